@@ -40,6 +40,7 @@ extern "C" {
 #define WNW_F32 0
 #define WNW_F16 1
 #define WNW_BF16 2
+#define WNW_E4M3 3 /* pages of a paged cache only: OCP 8-bit floats       */
 
 /* device error bits recorded by kernels (wnw_device_error) */
 #define WNW_DEVERR_BOUNDS 1   /* an offset pointed outside the given rows  */
@@ -744,6 +745,108 @@ int wnw_prefill_scores(const void* q, const void* k, const void* mask,
  */
 int wnw_read_stream(const void* src, int64_t bytes, int64_t n_wg, int form,
                     void* sink, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Paged cache                                                               */
+/* ------------------------------------------------------------------------ */
+/*
+ * A cache in pages (no reference counterpart; its segments are the flat
+ * cache's, src/common/kv/flat_cache.py:46-54).  Segment s = b * Hkv + h holds
+ * the rows of (sequence b, KV head h); its row i lies in row i % page_rows of
+ * page page_table[s, i / page_rows].  A page belongs to one segment while that
+ * segment is appended to; segments that are only read may share pages.  Table
+ * entries past a segment's rows are not read.
+ *
+ * page_dtype WNW_BF16 / WNW_F16: the rows themselves.  WNW_E4M3: codes that
+ * stand for code * k_scale[page] (v_scale for V); the scales are positive.
+ * Bad lengths, table entries and token offsets set the device error word:
+ * WNW_DEVERR_BOUNDS (an entry that is no page, a length below zero or past
+ * the table, token offsets that decrease or leave the tokens) or
+ * WNW_DEVERR_CAPACITY (an append past the table).  Nothing is read or written
+ * outside the arrays: rows in no page are not stored, and read as zeros;
+ * outputs of a segment with a bad length are zeros.
+ */
+typedef struct {
+  void* k_pages;             /* [n_pages, page_rows, head_dim]               */
+  void* v_pages;
+  float* k_scale;            /* [n_pages] with WNW_E4M3, else NULL           */
+  float* v_scale;
+  const int32_t* page_table; /* [n_seg, max_blocks]                          */
+  int64_t n_seg, n_pages, max_blocks;
+  int64_t page_rows;         /* 16, 32, 64, 128 or 256                       */
+  int64_t head_dim;          /* 64, 128 or 256                               */
+  int64_t k_stride, v_stride; /* elements from one page to the next          */
+  int64_t table_stride;      /* entries from one segment's row to the next   */
+  int32_t page_dtype;
+} wnw_paged_cache;
+
+/*
+ * Appends each sample's new tokens to its Hkv = n_seg / n_samples segments,
+ * rotating K on the way (and q beside it); new_len = seg_len + tokens.
+ *
+ * k, v: [n_tokens, Hkv, head_dim], q (or NULL): [n_tokens, Hkv * group,
+ * head_dim] with strides[6] = {q token, q head, k token, k head, v token, v
+ * head} in elements (multiples of 8); q_out contiguous, of q's type.  Sample b
+ * has tokens [cu_tokens[b], cu_tokens[b + 1]), at most max_tokens (a larger
+ * sample is refused on the device: WNW_DEVERR_BOUNDS); with cu_tokens NULL
+ * token b alone.
+ *
+ * positions (NULL: no rotation): [n_sections, n_tokens], int64 or int32
+ * (pos_bits), pos_stride entries from one axis to the next; inv_freq [rot / 2]
+ * double or float (freq_bits).  Pair j turns by positions[axis(j)] *
+ * inv_freq[j]; the first sections[0] pairs take axis 0, the next sections[1]
+ * axis 1 and so on (at most four, adding up to rot / 2).  A pair is elements
+ * (j, j + rot / 2), or (2 j, 2 j + 1) with `interleaved`; elements from rot on
+ * are not rotated.
+ *
+ * WNW_E4M3: a page's scale is the least power of two 2^e, e >= -64, with
+ * |x| <= 448 * 2^e for the rows in it; it never falls while the page fills,
+ * and rows already there are rescaled when it rises.  Infinities and NaN are
+ * stored as NaN and do not count for the scale.
+ */
+int wnw_paged_append(const wnw_paged_cache* cache, const int32_t* seg_len,
+                     int32_t* new_len, const void* q, const void* k,
+                     const void* v, void* q_out, const int64_t* strides,
+                     int64_t n_tokens, int64_t n_samples, int64_t group,
+                     const int32_t* cu_tokens, int64_t max_tokens,
+                     const void* positions, int pos_bits, int64_t pos_stride,
+                     const void* inv_freq, int freq_bits, int64_t rot,
+                     const int32_t* sections, int n_sections, int interleaved,
+                     int dtype, void* stream);
+
+/*
+ * Decode attention over the cache: q, out [n_seg, group, head_dim], group at
+ * most 16; 16-bit pages have q's type.  A segment without rows gives zeros.
+ * The first wnw_paged_counter_bytes of the workspace (256-byte aligned, of at
+ * least wnw_paged_decode_workspace_bytes(n_seg, group, head_dim)) must be zero
+ * before its first use and are left zero by every launch; launches that may
+ * overlap must not share one.
+ */
+int64_t wnw_paged_counter_bytes(int64_t n_seg);
+int64_t wnw_paged_decode_workspace_bytes(int64_t n_seg, int64_t rows,
+                                         int64_t head_dim);
+int wnw_paged_decode_attn(const wnw_paged_cache* cache, const int32_t* seg_len,
+                          const void* q, void* out, int64_t group, float scale,
+                          int dtype, void* workspace, int64_t workspace_bytes,
+                          void* stream);
+
+/*
+ * Causal attention of each sample's last n tokens over its segments, which
+ * hold them already: token i of n sees the first seg_len - n + i + 1 rows
+ * (none: zeros).  q, out: [n_tokens, Hkv * group, head_dim] with strides[4] =
+ * {q token, q head, out token, out head}; cu_tokens and max_tokens as for the
+ * append.  Up to 16 query rows per segment (max_tokens * group) run the decode
+ * kernel and need its workspace; wnw_paged_prompt_workspace_bytes gives the
+ * bytes either way.
+ */
+int64_t wnw_paged_prompt_workspace_bytes(const wnw_paged_cache* cache,
+                                         int64_t group, int64_t max_tokens);
+int wnw_paged_prompt_attn(const wnw_paged_cache* cache, const int32_t* seg_len,
+                          const void* q, void* out, const int64_t* strides,
+                          int64_t n_tokens, int64_t n_samples, int64_t group,
+                          const int32_t* cu_tokens, int64_t max_tokens,
+                          float scale, int dtype, void* workspace,
+                          int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -15,7 +15,7 @@ _BUILD = "build the HIP extension first (python -c 'import __graft_entry__ as g;
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libwnw_amd.so")
 
 WNW_OK, WNW_EINVAL, WNW_EHIP, WNW_ENOTSUP = 0, 1, 2, 3
-DT_F32, DT_F16, DT_BF16 = 0, 1, 2
+DT_F32, DT_F16, DT_BF16, DT_E4M3 = 0, 1, 2, 3
 ATTN_AUTO, ATTN_MFMA, ATTN_VALU, ATTN_STREAM = 0, 1, 2, 3
 DEVERR_BOUNDS, DEVERR_ORDER, DEVERR_CAPACITY = 1, 2, 4
 NOALLOC_SCRATCH_BYTES, NOALLOC_MAX_SEG = 16 << 20, 4096
@@ -66,6 +66,13 @@ _SIGNATURES = {
     "wnw_prefill_scores_workspace_bytes": (_i64, [_i64] * 5 + [_i32]),
     "wnw_prefill_scores": (_i32, [_vp] * 4 + [_i64] * 5 + [_vp, _vp, _vp, _i64, _vp, _i64, _i32, _f32, _i32, _i32, _i64,
                                                          _i64, _vp, _vp, _vp, _i64, _vp]),
+    "wnw_paged_append": (_i32, [_vp] * 8 + [_i64] * 3 + [_vp, _i64, _vp, _i32, _i64, _vp, _i32, _i64, _vp, _i32, _i32,
+                                                       _i32, _vp]),
+    "wnw_paged_counter_bytes": (_i64, [_i64]),
+    "wnw_paged_decode_workspace_bytes": (_i64, [_i64] * 3),
+    "wnw_paged_decode_attn": (_i32, [_vp] * 4 + [_i64, _f32, _i32, _vp, _i64, _vp]),
+    "wnw_paged_prompt_workspace_bytes": (_i64, [_vp, _i64, _i64]),
+    "wnw_paged_prompt_attn": (_i32, [_vp] * 5 + [_i64] * 3 + [_vp, _i64, _f32, _i32, _vp, _i64, _vp]),
     "wnw_read_stream": (_i32, [_vp, _i64, _i64, _i32, _vp, _vp]),
     # host planner (CPU only)
     "wnw_planner_create": (_vp, [_i32, _i32, _i32, _i32]),
@@ -98,6 +105,14 @@ _SIGNATURES = {
     "wnw_h2d_join": (_i32, [_vp]),
     "wnw_h2d_reserve": (_i32, [_vp, _i64, _i32, _vp]),
 }
+
+
+class PagedCache(ctypes.Structure):
+    """``wnw_paged_cache`` of include/wnw_amd.h."""
+
+    _fields_ = [("k_pages", _vp), ("v_pages", _vp), ("k_scale", _vp), ("v_scale", _vp), ("page_table", _vp),
+                ("n_seg", _i64), ("n_pages", _i64), ("max_blocks", _i64), ("page_rows", _i64), ("head_dim", _i64),
+                ("k_stride", _i64), ("v_stride", _i64), ("table_stride", _i64), ("page_dtype", ctypes.c_int32)]
 
 
 def exported_symbols() -> list[str]:

@@ -1,0 +1,453 @@
+// Prompt attention over the paged cache (gfx950): the tokens of a prompt or of
+// a chunk of one, each against the rows up to its own.
+//
+// Mathematics: as decode attention, causal: token i of a sample's n sees the
+// segment's first len - n + i + 1 rows.
+//
+// A workgroup takes 128 query rows of one segment, a row being (token, head of
+// the group): the group shares the keys.  A wave has 32 of them and walks the
+// 64-key tiles up to its last row's:
+//   S^T (64 keys x 32 queries) = K Q^T, Q in registers, K from LDS;
+//   O^T (D x 32) += V^T P^T, the weights in 16 bits (the largest is near 1),
+//       their sum in 32, V^T by transposed LDS reads in S^T's own order.
+// The tiles go through registers into LDS, where 8-bit codes become 16-bit
+// elements once for all four waves; one barrier per tile, the loads two tiles
+// ahead.  K's page scale multiplies the exponent, V's is added to it as its
+// logarithm relative to the largest so far (a part of 2^x either way), so that
+// scales cost a few instructions per 16 keys and any scale fits 16 bits.
+//
+// Few query rows and many keys: the tiles of each workgroup are cut into
+// splits, whose sums a second launch adds up.
+#include <algorithm>
+#include <type_traits>
+
+#include "paged.h"
+
+namespace wnw {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+int paged_decode_launch(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, void* out, const int64_t* strides,
+                        const PagedTokens& t, int64_t group, float scale, int dtype, void* workspace, int64_t bytes,
+                        void* stream);
+int paged_attn_check(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, const void* out,
+                     const int64_t* strides, int64_t group, float scale, int dtype);
+
+struct PagedPromptParams {
+  PagedCache c;
+  PagedTokens t;
+  const int32_t* seg_len;
+  const void* q;
+  void* out;
+  int64_t qt, qh, ot, oh;  // strides in elements
+  float* part;             // [grid.x, splits, 4 waves]: D / 32 x 16 sums a lane, then max, sum, scale
+  float scale_log2;
+  int32_t G, nqb, splits;
+  int32_t* err;
+};
+
+static constexpr int kPpQ = 128;    // query rows of a workgroup
+static constexpr int kPpKeys = 64;  // keys of a tile
+
+template <typename T>
+__device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f32x16& c) {
+  if constexpr (std::is_same<T, bf16_t>::value)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// What a workgroup's rows are.
+struct PromptRows {
+  int first, count, len, rows;  // the sample's tokens, the segment's rows, query rows
+};
+__device__ __forceinline__ PromptRows prompt_rows(const PagedPromptParams& p, int seg, bool tell) {
+  PromptRows r;
+  const bool told = paged_tokens_of(p.t, seg, &r.first, &r.count);
+  r.len = p.seg_len[seg];
+  const bool good = r.len >= 0 && r.len <= p.c.capacity;
+  if (tell && (!told || !good)) raise_device_error(p.err, WNW_DEVERR_BOUNDS);
+  if (!good) r.len = 0;
+  r.rows = r.count * p.G;
+  return r;
+}
+
+// The wave's rows out: lane (hi, n) has elements 32 i + 8 j + 4 hi + 0..3 of row n
+template <typename T, int D>
+__device__ __forceinline__ void prompt_store(const PagedPromptParams& p, const PromptRows& r, int row, int h, int hi,
+                                             const f32x16 (&o)[D / 32], float l, float ref) {
+  if (row >= r.rows) return;
+  const int i = row / p.G, g = row - i * p.G;
+  T* op = (T*)p.out + (int64_t)(r.first + i) * p.ot + (int64_t)(h * p.G + g) * p.oh;
+  const bool none = r.len - r.count + i + 1 <= 0;
+  const float inv = __builtin_amdgcn_exp2f(ref) / l;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = none ? 0.f : o[dt][4 * j + e] * inv;
+      store_quad<T>(op, 32 * dt + 8 * j + 4 * hi, y);
+    }
+}
+
+template <typename T, int D, bool Q8>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(PagedPromptParams p) {
+  using Ops = HalfOps<T>;
+  constexpr int RB = D * 2, CH = RB / 16, TB = kPpKeys * RB;  // a tile in LDS: 16-bit elements
+  constexpr int GB = D * (Q8 ? 1 : 2);                        // bytes of a row in its page
+  constexpr int NI = kPpKeys * GB / 4096;                     // 16-byte loads per thread and tensor
+  constexpr int KK = D / 16, DT = D / 32;
+  constexpr int NB = D == 256 ? 1 : 2;  // tiles in LDS
+  __shared__ __attribute__((aligned(16))) uint8_t lds[NB * 2 * TB];  // [NB][K, V]
+  __shared__ float scales[2][kPpKeys / 16][2];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hi = lane >> 5, n = lane & 31;
+  const int N = p.c.n_seg;
+  const int seg = blockIdx.x % N, qblk = p.nqb - 1 - blockIdx.x / N;  // the longest first; a segment's keys in one L2
+  const PromptRows r = prompt_rows(p, seg, tid == 0 && qblk == 0 && blockIdx.y == 0);
+  if (qblk * kPpQ >= r.rows) return;
+  const int h = seg % p.t.hkv;
+  const int base = r.len - r.count + 1;  // token i sees base + i rows
+  const int row = qblk * kPpQ + 32 * w + n;
+  const int ri = min(row, r.rows - 1) / p.G, rg = min(row, r.rows - 1) - ri * p.G;
+  const int limit = base + ri;
+  // of the wave: rows its first and last query see; of the workgroup: its last
+  const int wfirst = base + min(qblk * kPpQ + 32 * w, r.rows - 1) / p.G;
+  const int wlast = base + min(qblk * kPpQ + 32 * w + 31, r.rows - 1) / p.G;
+  const int last = base + min(qblk * kPpQ + kPpQ - 1, r.rows - 1) / p.G;
+  const int tiles = max((last + kPpKeys - 1) / kPpKeys, 0);
+  const int t0 = (int)((int64_t)tiles * blockIdx.y / p.splits), t1 = (int)((int64_t)tiles * (blockIdx.y + 1) / p.splits);
+  const int mine = min(t1, (wlast + kPpKeys - 1) / kPpKeys);  // the wave's tiles end here
+  u32x4 qr[KK];
+  {
+    const T* qp = (const T*)p.q + (int64_t)(r.first + ri) * p.qt + (int64_t)(h * p.G + rg) * p.qh + 8 * hi;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) qr[kk] = *gptr<u32x4>(qp + 16 * kk);
+  }
+  // staging: the thread's rows of a tile and its 16 bytes of each
+  const int32_t* table = p.c.table + seg * p.c.table_stride;
+  auto page_of = [&](int at) {  // the page of row `at` of the segment, -1: none
+    int id = -1;
+    if (at < r.len) {
+      id = table[at >> p.c.shift];
+      if (id < 0 || id >= p.c.n_pages) {
+        raise_device_error(p.err, WNW_DEVERR_BOUNDS);
+        id = -1;
+      }
+    }
+    return id;
+  };
+  constexpr int CG = GB / 16;      // 16-byte chunks of a row in its page
+  constexpr int RPL = 256 / CG;    // rows per load of the workgroup
+  const int srow = tid / CG, sch = tid % CG;
+  int pid[NI], spid = -1;
+  u32x4 kr[NI], vr[NI];
+  float sk = 1.f, sv = 1.f;
+  auto find = [&](int tile) {  // the pages of the thread's rows
+#pragma unroll
+    for (int u = 0; u < NI; ++u) pid[u] = tile < t1 ? page_of(tile * kPpKeys + u * RPL + srow) : -1;
+    if (Q8 && tid < kPpKeys / 16) spid = tile < t1 ? page_of(tile * kPpKeys + 16 * tid) : -1;
+  };
+  auto fetch = [&](int tile) {
+    const int in = (1 << p.c.shift) - 1;
+#pragma unroll
+    for (int u = 0; u < NI; ++u) {
+      const int at = ((tile * kPpKeys + u * RPL + srow) & in) * GB + sch * 16;
+      kr[u] = vr[u] = u32x4{0, 0, 0, 0};
+      if (pid[u] >= 0) {
+        kr[u] = *gptr<u32x4>(p.c.k + (int64_t)pid[u] * p.c.k_stride + at);
+        vr[u] = *gptr<u32x4>(p.c.v + (int64_t)pid[u] * p.c.v_stride + at);
+      }
+    }
+    if (Q8 && tid < kPpKeys / 16) {
+      sk = sv = 1.f;
+      if (spid >= 0) {
+        sk = p.c.k_scale[spid];
+        sv = p.c.v_scale[spid];
+      }
+    }
+  };
+  auto put = [&](int buf) {
+    uint8_t* kt = lds + (NB == 2 ? buf * 2 * TB : 0);
+    uint8_t* vt = kt + TB;
+#pragma unroll
+    for (int u = 0; u < NI; ++u) {
+      const int rr = u * RPL + srow;
+      if constexpr (Q8) {
+        *(u32x4*)(kt + rr * RB + (((2 * sch) ^ (rr % CH)) * 16)) = e4m3x8<T>(kr[u][0], kr[u][1]);
+        *(u32x4*)(kt + rr * RB + (((2 * sch + 1) ^ (rr % CH)) * 16)) = e4m3x8<T>(kr[u][2], kr[u][3]);
+        *(u32x4*)(vt + rr * RB + (((2 * sch) ^ (2 * (rr & 3))) * 16)) = e4m3x8<T>(vr[u][0], vr[u][1]);
+        *(u32x4*)(vt + rr * RB + (((2 * sch + 1) ^ (2 * (rr & 3))) * 16)) = e4m3x8<T>(vr[u][2], vr[u][3]);
+      } else {
+        *(u32x4*)(kt + rr * RB + ((sch ^ (rr % CH)) * 16)) = kr[u];
+        *(u32x4*)(vt + rr * RB + ((sch ^ (2 * (rr & 3))) * 16)) = vr[u];
+      }
+    }
+    if (Q8 && tid < kPpKeys / 16) {
+      scales[buf][tid][0] = fmaxf(sk, 7.888609e-31f);  // 0 would make a masked score NaN
+      scales[buf][tid][1] = sv;
+    }
+  };
+  // lane offsets of the operands inside a tile
+  uint32_t koff[KK], voff[DT];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) koff[kk] = n * RB + (((2 * kk + hi) ^ (n % CH)) * 16);
+  {
+    const int lc = lane & 15, dsub = (lane >> 4) & 1;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      voff[dt] = (4 * hi + (lc >> 2)) * RB + (((4 * dt + 2 * dsub + ((lc & 3) >> 1)) ^ (2 * (lc >> 2))) * 16) + (lc & 1) * 8;
+  }
+  f32x16 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
+  float m = kPgLowest, l = 0.f;
+  float ref = -100.f;  // log2 of the largest V scale so far (Q8)
+  auto tile = [&](int i, auto masked) {
+    const uint8_t* kt = lds + (NB == 2 ? (i & 1) * 2 * TB : 0);
+    const uint8_t* vt = kt + TB;
+    f32x16 s[2];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) s[mt] = f32x16{};
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) s[mt] = mma32<T>(*(const u32x4*)(kt + koff[kk] + mt * 32 * RB), qr[kk], s[mt]);
+    float ck[4], lv[4];  // per 16 keys
+    if constexpr (Q8) {
+      float most = ref;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        ck[b] = scales[i & 1][b][0] * p.scale_log2;
+        lv[b] = __builtin_amdgcn_logf(scales[i & 1][b][1]);
+        most = fmaxf(most, lv[b]);
+      }
+      if (most > ref) {
+        const float f = __builtin_amdgcn_exp2f(ref - most);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
+        ref = most;
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) lv[b] = fmaxf(lv[b] - ref, -100.f);  // less is nothing beside the largest
+    } else {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        ck[b] = p.scale_log2;
+        lv[b] = 0.f;
+      }
+    }
+    if constexpr (decltype(masked)::value) {
+      const int lim = limit - i * kPpKeys - 4 * hi;  // keys 32 mt + 8 j + c (+ 4 hi) below it
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (32 * mt + 8 * (e >> 2) + (e & 3) >= lim) s[mt][e] = -INFINITY;
+    }
+    float mx = m;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      float y = s[b >> 1][8 * (b & 1)];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) y = fmaxf(y, s[b >> 1][8 * (b & 1) + e]);
+      mx = fmaxf(mx, y * ck[b]);
+    }
+    mx = max_x32(mx);
+    if (__ballot(mx > m)) {
+      const float f = __builtin_amdgcn_exp2f(m - mx);
+      l *= f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
+      m = mx;
+    }
+    u32x4 pb[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const float off = lv[b] - m;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float y0 = __builtin_amdgcn_exp2f(fmaf(s[b >> 1][8 * (b & 1) + 2 * j], ck[b], off));
+        const float y1 = __builtin_amdgcn_exp2f(fmaf(s[b >> 1][8 * (b & 1) + 2 * j + 1], ck[b], off));
+        sum += y0 + y1;
+        pb[b][j] = Ops::pack2(y0, y1);
+      }
+      l = Q8 ? fmaf(sum, __builtin_amdgcn_exp2f(-lv[b]), l) : l + sum;
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const uint64_t v0 = Ops::read_tr(vt + voff[dt] + 16 * b * RB);
+        const uint64_t v1 = Ops::read_tr(vt + voff[dt] + (16 * b + 8) * RB);
+        o[dt] = mma32<T>(u32x4{(uint32_t)v0, (uint32_t)(v0 >> 32), (uint32_t)v1, (uint32_t)(v1 >> 32)}, pb[b], o[dt]);
+      }
+  };
+  if (t0 < t1) {
+    find(t0);
+    fetch(t0);
+    find(t0 + 1);
+    if constexpr (NB == 2) {
+      put(t0 & 1);
+      fetch(t0 + 1);
+      find(t0 + 2);
+    }
+    for (int i = t0; i < t1; ++i) {
+      if constexpr (NB == 2) {
+        __syncthreads();  // tile i is in LDS; everyone is done with tile i - 1
+        if (i + 1 < t1) {
+          put((i + 1) & 1);
+          fetch(i + 2);
+          find(i + 3);
+        }
+      } else {
+        __syncthreads();  // everyone is done with tile i - 1
+        put(i & 1);
+        fetch(i + 1);
+        find(i + 2);
+        __syncthreads();
+      }
+      if (i >= mine) continue;
+      if ((i + 1) * kPpKeys > wfirst)
+        tile(i, std::true_type());
+      else
+        tile(i, std::false_type());
+    }
+  }
+  l = sum_x32(l);
+  if (p.splits == 1) {
+    prompt_store<T, D>(p, r, row, h, hi, o, l, Q8 ? ref : 0.f);
+  } else {
+    float* part = p.part + (((int64_t)blockIdx.x * p.splits + blockIdx.y) * 4 + w) * (DT * 16 + 3) * 64;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *(WNW_GLOBAL f32x4*)gptr_w<float>(part + ((dt * 4 + j) * 64 + lane) * 4) =
+            f32x4{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
+    part += DT * 16 * 64;
+    part[lane] = m;
+    part[64 + lane] = l;
+    part[128 + lane] = Q8 ? ref : 0.f;
+  }
+}
+
+// The splits' sums added up, a wave for 32 query rows.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParams p) {
+  constexpr int DT = D / 32;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hi = lane >> 5, n = lane & 31;
+  const int N = p.c.n_seg;
+  const int seg = blockIdx.x % N, qblk = p.nqb - 1 - blockIdx.x / N;
+  const PromptRows r = prompt_rows(p, seg, false);
+  if (qblk * kPpQ + 32 * w >= r.rows) return;
+  constexpr int64_t kPart = (DT * 16 + 3) * 64;
+  const float* part = p.part + ((int64_t)blockIdx.x * p.splits * 4 + w) * kPart;
+  f32x16 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
+  float m = kPgLowest, l = 0.f, ref = -100.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float* at = part + s * 4 * kPart;
+    const float pm = at[DT * 16 * 64 + lane], pl = at[DT * 16 * 64 + 64 + lane], pr = at[DT * 16 * 64 + 128 + lane];
+    const float mx = fmaxf(m, pm), most = fmaxf(ref, pr);
+    const float f = __builtin_amdgcn_exp2f(m - mx), g = __builtin_amdgcn_exp2f(pm - mx);
+    const float fo = f * __builtin_amdgcn_exp2f(ref - most), go = g * __builtin_amdgcn_exp2f(pr - most);
+    l = l * f + pl * g;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 y = *gptr<f32x4>(at + ((dt * 4 + j) * 64 + lane) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[dt][4 * j + e] = o[dt][4 * j + e] * fo + y[e] * go;
+      }
+    m = mx;
+    ref = most;
+  }
+  prompt_store<T, D>(p, r, qblk * kPpQ + 32 * w + n, seg % p.t.hkv, hi, o, l, ref);
+}
+
+// Splits: enough workgroups for two per CU, where the longest row has the tiles for it.
+struct PromptPlan {
+  int64_t nqb, splits, bytes;
+};
+static PromptPlan prompt_plan(int64_t n_seg, int64_t group, int64_t max_tokens, int64_t capacity, int64_t D) {
+  PromptPlan y;
+  y.nqb = (max_tokens * group + kPpQ - 1) / kPpQ;
+  const int64_t wgs = std::max<int64_t>(n_seg * y.nqb, 1), want = 2ll * device_cus(), tiles = (capacity + kPpKeys - 1) / kPpKeys;
+  y.splits = std::max<int64_t>(1, std::min({want / wgs, tiles / 4, (int64_t)64}));
+  y.bytes = y.splits == 1 ? 0 : wgs * y.splits * 4 * (D / 2 + 3) * 64 * 4;
+  return y;
+}
+
+template <typename T, int D, bool Q8>
+static hipError_t launch_prompt_q(const PagedPromptParams& p, hipStream_t st) {
+  const dim3 grid((unsigned)(p.c.n_seg * (int64_t)p.nqb), (unsigned)p.splits);
+  hipLaunchKernelGGL((paged_prompt_kernel<T, D, Q8>), grid, dim3(256), 0, st, p);
+  if (p.splits > 1) hipLaunchKernelGGL((paged_prompt_join_kernel<T, D>), dim3(grid.x), dim3(256), 0, st, p);
+  return hipGetLastError();
+}
+template <typename T>
+static hipError_t launch_prompt(const PagedPromptParams& p, int64_t D, bool q8, hipStream_t st) {
+  if (D == 64) return q8 ? launch_prompt_q<T, 64, true>(p, st) : launch_prompt_q<T, 64, false>(p, st);
+  if (D == 128) return q8 ? launch_prompt_q<T, 128, true>(p, st) : launch_prompt_q<T, 128, false>(p, st);
+  return q8 ? launch_prompt_q<T, 256, true>(p, st) : launch_prompt_q<T, 256, false>(p, st);
+}
+
+static constexpr int kFewRows = 16;  // query rows of a segment that decode attention takes
+
+}  // namespace wnw
+
+using namespace wnw;
+
+extern "C" int64_t wnw_paged_prompt_workspace_bytes(const wnw_paged_cache* cache, int64_t group, int64_t max_tokens) {
+  PagedCache c;
+  if (!cache || group < 1 || group > 1024 || max_tokens < 0 || max_tokens >= (1 << 24)) return -1;
+  if (paged_cache_of(cache, false, &c)) return -1;
+  if (max_tokens == 0) return 0;
+  if (max_tokens * group <= kFewRows) return wnw_paged_decode_workspace_bytes(cache->n_seg, max_tokens * group, cache->head_dim);
+  return prompt_plan(cache->n_seg, group, max_tokens, c.capacity, cache->head_dim).bytes;
+}
+
+extern "C" int wnw_paged_prompt_attn(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, void* out,
+                                     const int64_t* strides, int64_t n_tokens, int64_t n_samples, int64_t group,
+                                     const int32_t* cu_tokens, int64_t max_tokens, float scale, int dtype, void* workspace,
+                                     int64_t workspace_bytes, void* stream) {
+  PagedPromptParams p = {};
+  if (int rc = paged_cache_of(cache, false, &p.c)) return rc;
+  const int64_t N = cache->n_seg, D = cache->head_dim;
+  WNW_CHECK_ARG(n_samples >= 0 && (n_samples > 0 ? N % n_samples == 0 : N == 0), "segments must be samples x KV heads");
+  WNW_CHECK_ARG(n_tokens >= 0 && n_tokens < (1 << 24) && max_tokens >= 0, "bad token counts");
+  if (N == 0 || n_tokens == 0) return WNW_OK;
+  WNW_CHECK_ARG(cu_tokens, "cu_tokens is null");
+  if (int rc = paged_attn_check(cache, seg_len, q, out, strides, group, scale, dtype)) return rc;
+  const int64_t most = std::min(max_tokens, n_tokens);
+  WNW_CHECK_ARG(most > 0, "max_tokens is zero");
+  p.t = PagedTokens{cu_tokens, (int32_t)n_tokens, (int32_t)(N / n_samples), (int32_t)most};
+  if (most * group <= kFewRows)
+    return paged_decode_launch(cache, seg_len, q, out, strides, p.t, group, scale, dtype, workspace, workspace_bytes, stream);
+  WNW_CHECK_ARG(most * group < (1ll << 30), "too many query rows");
+  const PromptPlan y = prompt_plan(N, group, most, p.c.capacity, D);
+  WNW_CHECK_ARG(N * y.nqb < (1ll << 31), "too many segments and tokens for one call");
+  WNW_CHECK_ARG(y.bytes == 0 || (workspace && workspace_bytes >= y.bytes), "workspace too small: %lld bytes, %lld needed",
+                (long long)workspace_bytes, (long long)y.bytes);
+  WNW_CHECK_ARG((uintptr_t)workspace % 256 == 0, "the workspace must be 256-byte aligned");
+  p.seg_len = seg_len;
+  p.q = q;
+  p.out = out;
+  p.qt = strides[0], p.qh = strides[1], p.ot = strides[2], p.oh = strides[3];
+  p.part = (float*)workspace;
+  p.scale_log2 = scale * kPgLog2e;
+  p.G = (int32_t)group;
+  p.nqb = (int32_t)y.nqb;
+  p.splits = (int32_t)y.splits;
+  p.err = device_error_word();
+  const hipError_t e = dtype == WNW_BF16 ? launch_prompt<bf16_t>(p, D, cache->page_dtype == WNW_E4M3, (hipStream_t)stream)
+                                         : launch_prompt<f16_t>(p, D, cache->page_dtype == WNW_E4M3, (hipStream_t)stream);
+  WNW_CHECK_HIP(e, "paged prompt attention launch");
+  return WNW_OK;
+}
