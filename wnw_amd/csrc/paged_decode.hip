@@ -7,9 +7,13 @@
 // 2^(m' - m) each, so any split of the rows gives the same sums.
 //
 // Work split: the segments' rows in steps of 32 (no step crosses a segment),
-// all steps cut evenly over the workgroups; a workgroup's steps of one segment
-// are dealt to its four waves in turn.  The lengths are read on the device, so a
-// captured launch stays right as segments grow.
+// all steps cut evenly over the workgroups, and a workgroup's steps dealt to its
+// waves by pieces: a piece (its steps of one segment) has as many waves as its
+// share, whole waves, so that no wave holds the sums of two pieces at once and
+// short segments run side by side.  A piece of one wave ends in its registers,
+// one of several in LDS; a segment cut between workgroups in memory, added up by
+// the last of them to arrive.  The lengths are read on the device, so a captured
+// launch stays right as segments grow.
 //
 // A step: S^T (rows x queries) = K Q^T with the rows' 16-byte chunks straight
 // from memory as matrix operands (any order of the elements of a dot will do,
@@ -43,31 +47,48 @@ struct PagedDecodeParams {
 };
 
 static constexpr int kPdStep = 32;  // rows of a step
-static constexpr int kPdWaves = 4;
-static constexpr int kPdMin = 4;    // steps of a workgroup at least
+static constexpr int kPdMin = 8;    // steps of a workgroup at least
 
 template <int D, bool Q8>
 struct PagedDecodeGeom {
-  static constexpr int RB = D * (Q8 ? 1 : 2);  // bytes of a row
-  static constexpr int KC = RB / 64;           // 16-byte chunks of a K row per lane
-  static constexpr int VI = kPdStep * RB / 1024;  // loads of a step's V per lane
-  static constexpr int kStage = kPdStep * RB;     // LDS of a wave's V
-  static constexpr int kState = 16 * (D + 4) * 4; // LDS of a wave's sums
-  static constexpr int kLds = kPdWaves * (kStage > kState ? kStage : kState);
-  // workgroups per CU
-  static constexpr int kWgs = D == 256 ? 2 : Q8 || D == 64 ? 4 : 3;
+  static constexpr int RB = D * (Q8 ? 1 : 2);      // bytes of a row
+  static constexpr int KC = RB / 64;               // 16-byte chunks of a K row per lane
+  static constexpr int VI = kPdStep * RB / 1024;   // loads of a step's V per lane
+  // Bytes in flight and registers: a step is 8 to 32 KB of loads per wave, and
+  // 128 KB a CU keep the memory busy.
+  static constexpr int kWaves = RB >= 512 ? 4 : 8;  // of a workgroup
+  static constexpr int kWgs = RB >= 256 ? 1 : 2;    // workgroups per CU
+  static constexpr int kStage = kPdStep * RB;       // LDS of a wave's V
+  static constexpr int kQ = D * 32;                 // of its q
+  static constexpr int kState = 16 * (D + 4) * 4;   // of its sums, in the place of both
+  static constexpr int kPart = kStage + kQ > kState ? kStage + kQ : kState;
 };
 
-// Row r's 16-byte chunk c of a step's V in LDS.  The transposed reads take 8
-// rows of one chunk (8 bits: rows 4 q .. + 3 and 16 + 4 q .. + 3) or 4 rows of
-// two chunks (16 bits) at a time: both without bank conflicts.
+// A step's V in LDS: row r's 16-byte chunk c lies at r * RB + 16 * (c ^ x(r)).
+// The transposed reads take 8 rows of one chunk (8 bits: rows 4 q .. + 3 and 16 +
+// 4 q .. + 3) or 4 rows of two chunks (16 bits) at a time; x keeps both, and the
+// writes of whole rows, free of bank conflicts.  x(r) is a lane's part and a
+// load's part that do not overlap, so an address is a lane's constant XOR a
+// number known at compile time.
 template <int D, bool Q8>
-__device__ __forceinline__ int v_at(int r, int c) {
-  constexpr int RB = PagedDecodeGeom<D, Q8>::RB;
-  if constexpr (!Q8) return r * RB + ((c ^ (2 * (r & 3))) * 16);
-  const int f = (r & 3) | ((r >> 4) & 1) << 2;
-  return r * RB + ((c ^ (RB == 64 ? f >> 1 : f)) * 16);
-}
+struct PagedDecodeV {
+  static constexpr int RB = PagedDecodeGeom<D, Q8>::RB, VI = PagedDecodeGeom<D, Q8>::VI, CH = RB / 16;
+  // load i writes rows i * 64 / CH + lane / CH
+  __device__ static uint32_t write_base(int lane) {
+    const int r = lane / CH, c = lane % CH;
+    const int x = !Q8 ? 2 * (r & 3) : CH == 4 ? r >> 1 & 1 : r & 3;
+    return r * RB + 16 * (c ^ x);
+  }
+  static constexpr uint32_t write_x(int i) {
+    return !Q8 ? (D == 256 ? 64 * (i & 1) : 0) : i >= VI / 2 ? (CH == 4 ? 32 : 64) : 0;
+  }
+  // 16 columns i * 16 .. of the lane's rows
+  __device__ static uint32_t read_base(int lq, int lc) {
+    if (!Q8) return (4 * lq + (lc >> 2)) * RB + 16 * (((lc & 3) >> 1) ^ (2 * (lc >> 2))) + 8 * (lc & 1);
+    return (4 * lq + (lc >> 1 & 3) + 16 * (lc >> 3)) * RB + 16 * (CH == 4 ? lc >> 2 : lc >> 1) + 8 * (lc & 1);
+  }
+  static constexpr uint32_t read_x(int i) { return (Q8 ? 16 : 32) * i; }
+};
 
 // Two positive values as two pairs of 16-bit parts
 template <typename T>
@@ -95,46 +116,174 @@ __device__ __forceinline__ void load_agent(const float* p, float* a, float* b) {
   *b = __uint_as_float((uint32_t)(x >> 32));
 }
 
+// x, as a value that the compiler does not know: what follows from it is worked
+// out here and not, ahead of the loops around, held in registers all along
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// A segment's result from its sums: element d .. d + 3 of query row col
+template <typename T, int D>
+__device__ __forceinline__ void paged_decode_out(const PagedDecodeParams& p, int seg, int n, int col, int d, const float* o,
+                                                 float L) {
+  int first, count;
+  paged_tokens_of(p.t, seg, &first, &count);
+  const int ti = col / p.G, h = seg % p.t.hkv;
+  const bool sees = n - count + ti + 1 > 0;  // else a row without keys
+  const float inv = 1.f / L;
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = sees ? o[i] * inv : 0.f;
+  store_quad<T>((T*)p.out + (int64_t)(first + ti) * p.ot + (int64_t)(h * p.G + col - ti * p.G) * p.oh, d, y);
+}
+__device__ __forceinline__ int paged_decode_cols(const PagedDecodeParams& p, int seg) {
+  int first, count;
+  paged_tokens_of(p.t, seg, &first, &count);
+  return min(count * p.G, p.cols);
+}
+
+// The sums of a piece's waves: the segment's result (done), or its partial in a slot
+template <typename T, int D, typename FM, typename FS>
+__device__ __forceinline__ void paged_decode_join(const PagedDecodeParams& p, int seg, int n, int tid, int threads, bool done,
+                                                  int slot, FM most, FS sums) {
+  tid = here(tid);
+  const int cols = paged_decode_cols(p, seg);
+  for (int e = tid; e < cols * (D / 4); e += threads) {
+    const int col = e / (D / 4), d = 4 * (e % (D / 4));
+    float M = kPgLowest, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    most(col, &M);
+    sums(col, d, M, &L, o);
+    if (done) {
+      paged_decode_out<T, D>(p, seg, n, col, d, o, L);
+    } else {
+      const int64_t to = (int64_t)slot * p.cols + col;
+      store_agent(p.part_acc + to * D + d, o[0], o[1]);
+      store_agent(p.part_acc + to * D + d + 2, o[2], o[3]);
+      if (d == 0) store_agent(p.part_ml + to * 2, M, L);
+    }
+  }
+}
+
+// The partials of workgroups [w0, w1] (the first in slot0, the others each in
+// its first slot) added up: in as many runs as there are threads for, then the
+// runs, by way of lds.
+template <typename T, int D, int NT>
+__device__ __forceinline__ void paged_decode_gather(const PagedDecodeParams& p, int seg, int n, int tid, int64_t slot0, int w0,
+                                                    int w1, float* lds) {
+  tid = here(tid);
+  const int items = paged_decode_cols(p, seg) * (D / 4), runs = max(1, min(NT / max(items, 1), 8));
+  const int each = (w1 - w0 + runs) / runs, run = runs > 1 ? tid / max(items, 1) : 0;
+  __syncthreads();
+  for (int e = tid - run * items; e < items && run < runs; e += runs > 1 ? items : NT) {
+    const int col = e / (D / 4), d = 4 * (e % (D / 4));
+    const int a0 = w0 + run * each, a1 = min(a0 + each - 1, w1);
+    float M = kPgLowest, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = a0; i0 <= a1; i0 += 4) {
+      float pm[4], pl[4], po[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int from = min(i0 + i, a1);
+        const int64_t at = (from == w0 ? slot0 : 2 * (int64_t)from) * p.cols + col;
+        load_agent(p.part_ml + at * 2, &pm[i], &pl[i]);
+        load_agent(p.part_acc + at * D + d, &po[i][0], &po[i][1]);
+        load_agent(p.part_acc + at * D + d + 2, &po[i][2], &po[i][3]);
+      }
+      float now = M;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) now = fmaxf(now, pm[i]);
+      const float f0 = __builtin_amdgcn_exp2f(M - now);
+      L *= f0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] *= f0;
+      M = now;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f = i0 + i <= a1 ? __builtin_amdgcn_exp2f(pm[i] - M) : 0.f;
+        L += f * pl[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] += f * po[i][j];
+      }
+    }
+    if (runs == 1) {
+      paged_decode_out<T, D>(p, seg, n, col, d, o, L);
+    } else {
+      float* to = lds + (run * items + e) * 8;
+      *(f32x4*)to = f32x4{o[0], o[1], o[2], o[3]};
+      to[4] = M;
+      to[5] = L;
+    }
+  }
+  if (runs == 1) return;
+  __syncthreads();
+  if (tid < items) {
+    float M = kPgLowest, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < runs; ++i) M = fmaxf(M, lds[(i * items + tid) * 8 + 4]);
+    for (int i = 0; i < runs; ++i) {
+      const float* at = lds + (i * items + tid) * 8;
+      const float f = __builtin_amdgcn_exp2f(at[4] - M);
+      L += f * at[5];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] += f * at[j];
+    }
+    paged_decode_out<T, D>(p, seg, n, tid / (D / 4), 4 * (tid % (D / 4)), o, L);
+  }
+}
+
 template <typename T, int D, bool Q8>
-__global__ __launch_bounds__(256, (PagedDecodeGeom<D, Q8>::kWgs)) void paged_decode_kernel(PagedDecodeParams p) {
+__global__ __launch_bounds__((64 * PagedDecodeGeom<D, Q8>::kWaves),
+                             (PagedDecodeGeom<D, Q8>::kWaves * PagedDecodeGeom<D, Q8>::kWgs / 4)) void
+paged_decode_kernel(PagedDecodeParams p) {
   using Ge = PagedDecodeGeom<D, Q8>;
   using VT = typename std::conditional<Q8, bf16_t, T>::type;  // the value product's type: any scale fits bf16
   using QO = HalfOps<T>;
   using VO = HalfOps<VT>;
+  using Vl = PagedDecodeV<D, Q8>;
+  constexpr int W = Ge::kWaves, NT = 64 * W;
   constexpr int RB = Ge::RB, KC = Ge::KC, VI = Ge::VI, DT = D / 16, KK = D / 32;
   // weights of f16 are held times 2^12: their lower parts reach 2^-36 of the largest
   constexpr float kBias = std::is_same<VT, f16_t>::value ? 12.f : 0.f;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[Ge::kLds];
-  __shared__ float st[kPdWaves][16][2];
-  __shared__ int32_t sh[8];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[W * Ge::kPart];
+  __shared__ float st[W][16][2];
+  __shared__ int32_t sh[W + 4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lq = lane >> 4, lc = lane & 15;
   const int N = p.c.n_seg, wg = blockIdx.x;
 
-  auto steps_of = [&](int s) {
-    const int n = p.seg_len[s];
-    return n >= 0 && n <= p.c.capacity ? (n + kPdStep - 1) / kPdStep : 0;
+  auto steps_of = [&](int n) { return n >= 0 && n <= p.c.capacity ? (n + kPdStep - 1) / kPdStep : 0; };
+  auto scan = [&](int x) {  // inclusive, over the wave
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(x, o);
+      if (lane >= o) x += y;
+    }
+    return x;
   };
-  // all steps, and where this workgroup's begin
-  const int per = (N + 255) / 256;
-  const int sa = min(tid * per, N), sb = min(sa + per, N);
-  int mine = 0;
-  for (int s = sa; s < sb; ++s) mine += steps_of(s);
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(incl, o);
-    if (lane >= o) incl += y;
+  // All steps, this workgroup's [x0, x1), and the window of 64 segments from
+  // its first one on: lane j has segment win + j, of `len` rows, whose `num`
+  // steps come after `at` others.
+  int win = 0, len = 0, num = 0, at = 0, S;
+  if (N <= 64) {
+    len = lane < N ? p.seg_len[lane] : 0;
+    num = steps_of(len);
+    at = scan(num);
+    S = __builtin_amdgcn_readlane(at, 63);
+    at -= num;
   }
-  if (lane == 63) sh[w] = incl;
-  __syncthreads();
-  int before = 0, S = 0;
+  int mine = 0, incl = 0, before = 0;
+  const int per = (N + NT - 1) / NT, sa = min(tid * per, N), sb = min(sa + per, N);
+  if (N > 64) {
+    for (int s = sa; s < sb; ++s) mine += steps_of(p.seg_len[s]);
+    incl = scan(mine);
+    if (lane == 63) sh[w] = incl;
+    __syncthreads();
+    S = 0;
 #pragma unroll
-  for (int i = 0; i < kPdWaves; ++i) {
-    if (i < w) before += sh[i];
-    S += sh[i];
+    for (int i = 0; i < W; ++i) {
+      if (i < w) before += sh[i];
+      S += sh[i];
+    }
+    S = __builtin_amdgcn_readfirstlane(S);
   }
-  S = __builtin_amdgcn_readfirstlane(S);
   const int P = min((int)gridDim.x, max(S / kPdMin, 1));
   const int share = S / P, more = S - share * P;  // the first `more` workgroups take one step more
   auto start_of = [&](int i) { return i * share + min(i, more); };
@@ -143,306 +292,324 @@ __global__ __launch_bounds__(256, (PagedDecodeGeom<D, Q8>::kWgs)) void paged_dec
     return x < big ? x / (share + 1) : more + (x - big) / max(share, 1);
   };
   const int x0 = wg < P ? start_of(wg) : 0, x1 = wg < P ? start_of(wg + 1) : 0;
-  if (x0 < x1) {
-    int e = before + incl - mine;  // steps before the thread's segments
-    if (e <= x0 && x0 < e + mine) {
-      int s = sa;
-      for (int n; e + (n = steps_of(s)) <= x0; ++s) e += n;
-      sh[4] = s;
-      sh[5] = e;
+  if (N > 64 && x0 < x1) {
+    const int e0 = before + incl - mine;  // steps before the thread's segments
+    if (e0 <= x0 && x0 < e0 + mine) {
+      int s = sa, e = e0;
+      for (int n; e + (n = steps_of(p.seg_len[s])) <= x0; ++s) e += n;
+      sh[W] = s;
+      sh[W + 1] = e;
     }
+    __syncthreads();
+    win = __builtin_amdgcn_readfirstlane(sh[W]);
+    at = __builtin_amdgcn_readfirstlane(sh[W + 1]);
   }
-  __syncthreads();
-  int seg = __builtin_amdgcn_readfirstlane(sh[4]), base = __builtin_amdgcn_readfirstlane(sh[5]);
 
-  for (int x = x0; x < x1 && seg < N; ++seg) {
-    const int len = p.seg_len[seg], ns = steps_of(seg);
-    if (ns == 0) continue;
-    const int a = x - base, b = min(ns, x1 - base);  // the piece: steps [a, b) of the segment
-    int first, count;
-    paged_tokens_of(p.t, seg, &first, &count);
-    const int h = seg % p.t.hkv;
-    const int cols = min(count * p.G, p.cols);
-    const int c = min(lc, max(cols - 1, 0)), ti = c / p.G, g = c - ti * p.G;
-    const int limit = len - count + ti + 1;           // rows that the lane's column sees
-    const int all_see = len - count + 1;              // rows that every column sees
-    // q, in the order of K's chunks
-    u32x4 qf[KK];
-    {
-      const T* qp = (const T*)p.q + (int64_t)(first + ti) * p.qt + (int64_t)(h * p.G + g) * p.qh;
-#pragma unroll
-      for (int i = 0; i < KK; ++i) {
-        const int d = Q8 ? 16 * (lq + 4 * (i >> 1)) + 8 * (i & 1) : 8 * (lq + 4 * i);
-        qf[i] = cols > 0 ? *gptr<u32x4>(qp + d) : u32x4{0, 0, 0, 0};
-      }
+  for (int x = x0; x < x1 && win < N;) {
+    if (N > 64) {
+      len = win + lane < N ? p.seg_len[win + lane] : 0;
+      num = steps_of(len);
+      at += scan(num) - num;
     }
-    f32x4 acc[DT];
+    // the pieces of this window, and the waves [wf, wt) of each; a piece that
+    // has none (wf == wt) is done by a wave beside its own
+    const int xe = min(x1, __builtin_amdgcn_readlane(at + num, 63));
+    const int pa = max(at, x), pb = min(at + num, xe), all = xe - x;
+    const bool some = pa < pb;
+    const int wf = some ? (2 * W * (pa - x) + all) / (2 * all) : 0, wt = some ? (2 * W * (pb - x) + all) / (2 * all) : 0;
+    const uint64_t several = __ballot(some && wt - wf > 1), cut = __ballot(some && (pa != at || pb != at + num));
+    const int waves = wf | wt << 8;
+    // segment win + j: its steps before the piece and up to its end
+    auto piece = [&](int j, int* a, int* b) {
+      const int e = __builtin_amdgcn_readlane(at, j);
+      *a = max(x - e, 0);
+      *b = min(xe - e, __builtin_amdgcn_readlane(num, j));
+      return e;
+    };
+    // those beside its own first: its own sums stay in its LDS
+    uint64_t beside = __ballot(some && wf == wt && min(wf, W - 1) == w), own = __ballot(some && wf <= w && w < wt);
+    while (beside | own) {
+      const int j = __builtin_ctzll(beside ? beside : own), ln = here(lane), lq = ln >> 4, lc = ln & 15;
+      const int seg = win + j, n = __builtin_amdgcn_readlane(len, j);
+      const int f = __builtin_amdgcn_readlane(waves, j) & 255, t = __builtin_amdgcn_readlane(waves, j) >> 8;
+      const int nw = max(t - f, 1), iw = t > f ? w - f : 0;
+      int a, b;  // the wave's steps of the segment: a, a + nw, ... below b
+      const int first_step = piece(j, &a, &b);
+      a += iw;
+      const int mysteps = (b - a + nw - 1) / nw;
+      int first, count;
+      paged_tokens_of(p.t, seg, &first, &count);
+      const int h = seg % p.t.hkv;
+      const int cols = min(count * p.G, p.cols);
+      const int c = min(lc, max(cols - 1, 0)), ti = c / p.G, g = c - ti * p.G;
+      const int limit = n - count + ti + 1;  // rows that the lane's column sees
+      const int all_see = n - count + 1;     // rows that every column sees
+      f32x4 acc[DT];
 #pragma unroll
-    for (int i = 0; i < DT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = kPgLowest, l = 0.f;
-    const int mysteps = (b - a - w + kPdWaves - 1) / kPdWaves;  // this wave's: a + w + 4 k
-    uint8_t* stage = lds + w * (Ge::kLds / kPdWaves);
+      for (int i = 0; i < DT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      float m = kPgLowest, l = 0.f;
+      uint8_t* stage = lds + w * Ge::kPart;
+      const uint32_t klane = lc * RB + lq * 16, vlane = ln * 16;
+      uint32_t vput = Vl::write_base(ln), vget = Vl::read_base(lq, lc);
+      u32x4* qs = (u32x4*)(stage + Ge::kStage) + lane;
 
-    // a window of 32 steps' pages: lane l has the page of half l & 1 of step l / 2
-    int pid = -1;
-    float ks = 1.f, vs = 1.f;
-    auto window = [&](int k0) {
-      const int step = a + w + kPdWaves * (k0 + (lane >> 1));
-      const int row = step * kPdStep + 16 * (lane & 1);
-      pid = -1;
-      if (step < b && row < len) {
-        pid = p.c.table[seg * p.c.table_stride + (row >> p.c.shift)];
-        if (pid < 0 || pid >= p.c.n_pages) {
-          raise_device_error(p.err, WNW_DEVERR_BOUNDS);
-          pid = -1;
+      // a window of 32 steps' pages: lane l has the page of half l & 1 of step l / 2
+      int pid = -1;
+      float ks = 1.f, vs = 1.f;
+      auto window = [&](int k0) {
+        const int step = a + nw * (k0 + (lane >> 1));
+        const int row = step * kPdStep + 16 * (lane & 1);
+        pid = -1;
+        if (step < b && row < n) {
+          pid = p.c.table[seg * p.c.table_stride + (row >> p.c.shift)];
+          if (pid < 0 || pid >= p.c.n_pages) {
+            raise_device_error(p.err, WNW_DEVERR_BOUNDS);
+            pid = -1;
+          }
         }
-        if (Q8 && pid >= 0) {
-          ks = p.c.k_scale[pid];
-          vs = p.c.v_scale[pid];
+        if (Q8) {
+          ks = p.c.k_scale[max(pid, 0)];
+          vs = p.c.v_scale[max(pid, 0)];
         }
-      }
-    };
-    u32x4 kr[2][KC], vr[VI];
-    float ks0, ks1, vs0, vs1;  // of the step whose rows are in kr and vr
-    int bad = 0;               // halves of that step that no page holds
-    auto load = [&](int k) {
-      const int at = 2 * (k & 31);
-      const int step = a + w + kPdWaves * k;
-      const int p0 = __builtin_amdgcn_readlane(pid, at), p1 = __builtin_amdgcn_readlane(pid, at + 1);
-      if (Q8) {
-        ks0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), at));
-        ks1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), at + 1));
-        vs0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), at));
-        vs1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), at + 1));
-      }
-      bad = (p0 < 0 ? 1 : 0) | (p1 < 0 ? 2 : 0);
-      const int in = (step * kPdStep) & ((1 << p.c.shift) - 1);             // first row in its page
-      const int in1 = (step * kPdStep + 16) & ((1 << p.c.shift) - 1);
-      const int r0 = p0 < 0 ? (p1 < 0 ? 0 : p1) : p0, r1 = p1 < 0 ? r0 : p1;  // a half in no page reads the other's
-      const uint8_t* k0 = p.c.k + (int64_t)r0 * p.c.k_stride + (p0 < 0 ? 0 : in) * RB;
-      const uint8_t* k1 = p.c.k + (int64_t)r1 * p.c.k_stride + (p1 < 0 ? 0 : in1) * RB;
-      const uint8_t* v0 = p.c.v + (int64_t)r0 * p.c.v_stride + (p0 < 0 ? 0 : in) * RB;
-      const uint8_t* v1 = p.c.v + (int64_t)r1 * p.c.v_stride + (p1 < 0 ? 0 : in1) * RB;
+      };
+      u32x4 kr[2][KC], vr[VI];
+      int bad = 0;  // halves of the loaded step that no page holds
+      auto load = [&](int k) {
+        const int from = 2 * (k & 31);
+        const int step = a + nw * k;
+        const int p0 = __builtin_amdgcn_readlane(pid, from), p1 = __builtin_amdgcn_readlane(pid, from + 1);
+        bad = (p0 < 0 ? 1 : 0) | (p1 < 0 ? 2 : 0);
+        const int in = (step * kPdStep) & ((1 << p.c.shift) - 1);  // first row in its page
+        const int in1 = (step * kPdStep + 16) & ((1 << p.c.shift) - 1);
+        const int r0 = p0 < 0 ? max(p1, 0) : p0, r1 = p1 < 0 ? r0 : p1;  // a half in no page reads the other's
+        const WNW_GLOBAL uint8_t* k0 = gptr<uint8_t>(p.c.k) + (int64_t)r0 * p.c.k_stride + (p0 < 0 ? 0 : in) * RB;
+        const WNW_GLOBAL uint8_t* k1 = gptr<uint8_t>(p.c.k) + (int64_t)r1 * p.c.k_stride + (p1 < 0 ? 0 : in1) * RB;
+        const WNW_GLOBAL uint8_t* v0 = gptr<uint8_t>(p.c.v) + (int64_t)r0 * p.c.v_stride + (p0 < 0 ? 0 : in) * RB;
+        const WNW_GLOBAL uint8_t* v1 = gptr<uint8_t>(p.c.v) + (int64_t)r1 * p.c.v_stride + (p1 < 0 ? 0 : in1) * RB;
+        const uint32_t kl = here(klane), vl = here(vlane);
 #pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        kr[0][i] = *gptr<u32x4>(k0 + lc * RB + (lq + 4 * i) * 16);
-        kr[1][i] = *gptr<u32x4>(k1 + lc * RB + (lq + 4 * i) * 16);
-      }
+        for (int i = 0; i < KC; ++i) {
+          kr[0][i] = *(const WNW_GLOBAL u32x4*)(k0 + (kl + 64 * i));
+          kr[1][i] = *(const WNW_GLOBAL u32x4*)(k1 + (kl + 64 * i));
+        }
 #pragma unroll
-      for (int i = 0; i < VI; ++i) vr[i] = *gptr<u32x4>((i < VI / 2 ? v0 : v1) + (i % (VI / 2)) * 1024 + lane * 16);
-    };
-    if (mysteps > 0) {
+        for (int i = 0; i < VI; ++i) vr[i] = *(const WNW_GLOBAL u32x4*)((i < VI / 2 ? v0 : v1) + (vl + (i % (VI / 2)) * 1024));
+      };
       window(0);
       load(0);
-    }
-    for (int k = 0; k < mysteps; ++k) {
-      const int row0 = (a + w + kPdWaves * k) * kPdStep;
-      const bool edge = row0 + kPdStep > all_see || bad;
-      const int bad_now = bad;
-      // scores of the step's rows: lane holds rows 16 t + 4 lq + i of column lc
-      float x[2][4];
+      // q, in the order of K's chunks
       {
-        const float s0 = Q8 ? p.scale_log2 * ks0 : p.scale_log2, s1 = Q8 ? p.scale_log2 * ks1 : p.scale_log2;
+        const T* qp = (const T*)p.q + (int64_t)(first + ti) * p.qt + (int64_t)(h * p.G + g) * p.qh;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < KK; ++i)
+          qs[64 * i] = cols > 0 ? *gptr<u32x4>(qp + (Q8 ? 16 * (lq + 4 * (i >> 1)) + 8 * (i & 1) : 8 * (lq + 4 * i)))
+                                : u32x4{0, 0, 0, 0};
+      }
+      for (int k = 0; k < mysteps; ++k) {
+        const int row0 = (a + nw * k) * kPdStep;
+        const bool edge = row0 + kPdStep > all_see || bad;
+        const int bad_now = bad, from = 2 * (k & 31);
+        // the 8 to 16 addresses made of these are worked out where they are used: held, they would cost registers
+        asm volatile("" : "+v"(vput), "+v"(vget));
+        // scores of the step's rows: lane holds rows 16 t + 4 lq + i of column lc
+        float y[2][4];
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) {
+          f32x4 z = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int i = 0; i < KK; ++i) {
             if constexpr (Q8)
-              y = QO::mma16(e4m3x8<T>(kr[t][i >> 1][2 * (i & 1)], kr[t][i >> 1][2 * (i & 1) + 1]), qf[i], y);
+              z = QO::mma16(e4m3x8<T>(kr[t2][i >> 1][2 * (i & 1)], kr[t2][i >> 1][2 * (i & 1) + 1]), qs[64 * i], z);
             else
-              y = QO::mma16(kr[t][i], qf[i], y);
+              z = QO::mma16(kr[t2][i], qs[64 * i], z);
+          }
+          const float sc = Q8 ? p.scale_log2 * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), from + t2))
+                              : p.scale_log2;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[t2][i] = z[i] * sc;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // V into LDS; rows that are not the segment's become zero
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < VI; ++i) {
+            const int r = (i * 1024 + lane * 16) / RB;
+            if (row0 + r >= n || (bad_now >> (r >> 4) & 1)) vr[i] = u32x4{0, 0, 0, 0};
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[t][i] = y[i] * (t ? s1 : s0);
-        }
-      }
-      // V into LDS; rows that are not the segment's become zero
-      if (edge) {
+          for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
-        for (int i = 0; i < VI; ++i) {
-          const int r = (i * 1024 + lane * 16) / RB;
-          if (row0 + r >= len || (bad_now >> (r >> 4) & 1)) vr[i] = u32x4{0, 0, 0, 0};
+            for (int i = 0; i < 4; ++i) {
+              if (bad_now >> t2 & 1) y[t2][i] = 0.f;
+              if (row0 + 16 * t2 + 4 * lq + i >= limit) y[t2][i] = -INFINITY;
+            }
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int i = 0; i < VI; ++i) *(u32x4*)(stage + ((vput ^ Vl::write_x(i)) + i * 1024)) = vr[i];
+        const float w0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), from));
+        const float w1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), from + 1));
+        if (k + 1 < mysteps) {
+          if (((k + 1) & 31) == 0) window(k + 1);
+          load(k + 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        float mx = m;
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, y[t2][i]);
+        mx = max_x32(max_x16(mx));
+        if (__ballot(mx > m)) {
+          const float r = __builtin_amdgcn_exp2f(m - mx);
+          l *= r;
+#pragma unroll
+          for (int i = 0; i < DT; ++i) acc[i] *= r;
+          m = mx;
+        }
+        u32x4 hi, lo;
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (bad_now >> t & 1) x[t][i] = 0.f;
-            if (row0 + 16 * t + 4 * lq + i >= limit) x[t][i] = -INFINITY;
+            y[t2][i] = __builtin_amdgcn_exp2f(y[t2][i] - m + kBias);
+            l += y[t2][i];
+            if (Q8) y[t2][i] *= t2 ? w1 : w0;
           }
-      }
 #pragma unroll
-      for (int i = 0; i < VI; ++i) {
-        const int at = i * 1024 + lane * 16;
-        *(u32x4*)(stage + v_at<D, Q8>(at / RB, at % RB / 16)) = vr[i];
-      }
-      const float w0 = vs0, w1 = vs1;
-      if (k + 1 < mysteps) {
-        if (((k + 1) & 31) == 0) window(k + 1);
-        load(k + 1);
-      }
-      float mx = m;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, x[t][i]);
-      mx = max_x32(max_x16(mx));
-      if (__ballot(mx > m)) {
-        const float f = __builtin_amdgcn_exp2f(m - mx);
-        l *= f;
-#pragma unroll
-        for (int i = 0; i < DT; ++i) acc[i] *= f;
-        m = mx;
-      }
-      u32x4 hi, lo;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        float y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          y[i] = __builtin_amdgcn_exp2f(x[t][i] - m + kBias);
-          l += y[i];
-          if (Q8) y[i] *= t ? w1 : w0;
+          for (int i = 0; i < 2; ++i) {
+            uint32_t uh, ul;
+            two_parts<VT>(y[t2][2 * i], y[t2][2 * i + 1], &uh, &ul);
+            hi[2 * t2 + i] = uh;
+            lo[2 * t2 + i] = ul;
+          }
         }
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t uh, ul;
-          two_parts<VT>(y[2 * i], y[2 * i + 1], &uh, &ul);
-          hi[2 * t + i] = uh;
-          lo[2 * t + i] = ul;
+        for (int i = 0; i < DT; ++i) {
+          if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+          u32x4 v;
+          if constexpr (Q8) {
+            typedef int i2 __attribute__((ext_vector_type(2)));
+            const i2 z = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                (__attribute__((address_space(3))) i2*)(stage + (vget ^ Vl::read_x(i))));
+            v = e4m3x8<VT>(z[0], z[1]);
+          } else {
+            const uint64_t z0 = VO::read_tr(stage + (vget ^ Vl::read_x(i)));
+            const uint64_t z1 = VO::read_tr(stage + ((vget ^ Vl::read_x(i)) + 16 * RB));
+            v = u32x4{(uint32_t)z0, (uint32_t)(z0 >> 32), (uint32_t)z1, (uint32_t)(z1 >> 32)};
+          }
+          acc[i] = VO::mma16(v, hi, acc[i]);
+          acc[i] = VO::mma16(v, lo, acc[i]);
         }
+        __builtin_amdgcn_wave_barrier();
       }
-      __builtin_amdgcn_wave_barrier();
+      l = sum_x32(sum_x16(l));
+      const int oq = here(lane) >> 4, oc = here(lane) & 15;
+      if (oc < cols) {
+        if (nw > 1) {  // the sums to LDS
+          float* state = (float*)stage + oc * (D + 4) + 4 * oq;
 #pragma unroll
-      for (int i = 0; i < DT; ++i) {
-        u32x4 v;
-        if constexpr (Q8) {
-          typedef int i2 __attribute__((ext_vector_type(2)));
-          const int r = 4 * lq + (lc >> 1 & 3) + (lc >> 3) * 16;
-          const i2 y = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-              (__attribute__((address_space(3))) i2*)(stage + v_at<D, true>(r, i) + (lc & 1) * 8));
-          v = e4m3x8<VT>(y[0], y[1]);
+          for (int i = 0; i < DT; ++i) *(f32x4*)(state + 16 * i) = acc[i];
+          if (oq == 0) {
+            st[w][oc][0] = m;
+            st[w][oc][1] = l;
+          }
+        } else if (!(cut >> j & 1)) {  // the whole segment
+          const int ot = oc / p.G, og = oc - ot * p.G;
+          const bool sees = n - count + ot + 1 > 0;
+          const float inv = sees ? 1.f / l : 0.f;
+          T* op = (T*)p.out + (int64_t)(first + ot) * p.ot + (int64_t)(h * p.G + og) * p.oh;
+#pragma unroll
+          for (int i = 0; i < DT; ++i) {
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = sees ? acc[i][e] * inv : 0.f;
+            store_quad<T>(op, 16 * i + 4 * oq, o);
+          }
         } else {
-          const int r = 4 * lq + (lc >> 2), ch = 2 * i + ((lc & 3) >> 1);
-          const uint64_t y0 = VO::read_tr(stage + v_at<D, false>(r, ch) + (lc & 1) * 8);
-          const uint64_t y1 = VO::read_tr(stage + v_at<D, false>(r + 16, ch) + (lc & 1) * 8);
-          v = u32x4{(uint32_t)y0, (uint32_t)(y0 >> 32), (uint32_t)y1, (uint32_t)(y1 >> 32)};
+          const int64_t slot = (int64_t)(2 * wg + (first_step + a == x0 ? 0 : 1)) * p.cols + oc;
+#pragma unroll
+          for (int i = 0; i < DT; ++i) {
+            float* to = p.part_acc + slot * D + 16 * i + 4 * oq;
+            store_agent(to, acc[i][0], acc[i][1]);
+            store_agent(to + 2, acc[i][2], acc[i][3]);
+          }
+          if (oq == 0) store_agent(p.part_ml + slot * 2, m, l);
         }
-        acc[i] = VO::mma16(v, hi, acc[i]);
-        acc[i] = VO::mma16(v, lo, acc[i]);
       }
       __builtin_amdgcn_wave_barrier();
+      if (beside)
+        beside &= beside - 1;
+      else
+        own = 0;  // a wave has one at most
     }
-    // the waves' sums through LDS
-    l = sum_x32(sum_x16(l));
-    __syncthreads();
-    {
-      float* state = (float*)stage + lc * (D + 4) + 4 * lq;
-      if (lc < cols) {
+
+    // pieces of several waves: their sums added up
+    if (several) {
+      __syncthreads();
+      for (uint64_t todo = several; todo; todo &= todo - 1) {
+        const int j = __builtin_ctzll(todo), seg = win + j;
+        const int f = __builtin_amdgcn_readlane(waves, j) & 255, t = __builtin_amdgcn_readlane(waves, j) >> 8;
+        const bool done = !(cut >> j & 1);
+        int a, b;
+        const int slot = 2 * wg + (piece(j, &a, &b) + a == x0 ? 0 : 1);
+        paged_decode_join<T, D>(p, seg, __builtin_amdgcn_readlane(len, j), tid, NT, done, slot,
+                                [&](int col, float* M) {
+                                  for (int i = f; i < t; ++i) *M = fmaxf(*M, st[i][col][0]);
+                                },
+                                [&](int col, int d, float M, float* L, float* o) {
+                                  for (int i = f; i < t; ++i) {
+                                    const float r = __builtin_amdgcn_exp2f(st[i][col][0] - M);
+                                    const f32x4 z = *(const f32x4*)((const float*)(lds + i * Ge::kPart) + col * (D + 4) + d);
+                                    *L += r * st[i][col][1];
 #pragma unroll
-        for (int i = 0; i < DT; ++i) *(f32x4*)(state + 16 * i) = acc[i];
-        if (lq == 0) {
-          st[w][lc][0] = m;
-          st[w][lc][1] = l;
-        }
+                                    for (int e = 0; e < 4; ++e) o[e] += r * z[e];
+                                  }
+                                });
       }
     }
-    __syncthreads();
-    const bool whole = a == 0 && b == ns;
-    const int slot = 2 * wg + (a > 0 || x == x0 ? 0 : 1);  // the first or the last piece of the workgroup
-    auto finish = [&](int col, int d, float* o, float L) {
-      const int t2 = col / p.G;
-      const bool none = len - count + t2 + 1 <= 0;  // a row that sees no key
-      const float inv = 1.f / L;
-      float y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = none ? 0.f : o[i] * inv;
-      T* op = (T*)p.out + (int64_t)(first + t2) * p.ot + (int64_t)(h * p.G + col - t2 * p.G) * p.oh;
-      store_quad<T>(op, d, y);
-    };
-    for (int e = tid; e < cols * (D / 4); e += 256) {
-      const int col = e / (D / 4), d = 4 * (e % (D / 4));
-      float M = kPgLowest, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < kPdWaves; ++i) M = fmaxf(M, st[i][col][0]);
-#pragma unroll
-      for (int i = 0; i < kPdWaves; ++i) {
-        const float f = __builtin_amdgcn_exp2f(st[i][col][0] - M);
-        const f32x4 y = *(const f32x4*)((const float*)(lds + i * (Ge::kLds / kPdWaves)) + col * (D + 4) + d);
-        L += f * st[i][col][1];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] += f * y[j];
-      }
-      if (whole) {
-        finish(col, d, o, L);
-      } else {
-        float* pa = p.part_acc + ((int64_t)slot * p.cols + col) * D + d;
-        store_agent(pa, o[0], o[1]);
-        store_agent(pa + 2, o[2], o[3]);
-        if (d == 0) store_agent(p.part_ml + ((int64_t)slot * p.cols + col) * 2, M, L);
-      }
-    }
-    if (!whole) {
-      // the last workgroup to arrive at a segment adds up its pieces, in their order
+    // segments cut between workgroups: the last one to arrive adds up the pieces, in their order
+    if (cut) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      const int w0 = owner_of(base), w1 = owner_of(base + ns - 1);
-      if (tid == 0) {
-        const int seen = __hip_atomic_fetch_add(p.counters + seg, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        sh[6] = seen == w1 - w0;
-        if (seen == w1 - w0) __hip_atomic_store(p.counters + seg, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int j0 = __builtin_ctzll(cut), j1 = 63 - __builtin_clzll(cut);  // at most the first and the last piece
+      const int b0 = __builtin_amdgcn_readlane(at, j0), b1 = __builtin_amdgcn_readlane(at, j1);
+      const int others0 = owner_of(b0 + __builtin_amdgcn_readlane(num, j0) - 1) - owner_of(b0);
+      const int others1 = owner_of(b1 + __builtin_amdgcn_readlane(num, j1) - 1) - owner_of(b1);
+      if (tid < 2 && (tid == 0 || j1 != j0)) {
+        const int j = tid ? j1 : j0, others = tid ? others1 : others0;
+        int* counter = p.counters + win + j;
+        const int seen = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (seen == others) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sh[W + 2 + tid] = seen == others;
       }
       __syncthreads();
-      if (sh[6]) {
-        for (int e = tid; e < cols * (D / 4); e += 256) {
-          const int col = e / (D / 4), d = 4 * (e % (D / 4));
-          float M = kPgLowest, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-          for (int i0 = w0; i0 <= w1; i0 += 8) {
-            float pm[8], pl[8], po[8][4];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int from = min(i0 + i, w1);
-              const int64_t sl = (int64_t)(2 * from + (base > start_of(from) ? 1 : 0)) * p.cols + col;
-              load_agent(p.part_ml + sl * 2, &pm[i], &pl[i]);
-              load_agent(p.part_acc + sl * D + d, &po[i][0], &po[i][1]);
-              load_agent(p.part_acc + sl * D + d + 2, &po[i][2], &po[i][3]);
-            }
-            float now = M;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) now = fmaxf(now, pm[i]);
-            const float f0 = __builtin_amdgcn_exp2f(M - now);
-            L *= f0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] *= f0;
-            M = now;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if (i0 + i > w1) continue;
-              const float f = __builtin_amdgcn_exp2f(pm[i] - M);
-              L += f * pl[i];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) o[j] += f * po[i][j];
-            }
-          }
-          finish(col, d, o, L);
-        }
+      for (int i = 0; i < (j1 != j0 ? 2 : 1); ++i) {
+        if (!sh[W + 2 + i]) continue;
+        const int j = i ? j1 : j0, seg = win + j;
+        const int b0 = __builtin_amdgcn_readlane(at, j), b1 = b0 + __builtin_amdgcn_readlane(num, j) - 1;
+        const int w0 = owner_of(b0), w1 = owner_of(b1);
+        const int64_t slot0 = 2 * w0 + (b0 > start_of(w0) ? 1 : 0);
+        paged_decode_gather<T, D, NT>(p, seg, __builtin_amdgcn_readlane(len, j), tid, slot0, w0, w1, (float*)lds);
       }
     }
-    __syncthreads();  // the next piece writes the LDS that this one's sums lie in
-    x += b - a;
-    base += ns;
+    if (N <= 64) break;
+    x = xe;
+    at = __builtin_amdgcn_readlane(at + num, 63);
+    win += 64;
+    __syncthreads();  // the next window's waves write the LDS that this one's sums lie in
   }
   // segments without rows, or that cannot be read: zeros
   for (int s = wg; s < N; s += gridDim.x) {
-    const int len = p.seg_len[s];
+    const int n = p.seg_len[s];
     int first, count;
     const bool told = paged_tokens_of(p.t, s, &first, &count);
-    if (tid == 0 && (!told || len < 0 || len > p.c.capacity)) raise_device_error(p.err, WNW_DEVERR_BOUNDS);
-    if (steps_of(s) > 0) continue;
+    if (tid == 0 && (!told || n < 0 || n > p.c.capacity)) raise_device_error(p.err, WNW_DEVERR_BOUNDS);
+    if (steps_of(n) > 0) continue;
     const int h = s % p.t.hkv, cols = min(count * p.G, p.cols);
     const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int e = tid; e < cols * (D / 4); e += 256) {
+    for (int e = here(tid); e < cols * (D / 4); e += NT) {
       const int col = e / (D / 4), t2 = col / p.G;
       store_quad<T>((T*)p.out + (int64_t)(first + t2) * p.ot + (int64_t)(h * p.G + col - t2 * p.G) * p.oh, 4 * (e % (D / 4)),
                     zero);
@@ -457,12 +624,9 @@ static int64_t counter_bytes(int64_t n_seg) { return (n_seg + 4095) / 4096 * 409
 struct PagedDecodeLayout {
   int64_t ml, acc, total;  // bytes: counters first
 };
-static int decode_grid(int D, bool q8) {
-  const int per = D == 256 ? 2 : q8 || D == 64 ? 4 : 3;
-  return device_cus() * per;
-}
+static int decode_grid(int D, bool q8) { return device_cus() * (D * (q8 ? 1 : 2) >= 256 ? 1 : 2); }
 static PagedDecodeLayout decode_layout(int64_t n_seg, int64_t cols, int64_t D) {
-  const int64_t slots = 2ll * 4 * device_cus();
+  const int64_t slots = 2ll * 2 * device_cus();
   PagedDecodeLayout y;
   y.ml = counter_bytes(n_seg);
   y.acc = y.ml + (slots * cols * 8 + 255) / 256 * 256;
@@ -473,9 +637,9 @@ static PagedDecodeLayout decode_layout(int64_t n_seg, int64_t cols, int64_t D) {
 template <typename T, int D>
 static void launch_decode(const PagedDecodeParams& p, bool q8, int grid, hipStream_t st) {
   if (q8)
-    hipLaunchKernelGGL((paged_decode_kernel<T, D, true>), dim3(grid), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((paged_decode_kernel<T, D, true>), dim3(grid), dim3(64 * PagedDecodeGeom<D, true>::kWaves), 0, st, p);
   else
-    hipLaunchKernelGGL((paged_decode_kernel<T, D, false>), dim3(grid), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((paged_decode_kernel<T, D, false>), dim3(grid), dim3(64 * PagedDecodeGeom<D, false>::kWaves), 0, st, p);
 }
 
 // Shared with the prompt attention's entry point, which hands it the calls of a few tokens.

@@ -295,27 +295,32 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
       fetch(t0 + 1);
       find(t0 + 2);
     }
-    for (int i = t0; i < t1; ++i) {
+    auto turn = [&](int i) {
+      __syncthreads();  // everyone is done with tile i - 1; with two buffers tile i is in LDS
       if constexpr (NB == 2) {
-        __syncthreads();  // tile i is in LDS; everyone is done with tile i - 1
         if (i + 1 < t1) {
           put((i + 1) & 1);
           fetch(i + 2);
           find(i + 3);
         }
       } else {
-        __syncthreads();  // everyone is done with tile i - 1
         put(i & 1);
         fetch(i + 1);
         find(i + 2);
         __syncthreads();
       }
-      if (i >= mine) continue;
-      if ((i + 1) * kPpKeys > wfirst)
-        tile(i, std::true_type());
-      else
-        tile(i, std::false_type());
+    };
+    // the tiles that every row of the wave sees whole, the others, the turns of the workgroup's later waves
+    int i = t0;
+    for (const int full = min(wfirst / kPpKeys, mine); i < full; ++i) {
+      turn(i);
+      tile(i, std::false_type());
     }
+    for (; i < mine; ++i) {
+      turn(i);
+      tile(i, std::true_type());
+    }
+    for (; i < t1; ++i) turn(i);
   }
   l = sum_x32(l);
   if (p.splits == 1) {
