@@ -47,7 +47,8 @@ struct PagedDecodeParams {
 };
 
 static constexpr int kPdStep = 32;  // rows of a step
-static constexpr int kPdMin = 8;    // steps of a workgroup at least
+static constexpr int kPdMin = 8;     // steps of a workgroup at least
+static constexpr int kPdWhole = 40;  // steps of a segment that is not cut
 
 template <int D, bool Q8>
 struct PagedDecodeGeom {
@@ -123,93 +124,97 @@ __device__ __forceinline__ int here(int x) {
   return x;
 }
 
-// A segment's result from its sums: element d .. d + 3 of query row col
-template <typename T, int D>
-__device__ __forceinline__ void paged_decode_out(const PagedDecodeParams& p, int seg, int n, int col, int d, const float* o,
+// What a segment's query rows are.  The divisions are branched around where
+// they are by one: code that a launch meets for the first time costs more
+// than its instructions (a cold line of the instruction cache is a memory round
+// trip), which is why what follows a piece is kept short and rolled.
+struct DecodeRows {
+  int first, count, h, n, cols;  // tokens, KV head, rows of the segment, query rows
+};
+__device__ __forceinline__ DecodeRows decode_rows(const PagedDecodeParams& p, int seg, int n) {
+  DecodeRows r;
+  if (p.t.hkv == 1 && !p.t.cu) {
+    r.first = seg;
+    r.count = 1;
+    r.h = 0;
+  } else {
+    paged_tokens_of(p.t, seg, &r.first, &r.count);
+    r.h = seg % p.t.hkv;
+  }
+  r.n = n;
+  r.cols = min(r.count * p.G, p.cols);
+  return r;
+}
+__device__ __forceinline__ int token_of(const PagedDecodeParams& p, const DecodeRows& r, int col) {
+  return r.count > 1 ? col / p.G : 0;
+}
+// Where query row col's result goes
+template <typename T>
+__device__ __forceinline__ T* out_row(const PagedDecodeParams& p, const DecodeRows& r, int col, int ti) {
+  return (T*)p.out + (int64_t)(r.first + ti) * p.ot + (int64_t)(r.h * p.G + col - ti * p.G) * p.oh;
+}
+// Elements d .. d + 3 of a result, from its sums
+template <typename T>
+__device__ __forceinline__ void paged_decode_out(const PagedDecodeParams& p, const DecodeRows& r, int col, int d, const f32x4& o,
                                                  float L) {
-  int first, count;
-  paged_tokens_of(p.t, seg, &first, &count);
-  const int ti = col / p.G, h = seg % p.t.hkv;
-  const bool sees = n - count + ti + 1 > 0;  // else a row without keys
-  const float inv = 1.f / L;
+  const int ti = token_of(p, r, col);
+  const bool sees = r.n - r.count + ti + 1 > 0;  // else a row without keys
+  const float inv = __builtin_amdgcn_rcpf(L);
   float y[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) y[i] = sees ? o[i] * inv : 0.f;
-  store_quad<T>((T*)p.out + (int64_t)(first + ti) * p.ot + (int64_t)(h * p.G + col - ti * p.G) * p.oh, d, y);
-}
-__device__ __forceinline__ int paged_decode_cols(const PagedDecodeParams& p, int seg) {
-  int first, count;
-  paged_tokens_of(p.t, seg, &first, &count);
-  return min(count * p.G, p.cols);
+  store_quad<T>(out_row<T>(p, r, col, ti), d, y);
 }
 
-// The sums of a piece's waves: the segment's result (done), or its partial in a slot
-template <typename T, int D, typename FM, typename FS>
-__device__ __forceinline__ void paged_decode_join(const PagedDecodeParams& p, int seg, int n, int tid, int threads, bool done,
-                                                  int slot, FM most, FS sums) {
-  tid = here(tid);
-  const int cols = paged_decode_cols(p, seg);
-  for (int e = tid; e < cols * (D / 4); e += threads) {
-    const int col = e / (D / 4), d = 4 * (e % (D / 4));
-    float M = kPgLowest, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    most(col, &M);
-    sums(col, d, M, &L, o);
-    if (done) {
-      paged_decode_out<T, D>(p, seg, n, col, d, o, L);
-    } else {
-      const int64_t to = (int64_t)slot * p.cols + col;
-      store_agent(p.part_acc + to * D + d, o[0], o[1]);
-      store_agent(p.part_acc + to * D + d + 2, o[2], o[3]);
-      if (d == 0) store_agent(p.part_ml + to * 2, M, L);
-    }
-  }
-}
-
-// The partials of workgroups [w0, w1] (the first in slot0, the others each in
-// its first slot) added up: in as many runs as there are threads for, then the
-// runs, by way of lds.
+// The partials of workgroups [w0, w1] (the first in slot 2 w0 + late, the
+// others each in its first slot) added up, in as many runs as there are threads
+// for, 8 at a time; the runs by way of lds.
 template <typename T, int D, int NT>
-__device__ __forceinline__ void paged_decode_gather(const PagedDecodeParams& p, int seg, int n, int tid, int64_t slot0, int w0,
+__device__ __forceinline__ void paged_decode_gather(const PagedDecodeParams& p, const DecodeRows& r, int tid, int late, int w0,
                                                     int w1, float* lds) {
+  constexpr int kSc1 = 16;  // buffer cache policy: coherent over the device
   tid = here(tid);
-  const int items = paged_decode_cols(p, seg) * (D / 4), runs = max(1, min(NT / max(items, 1), 8));
-  const int each = (w1 - w0 + runs) / runs, run = runs > 1 ? tid / max(items, 1) : 0;
+  const int items = r.cols * (D / 4), np = w1 - w0 + 1;
+  int runs = 1;
+  while (runs < 8 && 2 * runs * items <= NT && 2 * runs < np) runs *= 2;
+  const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(p.part_acc, 0, 0x7fffffff, 0x00027000);
+  const __amdgpu_buffer_rsrc_t rm = __builtin_amdgcn_make_buffer_rsrc(p.part_ml, 0, 0x7fffffff, 0x00027000);
   __syncthreads();
-  for (int e = tid - run * items; e < items && run < runs; e += runs > 1 ? items : NT) {
-    const int col = e / (D / 4), d = 4 * (e % (D / 4));
-    const int a0 = w0 + run * each, a1 = min(a0 + each - 1, w1);
-    float M = kPgLowest, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int i0 = a0; i0 <= a1; i0 += 4) {
-      float pm[4], pl[4], po[4][4];
+  for (int e = tid; e < items * runs; e += NT) {
+    const int run = runs > 1 ? e / items : 0, item = e - run * items, col = item / (D / 4);
+    float M = kPgLowest, L = 0.f;
+    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = run; k0 < np; k0 += 8 * runs) {
+      f32x4 po[8];
+      float pm[8], pl[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int from = min(i0 + i, a1);
-        const int64_t at = (from == w0 ? slot0 : 2 * (int64_t)from) * p.cols + col;
-        load_agent(p.part_ml + at * 2, &pm[i], &pl[i]);
-        load_agent(p.part_acc + at * D + d, &po[i][0], &po[i][1]);
-        load_agent(p.part_acc + at * D + d + 2, &po[i][2], &po[i][3]);
+      for (int i = 0; i < 8; ++i) {
+        const int k = min(k0 + i * runs, np - 1);  // past the last: the last again, without weight
+        const int slot = (2 * (w0 + k) + (k == 0 ? late : 0)) * p.cols;
+        po[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(ra, slot * (D * 4) + item * 16, 0, kSc1));
+        const auto ml = __builtin_amdgcn_raw_buffer_load_b64(rm, (slot + col) * 8, 0, kSc1);
+        pm[i] = __uint_as_float(ml[0]);
+        pl[i] = __uint_as_float(ml[1]);
       }
       float now = M;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) now = fmaxf(now, pm[i]);
+      for (int i = 0; i < 8; ++i) now = fmaxf(now, pm[i]);
       const float f0 = __builtin_amdgcn_exp2f(M - now);
       L *= f0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] *= f0;
+      o *= f0;
       M = now;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float f = i0 + i <= a1 ? __builtin_amdgcn_exp2f(pm[i] - M) : 0.f;
+      for (int i = 0; i < 8; ++i) {
+        const float f = k0 + i * runs < np ? __builtin_amdgcn_exp2f(pm[i] - M) : 0.f;
         L += f * pl[i];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] += f * po[i][j];
+        o += f * po[i];
       }
     }
     if (runs == 1) {
-      paged_decode_out<T, D>(p, seg, n, col, d, o, L);
+      paged_decode_out<T>(p, r, col, 4 * (item % (D / 4)), o, L);
     } else {
-      float* to = lds + (run * items + e) * 8;
-      *(f32x4*)to = f32x4{o[0], o[1], o[2], o[3]};
+      float* to = lds + e * 8;
+      *(f32x4*)to = o;
       to[4] = M;
       to[5] = L;
     }
@@ -217,16 +222,17 @@ __device__ __forceinline__ void paged_decode_gather(const PagedDecodeParams& p, 
   if (runs == 1) return;
   __syncthreads();
   if (tid < items) {
-    float M = kPgLowest, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < runs; ++i) M = fmaxf(M, lds[(i * items + tid) * 8 + 4]);
+    float M = kPgLowest, L = 0.f;
+    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
     for (int i = 0; i < runs; ++i) {
       const float* at = lds + (i * items + tid) * 8;
-      const float f = __builtin_amdgcn_exp2f(at[4] - M);
-      L += f * at[5];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] += f * at[j];
+      const float now = fmaxf(M, at[4]), f = __builtin_amdgcn_exp2f(M - now), g = __builtin_amdgcn_exp2f(at[4] - now);
+      L = L * f + g * at[5];
+      o = o * f + g * *(const f32x4*)at;
+      M = now;
     }
-    paged_decode_out<T, D>(p, seg, n, tid / (D / 4), 4 * (tid % (D / 4)), o, L);
+    paged_decode_out<T>(p, r, tid / (D / 4), 4 * (tid % (D / 4)), o, L);
   }
 }
 
@@ -245,7 +251,7 @@ paged_decode_kernel(PagedDecodeParams p) {
   constexpr float kBias = std::is_same<VT, f16_t>::value ? 12.f : 0.f;
   __shared__ __attribute__((aligned(16))) uint8_t lds[W * Ge::kPart];
   __shared__ float st[W][16][2];
-  __shared__ int32_t sh[W + 4];
+  __shared__ int32_t sh[2 * W];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int N = p.c.n_seg, wg = blockIdx.x;
 
@@ -258,51 +264,81 @@ paged_decode_kernel(PagedDecodeParams p) {
     }
     return x;
   };
-  // All steps, this workgroup's [x0, x1), and the window of 64 segments from
-  // its first one on: lane j has segment win + j, of `len` rows, whose `num`
-  // steps come after `at` others.
-  int win = 0, len = 0, num = 0, at = 0, S;
+  // All steps and the most of a segment, this workgroup's [x0, x1), and the
+  // window of 64 segments from its first one on: lane j has segment win + j, of
+  // `len` rows, whose `num` steps come after `at` others.
+  int win = 0, len = 0, num = 0, at = 0, S, longest;
+  int mine = 0, incl = 0, before = 0;
+  const int per = (N + NT - 1) / NT, sa = min(tid * per, N), sb = min(sa + per, N);
   if (N <= 64) {
     len = lane < N ? p.seg_len[lane] : 0;
     num = steps_of(len);
     at = scan(num);
     S = __builtin_amdgcn_readlane(at, 63);
     at -= num;
-  }
-  int mine = 0, incl = 0, before = 0;
-  const int per = (N + NT - 1) / NT, sa = min(tid * per, N), sb = min(sa + per, N);
-  if (N > 64) {
-    for (int s = sa; s < sb; ++s) mine += steps_of(p.seg_len[s]);
+    longest = (int)wave_max((float)num);  // steps are below 2^25: exact
+  } else {
+    int most = 0;
+    for (int s = sa; s < sb; ++s) {
+      const int n = steps_of(p.seg_len[s]);
+      mine += n;
+      most = max(most, n);
+    }
     incl = scan(mine);
-    if (lane == 63) sh[w] = incl;
+    most = (int)wave_max((float)most);
+    if (lane == 63) {
+      sh[w] = incl;
+      sh[W + w] = most;
+    }
     __syncthreads();
-    S = 0;
+    S = longest = 0;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       if (i < w) before += sh[i];
       S += sh[i];
+      longest = max(longest, sh[W + i]);
     }
     S = __builtin_amdgcn_readfirstlane(S);
+    __syncthreads();
   }
-  const int P = min((int)gridDim.x, max(S / kPdMin, 1));
-  const int share = S / P, more = S - share * P;  // the first `more` workgroups take one step more
+  longest = __builtin_amdgcn_readfirstlane(longest);
+  // Short segments are not cut (a workgroup takes whole ones): what adds up the
+  // pieces of a cut one costs as much as the steps of kPdWhole.
+  const bool uncut = longest <= kPdWhole;
+  const int total = uncut ? N : S, P = min((int)gridDim.x, uncut ? N : max(S / kPdMin, 1));
+  const int share = total / P, more = total - share * P;  // the first `more` workgroups take one more
   auto start_of = [&](int i) { return i * share + min(i, more); };
   auto owner_of = [&](int x) {  // the workgroup that has step x
     const int big = more * (share + 1);
     return x < big ? x / (share + 1) : more + (x - big) / max(share, 1);
   };
-  const int x0 = wg < P ? start_of(wg) : 0, x1 = wg < P ? start_of(wg + 1) : 0;
-  if (N > 64 && x0 < x1) {
-    const int e0 = before + incl - mine;  // steps before the thread's segments
-    if (e0 <= x0 && x0 < e0 + mine) {
-      int s = sa, e = e0;
-      for (int n; e + (n = steps_of(p.seg_len[s])) <= x0; ++s) e += n;
-      sh[W] = s;
-      sh[W + 1] = e;
+  int x0 = wg < P ? start_of(wg) : 0, x1 = wg < P ? start_of(wg + 1) : 0;
+  if (x0 < x1) {
+    const int s0 = x0, s1 = x1;  // segments, if uncut
+    if (N <= 64) {
+      if (uncut) {
+        x0 = __builtin_amdgcn_readlane(at, s0);
+        x1 = s1 < N ? __builtin_amdgcn_readlane(at, s1) : S;
+      }
+    } else {
+      int e = before + incl - mine;  // steps before the thread's segments
+      for (int s = sa; s < sb; ++s) {
+        const int n = steps_of(p.seg_len[s]);
+        if (uncut ? s == s0 : e <= x0 && x0 < e + n) {
+          sh[0] = s;
+          sh[1] = e;
+        }
+        if (uncut && s == s1) sh[2] = e;
+        e += n;
+      }
+      __syncthreads();
+      win = __builtin_amdgcn_readfirstlane(sh[0]);
+      at = __builtin_amdgcn_readfirstlane(sh[1]);
+      if (uncut) {
+        x0 = at;
+        x1 = s1 < N ? __builtin_amdgcn_readfirstlane(sh[2]) : S;
+      }
     }
-    __syncthreads();
-    win = __builtin_amdgcn_readfirstlane(sh[W]);
-    at = __builtin_amdgcn_readfirstlane(sh[W + 1]);
   }
 
   for (int x = x0; x < x1 && win < N;) {
@@ -337,13 +373,11 @@ paged_decode_kernel(PagedDecodeParams p) {
       const int first_step = piece(j, &a, &b);
       a += iw;
       const int mysteps = (b - a + nw - 1) / nw;
-      int first, count;
-      paged_tokens_of(p.t, seg, &first, &count);
-      const int h = seg % p.t.hkv;
-      const int cols = min(count * p.G, p.cols);
-      const int c = min(lc, max(cols - 1, 0)), ti = c / p.G, g = c - ti * p.G;
-      const int limit = n - count + ti + 1;  // rows that the lane's column sees
-      const int all_see = n - count + 1;     // rows that every column sees
+      const DecodeRows r = decode_rows(p, seg, n);
+      const int cols = r.cols;
+      const int c = min(lc, max(cols - 1, 0)), ti = token_of(p, r, c);
+      const int limit = n - r.count + ti + 1;  // rows that the lane's column sees
+      const int all_see = n - r.count + 1;     // rows that every column sees
       f32x4 acc[DT];
 #pragma unroll
       for (int i = 0; i < DT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -389,22 +423,25 @@ paged_decode_kernel(PagedDecodeParams p) {
         const uint32_t kl = here(klane), vl = here(vlane);
 #pragma unroll
         for (int i = 0; i < KC; ++i) {
-          kr[0][i] = *(const WNW_GLOBAL u32x4*)(k0 + (kl + 64 * i));
-          kr[1][i] = *(const WNW_GLOBAL u32x4*)(k1 + (kl + 64 * i));
+          kr[0][i] = __builtin_nontemporal_load((const WNW_GLOBAL u32x4*)(k0 + (kl + 64 * i)));
+          kr[1][i] = __builtin_nontemporal_load((const WNW_GLOBAL u32x4*)(k1 + (kl + 64 * i)));
         }
 #pragma unroll
-        for (int i = 0; i < VI; ++i) vr[i] = *(const WNW_GLOBAL u32x4*)((i < VI / 2 ? v0 : v1) + (vl + (i % (VI / 2)) * 1024));
+        for (int i = 0; i < VI; ++i) vr[i] = __builtin_nontemporal_load((const WNW_GLOBAL u32x4*)((i < VI / 2 ? v0 : v1) + (vl + (i % (VI / 2)) * 1024)));
       };
-      window(0);
-      load(0);
       // q, in the order of K's chunks
+      u32x4 qf[KK];
       {
-        const T* qp = (const T*)p.q + (int64_t)(first + ti) * p.qt + (int64_t)(h * p.G + g) * p.qh;
+        const T* qp = (const T*)p.q + (int64_t)(r.first + ti) * p.qt + (int64_t)(r.h * p.G + c - ti * p.G) * p.qh;
 #pragma unroll
         for (int i = 0; i < KK; ++i)
-          qs[64 * i] = cols > 0 ? *gptr<u32x4>(qp + (Q8 ? 16 * (lq + 4 * (i >> 1)) + 8 * (i & 1) : 8 * (lq + 4 * i)))
+          qf[i] = cols > 0 ? *gptr<u32x4>(qp + (Q8 ? 16 * (lq + 4 * (i >> 1)) + 8 * (i & 1) : 8 * (lq + 4 * i)))
                                 : u32x4{0, 0, 0, 0};
       }
+      window(0);
+      load(0);
+#pragma unroll
+      for (int i = 0; i < KK; ++i) qs[64 * i] = qf[i];
       for (int k = 0; k < mysteps; ++k) {
         const int row0 = (a + nw * k) * kPdStep;
         const bool edge = row0 + kPdStep > all_see || bad;
@@ -433,8 +470,8 @@ paged_decode_kernel(PagedDecodeParams p) {
         if (edge) {
 #pragma unroll
           for (int i = 0; i < VI; ++i) {
-            const int r = (i * 1024 + lane * 16) / RB;
-            if (row0 + r >= n || (bad_now >> (r >> 4) & 1)) vr[i] = u32x4{0, 0, 0, 0};
+            const int rr = (i * 1024 + lane * 16) / RB;
+            if (row0 + rr >= n || (bad_now >> (rr >> 4) & 1)) vr[i] = u32x4{0, 0, 0, 0};
           }
 #pragma unroll
           for (int t2 = 0; t2 < 2; ++t2)
@@ -460,10 +497,10 @@ paged_decode_kernel(PagedDecodeParams p) {
           for (int i = 0; i < 4; ++i) mx = fmaxf(mx, y[t2][i]);
         mx = max_x32(max_x16(mx));
         if (__ballot(mx > m)) {
-          const float r = __builtin_amdgcn_exp2f(m - mx);
-          l *= r;
+          const float fall = __builtin_amdgcn_exp2f(m - mx);
+          l *= fall;
 #pragma unroll
-          for (int i = 0; i < DT; ++i) acc[i] *= r;
+          for (int i = 0; i < DT; ++i) acc[i] *= fall;
           m = mx;
         }
         u32x4 hi, lo;
@@ -516,17 +553,8 @@ paged_decode_kernel(PagedDecodeParams p) {
             st[w][oc][1] = l;
           }
         } else if (!(cut >> j & 1)) {  // the whole segment
-          const int ot = oc / p.G, og = oc - ot * p.G;
-          const bool sees = n - count + ot + 1 > 0;
-          const float inv = sees ? 1.f / l : 0.f;
-          T* op = (T*)p.out + (int64_t)(first + ot) * p.ot + (int64_t)(h * p.G + og) * p.oh;
 #pragma unroll
-          for (int i = 0; i < DT; ++i) {
-            float o[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = sees ? acc[i][e] * inv : 0.f;
-            store_quad<T>(op, 16 * i + 4 * oq, o);
-          }
+          for (int i = 0; i < DT; ++i) paged_decode_out<T>(p, r, oc, 16 * i + 4 * oq, acc[i], l);
         } else {
           const int64_t slot = (int64_t)(2 * wg + (first_step + a == x0 ? 0 : 1)) * p.cols + oc;
 #pragma unroll
@@ -549,24 +577,32 @@ paged_decode_kernel(PagedDecodeParams p) {
     if (several) {
       __syncthreads();
       for (uint64_t todo = several; todo; todo &= todo - 1) {
-        const int j = __builtin_ctzll(todo), seg = win + j;
+        const int j = __builtin_ctzll(todo);
         const int f = __builtin_amdgcn_readlane(waves, j) & 255, t = __builtin_amdgcn_readlane(waves, j) >> 8;
-        const bool done = !(cut >> j & 1);
+        const DecodeRows r = decode_rows(p, win + j, __builtin_amdgcn_readlane(len, j));
         int a, b;
-        const int slot = 2 * wg + (piece(j, &a, &b) + a == x0 ? 0 : 1);
-        paged_decode_join<T, D>(p, seg, __builtin_amdgcn_readlane(len, j), tid, NT, done, slot,
-                                [&](int col, float* M) {
-                                  for (int i = f; i < t; ++i) *M = fmaxf(*M, st[i][col][0]);
-                                },
-                                [&](int col, int d, float M, float* L, float* o) {
-                                  for (int i = f; i < t; ++i) {
-                                    const float r = __builtin_amdgcn_exp2f(st[i][col][0] - M);
-                                    const f32x4 z = *(const f32x4*)((const float*)(lds + i * Ge::kPart) + col * (D + 4) + d);
-                                    *L += r * st[i][col][1];
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) o[e] += r * z[e];
-                                  }
-                                });
+        const int slot = (2 * wg + (piece(j, &a, &b) + a == x0 ? 0 : 1)) * p.cols;
+        for (int e = here(tid); e < r.cols * (D / 4); e += NT) {
+          const int col = e / (D / 4), d = 4 * (e % (D / 4));
+          float M = kPgLowest, L = 0.f;
+          f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+          for (int i = f; i < t; ++i) {
+            const float mi = st[i][col][0], now = fmaxf(M, mi);
+            const float u = __builtin_amdgcn_exp2f(M - now), v = __builtin_amdgcn_exp2f(mi - now);
+            L = L * u + v * st[i][col][1];
+            o = o * u + v * *(const f32x4*)((const float*)(lds + i * Ge::kPart) + col * (D + 4) + d);
+            M = now;
+          }
+          if (!(cut >> j & 1)) {
+            paged_decode_out<T>(p, r, col, d, o, L);
+          } else {
+            float* to = p.part_acc + (slot + col) * D + d;
+            store_agent(to, o[0], o[1]);
+            store_agent(to + 2, o[2], o[3]);
+            if (d == 0) store_agent(p.part_ml + (slot + col) * 2, M, L);
+          }
+        }
       }
     }
     // segments cut between workgroups: the last one to arrive adds up the pieces, in their order
@@ -574,24 +610,27 @@ paged_decode_kernel(PagedDecodeParams p) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       const int j0 = __builtin_ctzll(cut), j1 = 63 - __builtin_clzll(cut);  // at most the first and the last piece
-      const int b0 = __builtin_amdgcn_readlane(at, j0), b1 = __builtin_amdgcn_readlane(at, j1);
-      const int others0 = owner_of(b0 + __builtin_amdgcn_readlane(num, j0) - 1) - owner_of(b0);
-      const int others1 = owner_of(b1 + __builtin_amdgcn_readlane(num, j1) - 1) - owner_of(b1);
+      int a, b;
+      piece(j0, &a, &b);
+      const int mine0 = b - a, all0 = __builtin_amdgcn_readlane(num, j0);
+      piece(j1, &a, &b);
+      const int mine1 = b - a, all1 = __builtin_amdgcn_readlane(num, j1);
       if (tid < 2 && (tid == 0 || j1 != j0)) {
-        const int j = tid ? j1 : j0, others = tid ? others1 : others0;
-        int* counter = p.counters + win + j;
-        const int seen = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (seen == others) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        sh[W + 2 + tid] = seen == others;
+        // the counter has the steps that are done
+        int* counter = p.counters + win + (tid ? j1 : j0);
+        const int add = tid ? mine1 : mine0;
+        const int seen = __hip_atomic_fetch_add(counter, add, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool last = seen + add == (tid ? all1 : all0);
+        if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sh[tid] = last;
       }
       __syncthreads();
+#pragma unroll 1
       for (int i = 0; i < (j1 != j0 ? 2 : 1); ++i) {
-        if (!sh[W + 2 + i]) continue;
-        const int j = i ? j1 : j0, seg = win + j;
-        const int b0 = __builtin_amdgcn_readlane(at, j), b1 = b0 + __builtin_amdgcn_readlane(num, j) - 1;
-        const int w0 = owner_of(b0), w1 = owner_of(b1);
-        const int64_t slot0 = 2 * w0 + (b0 > start_of(w0) ? 1 : 0);
-        paged_decode_gather<T, D, NT>(p, seg, __builtin_amdgcn_readlane(len, j), tid, slot0, w0, w1, (float*)lds);
+        if (!sh[i]) continue;
+        const int j = i ? j1 : j0, b0 = __builtin_amdgcn_readlane(at, j), w0 = owner_of(b0);
+        paged_decode_gather<T, D, NT>(p, decode_rows(p, win + j, __builtin_amdgcn_readlane(len, j)), tid, b0 > start_of(w0), w0,
+                                      owner_of(b0 + __builtin_amdgcn_readlane(num, j) - 1), (float*)lds);
       }
     }
     if (N <= 64) break;
@@ -603,16 +642,16 @@ paged_decode_kernel(PagedDecodeParams p) {
   // segments without rows, or that cannot be read: zeros
   for (int s = wg; s < N; s += gridDim.x) {
     const int n = p.seg_len[s];
-    int first, count;
-    const bool told = paged_tokens_of(p.t, s, &first, &count);
-    if (tid == 0 && (!told || n < 0 || n > p.c.capacity)) raise_device_error(p.err, WNW_DEVERR_BOUNDS);
+    if (tid == 0) {
+      int first, count;
+      if (!paged_tokens_of(p.t, s, &first, &count) || n < 0 || n > p.c.capacity) raise_device_error(p.err, WNW_DEVERR_BOUNDS);
+    }
     if (steps_of(n) > 0) continue;
-    const int h = s % p.t.hkv, cols = min(count * p.G, p.cols);
+    const DecodeRows r = decode_rows(p, s, 0);
     const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int e = here(tid); e < cols * (D / 4); e += NT) {
-      const int col = e / (D / 4), t2 = col / p.G;
-      store_quad<T>((T*)p.out + (int64_t)(first + t2) * p.ot + (int64_t)(h * p.G + col - t2 * p.G) * p.oh, 4 * (e % (D / 4)),
-                    zero);
+    for (int e = here(tid); e < r.cols * (D / 4); e += NT) {
+      const int col = e / (D / 4);
+      store_quad<T>(out_row<T>(p, r, col, token_of(p, r, col)), 4 * (e % (D / 4)), zero);
     }
   }
 }
