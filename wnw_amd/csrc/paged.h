@@ -50,6 +50,14 @@ __device__ __forceinline__ bool paged_tokens_of(const PagedTokens& t, int s, int
   return true;
 }
 
+// x, as a value that the compiler does not know: what follows from it is worked
+// out here and not, ahead of the loops around, held in registers all along
+template <typename I>
+__device__ __forceinline__ I here(I x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 template <typename T>
 struct HalfOps;
 template <>

@@ -117,13 +117,6 @@ __device__ __forceinline__ void load_agent(const float* p, float* a, float* b) {
   *b = __uint_as_float((uint32_t)(x >> 32));
 }
 
-// x, as a value that the compiler does not know: what follows from it is worked
-// out here and not, ahead of the loops around, held in registers all along
-__device__ __forceinline__ int here(int x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
-
 // What a segment's query rows are.  The divisions are branched around where
 // they are by one: code that a launch meets for the first time costs more
 // than its instructions (a cold line of the instruction cache is a memory round

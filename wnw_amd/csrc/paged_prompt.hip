@@ -46,8 +46,13 @@ struct PagedPromptParams {
   int32_t* err;
 };
 
-static constexpr int kPpQ = 128;    // query rows of a workgroup
+// waves of a workgroup, each with 32 query rows
+__host__ __device__ constexpr int prompt_waves(int D) { return D == 128 ? 8 : 4; }
 static constexpr int kPpKeys = 64;  // keys of a tile
+// log2 of how far the maximum that the weights are taken against may trail the
+// running one: weights up to 2^6 round like weights up to 1, and most tiles
+// then leave the sums as they are.
+static constexpr float kPpTrail = 6.f;
 
 template <typename T>
 __device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f32x16& c) {
@@ -93,13 +98,16 @@ __device__ __forceinline__ void prompt_store(const PagedPromptParams& p, const P
 }
 
 template <typename T, int D, bool Q8>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(PagedPromptParams p) {
+__global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void paged_prompt_kernel(PagedPromptParams p) {
   using Ops = HalfOps<T>;
+  constexpr int W = prompt_waves(D), kPpQ = 32 * W;
   constexpr int RB = D * 2, CH = RB / 16, TB = kPpKeys * RB;  // a tile in LDS: 16-bit elements
   constexpr int GB = D * (Q8 ? 1 : 2);                        // bytes of a row in its page
-  constexpr int NI = kPpKeys * GB / 4096;                     // 16-byte loads per thread and tensor
+  constexpr int NI = kPpKeys * GB / (1024 * W);                     // 16-byte loads per thread and tensor
   constexpr int KK = D / 16, DT = D / 32;
   constexpr int NB = D == 256 ? 1 : 2;  // tiles in LDS
+  // f16 weights are held times 2^8 (2^14 at most): normal numbers down to 2^-22 of the largest
+  constexpr float kBias = std::is_same<T, f16_t>::value ? 8.f : 0.f;
   __shared__ __attribute__((aligned(16))) uint8_t lds[NB * 2 * TB];  // [NB][K, V]
   __shared__ float scales[2][kPpKeys / 16][2];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -126,68 +134,109 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) qr[kk] = *gptr<u32x4>(qp + 16 * kk);
   }
-  // staging: the thread's rows of a tile and its 16 bytes of each
-  const int32_t* table = p.c.table + seg * p.c.table_stride;
-  auto page_of = [&](int at) {  // the page of row `at` of the segment, -1: none
-    int id = -1;
-    if (at < r.len) {
-      id = table[at >> p.c.shift];
-      if (id < 0 || id >= p.c.n_pages) {
-        raise_device_error(p.err, WNW_DEVERR_BOUNDS);
-        id = -1;
-      }
-    }
-    return id;
-  };
-  constexpr int CG = GB / 16;      // 16-byte chunks of a row in its page
-  constexpr int RPL = 256 / CG;    // rows per load of the workgroup
+  // Staging: a wave's load is 16 bytes of each of 64 / CG (2 to 16) rows that
+  // lie in one page, so a load's page and its address are scalars.  They come
+  // from a window of 64 x 16 keys (16 tiles) that a wave keeps in registers: lane j
+  // has the page, and K's and V's scale, of keys 16 j ...  The next window's
+  // pages are loaded when a window is entered, its scales half way through.
+  constexpr int CG = GB / 16;     // 16-byte chunks of a row in its page
+  constexpr int RPL = 64 * W / CG;   // rows per load of the workgroup
+  constexpr int kWin = 16;        // tiles of a window
   const int srow = tid / CG, sch = tid % CG;
-  int pid[NI], spid = -1;
+  // 8 bits: a lane has 8 codes of either half of a row, so that what it writes,
+  // a 16-byte chunk of 16-bit elements each, meets every LDS bank once per row
+  uint32_t soff = (uint32_t)((lane / CG) * GB + sch * (Q8 ? 8 : 16));
+  // the lane's place in a tile's K and V in LDS (load u: u * RPL rows on); K's
+  // second half has the chunk's top bit turned, V's lies half a row on
+  constexpr uint32_t kHalf = RB / 2;
+  static_assert(RPL % 4 == 0 && (RPL % CH == 0 || CH % RPL == 0), "rows of a load: whole turns of the swizzle, or a part of one");
+  uint32_t kput = srow * RB + ((sch ^ (srow % CH)) * 16), vput = srow * RB + ((sch ^ (2 * (srow & 3))) * 16);
+  const int32_t* table = p.c.table + seg * p.c.table_stride;
+  int pid = 0, pid_next = 0;  // of the window that fetch() is in, and of the next
+  float ks = 1.f, vs = 1.f, ks_next = 1.f, vs_next = 1.f;
+  bool wrong = false;
+  // Rows past the segment's take its last page; an entry that is no page page
+  // 0, with its sign bit set.
+  auto find = [&](int window) {
+    const int id = table[min((window * 64 + lane) * 16, r.len - 1) >> p.c.shift];
+    const bool is = (uint32_t)id < (uint32_t)p.c.n_pages;
+    wrong |= !is;
+    pid_next = is ? id : (int)0x80000000;
+  };
+  auto find_scales = [&]() {
+    if constexpr (Q8) {
+      const int id = pid_next & 0x7fffffff;
+      ks_next = pid_next < 0 ? 1.f : p.c.k_scale[id];
+      vs_next = pid_next < 0 ? 1.f : p.c.v_scale[id];
+    }
+  };
+  auto enter = [&](int window) {
+    pid = pid_next;
+    ks = ks_next;
+    vs = vs_next;
+    find(window + 1);
+  };
   u32x4 kr[NI], vr[NI];
-  float sk = 1.f, sv = 1.f;
-  auto find = [&](int tile) {  // the pages of the thread's rows
-#pragma unroll
-    for (int u = 0; u < NI; ++u) pid[u] = tile < t1 ? page_of(tile * kPpKeys + u * RPL + srow) : -1;
-    if (Q8 && tid < kPpKeys / 16) spid = tile < t1 ? page_of(tile * kPpKeys + 16 * tid) : -1;
-  };
+  int gone[NI];  // rows of kr and vr in no page: negative
   auto fetch = [&](int tile) {
+    if (tile % kWin == 0)
+      enter(tile / kWin);
+    else if (tile % kWin == kWin / 2)
+      find_scales();
     const int in = (1 << p.c.shift) - 1;
+    typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+    soff = here(soff);
 #pragma unroll
     for (int u = 0; u < NI; ++u) {
-      const int at = ((tile * kPpKeys + u * RPL + srow) & in) * GB + sch * 16;
-      kr[u] = vr[u] = u32x4{0, 0, 0, 0};
-      if (pid[u] >= 0) {
-        kr[u] = *gptr<u32x4>(p.c.k + (int64_t)pid[u] * p.c.k_stride + at);
-        vr[u] = *gptr<u32x4>(p.c.v + (int64_t)pid[u] * p.c.v_stride + at);
+      const int row = tile * kPpKeys + u * RPL + w * (64 / CG);
+      const int id = __builtin_amdgcn_readlane(pid, (row >> 4) & 63);
+      const int64_t page = id & 0x7fffffff;
+      const WNW_GLOBAL uint8_t* kp = gptr<uint8_t>(p.c.k) + (page * p.c.k_stride + (row & in) * GB);
+      const WNW_GLOBAL uint8_t* vp = gptr<uint8_t>(p.c.v) + (page * p.c.v_stride + (row & in) * GB);
+      if constexpr (Q8) {
+        const u32x2_t k0 = *(const WNW_GLOBAL u32x2_t*)(kp + soff), k1 = *(const WNW_GLOBAL u32x2_t*)(kp + (soff + GB / 2));
+        const u32x2_t v0 = *(const WNW_GLOBAL u32x2_t*)(vp + soff), v1 = *(const WNW_GLOBAL u32x2_t*)(vp + (soff + GB / 2));
+        kr[u] = u32x4{k0[0], k0[1], k1[0], k1[1]};
+        vr[u] = u32x4{v0[0], v0[1], v1[0], v1[1]};
+      } else {
+        kr[u] = *(const WNW_GLOBAL u32x4*)(kp + soff);
+        vr[u] = *(const WNW_GLOBAL u32x4*)(vp + soff);
       }
-    }
-    if (Q8 && tid < kPpKeys / 16) {
-      sk = sv = 1.f;
-      if (spid >= 0) {
-        sk = p.c.k_scale[spid];
-        sv = p.c.v_scale[spid];
-      }
+      gone[u] = id;
     }
   };
-  auto put = [&](int buf) {
-    uint8_t* kt = lds + (NB == 2 ? buf * 2 * TB : 0);
-    uint8_t* vt = kt + TB;
+  auto clear = [&](int tile) {  // rows of kr and vr that are not the segment's
+    int any = (tile + 1) * kPpKeys > r.len;
+#pragma unroll
+    for (int u = 0; u < NI; ++u) any |= gone[u] < 0;
+    if (!any) return;
 #pragma unroll
     for (int u = 0; u < NI; ++u) {
-      const int rr = u * RPL + srow;
-      if constexpr (Q8) {
-        *(u32x4*)(kt + rr * RB + (((2 * sch) ^ (rr % CH)) * 16)) = e4m3x8<T>(kr[u][0], kr[u][1]);
-        *(u32x4*)(kt + rr * RB + (((2 * sch + 1) ^ (rr % CH)) * 16)) = e4m3x8<T>(kr[u][2], kr[u][3]);
-        *(u32x4*)(vt + rr * RB + (((2 * sch) ^ (2 * (rr & 3))) * 16)) = e4m3x8<T>(vr[u][0], vr[u][1]);
-        *(u32x4*)(vt + rr * RB + (((2 * sch + 1) ^ (2 * (rr & 3))) * 16)) = e4m3x8<T>(vr[u][2], vr[u][3]);
-      } else {
-        *(u32x4*)(kt + rr * RB + ((sch ^ (rr % CH)) * 16)) = kr[u];
-        *(u32x4*)(vt + rr * RB + ((sch ^ (2 * (rr & 3))) * 16)) = vr[u];
-      }
+      if (gone[u] < 0) kr[u] = u32x4{0, 0, 0, 0};
+      if (gone[u] < 0 || tile * kPpKeys + u * RPL + srow >= r.len) vr[u] = u32x4{0, 0, 0, 0};
     }
-    if (Q8 && tid < kPpKeys / 16) {
-      scales[buf][tid][0] = fmaxf(sk, 7.888609e-31f);  // 0 would make a masked score NaN
-      scales[buf][tid][1] = sv;
+  };
+  auto put = [&](int tile) {
+    uint8_t* kt = lds + (NB == 2 ? (tile & 1) * 2 * TB : 0);
+    uint8_t* vt = kt + TB;
+    kput = here(kput);
+    vput = here(vput);
+#pragma unroll
+    for (int u = 0; u < NI; ++u) {
+      // load u's rows lie u * RPL further; where that changes the row's place in the swizzle, so do the chunks
+      constexpr int kRot = RPL % CH;
+      const uint32_t kx = kRot ? ((u * kRot) % CH) * 16 : 0;
+      uint8_t* const kd = kt + u * RPL * RB;
+      uint8_t* const vd = vt + u * RPL * RB;
+      if constexpr (Q8) {
+        *(u32x4*)(kd + (kput ^ kx)) = e4m3x8<T>(kr[u][0], kr[u][1]);
+        *(u32x4*)(kd + (kput ^ kx ^ kHalf)) = e4m3x8<T>(kr[u][2], kr[u][3]);
+        *(u32x4*)(vd + vput) = e4m3x8<T>(vr[u][0], vr[u][1]);
+        *(u32x4*)(vd + (vput ^ kHalf)) = e4m3x8<T>(vr[u][2], vr[u][3]);
+      } else {
+        *(u32x4*)(kd + (kput ^ kx)) = kr[u];
+        *(u32x4*)(vd + vput) = vr[u];
+      }
     }
   };
   // lane offsets of the operands inside a tile
@@ -204,7 +253,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
   float m = kPgLowest, l = 0.f;
-  float ref = -100.f;  // log2 of the largest V scale so far (Q8)
+  // Q8, per 16 keys of the window that the products are in: what a score is
+  // worth in the exponent, the logarithm of V's scale relative to the largest so
+  // far (ref), and what undoes it
+  float ref = -100.f, wk = 0.f, wl = 0.f, wu = 0.f;
+  auto enter_scales = [&]() {
+    wk = fmaxf(ks, 7.888609e-31f) * p.scale_log2;  // a scale of 0 would make a masked score NaN
+    const float lg = __builtin_amdgcn_logf(vs), most = fmaxf(ref, wave_max(lg));
+    const float f = __builtin_amdgcn_exp2f(ref - most);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
+    ref = most;
+    wl = fmaxf(lg - ref, -100.f);  // less is nothing beside the largest
+    wu = __builtin_amdgcn_exp2f(-wl);
+  };
   auto tile = [&](int i, auto masked) {
     const uint8_t* kt = lds + (NB == 2 ? (i & 1) * 2 * TB : 0);
     const uint8_t* vt = kt + TB;
@@ -215,29 +277,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) s[mt] = mma32<T>(*(const u32x4*)(kt + koff[kk] + mt * 32 * RB), qr[kk], s[mt]);
-    float ck[4], lv[4];  // per 16 keys
-    if constexpr (Q8) {
-      float most = ref;
+    if constexpr (NB == 2) {  // among the products: the next tile into the other buffer, the one after it on its way
+      put(i + 1);
+      fetch(i + 2);
+    }
+    float ck[4], lv[4], un[4];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        ck[b] = scales[i & 1][b][0] * p.scale_log2;
-        lv[b] = __builtin_amdgcn_logf(scales[i & 1][b][1]);
-        most = fmaxf(most, lv[b]);
-      }
-      if (most > ref) {
-        const float f = __builtin_amdgcn_exp2f(ref - most);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
-        ref = most;
-      }
-#pragma unroll
-      for (int b = 0; b < 4; ++b) lv[b] = fmaxf(lv[b] - ref, -100.f);  // less is nothing beside the largest
-    } else {
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        ck[b] = p.scale_log2;
-        lv[b] = 0.f;
-      }
+    for (int b = 0; b < 4; ++b) {
+      auto at = [&](float x) {
+        return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), (4 * i + b) & 63));
+      };
+      ck[b] = Q8 ? at(wk) : p.scale_log2;
+      lv[b] = Q8 ? at(wl) : 0.f;
+      un[b] = Q8 ? at(wu) : 1.f;
     }
     if constexpr (decltype(masked)::value) {
       const int lim = limit - i * kPpKeys - 4 * hi;  // keys 32 mt + 8 j + c (+ 4 hi) below it
@@ -256,17 +308,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
       mx = fmaxf(mx, y * ck[b]);
     }
     mx = max_x32(mx);
-    if (__ballot(mx > m)) {
+    if (__ballot(mx > m + kPpTrail)) {
       const float f = __builtin_amdgcn_exp2f(m - mx);
       l *= f;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
       m = mx;
     }
+    __builtin_amdgcn_s_setprio(1);  // a wave at these products before another's other work: 222 -> 218 us
     u32x4 pb[4];
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const float off = lv[b] - m;
+      const float off = lv[b] - m + kBias;
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -275,7 +328,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
         sum += y0 + y1;
         pb[b][j] = Ops::pack2(y0, y1);
       }
-      l = Q8 ? fmaf(sum, __builtin_amdgcn_exp2f(-lv[b]), l) : l + sum;
+      l = Q8 ? fmaf(sum, un[b], l) : l + sum;
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b)
@@ -285,28 +338,31 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
         const uint64_t v1 = Ops::read_tr(vt + voff[dt] + (16 * b + 8) * RB);
         o[dt] = mma32<T>(u32x4{(uint32_t)v0, (uint32_t)(v0 >> 32), (uint32_t)v1, (uint32_t)(v1 >> 32)}, pb[b], o[dt]);
       }
+    __builtin_amdgcn_s_setprio(0);
   };
   if (t0 < t1) {
-    find(t0);
+    find(t0 / kWin);
+    find_scales();
+    if (t0 % kWin != 0) enter(t0 / kWin);
     fetch(t0);
-    find(t0 + 1);
+    if (t0 % kWin >= kWin / 2) find_scales();
     if constexpr (NB == 2) {
-      put(t0 & 1);
-      fetch(t0 + 1);
-      find(t0 + 2);
+      clear(t0);
+      put(t0);
     }
+    if (Q8) enter_scales();
+    if constexpr (NB == 2) fetch(t0 + 1);
+    // (the tile after next is fetched while a tile is used, or the next one with
+    // one buffer: the window of the products follows that of fetch() by as much)
     auto turn = [&](int i) {
+      if (Q8 && i % kWin == 0 && i > t0) enter_scales();
       __syncthreads();  // everyone is done with tile i - 1; with two buffers tile i is in LDS
       if constexpr (NB == 2) {
-        if (i + 1 < t1) {
-          put((i + 1) & 1);
-          fetch(i + 2);
-          find(i + 3);
-        }
+        clear(i + 1);
       } else {
-        put(i & 1);
+        clear(i);
+        put(i);
         fetch(i + 1);
-        find(i + 2);
         __syncthreads();
       }
     };
@@ -320,13 +376,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
       turn(i);
       tile(i, std::true_type());
     }
-    for (; i < t1; ++i) turn(i);
+    for (; i < t1; ++i) {
+      turn(i);
+      if constexpr (NB == 2) {
+        put(i + 1);
+        fetch(i + 2);
+      }
+    }
+    if (wrong) raise_device_error(p.err, WNW_DEVERR_BOUNDS);
   }
   l = sum_x32(l);
   if (p.splits == 1) {
     prompt_store<T, D>(p, r, row, h, hi, o, l, Q8 ? ref : 0.f);
   } else {
-    float* part = p.part + (((int64_t)blockIdx.x * p.splits + blockIdx.y) * 4 + w) * (DT * 16 + 3) * 64;
+    float* part = p.part + (((int64_t)blockIdx.x * p.splits + blockIdx.y) * W + w) * (DT * 16 + 3) * 64;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -342,21 +405,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
 
 // The splits' sums added up, a wave for 32 query rows.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParams p) {
-  constexpr int DT = D / 32;
+__global__ __launch_bounds__(64 * prompt_waves(D)) void paged_prompt_join_kernel(PagedPromptParams p) {
+  constexpr int DT = D / 32, W = prompt_waves(D), kPpQ = 32 * W;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hi = lane >> 5, n = lane & 31;
   const int N = p.c.n_seg;
   const int seg = blockIdx.x % N, qblk = p.nqb - 1 - blockIdx.x / N;
   const PromptRows r = prompt_rows(p, seg, false);
   if (qblk * kPpQ + 32 * w >= r.rows) return;
   constexpr int64_t kPart = (DT * 16 + 3) * 64;
-  const float* part = p.part + ((int64_t)blockIdx.x * p.splits * 4 + w) * kPart;
+  const float* part = p.part + ((int64_t)blockIdx.x * p.splits * W + w) * kPart;
   f32x16 o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
   float m = kPgLowest, l = 0.f, ref = -100.f;
   for (int s = 0; s < p.splits; ++s) {
-    const float* at = part + s * 4 * kPart;
+    const float* at = part + s * W * kPart;
     const float pm = at[DT * 16 * 64 + lane], pl = at[DT * 16 * 64 + 64 + lane], pr = at[DT * 16 * 64 + 128 + lane];
     const float mx = fmaxf(m, pm), most = fmaxf(ref, pr);
     const float f = __builtin_amdgcn_exp2f(m - mx), g = __builtin_amdgcn_exp2f(pm - mx);
@@ -382,18 +445,19 @@ struct PromptPlan {
 };
 static PromptPlan prompt_plan(int64_t n_seg, int64_t group, int64_t max_tokens, int64_t capacity, int64_t D) {
   PromptPlan y;
+  const int W = prompt_waves((int)D), kPpQ = 32 * W;
   y.nqb = (max_tokens * group + kPpQ - 1) / kPpQ;
-  const int64_t wgs = std::max<int64_t>(n_seg * y.nqb, 1), want = 2ll * device_cus(), tiles = (capacity + kPpKeys - 1) / kPpKeys;
+  const int64_t wgs = std::max<int64_t>(n_seg * y.nqb, 1), want = (W == 8 ? 1ll : 2ll) * device_cus(), tiles = (capacity + kPpKeys - 1) / kPpKeys;
   y.splits = std::max<int64_t>(1, std::min({want / wgs, tiles / 4, (int64_t)64}));
-  y.bytes = y.splits == 1 ? 0 : wgs * y.splits * 4 * (D / 2 + 3) * 64 * 4;
+  y.bytes = y.splits == 1 ? 0 : wgs * y.splits * W * (D / 2 + 3) * 64 * 4;
   return y;
 }
 
 template <typename T, int D, bool Q8>
 static hipError_t launch_prompt_q(const PagedPromptParams& p, hipStream_t st) {
   const dim3 grid((unsigned)(p.c.n_seg * (int64_t)p.nqb), (unsigned)p.splits);
-  hipLaunchKernelGGL((paged_prompt_kernel<T, D, Q8>), grid, dim3(256), 0, st, p);
-  if (p.splits > 1) hipLaunchKernelGGL((paged_prompt_join_kernel<T, D>), dim3(grid.x), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((paged_prompt_kernel<T, D, Q8>), grid, dim3(64 * prompt_waves(D)), 0, st, p);
+  if (p.splits > 1) hipLaunchKernelGGL((paged_prompt_join_kernel<T, D>), dim3(grid.x), dim3(64 * prompt_waves(D)), 0, st, p);
   return hipGetLastError();
 }
 template <typename T>
