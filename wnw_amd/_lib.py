@@ -148,10 +148,11 @@ def callpath():
         except ImportError as e:
             raise RuntimeError(f"wnw_amd/_callpath.so is missing or does not load ({e}): {_BUILD}") from e
         from .kv.fused_attn import call_workspace
+        from .kv.paged import call_workspace as paged_workspace
         from .wnw.kernels import call_score_workspace
 
         mod.setup(_raw_stream if _raw_stream is not None else lambda i: raw_stream(torch.device("cuda", i)),
-                  call_workspace, call_score_workspace, check)
+                  call_workspace, call_score_workspace, paged_workspace, check)
         _callpath = mod
     return _callpath
 

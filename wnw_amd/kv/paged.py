@@ -41,22 +41,28 @@ _PAGE_DTYPES = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16, E4M3: 
 _workspaces: dict[tuple[int, int], list] = {}
 
 
-def _workspace(dev: torch.device, n_seg: int, need: int) -> Tensor | None:
-    if need <= 0:
-        return None
-    counters = int(_lib.lib().wnw_paged_counter_bytes(n_seg))
-    if torch.cuda.is_current_stream_capturing():
-        buf = torch.empty(need, dtype=torch.uint8, device=dev)
-    else:
-        key = (dev.index if dev.index is not None else torch.cuda.current_device(), _lib.raw_stream(dev))
-        held = _workspaces.get(key)
-        if held is not None and held[0].numel() >= need and held[1] == counters:
-            return held[0]
-        size = need if held is None else max(need, held[0].numel())
-        buf = torch.empty(size, dtype=torch.uint8, device=dev)
-        _workspaces[key] = [buf, counters]
-    _lib.check(_lib.lib().wnw_workspace_init(_lib.ptr(buf), counters, _lib.stream_of(dev)), "workspace init")
+_is_capturing = torch.cuda.is_current_stream_capturing
+
+
+def call_workspace(idx: int, stream: int, n_seg: int, need: int) -> Tensor:
+    """The workspace of an attention call on ``stream`` of device ``idx`` (the
+    current one), its counters zero."""
+    _lib.ensure_init_index(idx)
+    counters = (n_seg + 4095) // 4096 * 16384  # wnw_paged_counter_bytes
+    capturing = _is_capturing()
+    held = _workspaces.get((idx, stream))
+    if not capturing and held is not None and held[1] == counters and held[0].numel() >= need:
+        return held[0]
+    size = need if capturing or held is None else max(need, held[0].numel())
+    buf = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", idx))
+    _lib.check(_lib.lib().wnw_workspace_init(_lib.ptr(buf), counters, ctypes.c_void_p(stream)), "workspace init")
+    if not capturing:
+        _workspaces[(idx, stream)] = [buf, counters]
     return buf
+
+
+def _workspace(dev: torch.device, n_seg: int, need: int) -> Tensor:
+    return call_workspace(dev.index if dev.index is not None else torch.cuda.current_device(), _lib.raw_stream(dev), n_seg, need)
 
 
 def _cache(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seg_len: Tensor, k_scale: Tensor | None,
@@ -151,6 +157,12 @@ def paged_append(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_ta
 
     ``new_len``: where to put the new lengths (not ``seg_len`` itself).  16-bit
     pages must have the type of ``k``."""
+    if new_len is None:  # the plain form (tensors that need no copy): checked and launched natively
+        done = (_lib._callpath or _lib.callpath()).paged_append(
+            k, v, k_pages, v_pages, page_table, seg_len, q, positions, inv_freq, sections, interleaved, cu_tokens, max_tokens,
+            k_scale, v_scale)
+        if done is not None:
+            return done
     cache = _cache(k_pages, v_pages, page_table, seg_len, k_scale, v_scale, k, v, q, positions, inv_freq, cu_tokens, new_len)
     N, D = cache.n_seg, cache.head_dim
     if k.dtype not in (torch.bfloat16, torch.float16) or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
@@ -235,6 +247,10 @@ def paged_decode_attn(q_flat: Tensor, k_pages: Tensor, v_pages: Tensor, page_tab
     segment without rows gives zeros.  ``out``: a contiguous tensor for the
     result.  The lengths are read on the device; ``page_table.shape[1]`` bounds
     them and sizes the grid."""
+    done = (_lib._callpath or _lib.callpath()).paged_decode(q_flat, k_pages, v_pages, page_table, seg_len, scale, k_scale,
+                                                            v_scale, out)
+    if done is not None:
+        return done
     cache = _cache(k_pages, v_pages, page_table, seg_len, k_scale, v_scale, q_flat, out)
     _check_q(q_flat, k_pages, scale)
     N, D = cache.n_seg, cache.head_dim
@@ -270,6 +286,10 @@ def paged_prompt_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: T
     [T, Hq, D].  ``max_tokens``, the most tokens of a sample, sizes the grid
     (default T); a sample with more sets the device error word and its rows of
     the result are not written."""
+    done = (_lib._callpath or _lib.callpath()).paged_prompt(q, k_pages, v_pages, page_table, seg_len, cu_tokens, scale,
+                                                            max_tokens, k_scale, v_scale, out)
+    if done is not None:
+        return done
     cache = _cache(k_pages, v_pages, page_table, seg_len, k_scale, v_scale, q, cu_tokens, out)
     _check_q(q, k_pages, scale)
     N, D = cache.n_seg, cache.head_dim
