@@ -39,13 +39,12 @@ struct PagedAppendParams {
   int32_t* err;
 };
 
-// sin and cos of x * f, x * f in radians
-__device__ __forceinline__ void turn_of(double x, double f, float* sn, float* cs) {
-  double u = x * f * 0.15915494309189535;  // turns
-  u = 4.0 * (u - __builtin_rint(u));       // quarter turns, [-2, 2]
-  const double k = __builtin_rint(u);
-  const float y = (float)((u - k) * 1.5707963267948966);  // [-pi / 4, pi / 4]
-  const int quarter = (int)k & 3;
+// sin and cos of u quarter turns, |u| < 2^51
+__device__ __forceinline__ void turn_of(double u, float* sn, float* cs) {
+  // adding 1.5 * 2^52 leaves the nearest whole number in the low bits
+  const double t = u + 6755399441055744.0;
+  const int quarter = (int)__builtin_bit_cast(uint64_t, t);
+  const float y = (float)(u - (t - 6755399441055744.0)) * 1.57079633f;  // [-pi / 4, pi / 4]
   const float z = y * y;
   float s = fmaf(z, 2.7557319e-6f, -1.9841270e-4f);
   s = fmaf(z, s, 8.3333333e-3f);
@@ -57,25 +56,27 @@ __device__ __forceinline__ void turn_of(double x, double f, float* sn, float* cs
   c = fmaf(z, c, -0.5f);
   c = fmaf(z, c, 1.0f);
   const float a = quarter & 1 ? c : s, b = quarter & 1 ? s : c;
-  *sn = quarter & 2 ? -a : a;
-  *cs = (quarter == 1 || quarter == 2) ? -b : b;
+  *sn = __uint_as_float(__float_as_uint(a) ^ (uint32_t)(quarter & 2) << 30);
+  *cs = __uint_as_float(__float_as_uint(b) ^ (uint32_t)((quarter + 1) & 2) << 30);
 }
 
-// n consecutive 16-bit elements (n = 2 or 8) as floats, and back
+// PP consecutive 16-bit elements (2 or 8): as they lie, as floats, and back
+template <int PP>
+using Run = typename std::conditional<PP == 8, u32x4, uint32_t>::type;
 template <typename T, int PP>
-__device__ __forceinline__ void load_elems(const T* p, float (&x)[PP]) {
+__device__ __forceinline__ Run<PP> load_run(const T* p) {
+  return *gptr<Run<PP>>(p);
+}
+template <typename T, int PP>
+__device__ __forceinline__ void elems_of(const Run<PP>& w, float (&x)[PP]) {
   if constexpr (PP == 8) {
-    const u32x4 w = *gptr<u32x4>(p);
     unpack8(w, x, (T*)nullptr);
+  } else if constexpr (std::is_same<T, bf16_t>::value) {
+    x[0] = bf16_lo(w);
+    x[1] = bf16_hi(w);
   } else {
-    const uint32_t w = *gptr<uint32_t>(p);
-    if constexpr (std::is_same<T, bf16_t>::value) {
-      x[0] = bf16_lo(w);
-      x[1] = bf16_hi(w);
-    } else {
-      x[0] = f16_bits_to_f32(w & 0xffffu);
-      x[1] = f16_bits_to_f32(w >> 16);
-    }
+    x[0] = f16_bits_to_f32(w & 0xffffu);
+    x[1] = f16_bits_to_f32(w >> 16);
   }
 }
 template <typename T, int PP>
@@ -117,19 +118,21 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 // A workgroup takes one unit: the rows of one append that fall into one page of
 // one segment, so that the page's largest magnitude is known before a code is
 // written.  A thread holds PP pairs of a row (2 PP elements in two runs of PP)
-// and up to NIT rows.
+// and up to NIT rows.  V's loads go out first and a q head's before the one
+// ahead of it is stored.
 //   PP = 8 (chunks of prompts): 16-byte loads; the unit does K, V and the
-//       group's q heads, so a row's sines are worked out once for all of them.
+//       group's q heads, so a row's sines are worked out once for all of them;
+//       with few units the q heads are shared out over blockIdx.y.
 //   PP = 2 (a few tokens): K, V and each q head in workgroups of their own
 //       (blockIdx.y), a quarter of the sines in each thread: with one token the
 //       time is one chain of loads, sines and stores.
-template <typename T, int PP, bool Q8, int NT>
+template <typename T, int PP, bool Q8, int NT, int NIT>
 __global__ __launch_bounds__(NT) void paged_append_kernel(PagedAppendParams p, int D) {
-  constexpr int NIT = 4;
   __shared__ float red[2][NT / 64];
   const int tid = threadIdx.x;
   const int s = blockIdx.x / p.units, unit = blockIdx.x - s * p.units;
-  const int what = PP == 8 ? -1 : blockIdx.y;  // -1: all; 0: K, 1: V, 2 + g: q head g
+  // PP = 2: 0 K, 1 V, 2 + g q head g.  PP = 8: -1 K, V and the first share of the q heads, 2 another share
+  const int what = PP == 2 ? (int)blockIdx.y : blockIdx.y == 0 ? -1 : 2;
   const int h = s % p.t.hkv;
   int first, count;
   const bool told = paged_tokens_of(p.t, s, &first, &count);
@@ -169,15 +172,32 @@ __global__ __launch_bounds__(NT) void paged_append_kernel(PagedAppendParams p, i
   }
   const int n = row1 - row0, t0 = first + row0 - len;
 
-  auto sines = [&](int row, float (&sn)[PP], float (&cs)[PP]) {
+  // what a position is worth in quarter turns, pair by pair, and the pairs' axes
+  double fq[PP];
+  const int64_t axis0 = ((cth * PP >= p.sec1) + (cth * PP >= p.sec2) + (cth * PP >= p.sec3)) * p.pos_axis;
+  const int last = cth * PP + PP - 1;
+  const bool one_axis = axis0 == ((last >= p.sec1) + (last >= p.sec2) + (last >= p.sec3)) * p.pos_axis;
+  if (turns && what != 1) {
 #pragma unroll
     for (int i = 0; i < PP; ++i) {
       const int j = cth * PP + i;
-      const int axis = (j >= p.sec1) + (j >= p.sec2) + (j >= p.sec3);
-      const int64_t at = axis * p.pos_axis + t0 + row;
-      const double x = p.pos64 ? (double)gptr<int64_t>(p.pos)[at] : (double)gptr<int32_t>(p.pos)[at];
-      const double f = p.freq64 ? gptr<double>(p.inv_freq)[j] : (double)gptr<float>(p.inv_freq)[j];
-      turn_of(x, f, &sn[i], &cs[i]);
+      fq[i] = (p.freq64 ? gptr<double>(p.inv_freq)[j] : (double)gptr<float>(p.inv_freq)[j]) * 0.63661977236758134;
+    }
+  }
+  auto position = [&](int64_t at) {
+    return p.pos64 ? (double)gptr<int64_t>(p.pos)[at] : (double)gptr<int32_t>(p.pos)[at];
+  };
+  auto sines = [&](int row, float (&sn)[PP], float (&cs)[PP]) {
+    if (one_axis) {
+      const double x = position(axis0 + t0 + row);
+#pragma unroll
+      for (int i = 0; i < PP; ++i) turn_of(x * fq[i], &sn[i], &cs[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PP; ++i) {
+        const int j = cth * PP + i;
+        turn_of(position(((j >= p.sec1) + (j >= p.sec2) + (j >= p.sec3)) * p.pos_axis + t0 + row) * fq[i], &sn[i], &cs[i]);
+      }
     }
   };
   auto turned = [&](float (&a)[PP], float (&b)[PP], const float (&sn)[PP], const float (&cs)[PP]) {
@@ -261,6 +281,19 @@ __global__ __launch_bounds__(NT) void paged_append_kernel(PagedAppendParams p, i
     }
   };
 
+  // V's loads first, where there are registers for them
+  constexpr bool kEarly = NIT <= 2;
+  Run<PP> vr[NIT][2];
+  auto load_v = [&]() {
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+      // rows past the unit's repeat its last
+      const T* row = (const T*)p.v + (int64_t)(t0 + min(it * rpp + rth, n - 1)) * p.vt + h * p.vh;
+      vr[it][0] = load_run<T, PP>(row + e0);
+      vr[it][1] = load_run<T, PP>(row + e1);
+    }
+  };
+  if (kEarly && (what == -1 || what == 1)) load_v();
   float x[NIT][2][PP];
   if (what != 1) {
 #pragma unroll
@@ -269,63 +302,83 @@ __global__ __launch_bounds__(NT) void paged_append_kernel(PagedAppendParams p, i
 #pragma unroll
       for (int i = 0; i < PP; ++i) x[it][0][i] = x[it][1][i] = 0.f;
       if (r >= n) continue;
+      Run<PP> ka, kb, qa, qb;
+      if (what <= 0) {
+        const T* row = (const T*)p.k + (int64_t)(t0 + r) * p.kt + h * p.kh;
+        ka = load_run<T, PP>(row + e0);
+        kb = load_run<T, PP>(row + e1);
+      }
+      const int g0 = PP == 2 ? what - 2 : p.G * (int)blockIdx.y / (int)gridDim.y;
+      const int g1 = PP == 2 ? what - 1 : p.G * ((int)blockIdx.y + 1) / (int)gridDim.y;
+      const T* qp = (const T*)p.q + (int64_t)(t0 + r) * p.qt + (h * p.G + g0) * p.qh;
+      if (p.q && what != 0 && g0 < g1) {
+        qa = load_run<T, PP>(qp + e0);
+        qb = load_run<T, PP>(qp + e1);
+      }
       float sn[PP], cs[PP];
       if (turns) sines(r, sn, cs);
       if (what <= 0) {
-        const T* row = (const T*)p.k + (int64_t)(t0 + r) * p.kt + h * p.kh;
-        load_elems<T, PP>(row + e0, x[it][0]);
-        load_elems<T, PP>(row + e1, x[it][1]);
+        elems_of<T, PP>(ka, x[it][0]);
+        elems_of<T, PP>(kb, x[it][1]);
         turned(x[it][0], x[it][1], sn, cs);
       }
       if (p.q && what != 0) {
-        const int g0 = what < 0 ? 0 : what - 2, g1 = what < 0 ? p.G : what - 1;
+        T* dst = (T*)p.q_out + ((int64_t)(t0 + r) * (p.t.hkv * p.G) + h * p.G + g0) * D;
         for (int g = g0; g < g1; ++g) {
-          const int head = h * p.G + g;
-          const T* row = (const T*)p.q + (int64_t)(t0 + r) * p.qt + head * p.qh;
-          T* dst = (T*)p.q_out + ((int64_t)(t0 + r) * (p.t.hkv * p.G) + head) * D;
           float a[PP], b[PP];
-          load_elems<T, PP>(row + e0, a);
-          load_elems<T, PP>(row + e1, b);
+          elems_of<T, PP>(qa, a);
+          elems_of<T, PP>(qb, b);
+          if (g + 1 < g1) {
+            qp += p.qh;
+            qa = load_run<T, PP>(qp + e0);
+            qb = load_run<T, PP>(qp + e1);
+          }
           turned(a, b, sn, cs);
           store_elems<T, PP>(dst + e0, a);
           store_elems<T, PP>(dst + e1, b);
+          dst += D;
         }
       }
     }
     if (what <= 0) put(x, p.c.k, p.c.k_stride, p.c.k_scale, red[0]);
   }
   if (what == -1 || what == 1) {
+    if (!kEarly) load_v();
 #pragma unroll
     for (int it = 0; it < NIT; ++it) {
-      const int r = it * rpp + rth;
-#pragma unroll
-      for (int i = 0; i < PP; ++i) x[it][0][i] = x[it][1][i] = 0.f;
-      if (r >= n) continue;
-      const T* row = (const T*)p.v + (int64_t)(t0 + r) * p.vt + h * p.vh;
-      load_elems<T, PP>(row + e0, x[it][0]);
-      load_elems<T, PP>(row + e1, x[it][1]);
+      elems_of<T, PP>(vr[it][0], x[it][0]);
+      elems_of<T, PP>(vr[it][1], x[it][1]);
     }
     put(x, p.c.v, p.c.v_stride, p.c.v_scale, red[1]);
   }
 }
 
+static constexpr int64_t kPaWgs = 1536;  // workgroups that shares of the q heads are made for
+
 template <typename T, bool Q8>
 static hipError_t launch_append(const PagedAppendParams& p, int D, int64_t most, hipStream_t st) {
   const int R = 1 << p.c.shift;
-  // rows of a unit, and threads so that no thread holds more than 4 of its rows
+  // rows of a unit; threads for them
   const int64_t rows = std::min<int64_t>(R, most);
   const dim3 grid((unsigned)((int64_t)p.c.n_seg * p.units));
-  if (rows * D <= 4 * 4 * 256) {  // a few tokens: 2 pairs a thread
-    const dim3 heads(grid.x, p.q ? 2 + p.G : 2);
-    if (rows * D <= 4 * 64)  // one pass of a wave
-      hipLaunchKernelGGL((paged_append_kernel<T, 2, Q8, 64>), heads, dim3(64), 0, st, p, D);
-    else
-      hipLaunchKernelGGL((paged_append_kernel<T, 2, Q8, 256>), heads, dim3(256), 0, st, p, D);
-  } else if (rows * D <= 4 * 16 * 256) {
-    hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 256>), grid, dim3(256), 0, st, p, D);
-  } else {
-    hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 1024>), grid, dim3(1024), 0, st, p, D);
-  }
+  const dim3 heads(grid.x, p.q ? 2 + p.G : 2);
+  const dim3 shares(grid.x, p.q ? (unsigned)std::max<int64_t>(1, std::min<int64_t>(p.G, kPaWgs / grid.x)) : 1u);
+  if (rows * D <= 4 * 64)  // one token, or a few: one pass of a wave
+    hipLaunchKernelGGL((paged_append_kernel<T, 2, Q8, 64, 1>), heads, dim3(64), 0, st, p, D);
+  else if (rows * D <= 4 * 256)
+    hipLaunchKernelGGL((paged_append_kernel<T, 2, Q8, 256, 1>), heads, dim3(256), 0, st, p, D);
+  else if (rows * D <= 16 * 128)
+    hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 128, 1>), shares, dim3(128), 0, st, p, D);
+  else if (rows * D <= 16 * 256)
+    hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 256, 1>), shares, dim3(256), 0, st, p, D);
+  else if (rows * D <= 2 * 16 * 256)
+    hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 256, 2>), shares, dim3(256), 0, st, p, D);
+  else if (rows * D <= 4 * 16 * 256)
+    hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 512, 2>), shares, dim3(512), 0, st, p, D);
+  else if (rows * D <= 8 * 16 * 256)
+    hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 512, 4>), shares, dim3(512), 0, st, p, D);
+  else
+    hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 1024, 4>), shares, dim3(1024), 0, st, p, D);
   return hipGetLastError();
 }
 

@@ -49,10 +49,6 @@ struct PagedPromptParams {
 // waves of a workgroup, each with 32 query rows
 __host__ __device__ constexpr int prompt_waves(int D) { return D == 128 ? 8 : 4; }
 static constexpr int kPpKeys = 64;  // keys of a tile
-// log2 of how far the maximum that the weights are taken against may trail the
-// running one: weights up to 2^6 round like weights up to 1, and most tiles
-// then leave the sums as they are.
-static constexpr float kPpTrail = 6.f;
 
 template <typename T>
 __device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f32x16& c) {
@@ -106,7 +102,7 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
   constexpr int NI = kPpKeys * GB / (1024 * W);                     // 16-byte loads per thread and tensor
   constexpr int KK = D / 16, DT = D / 32;
   constexpr int NB = D == 256 ? 1 : 2;  // tiles in LDS
-  // f16 weights are held times 2^8 (2^14 at most): normal numbers down to 2^-22 of the largest
+  // f16 weights are held times 2^8: normal numbers down to 2^-22 of the largest
   constexpr float kBias = std::is_same<T, f16_t>::value ? 8.f : 0.f;
   __shared__ __attribute__((aligned(16))) uint8_t lds[NB * 2 * TB];  // [NB][K, V]
   __shared__ float scales[2][kPpKeys / 16][2];
@@ -308,14 +304,13 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
       mx = fmaxf(mx, y * ck[b]);
     }
     mx = max_x32(mx);
-    if (__ballot(mx > m + kPpTrail)) {
+    if (__ballot(mx > m)) {
       const float f = __builtin_amdgcn_exp2f(m - mx);
       l *= f;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
       m = mx;
     }
-    __builtin_amdgcn_s_setprio(1);  // a wave at these products before another's other work: 222 -> 218 us
     u32x4 pb[4];
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
@@ -338,7 +333,6 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
         const uint64_t v1 = Ops::read_tr(vt + voff[dt] + (16 * b + 8) * RB);
         o[dt] = mma32<T>(u32x4{(uint32_t)v0, (uint32_t)(v0 >> 32), (uint32_t)v1, (uint32_t)(v1 >> 32)}, pb[b], o[dt]);
       }
-    __builtin_amdgcn_s_setprio(0);
   };
   if (t0 < t1) {
     find(t0 / kWin);
