@@ -73,23 +73,24 @@ __device__ __forceinline__ PromptRows prompt_rows(const PagedPromptParams& p, in
   return r;
 }
 
-// The wave's rows out: lane (hi, n) has elements 32 i + 8 j + 4 hi + 0..3 of row n
-template <typename T, int D>
-__device__ __forceinline__ void prompt_store(const PagedPromptParams& p, const PromptRows& r, int row, int h, int hi,
-                                             const f32x16 (&o)[D / 32], float l, float ref) {
+// The wave's rows out, 32-element parts dt0 .. dt0 + NT - 1: lane (hi, n) has
+// elements 32 i + 8 j + 4 hi + 0..3 of row n
+template <typename T, int NT>
+__device__ __forceinline__ void prompt_store(const PagedPromptParams& p, const PromptRows& r, int row, int h, int hi, int dt0,
+                                             const f32x16* o, float l, float ref) {
   if (row >= r.rows) return;
   const int i = row / p.G, g = row - i * p.G;
   T* op = (T*)p.out + (int64_t)(r.first + i) * p.ot + (int64_t)(h * p.G + g) * p.oh;
   const bool none = r.len - r.count + i + 1 <= 0;
   const float inv = __builtin_amdgcn_exp2f(ref) / l;
 #pragma unroll
-  for (int dt = 0; dt < D / 32; ++dt)
+  for (int dt = 0; dt < NT; ++dt)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float y[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = none ? 0.f : o[dt][4 * j + e] * inv;
-      store_quad<T>(op, 32 * dt + 8 * j + 4 * hi, y);
+      store_quad<T>(op, 32 * (dt0 + dt) + 8 * j + 4 * hi, y);
     }
 }
 
@@ -123,7 +124,8 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
   const int last = base + min(qblk * kPpQ + kPpQ - 1, r.rows - 1) / p.G;
   const int tiles = max((last + kPpKeys - 1) / kPpKeys, 0);
   const int t0 = (int)((int64_t)tiles * blockIdx.y / p.splits), t1 = (int)((int64_t)tiles * (blockIdx.y + 1) / p.splits);
-  const int mine = min(t1, (wlast + kPpKeys - 1) / kPpKeys);  // the wave's tiles end here
+  const bool busy = qblk * kPpQ + 32 * w < r.rows;  // a wave without rows only moves tiles
+  const int mine = busy ? min(t1, (wlast + kPpKeys - 1) / kPpKeys) : t0;  // the wave's tiles end here
   u32x4 qr[KK];
   {
     const T* qp = (const T*)p.q + (int64_t)(r.first + ri) * p.qt + (int64_t)(h * p.G + rg) * p.qh + 8 * hi;
@@ -381,8 +383,8 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
   }
   l = sum_x32(l);
   if (p.splits == 1) {
-    prompt_store<T, D>(p, r, row, h, hi, o, l, Q8 ? ref : 0.f);
-  } else {
+    prompt_store<T, DT>(p, r, row, h, hi, 0, o, l, Q8 ? ref : 0.f);
+  } else if (busy) {
     float* part = p.part + (((int64_t)blockIdx.x * p.splits + blockIdx.y) * W + w) * (DT * 16 + 3) * 64;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -397,40 +399,59 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
   }
 }
 
-// The splits' sums added up, a wave for 32 query rows.
+// The splits' sums added up: a workgroup for 32 query rows and 32 elements of
+// them, its four waves a quarter of the splits each, joined through LDS.
 template <typename T, int D>
-__global__ __launch_bounds__(64 * prompt_waves(D)) void paged_prompt_join_kernel(PagedPromptParams p) {
+__global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParams p) {
   constexpr int DT = D / 32, W = prompt_waves(D), kPpQ = 32 * W;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hi = lane >> 5, n = lane & 31;
-  const int N = p.c.n_seg;
-  const int seg = blockIdx.x % N, qblk = p.nqb - 1 - blockIdx.x / N;
+  __shared__ float sums[4][19][64];
+  const int lane = threadIdx.x & 63, k = threadIdx.x >> 6, hi = lane >> 5, n = lane & 31;
+  const int N = p.c.n_seg, block = blockIdx.x / (W * DT), w = blockIdx.x / DT % W, dt = blockIdx.x % DT;
+  const int seg = block % N, qblk = p.nqb - 1 - block / N;
   const PromptRows r = prompt_rows(p, seg, false);
   if (qblk * kPpQ + 32 * w >= r.rows) return;
   constexpr int64_t kPart = (DT * 16 + 3) * 64;
-  const float* part = p.part + ((int64_t)blockIdx.x * p.splits * W + w) * kPart;
-  f32x16 o[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
+  const float* part = p.part + ((int64_t)block * p.splits * W + w) * kPart;
+  f32x16 o = f32x16{};
   float m = kPgLowest, l = 0.f, ref = -100.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float* at = part + s * W * kPart;
-    const float pm = at[DT * 16 * 64 + lane], pl = at[DT * 16 * 64 + 64 + lane], pr = at[DT * 16 * 64 + 128 + lane];
+  auto add = [&](float pm, float pl, float pr, const f32x16& y) {
     const float mx = fmaxf(m, pm), most = fmaxf(ref, pr);
     const float f = __builtin_amdgcn_exp2f(m - mx), g = __builtin_amdgcn_exp2f(pm - mx);
     const float fo = f * __builtin_amdgcn_exp2f(ref - most), go = g * __builtin_amdgcn_exp2f(pr - most);
     l = l * f + pl * g;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 y = *gptr<f32x4>(at + ((dt * 4 + j) * 64 + lane) * 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[dt][4 * j + e] = o[dt][4 * j + e] * fo + y[e] * go;
-      }
+    for (int e = 0; e < 16; ++e) o[e] = o[e] * fo + y[e] * go;
     m = mx;
     ref = most;
+  };
+#pragma unroll 2
+  for (int s = k; s < p.splits; s += 4) {
+    const float* at = part + s * W * kPart;
+    f32x16 y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4 z = *gptr<f32x4>(at + ((dt * 4 + j) * 64 + lane) * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[4 * j + e] = z[e];
+    }
+    at += DT * 16 * 64 + lane;
+    add(gptr<float>(at)[0], gptr<float>(at)[64], gptr<float>(at)[128], y);
   }
-  prompt_store<T, D>(p, r, qblk * kPpQ + 32 * w + n, seg % p.t.hkv, hi, o, l, ref);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sums[k][e][lane] = o[e];
+  sums[k][16][lane] = m;
+  sums[k][17][lane] = l;
+  sums[k][18][lane] = ref;
+  __syncthreads();
+  if (k != 0) return;
+#pragma unroll 1
+  for (int i = 1; i < 4; ++i) {
+    f32x16 y;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) y[e] = sums[i][e][lane];
+    add(sums[i][16][lane], sums[i][17][lane], sums[i][18][lane], y);
+  }
+  prompt_store<T, 1>(p, r, qblk * kPpQ + 32 * w + n, seg % p.t.hkv, hi, dt, &o, l, ref);
 }
 
 // Splits: enough workgroups for two per CU, where the longest row has the tiles for it.
@@ -451,7 +472,7 @@ template <typename T, int D, bool Q8>
 static hipError_t launch_prompt_q(const PagedPromptParams& p, hipStream_t st) {
   const dim3 grid((unsigned)(p.c.n_seg * (int64_t)p.nqb), (unsigned)p.splits);
   hipLaunchKernelGGL((paged_prompt_kernel<T, D, Q8>), grid, dim3(64 * prompt_waves(D)), 0, st, p);
-  if (p.splits > 1) hipLaunchKernelGGL((paged_prompt_join_kernel<T, D>), dim3(grid.x), dim3(64 * prompt_waves(D)), 0, st, p);
+  if (p.splits > 1) hipLaunchKernelGGL((paged_prompt_join_kernel<T, D>), dim3(grid.x * prompt_waves(D) * (D / 32)), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 template <typename T>
@@ -495,7 +516,7 @@ extern "C" int wnw_paged_prompt_attn(const wnw_paged_cache* cache, const int32_t
     return paged_decode_launch(cache, seg_len, q, out, strides, p.t, group, scale, dtype, workspace, workspace_bytes, stream);
   WNW_CHECK_ARG(most * group < (1ll << 30), "too many query rows");
   const PromptPlan y = prompt_plan(N, group, most, p.c.capacity, D);
-  WNW_CHECK_ARG(N * y.nqb < (1ll << 31), "too many segments and tokens for one call");
+  WNW_CHECK_ARG(N * y.nqb < (1ll << 25), "too many segments and tokens for one call");
   WNW_CHECK_ARG(y.bytes == 0 || (workspace && workspace_bytes >= y.bytes), "workspace too small: %lld bytes, %lld needed",
                 (long long)workspace_bytes, (long long)y.bytes);
   WNW_CHECK_ARG((uintptr_t)workspace % 256 == 0, "the workspace must be 256-byte aligned");
