@@ -1,6 +1,8 @@
 // The paged K/V cache: what its append and its attention kernels share.
 #pragma once
 
+#include <type_traits>
+
 #include "wnw_common.h"
 
 namespace wnw {
@@ -23,7 +25,7 @@ struct PagedCache {
 
 // Checks a cache description and fills *out; WNW_OK or the status of the
 // refusal (wnw_last_error set).
-int paged_cache_of(const wnw_paged_cache* c, bool writes, PagedCache* out);
+int paged_cache_of(const wnw_paged_cache* c, PagedCache* out);
 
 // A token sequence of samples: cu_tokens, or one token per sample.
 struct PagedTokens {
@@ -101,6 +103,56 @@ struct HalfOps<f16_t> {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, v2));
   }
 };
+
+// Infinities and NaN among V's elements.  Where a product's columns do not all
+// see a row, its weight 0 does not take them out (0 times either is NaN): there
+// they are staged as zeros, and added to the sums of the columns that see them at
+// the end.  E: the page's element, uint8_t for e4m3 codes.
+//
+// All ones in the elements of w that are infinite or NaN
+template <typename E>
+__device__ __forceinline__ uint32_t odd_elems(uint32_t w) {
+  constexpr bool kCodes = std::is_same<E, uint8_t>::value;
+  constexpr uint32_t kMost = kCodes ? 0x7f7f7f7fu : std::is_same<E, bf16_t>::value ? 0x7f807f80u : 0x7c007c00u;
+  constexpr uint32_t kOne = kMost & ~(kMost << 1);  // the lowest bit of each field
+  const uint32_t top = ((w & kMost) + kOne) & (kCodes ? 0x80808080u : 0x80008000u);
+  return kCodes ? (top >> 7) * 0xffu : (top >> 15) * 0xffffu;
+}
+// Takes them out of x; whether there were any
+template <typename E>
+__device__ __forceinline__ bool take_odd(u32x4& x) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t m = odd_elems<E>(x[i]);
+    any |= m;
+    x[i] &= ~m;
+  }
+  return any != 0;
+}
+// Elements d .. d + 3 of a row in its page: those that are infinite or NaN, else zeros
+template <typename E>
+__device__ __forceinline__ f32x4 odd_quad(const uint8_t* row, int d) {
+  f32x4 y;
+  if constexpr (std::is_same<E, uint8_t>::value) {
+    const uint32_t m = odd_elems<E>(*gptr<uint32_t>(row + d));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = m >> (8 * e) & 1 ? __builtin_nanf("") : 0.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t w = gptr<uint32_t>(row + 2 * d)[i], x = w & odd_elems<E>(w);
+      y[2 * i] = std::is_same<E, bf16_t>::value ? bf16_lo(x) : f16_bits_to_f32(x & 0xffffu);
+      y[2 * i + 1] = std::is_same<E, bf16_t>::value ? bf16_hi(x) : f16_bits_to_f32(x >> 16);
+    }
+  }
+  return y;
+}
+// Row `row` of segment seg in V's pages; null where no page holds it
+__device__ __forceinline__ const uint8_t* paged_v_row(const PagedCache& c, int seg, int row, int row_bytes) {
+  const int page = c.table[seg * c.table_stride + (row >> c.shift)];
+  return (uint32_t)page < (uint32_t)c.n_pages ? c.v + page * c.v_stride + (row & ((1 << c.shift) - 1)) * row_bytes : nullptr;
+}
 
 // 8 codes (two words) as 8 elements of T
 template <typename T>

@@ -382,7 +382,7 @@ static hipError_t launch_append(const PagedAppendParams& p, int D, int64_t most,
   return hipGetLastError();
 }
 
-int paged_cache_of(const wnw_paged_cache* c, bool writes, PagedCache* out) {
+int paged_cache_of(const wnw_paged_cache* c, PagedCache* out) {
   WNW_CHECK_ARG(c != nullptr, "the cache description is null");
   WNW_CHECK_ARG(c->page_dtype == WNW_BF16 || c->page_dtype == WNW_F16 || c->page_dtype == WNW_E4M3, "bad page type %d",
                 c->page_dtype);
@@ -407,7 +407,6 @@ int paged_cache_of(const wnw_paged_cache* c, bool writes, PagedCache* out) {
     WNW_CHECK_ARG(c->n_pages == 0 || (c->k_scale && c->v_scale), "8-bit pages need k_scale and v_scale");
   else
     WNW_CHECK_ARG(!c->k_scale && !c->v_scale, "16-bit pages have no scales");
-  (void)writes;
   out->k = (uint8_t*)c->k_pages;
   out->v = (uint8_t*)c->v_pages;
   out->k_scale = c->k_scale;
@@ -435,7 +434,7 @@ extern "C" int wnw_paged_append(const wnw_paged_cache* cache, const int32_t* seg
                                 int64_t rot, const int32_t* sections, int n_sections, int interleaved, int dtype,
                                 void* stream) {
   PagedAppendParams p = {};
-  if (int rc = paged_cache_of(cache, true, &p.c)) return rc;
+  if (int rc = paged_cache_of(cache, &p.c)) return rc;
   const int64_t D = cache->head_dim, N = cache->n_seg;
   WNW_CHECK_ARG(dtype == WNW_BF16 || dtype == WNW_F16, "q, k and v must be bf16 or f16");
   WNW_CHECK_ARG(cache->page_dtype == WNW_E4M3 || cache->page_dtype == dtype, "16-bit pages must have the type of k and v");
@@ -446,7 +445,9 @@ extern "C" int wnw_paged_append(const wnw_paged_cache* cache, const int32_t* seg
   if (N == 0) return WNW_OK;
   WNW_CHECK_ARG(seg_len && new_len && strides, "null pointer argument");
   WNW_CHECK_ARG(n_tokens == 0 || (k && v), "k or v is null");
-  WNW_CHECK_ARG(seg_len != new_len, "new_len must not alias seg_len");
+  WNW_CHECK_ARG(seg_len + N <= new_len || new_len + N <= seg_len, "new_len must not overlap seg_len");
+  WNW_CHECK_ARG(cache->n_pages == 0 || (cache->k_pages != cache->v_pages && (!cache->k_scale || cache->k_scale != cache->v_scale)),
+                "K and V need pages and scales of their own");
   WNW_CHECK_ARG((q == nullptr) == (q_out == nullptr), "q and q_out come together");
   for (int i = 0; i < 6; ++i)
     WNW_CHECK_ARG(strides[i] >= 0 && strides[i] % 8 == 0 && strides[i] < (1ll << 40), "strides must be multiples of 8 elements");

@@ -235,6 +235,7 @@ __global__ __launch_bounds__((64 * PagedDecodeGeom<D, Q8>::kWaves),
 paged_decode_kernel(PagedDecodeParams p) {
   using Ge = PagedDecodeGeom<D, Q8>;
   using VT = typename std::conditional<Q8, bf16_t, T>::type;  // the value product's type: any scale fits bf16
+  using PE = typename std::conditional<Q8, uint8_t, T>::type;  // the pages' elements
   using QO = HalfOps<T>;
   using VO = HalfOps<VT>;
   using Vl = PagedDecodeV<D, Q8>;
@@ -269,7 +270,7 @@ paged_decode_kernel(PagedDecodeParams p) {
     at = scan(num);
     S = __builtin_amdgcn_readlane(at, 63);
     at -= num;
-    longest = (int)wave_max((float)num);  // steps are below 2^25: exact
+    longest = (int)wave_max((float)num);  // as good as exact: it is compared with kPdWhole
   } else {
     int most = 0;
     for (int s = sa; s < sb; ++s) {
@@ -400,6 +401,7 @@ paged_decode_kernel(PagedDecodeParams p) {
         }
       };
       u32x4 kr[2][KC], vr[VI];
+      int odd = 0;  // V had infinities or NaN where not every column sees its row
       int bad = 0;  // halves of the loaded step that no page holds
       auto load = [&](int k) {
         const int from = 2 * (k & 31);
@@ -465,6 +467,13 @@ paged_decode_kernel(PagedDecodeParams p) {
           for (int i = 0; i < VI; ++i) {
             const int rr = (i * 1024 + lane * 16) / RB;
             if (row0 + rr >= n || (bad_now >> (rr >> 4) & 1)) vr[i] = u32x4{0, 0, 0, 0};
+          }
+          if (row0 + kPdStep > all_see && r.count > 1) {
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < VI; ++i)
+              if (row0 + (i * 1024 + lane * 16) / RB >= all_see) any |= take_odd<PE>(vr[i]);
+            if (__ballot(any)) odd = 1;
           }
 #pragma unroll
           for (int t2 = 0; t2 < 2; ++t2)
@@ -533,6 +542,19 @@ paged_decode_kernel(PagedDecodeParams p) {
           acc[i] = VO::mma16(v, lo, acc[i]);
         }
         __builtin_amdgcn_wave_barrier();
+      }
+      if (odd) {
+#pragma unroll 1
+        for (int row = max(all_see, 0); row < n; ++row) {
+          const int step = row / kPdStep - a;  // nw apart in the wave
+          const uint8_t* from = step >= 0 && step % nw == 0 && row / kPdStep < b ? paged_v_row(p.c, seg, row, RB) : nullptr;
+          if (!from || row >= limit) continue;
+#pragma unroll
+          for (int i = 0; i < DT; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            acc[i] += odd_quad<PE>(from, 16 * i + 4 * lq);
+          }
+        }
       }
       l = sum_x32(sum_x16(l));
       const int oq = here(lane) >> 4, oc = here(lane) & 15;
@@ -679,7 +701,7 @@ int paged_decode_launch(const wnw_paged_cache* cache, const int32_t* seg_len, co
                         const PagedTokens& t, int64_t group, float scale, int dtype, void* workspace, int64_t bytes,
                         void* stream) {
   PagedDecodeParams p = {};
-  if (int rc = paged_cache_of(cache, false, &p.c)) return rc;
+  if (int rc = paged_cache_of(cache, &p.c)) return rc;
   const int64_t N = cache->n_seg, D = cache->head_dim, cols = group * t.most;
   const PagedDecodeLayout y = decode_layout(N, cols, D);
   WNW_CHECK_ARG(workspace && bytes >= y.total, "workspace too small: %lld bytes, %lld needed", (long long)bytes,

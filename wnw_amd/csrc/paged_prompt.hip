@@ -97,6 +97,7 @@ __device__ __forceinline__ void prompt_store(const PagedPromptParams& p, const P
 template <typename T, int D, bool Q8>
 __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void paged_prompt_kernel(PagedPromptParams p) {
   using Ops = HalfOps<T>;
+  using PE = typename std::conditional<Q8, uint8_t, T>::type;  // the pages' elements
   constexpr int W = prompt_waves(D), kPpQ = 32 * W;
   constexpr int RB = D * 2, CH = RB / 16, TB = kPpKeys * RB;  // a tile in LDS: 16-bit elements
   constexpr int GB = D * (Q8 ? 1 : 2);                        // bytes of a row in its page
@@ -106,7 +107,7 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
   // f16 weights are held times 2^8: normal numbers down to 2^-22 of the largest
   constexpr float kBias = std::is_same<T, f16_t>::value ? 8.f : 0.f;
   __shared__ __attribute__((aligned(16))) uint8_t lds[NB * 2 * TB];  // [NB][K, V]
-  __shared__ float scales[2][kPpKeys / 16][2];
+  __shared__ int odd;  // V had infinities or NaN in such a tile
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hi = lane >> 5, n = lane & 31;
   const int N = p.c.n_seg;
@@ -118,10 +119,10 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
   const int row = qblk * kPpQ + 32 * w + n;
   const int ri = min(row, r.rows - 1) / p.G, rg = min(row, r.rows - 1) - ri * p.G;
   const int limit = base + ri;
-  // of the wave: rows its first and last query see; of the workgroup: its last
+  // rows that the first and the last query see: of the wave, of the workgroup
   const int wfirst = base + min(qblk * kPpQ + 32 * w, r.rows - 1) / p.G;
   const int wlast = base + min(qblk * kPpQ + 32 * w + 31, r.rows - 1) / p.G;
-  const int last = base + min(qblk * kPpQ + kPpQ - 1, r.rows - 1) / p.G;
+  const int first = base + qblk * kPpQ / p.G, last = base + min(qblk * kPpQ + kPpQ - 1, r.rows - 1) / p.G;
   const int tiles = max((last + kPpKeys - 1) / kPpKeys, 0);
   const int t0 = (int)((int64_t)tiles * blockIdx.y / p.splits), t1 = (int)((int64_t)tiles * (blockIdx.y + 1) / p.splits);
   const bool busy = qblk * kPpQ + 32 * w < r.rows;  // a wave without rows only moves tiles
@@ -213,6 +214,14 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
       if (gone[u] < 0) kr[u] = u32x4{0, 0, 0, 0};
       if (gone[u] < 0 || tile * kPpKeys + u * RPL + srow >= r.len) vr[u] = u32x4{0, 0, 0, 0};
     }
+  };
+  // takes infinities and NaN out of the V of a tile that not every row of the workgroup sees whole
+  auto even = [&](int tile) {
+    if ((tile + 1) * kPpKeys <= first) return;
+    bool any = false;
+#pragma unroll
+    for (int u = 0; u < NI; ++u) any |= take_odd<PE>(vr[u]);
+    if (any) odd = 1;
   };
   auto put = [&](int tile) {
     uint8_t* kt = lds + (NB == 2 ? (tile & 1) * 2 * TB : 0);
@@ -337,6 +346,8 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
       }
   };
   if (t0 < t1) {
+    if (tid == 0) odd = 0;
+    __syncthreads();
     find(t0 / kWin);
     find_scales();
     if (t0 % kWin != 0) enter(t0 / kWin);
@@ -344,6 +355,7 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
     if (t0 % kWin >= kWin / 2) find_scales();
     if constexpr (NB == 2) {
       clear(t0);
+      even(t0);
       put(t0);
     }
     if (Q8) enter_scales();
@@ -355,8 +367,10 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
       __syncthreads();  // everyone is done with tile i - 1; with two buffers tile i is in LDS
       if constexpr (NB == 2) {
         clear(i + 1);
+        even(i + 1);
       } else {
         clear(i);
+        even(i);
         put(i);
         fetch(i + 1);
         __syncthreads();
@@ -380,6 +394,23 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
       }
     }
     if (wrong) raise_device_error(p.err, WNW_DEVERR_BOUNDS);
+    if (odd) {  // what even() took out, to the rows that see it (the wave's tiles are behind a barrier)
+      const int from = max(t0, max(first, 0) / kPpKeys) * kPpKeys, to = min(t1 * kPpKeys, wlast);
+#pragma unroll 1
+      for (int key = from; key < to; ++key) {
+        const uint8_t* at = paged_v_row(p.c, seg, key, GB);
+        if (!at || key >= limit) continue;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            __builtin_amdgcn_sched_barrier(0);
+            const f32x4 x = odd_quad<PE>(at, 32 * dt + 8 * j + 4 * hi);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[dt][4 * j + e] += x[e];
+          }
+      }
+    }
   }
   l = sum_x32(l);
   if (p.splits == 1) {
@@ -491,7 +522,7 @@ using namespace wnw;
 extern "C" int64_t wnw_paged_prompt_workspace_bytes(const wnw_paged_cache* cache, int64_t group, int64_t max_tokens) {
   PagedCache c;
   if (!cache || group < 1 || group > 1024 || max_tokens < 0 || max_tokens >= (1 << 24)) return -1;
-  if (paged_cache_of(cache, false, &c)) return -1;
+  if (paged_cache_of(cache, &c)) return -1;
   if (max_tokens == 0) return 0;
   if (max_tokens * group <= kFewRows) return wnw_paged_decode_workspace_bytes(cache->n_seg, max_tokens * group, cache->head_dim);
   return prompt_plan(cache->n_seg, group, max_tokens, c.capacity, cache->head_dim).bytes;
@@ -502,13 +533,19 @@ extern "C" int wnw_paged_prompt_attn(const wnw_paged_cache* cache, const int32_t
                                      const int32_t* cu_tokens, int64_t max_tokens, float scale, int dtype, void* workspace,
                                      int64_t workspace_bytes, void* stream) {
   PagedPromptParams p = {};
-  if (int rc = paged_cache_of(cache, false, &p.c)) return rc;
+  if (int rc = paged_cache_of(cache, &p.c)) return rc;
   const int64_t N = cache->n_seg, D = cache->head_dim;
   WNW_CHECK_ARG(n_samples >= 0 && (n_samples > 0 ? N % n_samples == 0 : N == 0), "segments must be samples x KV heads");
   WNW_CHECK_ARG(n_tokens >= 0 && n_tokens < (1 << 24) && max_tokens >= 0, "bad token counts");
   if (N == 0 || n_tokens == 0) return WNW_OK;
   WNW_CHECK_ARG(cu_tokens, "cu_tokens is null");
   if (int rc = paged_attn_check(cache, seg_len, q, out, strides, group, scale, dtype)) return rc;
+  {
+    const int64_t heads = N / n_samples * group, t = strides[2], h = strides[3];
+    const bool apart = t >= h ? (heads == 1 || h >= D) && (n_tokens == 1 || t >= h * (heads - 1) + D)
+                              : (n_tokens == 1 || t >= D) && (heads == 1 || h >= t * (n_tokens - 1) + D);
+    WNW_CHECK_ARG(apart, "the rows of out overlap");
+  }
   const int64_t most = std::min(max_tokens, n_tokens);
   WNW_CHECK_ARG(most > 0, "max_tokens is zero");
   p.t = PagedTokens{cu_tokens, (int32_t)n_tokens, (int32_t)(N / n_samples), (int32_t)most};
