@@ -95,7 +95,7 @@ __device__ __forceinline__ void prompt_store(const PagedPromptParams& p, const P
 }
 
 template <typename T, int D, bool Q8>
-__global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void paged_prompt_kernel(PagedPromptParams p) {
+__global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 && !Q8 ? 1 : 2)) void paged_prompt_kernel(PagedPromptParams p) {
   using Ops = HalfOps<T>;
   using PE = typename std::conditional<Q8, uint8_t, T>::type;  // the pages' elements
   constexpr int W = prompt_waves(D), kPpQ = 32 * W;
@@ -104,6 +104,7 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
   constexpr int NI = kPpKeys * GB / (1024 * W);                     // 16-byte loads per thread and tensor
   constexpr int KK = D / 16, DT = D / 32;
   constexpr int NB = D == 256 ? 1 : 2;  // tiles in LDS
+  constexpr bool kAhead = D != 256 || !Q8;  // the next tile's loads are on their way during the products
   // f16 weights are held times 2^8: normal numbers down to 2^-22 of the largest
   constexpr float kBias = std::is_same<T, f16_t>::value ? 8.f : 0.f;
   __shared__ __attribute__((aligned(16))) uint8_t lds[NB * 2 * TB];  // [NB][K, V]
@@ -246,15 +247,13 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
       }
     }
   };
-  // lane offsets of the operands inside a tile
-  uint32_t koff[KK], voff[DT];
-#pragma unroll
-  for (int kk = 0; kk < KK; ++kk) koff[kk] = n * RB + (((2 * kk + hi) ^ (n % CH)) * 16);
+  // The lane's operands inside a tile: K's chunks 2 kk + hi of row n, V's chunks
+  // 4 dt .. + 3; the swizzle leaves kk and dt to a XOR, which head_dim 256, short
+  // of registers, does at each read.
+  uint32_t kget = n * RB + ((hi ^ (n % CH)) * 16), vget;
   {
     const int lc = lane & 15, dsub = (lane >> 4) & 1;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-      voff[dt] = (4 * hi + (lc >> 2)) * RB + (((4 * dt + 2 * dsub + ((lc & 3) >> 1)) ^ (2 * (lc >> 2))) * 16) + (lc & 1) * 8;
+    vget = (4 * hi + (lc >> 2)) * RB + (((2 * dsub + ((lc & 3) >> 1)) ^ (2 * (lc >> 2))) * 16) + (lc & 1) * 8;
   }
   f32x16 o[DT];
 #pragma unroll
@@ -277,13 +276,17 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
   auto tile = [&](int i, auto masked) {
     const uint8_t* kt = lds + (NB == 2 ? (i & 1) * 2 * TB : 0);
     const uint8_t* vt = kt + TB;
+    if (D == 256) {
+      kget = here(kget);
+      vget = here(vget);
+    }
     f32x16 s[2];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) s[mt] = f32x16{};
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) s[mt] = mma32<T>(*(const u32x4*)(kt + koff[kk] + mt * 32 * RB), qr[kk], s[mt]);
+      for (int mt = 0; mt < 2; ++mt) s[mt] = mma32<T>(*(const u32x4*)(kt + (kget ^ 32 * kk) + mt * 32 * RB), qr[kk], s[mt]);
     if constexpr (NB == 2) {  // among the products: the next tile into the other buffer, the one after it on its way
       put(i + 1);
       fetch(i + 2);
@@ -340,8 +343,8 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
     for (int b = 0; b < 4; ++b)
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const uint64_t v0 = Ops::read_tr(vt + voff[dt] + 16 * b * RB);
-        const uint64_t v1 = Ops::read_tr(vt + voff[dt] + (16 * b + 8) * RB);
+        const uint64_t v0 = Ops::read_tr(vt + (vget ^ 64 * dt) + 16 * b * RB);
+        const uint64_t v1 = Ops::read_tr(vt + (vget ^ 64 * dt) + (16 * b + 8) * RB);
         o[dt] = mma32<T>(u32x4{(uint32_t)v0, (uint32_t)(v0 >> 32), (uint32_t)v1, (uint32_t)(v1 >> 32)}, pb[b], o[dt]);
       }
   };
@@ -351,19 +354,20 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
     find(t0 / kWin);
     find_scales();
     if (t0 % kWin != 0) enter(t0 / kWin);
-    fetch(t0);
+    if (kAhead) fetch(t0);
     if (t0 % kWin >= kWin / 2) find_scales();
     if constexpr (NB == 2) {
       clear(t0);
       even(t0);
       put(t0);
     }
-    if (Q8) enter_scales();
+    if (Q8 && kAhead) enter_scales();
     if constexpr (NB == 2) fetch(t0 + 1);
     // (the tile after next is fetched while a tile is used, or the next one with
     // one buffer: the window of the products follows that of fetch() by as much)
     auto turn = [&](int i) {
-      if (Q8 && i % kWin == 0 && i > t0) enter_scales();
+      if (!kAhead) fetch(i);
+      if (Q8 && (kAhead ? i % kWin == 0 && i > t0 : i % kWin == 0 || i == t0)) enter_scales();
       __syncthreads();  // everyone is done with tile i - 1; with two buffers tile i is in LDS
       if constexpr (NB == 2) {
         clear(i + 1);
@@ -372,7 +376,7 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 ? 1 : 2)) void pa
         clear(i);
         even(i);
         put(i);
-        fetch(i + 1);
+        if (kAhead) fetch(i + 1);
         __syncthreads();
       }
     };
