@@ -4,20 +4,32 @@
 // Mathematics: as decode attention, causal: token i of a sample's n sees the
 // segment's first len - n + i + 1 rows.
 //
-// A workgroup takes 128 query rows of one segment, a row being (token, head of
-// the group): the group shares the keys.  A wave has 32 of them and walks the
-// 64-key tiles up to its last row's:
+// A workgroup takes 128 or 256 query rows of one segment, a row being (token,
+// head of the group): the group shares the keys.  A wave has 32 of them and
+// walks the 64-key tiles up to its last row's:
 //   S^T (64 keys x 32 queries) = K Q^T, Q in registers, K from LDS;
-//   O^T (D x 32) += V^T P^T, the weights in 16 bits (the largest is near 1),
-//       their sum in 32, V^T by transposed LDS reads in S^T's own order.
+//   O^T (D x 32) += V^T P^T, the weights in 16 bits (f16's held times 2^8), their
+//       sum in 32, V^T by transposed LDS reads in S^T's own order.
+// The weights are relative to the running maximum itself: one that trails it by
+// a bounded factor saved the rescaling of O (2 %), but its weights above 1 cost a
+// quarter more of the 16-bit rounding.
 // The tiles go through registers into LDS, where 8-bit codes become 16-bit
-// elements once for all four waves; one barrier per tile, the loads two tiles
-// ahead.  K's page scale multiplies the exponent, V's is added to it as its
-// logarithm relative to the largest so far (a part of 2^x either way), so that
-// scales cost a few instructions per 16 keys and any scale fits 16 bits.
+// elements once for all waves; one barrier per tile, the next tile written among
+// the products of S and the one after it loaded then (head_dim 256: one buffer,
+// two barriers).  K's page scale multiplies the exponent, V's is added to it as
+// its logarithm relative to the largest so far (a part of 2^x either way), so
+// that scales cost a few instructions per 16 keys and any scale fits 16 bits.
 //
-// Few query rows and many keys: the tiles of each workgroup are cut into
+// Few query rows and many keys: the tiles of each block of rows are cut into
 // splits, whose sums a second launch adds up.
+//
+// What bounds it: per tile and SIMD the matrix products (2 x 1,024 cycles for two
+// waves at head_dim 128), the exponentials and the LDS reads (each of 8 waves
+// reads the tile) come to the same 0.85 us each, and a wave's turn is these one
+// after another; about half overlaps.  The large products run at 0.86 PFLOP/s
+// (8,192-sized plain bf16 ones: 1.2).  Tried without gain: the next tile's
+// scores computed among the softmax (2 to 5 % slower: registers), loads two
+// tiles ahead, raised wave priority in the products.
 #include <algorithm>
 #include <type_traits>
 
@@ -40,14 +52,12 @@ struct PagedPromptParams {
   const void* q;
   void* out;
   int64_t qt, qh, ot, oh;  // strides in elements
-  float* part;             // [grid.x, splits, 4 waves]: D / 32 x 16 sums a lane, then max, sum, scale
+  float* part;             // [blocks, splits, waves]: D / 32 x 16 sums a lane, then max, sum, scale
   float scale_log2;
   int32_t G, nqb, splits;
   int32_t* err;
 };
 
-// waves of a workgroup, each with 32 query rows
-__host__ __device__ constexpr int prompt_waves(int D) { return D == 128 ? 8 : 4; }
 static constexpr int kPpKeys = 64;  // keys of a tile
 
 template <typename T>
@@ -94,11 +104,11 @@ __device__ __forceinline__ void prompt_store(const PagedPromptParams& p, const P
     }
 }
 
-template <typename T, int D, bool Q8>
-__global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 && !Q8 ? 1 : 2)) void paged_prompt_kernel(PagedPromptParams p) {
+template <typename T, int D, bool Q8, int W>
+__global__ __launch_bounds__((64 * W), (D == 256 && !Q8 ? 1 : 2)) void paged_prompt_kernel(PagedPromptParams p) {
   using Ops = HalfOps<T>;
   using PE = typename std::conditional<Q8, uint8_t, T>::type;  // the pages' elements
-  constexpr int W = prompt_waves(D), kPpQ = 32 * W;
+  constexpr int kPpQ = 32 * W;
   constexpr int RB = D * 2, CH = RB / 16, TB = kPpKeys * RB;  // a tile in LDS: 16-bit elements
   constexpr int GB = D * (Q8 ? 1 : 2);                        // bytes of a row in its page
   constexpr int NI = kPpKeys * GB / (1024 * W);                     // 16-byte loads per thread and tensor
@@ -112,8 +122,10 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 && !Q8 ? 1 : 2)) 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hi = lane >> 5, n = lane & 31;
   const int N = p.c.n_seg;
-  const int seg = blockIdx.x % N, qblk = p.nqb - 1 - blockIdx.x / N;  // the longest first; a segment's keys in one L2
-  const PromptRows r = prompt_rows(p, seg, tid == 0 && qblk == 0 && blockIdx.y == 0);
+  // the blocks with the most tiles first; workgroups of one segment N apart (8 segments: each in one L2)
+  const int seg = blockIdx.x % N, rank = blockIdx.x / N;
+  const int block = rank / p.splits, split = rank - block * p.splits, qblk = p.nqb - 1 - block;
+  const PromptRows r = prompt_rows(p, seg, tid == 0 && qblk == 0 && split == 0);
   if (qblk * kPpQ >= r.rows) return;
   const int h = seg % p.t.hkv;
   const int base = r.len - r.count + 1;  // token i sees base + i rows
@@ -125,7 +137,7 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 && !Q8 ? 1 : 2)) 
   const int wlast = base + min(qblk * kPpQ + 32 * w + 31, r.rows - 1) / p.G;
   const int first = base + qblk * kPpQ / p.G, last = base + min(qblk * kPpQ + kPpQ - 1, r.rows - 1) / p.G;
   const int tiles = max((last + kPpKeys - 1) / kPpKeys, 0);
-  const int t0 = (int)((int64_t)tiles * blockIdx.y / p.splits), t1 = (int)((int64_t)tiles * (blockIdx.y + 1) / p.splits);
+  const int t0 = (int)((int64_t)tiles * split / p.splits), t1 = (int)((int64_t)tiles * (split + 1) / p.splits);
   const bool busy = qblk * kPpQ + 32 * w < r.rows;  // a wave without rows only moves tiles
   const int mine = busy ? min(t1, (wlast + kPpKeys - 1) / kPpKeys) : t0;  // the wave's tiles end here
   u32x4 qr[KK];
@@ -420,7 +432,7 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 && !Q8 ? 1 : 2)) 
   if (p.splits == 1) {
     prompt_store<T, DT>(p, r, row, h, hi, 0, o, l, Q8 ? ref : 0.f);
   } else if (busy) {
-    float* part = p.part + (((int64_t)blockIdx.x * p.splits + blockIdx.y) * W + w) * (DT * 16 + 3) * 64;
+    float* part = p.part + ((((int64_t)block * N + seg) * p.splits + split) * W + w) * (DT * 16 + 3) * 64;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -436,9 +448,9 @@ __global__ __launch_bounds__((64 * prompt_waves(D)), (D == 256 && !Q8 ? 1 : 2)) 
 
 // The splits' sums added up: a workgroup for 32 query rows and 32 elements of
 // them, its four waves a quarter of the splits each, joined through LDS.
-template <typename T, int D>
+template <typename T, int D, int W>
 __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParams p) {
-  constexpr int DT = D / 32, W = prompt_waves(D), kPpQ = 32 * W;
+  constexpr int DT = D / 32, kPpQ = 32 * W;
   __shared__ float sums[4][19][64];
   const int lane = threadIdx.x & 63, k = threadIdx.x >> 6, hi = lane >> 5, n = lane & 31;
   const int N = p.c.n_seg, block = blockIdx.x / (W * DT), w = blockIdx.x / DT % W, dt = blockIdx.x % DT;
@@ -489,32 +501,50 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParam
   prompt_store<T, 1>(p, r, qblk * kPpQ + 32 * w + n, seg % p.t.hkv, hi, dt, &o, l, ref);
 }
 
-// Splits: enough workgroups for two per CU, where the longest row has the tiles for it.
+// How a call is cut, from what the host knows of it (us measured on one GPU, bf16
+// queries in 8 KV heads of 4, 8-bit pages).
+//
+// Waves of a workgroup, 32 query rows each.  head_dim 128 takes 8: K and V go
+// through LDS once for 256 rows (1,024 tokens after 4,000 rows: 108 us, with 4
+// waves 112; 3,500 tokens: 128 and 136).  But where such workgroups would be one
+// per CU at most and the rows mainly the call's own tokens, so that the last
+// tokens' workgroup sets the time, smaller ones are shorter (2,048 tokens: 79 us,
+// with 4 waves 67; 1,500: 56 and 49; 300: 19 and 16).  head_dim 64 and 256 keep 4:
+// registers and LDS for two or more workgroups per CU.
+//
+// Splits of a block's tiles: as many workgroups as the CUs hold, of at least 4
+// tiles each (64 tokens after 8,000 rows, 126 tiles: 32 us; with 8 tiles 38, with 32 tiles 91), where that
+// takes away 8 tiles or more: the second launch costs as much as 5 to 8 (700
+// tokens, 11 tiles: 25 us, cut in two 31).
 struct PromptPlan {
-  int64_t nqb, splits, bytes;
+  int64_t waves, nqb, splits, bytes;
 };
 static PromptPlan prompt_plan(int64_t n_seg, int64_t group, int64_t max_tokens, int64_t capacity, int64_t D) {
   PromptPlan y;
-  const int W = prompt_waves((int)D), kPpQ = 32 * W;
-  y.nqb = (max_tokens * group + kPpQ - 1) / kPpQ;
-  const int64_t wgs = std::max<int64_t>(n_seg * y.nqb, 1), want = (W == 8 ? 1ll : 2ll) * device_cus(), tiles = (capacity + kPpKeys - 1) / kPpKeys;
+  const int64_t rows = max_tokens * group, cus = device_cus(), tiles = (capacity + kPpKeys - 1) / kPpKeys;
+  const bool own = n_seg * ((rows + 255) / 256) <= cus && 2 * max_tokens >= capacity;
+  y.waves = D == 128 && !own ? 8 : 4;
+  y.nqb = (rows + 32 * y.waves - 1) / (32 * y.waves);
+  const int64_t wgs = std::max<int64_t>(n_seg * y.nqb, 1), want = (y.waves == 8 ? 1 : 2) * cus;
   y.splits = std::max<int64_t>(1, std::min({want / wgs, tiles / 4, (int64_t)64}));
-  y.bytes = y.splits == 1 ? 0 : wgs * y.splits * W * (D / 2 + 3) * 64 * 4;
+  if (tiles - tiles / y.splits < 8) y.splits = 1;
+  y.bytes = y.splits == 1 ? 0 : wgs * y.splits * y.waves * (D / 2 + 3) * 64 * 4;
   return y;
 }
 
-template <typename T, int D, bool Q8>
+template <typename T, int D, bool Q8, int W>
 static hipError_t launch_prompt_q(const PagedPromptParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.c.n_seg * (int64_t)p.nqb), (unsigned)p.splits);
-  hipLaunchKernelGGL((paged_prompt_kernel<T, D, Q8>), grid, dim3(64 * prompt_waves(D)), 0, st, p);
-  if (p.splits > 1) hipLaunchKernelGGL((paged_prompt_join_kernel<T, D>), dim3(grid.x * prompt_waves(D) * (D / 32)), dim3(256), 0, st, p);
+  const unsigned blocks = (unsigned)(p.c.n_seg * (int64_t)p.nqb);
+  hipLaunchKernelGGL((paged_prompt_kernel<T, D, Q8, W>), dim3(blocks * p.splits), dim3(64 * W), 0, st, p);
+  if (p.splits > 1) hipLaunchKernelGGL((paged_prompt_join_kernel<T, D, W>), dim3(blocks * W * (D / 32)), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 template <typename T>
-static hipError_t launch_prompt(const PagedPromptParams& p, int64_t D, bool q8, hipStream_t st) {
-  if (D == 64) return q8 ? launch_prompt_q<T, 64, true>(p, st) : launch_prompt_q<T, 64, false>(p, st);
-  if (D == 128) return q8 ? launch_prompt_q<T, 128, true>(p, st) : launch_prompt_q<T, 128, false>(p, st);
-  return q8 ? launch_prompt_q<T, 256, true>(p, st) : launch_prompt_q<T, 256, false>(p, st);
+static hipError_t launch_prompt(const PagedPromptParams& p, int64_t D, bool q8, int64_t waves, hipStream_t st) {
+  if (D == 64) return q8 ? launch_prompt_q<T, 64, true, 4>(p, st) : launch_prompt_q<T, 64, false, 4>(p, st);
+  if (D == 256) return q8 ? launch_prompt_q<T, 256, true, 4>(p, st) : launch_prompt_q<T, 256, false, 4>(p, st);
+  if (waves == 8) return q8 ? launch_prompt_q<T, 128, true, 8>(p, st) : launch_prompt_q<T, 128, false, 8>(p, st);
+  return q8 ? launch_prompt_q<T, 128, true, 4>(p, st) : launch_prompt_q<T, 128, false, 4>(p, st);
 }
 
 static constexpr int kFewRows = 16;  // query rows of a segment that decode attention takes
@@ -540,7 +570,7 @@ extern "C" int wnw_paged_prompt_attn(const wnw_paged_cache* cache, const int32_t
   if (int rc = paged_cache_of(cache, &p.c)) return rc;
   const int64_t N = cache->n_seg, D = cache->head_dim;
   WNW_CHECK_ARG(n_samples >= 0 && (n_samples > 0 ? N % n_samples == 0 : N == 0), "segments must be samples x KV heads");
-  WNW_CHECK_ARG(n_tokens >= 0 && n_tokens < (1 << 24) && max_tokens >= 0, "bad token counts");
+  WNW_CHECK_ARG(n_tokens >= 0 && n_tokens < (1 << 24) && max_tokens >= 0 && max_tokens < (1 << 24), "bad token counts");
   if (N == 0 || n_tokens == 0) return WNW_OK;
   WNW_CHECK_ARG(cu_tokens, "cu_tokens is null");
   if (int rc = paged_attn_check(cache, seg_len, q, out, strides, group, scale, dtype)) return rc;
@@ -550,7 +580,7 @@ extern "C" int wnw_paged_prompt_attn(const wnw_paged_cache* cache, const int32_t
                               : (n_tokens == 1 || t >= D) && (heads == 1 || h >= t * (n_tokens - 1) + D);
     WNW_CHECK_ARG(apart, "the rows of out overlap");
   }
-  const int64_t most = std::min(max_tokens, n_tokens);
+  const int64_t most = max_tokens;  // as the workspace's size was asked for
   WNW_CHECK_ARG(most > 0, "max_tokens is zero");
   p.t = PagedTokens{cu_tokens, (int32_t)n_tokens, (int32_t)(N / n_samples), (int32_t)most};
   if (most * group <= kFewRows)
@@ -571,8 +601,8 @@ extern "C" int wnw_paged_prompt_attn(const wnw_paged_cache* cache, const int32_t
   p.nqb = (int32_t)y.nqb;
   p.splits = (int32_t)y.splits;
   p.err = device_error_word();
-  const hipError_t e = dtype == WNW_BF16 ? launch_prompt<bf16_t>(p, D, cache->page_dtype == WNW_E4M3, (hipStream_t)stream)
-                                         : launch_prompt<f16_t>(p, D, cache->page_dtype == WNW_E4M3, (hipStream_t)stream);
+  const hipError_t e = dtype == WNW_BF16 ? launch_prompt<bf16_t>(p, D, cache->page_dtype == WNW_E4M3, y.waves, (hipStream_t)stream)
+                                         : launch_prompt<f16_t>(p, D, cache->page_dtype == WNW_E4M3, y.waves, (hipStream_t)stream);
   WNW_CHECK_HIP(e, "paged prompt attention launch");
   return WNW_OK;
 }
