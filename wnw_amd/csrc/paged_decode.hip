@@ -47,8 +47,17 @@ struct PagedDecodeParams {
 };
 
 static constexpr int kPdStep = 32;  // rows of a step
-static constexpr int kPdMin = 8;     // steps of a workgroup at least
-static constexpr int kPdWhole = 40;  // steps of a segment that is not cut
+// Where segments are cut.  More workgroups have fewer steps each, but whoever adds
+// up a segment's pieces reads as many partial sums, one round trip to memory for 8.
+// A workgroup has kPdMin steps at least (8 sequences of 2 x 7,564 and 6 x 512 rows:
+// 18.7 us; with 4: 18.9, 12: 20.0, 16: 20.9), a segment about kPdPieces pieces at
+// most, or half as many of 2,048 sums or more (30,000 rows of 2 heads: 4 query
+// heads 20.9 us with 117 pieces, 19.1 with 58, 20.2 with 39; 16 query heads 31.4,
+// 24.3, 22.5), and segments of up to kPdWhole steps stay whole (26 steps: 11.2 us,
+// cut 12.4).
+static constexpr int kPdMin = 8;
+static constexpr int kPdPieces = 64;
+static constexpr int kPdWhole = 40;
 
 template <int D, bool Q8>
 struct PagedDecodeGeom {
@@ -296,10 +305,11 @@ paged_decode_kernel(PagedDecodeParams p) {
     __syncthreads();
   }
   longest = __builtin_amdgcn_readfirstlane(longest);
-  // Short segments are not cut (a workgroup takes whole ones): what adds up the
-  // pieces of a cut one costs as much as the steps of kPdWhole.
+  // Short segments are not cut (a workgroup takes whole ones), others not into pieces
+  // of less than `least` steps.
   const bool uncut = longest <= kPdWhole;
-  const int total = uncut ? N : S, P = min((int)gridDim.x, uncut ? N : max(S / kPdMin, 1));
+  const int least = max(kPdMin, longest / (p.cols * D >= 2048 ? kPdPieces / 2 : kPdPieces));
+  const int total = uncut ? N : S, P = min((int)gridDim.x, uncut ? N : max(S / least, 1));
   const int share = total / P, more = total - share * P;  // the first `more` workgroups take one more
   auto start_of = [&](int i) { return i * share + min(i, more); };
   auto owner_of = [&](int x) {  // the workgroup that has step x
