@@ -3,11 +3,16 @@
 // Mathematics.  Pair j of a head (j < rot / 2; elements (j, j + rot / 2), or
 // (2 j, 2 j + 1) interleaved) at position x of its axis turns by the angle
 // x * inv_freq[j]: (a, b) -> (a cos - b sin, b cos + a sin).  The angle is a
-// product in 64 bits, reduced to an eighth of a turn there: at position 10^5 a
-// 32-bit product is off by 2^-8 of a radian.  Sine and cosine of what is left are
-// their Taylor series in 32 bits (|x| <= pi / 4; the terms left out are below
-// 2 * 10^-9 and 3 * 10^-10).  All else is 32-bit, rounded once where a value is
-// stored.
+// product in 64 bits, in quarter turns, and the whole ones are taken off there:
+// at position 10^5 a 32-bit product is off by 2^-8 of a radian.  Sine and cosine
+// of what is left are their Taylor series in 32 bits (|x| <= pi / 4; the terms
+// left out, x^11 / 11! and x^12 / 12!, are below 2 * 10^-9 and 2 * 10^-10).  All
+// else is 32-bit, rounded once where a value is stored.
+//
+// What bounds it: memory.  A prompt of 4,564 tokens (40 q and K / V heads of 128
+// into 8 bits, 103 MB) takes 21.8 us, 4.7 TB/s, a large copy 5.1.  One token
+// takes 4.3 us, most of it the launch and one chain of dependent loads: length,
+// table entry, position, row.
 //
 // 8-bit pages hold e4m3 codes under one scale per page, the least power of two
 // 2^e (e >= -64) with |x| <= 448 * 2^e for all its rows.  e4m3 has the same
@@ -34,7 +39,7 @@ struct PagedAppendParams {
   const void* pos;         // [axes, tokens] int64 or int32; null: no rotation
   const void* inv_freq;    // [rot / 2] double or float
   int64_t pos_axis;        // elements from one axis to the next
-  int32_t pos64, freq64, interleaved, rot, G, units;
+  int32_t pos64, freq64, interleaved, rot, G, units, unit_shift;
   int32_t sec1, sec2, sec3;  // first pair of the second, third and fourth axis
   int32_t* err;
 };
@@ -117,7 +122,9 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 
 // A workgroup takes one unit: the rows of one append that fall into one page of
 // one segment, so that the page's largest magnitude is known before a code is
-// written.  A thread holds PP pairs of a row (2 PP elements in two runs of PP)
+// written (with 16-bit pages, into 4,096 elements of one: pages of 256 rows
+// of 128 take a long prompt 24.2 us by 32 rows, 26.1 by 16, 25.9 by 64, 32.1 whole;
+// of 256 elements 22.0 by 32 rows, 18.5 by 16, 25.1 by 64).  A thread holds PP pairs of a row (2 PP elements in two runs of PP)
 // and up to NIT rows.  V's loads go out first and a q head's before the one
 // ahead of it is stored.
 //   PP = 8 (chunks of prompts): 16-byte loads; the unit does K, V and the
@@ -144,12 +151,13 @@ __global__ __launch_bounds__(NT) void paged_append_kernel(PagedAppendParams p, i
     if (!told) raise_device_error(p.err, WNW_DEVERR_BOUNDS);
     if (!good_len) raise_device_error(p.err, WNW_DEVERR_CAPACITY);
   }
-  const int R = 1 << p.c.shift;
-  const int block = (len >> p.c.shift) + unit;
-  const int row0 = max(block << p.c.shift, len), row1 = min((block + 1) << p.c.shift, len + count);  // rows of the segment
+  const int R = 1 << p.c.shift, us = p.unit_shift;
+  const int at = (len >> us) + unit;
+  const int row0 = max(at << us, len), row1 = min((at + 1) << us, len + count);  // rows of the segment
   if (row0 >= row1) return;
   // where they go: rows past the table, or in no page, are not stored
   int page = -1;
+  const int block = row0 >> p.c.shift;
   if (good_len && block < p.c.max_blocks) {
     page = p.c.table[s * p.c.table_stride + block];
     if (page < 0 || page >= p.c.n_pages) {
@@ -353,32 +361,44 @@ __global__ __launch_bounds__(NT) void paged_append_kernel(PagedAppendParams p, i
   }
 }
 
-static constexpr int64_t kPaWgs = 1536;  // workgroups that shares of the q heads are made for
+// Workgroups that shares of the q heads are made for: 568 of a 4,564-token prompt
+// take 21.8 us in one or two shares and 28.1 in four (the sines again in each),
+// 256 of ragged chunks 10.8, 9.5 and 9.0.
+static constexpr int64_t kPaWgs = 1536;
 
 template <typename T, bool Q8>
 static hipError_t launch_append(const PagedAppendParams& p, int D, int64_t most, hipStream_t st) {
-  const int R = 1 << p.c.shift;
-  // rows of a unit; threads for them
-  const int64_t rows = std::min<int64_t>(R, most);
+  // Rows of a unit and threads for them, measured on both sides (us):
+  //   PP = 2 up to 1,024 elements (one token 4.4, with PP = 8 6.6; 7 tokens of 8
+  //   samples 4.7 and 6.8; but units of 16 rows of a long prompt 58.8 and 23.4);
+  //   then the most workgroups that hide each other's loads: pages of 4,096
+  //   elements 20.9 with 256 threads and one row each, 22.1 with 128; 8,192:
+  //   22.3 (two rows), with 512 threads 22.9, 128 22.2 but 13.9 for 10.7 with few
+  //   units; 16,384: 27.3 (256, four rows), 512 34.0; 32,768: 30.5 (512), 1,024
+  //   41.2; 65,536: 30.6 (512, eight rows), 1,024 39.2.
+  const int64_t rows = std::min<int64_t>(1 << p.unit_shift, most);
   const dim3 grid((unsigned)((int64_t)p.c.n_seg * p.units));
   const dim3 heads(grid.x, p.q ? 2 + p.G : 2);
   const dim3 shares(grid.x, p.q ? (unsigned)std::max<int64_t>(1, std::min<int64_t>(p.G, kPaWgs / grid.x)) : 1u);
-  if (rows * D <= 4 * 64)  // one token, or a few: one pass of a wave
+  if (rows * D <= 4 * 64)
     hipLaunchKernelGGL((paged_append_kernel<T, 2, Q8, 64, 1>), heads, dim3(64), 0, st, p, D);
   else if (rows * D <= 4 * 256)
     hipLaunchKernelGGL((paged_append_kernel<T, 2, Q8, 256, 1>), heads, dim3(256), 0, st, p, D);
   else if (rows * D <= 16 * 128)
     hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 128, 1>), shares, dim3(128), 0, st, p, D);
-  else if (rows * D <= 16 * 256)
+  else if (rows * D <= 4096 || !Q8)
     hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 256, 1>), shares, dim3(256), 0, st, p, D);
-  else if (rows * D <= 2 * 16 * 256)
-    hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 256, 2>), shares, dim3(256), 0, st, p, D);
-  else if (rows * D <= 4 * 16 * 256)
-    hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 512, 2>), shares, dim3(512), 0, st, p, D);
-  else if (rows * D <= 8 * 16 * 256)
-    hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 512, 4>), shares, dim3(512), 0, st, p, D);
-  else
-    hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 1024, 4>), shares, dim3(1024), 0, st, p, D);
+  if constexpr (Q8) {  // a page that is one unit, however large
+    if (rows * D <= 4096) return hipGetLastError();
+    if (rows * D <= 2 * 4096)
+      hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 256, 2>), shares, dim3(256), 0, st, p, D);
+    else if (rows * D <= 4 * 4096)
+      hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 256, 4>), shares, dim3(256), 0, st, p, D);
+    else if (rows * D <= 8 * 4096)
+      hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 512, 4>), shares, dim3(512), 0, st, p, D);
+    else
+      hipLaunchKernelGGL((paged_append_kernel<T, 8, Q8, 512, 8>), shares, dim3(512), 0, st, p, D);
+  }
   return hipGetLastError();
 }
 
@@ -472,7 +492,9 @@ extern "C" int wnw_paged_append(const wnw_paged_cache* cache, const int32_t* seg
     WNW_CHECK_ARG(n_sections == 1 || pos_stride >= n_tokens, "positions must be [axes, tokens]");
   }
   const int64_t most = cu_tokens ? std::min(max_tokens, n_tokens) : 1;
-  const int64_t units = (std::max<int64_t>(most, 1) + cache->page_rows - 2) / cache->page_rows + 1;
+  const bool q8 = cache->page_dtype == WNW_E4M3;
+  const int64_t unit_rows = q8 ? cache->page_rows : std::min(cache->page_rows, 4096 / D);
+  const int64_t units = (std::max<int64_t>(most, 1) + unit_rows - 2) / unit_rows + 1;
   WNW_CHECK_ARG(N * units < (1ll << 31), "too many segments and tokens for one call");
   p.t = PagedTokens{cu_tokens, (int32_t)n_tokens, (int32_t)hkv, (int32_t)most};
   p.seg_len = seg_len;
@@ -492,7 +514,7 @@ extern "C" int wnw_paged_append(const wnw_paged_cache* cache, const int32_t* seg
   p.G = (int32_t)group;
   p.units = (int32_t)units;
   p.err = device_error_word();
-  const bool q8 = cache->page_dtype == WNW_E4M3;
+  p.unit_shift = __builtin_ctzll(unit_rows);
   const int64_t rows = std::max<int64_t>(most, 1);
   hipStream_t st = (hipStream_t)stream;
   const hipError_t e = dtype == WNW_BF16 ? (q8 ? launch_append<bf16_t, true>(p, (int)D, rows, st)

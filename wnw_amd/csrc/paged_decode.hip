@@ -24,6 +24,12 @@
 // multiplies the scores, V's scale the weights.  Weights go through two 16-bit
 // parts (the upper cut off, not rounded, and neither ever zero, so that an
 // infinity in V stays one): 16 bits of each, beside 32-bit sums.
+//
+// What bounds it: with many rows memory (256 segments of up to 5,003 16-bit rows,
+// 224 MB: 48.0 us, 4.7 TB/s, a large copy 5.1; loads that leave the caches alone,
+// as each byte is used once: 51.3 us without); with few, the launch and one chain of
+// dependent round trips: lengths, table, pages, partial sums, counter (8 segments
+// of at most 813 rows: 11.3 us).
 #include <algorithm>
 #include <type_traits>
 
@@ -64,8 +70,9 @@ struct PagedDecodeGeom {
   static constexpr int RB = D * (Q8 ? 1 : 2);      // bytes of a row
   static constexpr int KC = RB / 64;               // 16-byte chunks of a K row per lane
   static constexpr int VI = kPdStep * RB / 1024;   // loads of a step's V per lane
-  // Bytes in flight and registers: a step is 8 to 32 KB of loads per wave, and
-  // 128 KB a CU keep the memory busy.
+  // Bytes in flight and registers: a step is 4 to 32 KB of loads per wave, and
+  // 128 KB a CU keep the memory busy.  Two workgroups of 8 waves a CU, where the
+  // registers allow it, take 18.7 us where one of 16 takes 20.7.
   static constexpr int kWaves = RB >= 512 ? 4 : 8;  // of a workgroup
   static constexpr int kWgs = RB >= 256 ? 1 : 2;    // workgroups per CU
   static constexpr int kStage = kPdStep * RB;       // LDS of a wave's V
