@@ -122,11 +122,11 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 
 // A workgroup takes one unit: the rows of one append that fall into one page of
 // one segment, so that the page's largest magnitude is known before a code is
-// written (with 16-bit pages, into 4,096 elements of one: pages of 256 rows
-// of 128 take a long prompt 24.2 us by 32 rows, 26.1 by 16, 25.9 by 64, 32.1 whole;
-// of 256 elements 22.0 by 32 rows, 18.5 by 16, 25.1 by 64).  A thread holds PP pairs of a row (2 PP elements in two runs of PP)
-// and up to NIT rows.  V's loads go out first and a q head's before the one
-// ahead of it is stored.
+// written.  With 16-bit pages it is 4,096 elements of one (a long prompt into
+// pages of 256 rows of 128: 24.2 us by 32 rows, 26.1 by 16, 25.9 by 64, 32.1 whole;
+// of 256 elements: 22.0 by 32 rows, 18.5 by 16, 25.1 by 64).  A thread holds PP
+// pairs of a row (2 PP elements in two runs of PP) and up to NIT rows.  V's loads
+// go out first and a q head's before the one ahead of it is stored.
 //   PP = 8 (chunks of prompts): 16-byte loads; the unit does K, V and the
 //       group's q heads, so a row's sines are worked out once for all of them;
 //       with few units the q heads are shared out over blockIdx.y.

@@ -23,13 +23,15 @@
 // Few query rows and many keys: the tiles of each block of rows are cut into
 // splits, whose sums a second launch adds up.
 //
-// What bounds it: per tile and SIMD the matrix products (2 x 1,024 cycles for two
-// waves at head_dim 128), the exponentials and the LDS reads (each of 8 waves
-// reads the tile) come to the same 0.85 us each, and a wave's turn is these one
-// after another; about half overlaps.  The large products run at 0.86 PFLOP/s
-// (8,192-sized plain bf16 ones: 1.2).  Tried without gain: the next tile's
-// scores computed among the softmax (2 to 5 % slower: registers), loads two
-// tiles ahead, raised wave priority in the products.
+// What bounds it: the instructions.  Per tile and wave at head_dim 128 the products
+// take 1,024 cycles of the matrix unit, 32 exponentials 512 and about 230 other
+// vector instructions 920, and on one SIMD these add up: 4,564 tokens take 213 us
+// of kernel, in which matrix instructions run for 37 % and vector ones for 51 % of
+// the cycles.  That is 0.8 PFLOP/s (plain bf16 products of size 8,192: 1.2).
+// Without gain: half of the waves a phase behind the others, so that one's
+// products meet the other's exponentials (231 us; 214 without); the next tile's
+// scores among the exponentials (2 to 5 % slower); loads two tiles ahead; raised
+// wave priority in the products.
 #include <algorithm>
 #include <type_traits>
 
