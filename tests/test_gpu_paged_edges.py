@@ -180,3 +180,79 @@ def test_overlapping_outputs_are_refused(gpu):
     got = paged_prompt_attn(q, *c.args(), cu, 0.1, out=out, **ok)
     assert torch.equal(got, paged_prompt_attn(q, *c.args(), cu, 0.1, **ok))
     _clean()
+
+
+@pytest.mark.parametrize("dtype,D,G", [(BF, 128, 4), (FP, 64, 1), (BF, 256, 2), (FP, 128, 16)])
+@pytest.mark.parametrize("new,old", [(3, 50), (15, 17), (40, 70)], ids=lambda x: str(x))
+def test_huge_values_in_masked_rows(gpu, dtype, D, G, new, old):
+    """K and V of a later token at the type's largest number: the earlier tokens' results do not move."""
+    c = Cache(gpu, [old + new], 64, D, dtype, False, seed=D + new)
+    q = _q(gpu, new, G, D, dtype)
+    want = paged_prompt_attn(q, *c.args(), _cu([new], gpu), D ** -0.5)
+    p, at = c.table[0, (old + new - 1) // 64].item(), (old + new - 1) % 64
+    c.k[p, at] = c.v[p, at] = torch.finfo(dtype).max
+    got = paged_prompt_attn(q, *c.args(), _cu([new], gpu), D ** -0.5)
+    _clean()
+    assert torch.equal(got[:-1], want[:-1])  # a weight of 0 times any finite number is 0
+
+
+def test_table_without_blocks(gpu):
+    """A page table of no columns: no rows to see, no room to append to."""
+    c = Cache(gpu, [5, 9], 32, 64, BF, True, seed=26)
+    table, lens = c.table[:, :0], torch.zeros(2, dtype=torch.int32, device=gpu)
+    q, ok = _q(gpu, 2, 4, 64, BF), c.scales()
+    assert int(torch.count_nonzero(paged_decode_attn(q, c.k, c.v, table, lens, 0.1, **ok))) == 0
+    long = _q(gpu, 90, 8, 64, BF)
+    assert int(torch.count_nonzero(paged_prompt_attn(long, c.k, c.v, table, lens, _cu([90], gpu), 0.1, **ok))) == 0
+    _clean()
+    kv, was = torch.ones(2, 1, 64, device=gpu, dtype=BF), _snapshot(c)
+    _, nl = paged_append(kv, kv, c.k, c.v, table, lens, **ok)
+    torch.cuda.synchronize()
+    assert _lib.device_error() == _lib.DEVERR_CAPACITY and nl.tolist() == [1, 1]
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(_snapshot(c), was))
+
+
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("new,room", [(3, 1), (60, 1), (60, 60), (700, 1)], ids=lambda x: str(x))
+def test_prompts_captured(gpu, q8, new, room):
+    """An append and its prompt attention captured, each form of the attention; replays follow the lengths between eager
+    calls, and equal them."""
+    H, G, D = 2, 4, 128
+    c = Cache(gpu, [90, 333], 64, D, BF, q8, seed=27, room=room + 4 * new // 64 + 2)
+    eager = Cache.__new__(Cache)
+    eager.__dict__.update(c.__dict__)
+    for name in ("k", "v", "k_scale", "v_scale", "seg_len"):
+        if getattr(c, name) is not None:
+            setattr(eager, name, getattr(c, name).clone())
+    cu = _cu([new], gpu)
+    q, k, v = (torch.zeros(new, n, D, device=gpu, dtype=BF) for n in (H * G, H, H))
+
+    def step(x):
+        _, nl = paged_append(k, v, *x.args(), cu_tokens=cu, max_tokens=new, **x.scales())
+        out = paged_prompt_attn(q, x.k, x.v, x.table, nl, cu, 0.1, max_tokens=new, **x.scales())
+        x.seg_len.copy_(nl)
+        return out
+
+    state = [x.clone() for x in (*_snapshot(c), c.seg_len) if x is not None]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(c)
+    torch.cuda.current_stream().wait_stream(side)
+    for x, y in zip([t for t in (c.k, c.v, c.k_scale, c.v_scale, c.seg_len) if t is not None], state):
+        x.copy_(y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(c)
+    for i in range(3):
+        gen = torch.Generator(device=gpu).manual_seed(i)
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, device=gpu, generator=gen))
+        graph.replay()
+        want = step(eager)
+        assert torch.equal(out, want), i
+        if i == 1:
+            torch.cuda.synchronize()
+    _clean()
+    assert torch.equal(c.seg_len, eager.seg_len) and c.seg_len.tolist() == [90 + 3 * new, 333 + 3 * new]
+    assert torch.equal(c.k.view(torch.uint8), eager.k.view(torch.uint8))

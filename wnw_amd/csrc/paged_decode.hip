@@ -22,8 +22,7 @@
 // rows follow its order.  The next step's rows are loaded while a step is used.
 // 8-bit codes become 16-bit elements in registers (exact); K's scale
 // multiplies the scores, V's scale the weights.  Weights go through two 16-bit
-// parts (the upper cut off, not rounded, and neither ever zero, so that an
-// infinity in V stays one): 16 bits of each, beside 32-bit sums.
+// parts, the upper cut off, not rounded: 16 bits of each, beside 32-bit sums.
 //
 // What bounds it: with many rows memory (256 segments of up to 5,003 16-bit rows,
 // 224 MB: 48.0 us, 4.7 TB/s, a large copy 5.1; loads that leave the caches alone,
@@ -107,18 +106,18 @@ struct PagedDecodeV {
   static constexpr uint32_t read_x(int i) { return (Q8 ? 16 : 32) * i; }
 };
 
-// Two positive values as two pairs of 16-bit parts
+// Two values, positive or zero, as two pairs of 16-bit parts, the lower ones at least `least`
 template <typename T>
-__device__ __forceinline__ void two_parts(float a, float b, uint32_t* hi, uint32_t* lo) {
+__device__ __forceinline__ void two_parts(float a, float b, float least, uint32_t* hi, uint32_t* lo) {
   if constexpr (std::is_same<T, bf16_t>::value) {
     const uint32_t ua = __float_as_uint(a) & 0xffff0000u, ub = __float_as_uint(b) & 0xffff0000u;
     *hi = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
-    const float la = fmaxf(a - __uint_as_float(ua), 7.888609e-31f), lb = fmaxf(b - __uint_as_float(ub), 7.888609e-31f);
+    const float la = fmaxf(a - __uint_as_float(ua), least), lb = fmaxf(b - __uint_as_float(ub), least);
     *lo = __builtin_amdgcn_perm(__float_as_uint(lb), __float_as_uint(la), 0x07060302u);
   } else {
     const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
     *hi = __builtin_bit_cast(uint32_t, h);
-    const float la = fmaxf(a - (float)h[0], 5.9604645e-8f), lb = fmaxf(b - (float)h[1], 5.9604645e-8f);
+    const float la = fmaxf(a - (float)h[0], least), lb = fmaxf(b - (float)h[1], least);
     *lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(la, lb));
   }
 }
@@ -522,6 +521,8 @@ paged_decode_kernel(PagedDecodeParams p) {
           for (int i = 0; i < DT; ++i) acc[i] *= fall;
           m = mx;
         }
+        // the type's least number, so that an infinity that a column sees stays one; none beside masked rows
+        const float least_part = edge && r.count > 1 ? 0.f : std::is_same<VT, f16_t>::value ? 5.9604645e-8f : 1.17549435e-38f;
         u32x4 hi, lo;
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
@@ -534,7 +535,7 @@ paged_decode_kernel(PagedDecodeParams p) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             uint32_t uh, ul;
-            two_parts<VT>(y[t2][2 * i], y[t2][2 * i + 1], &uh, &ul);
+            two_parts<VT>(y[t2][2 * i], y[t2][2 * i + 1], least_part, &uh, &ul);
             hi[2 * t2 + i] = uh;
             lo[2 * t2 + i] = ul;
           }
