@@ -8,7 +8,7 @@ import torch
 from tests.paged_ref import E4M3, HALF, Cache, attend
 from tests.test_gpu_paged import BF, FP, _check, _clean, _cu, _decode_check, _prompt_check, _q, _snapshot
 from wnw_amd import _lib
-from wnw_amd.kv.paged import paged_append, paged_decode_attn, paged_prompt_attn
+from wnw_amd.kv.paged import PagedWorkspace, paged_append, paged_decode_attn, paged_prompt_attn
 
 pytestmark = pytest.mark.gpu
 
@@ -256,3 +256,42 @@ def test_prompts_captured(gpu, q8, new, room):
     _clean()
     assert torch.equal(c.seg_len, eager.seg_len) and c.seg_len.tolist() == [90 + 3 * new, 333 + 3 * new]
     assert torch.equal(c.k.view(torch.uint8), eager.k.view(torch.uint8))
+
+
+def test_own_workspace(gpu):
+    """Calls with a workspace of the caller's: eager and captured, two graphs of different sizes replayed in turn on it."""
+    cs = [Cache(gpu, lens, 64, 128, BF, True, seed=28 + i) for i, lens in enumerate(([6000, 90, 2500], [3000] * 70))]
+    qs = [_q(gpu, len(c.lens), 4, 128, BF) for c in cs]
+    few = [_q(gpu, 3, 4 * len(c.lens), 128, BF) for c in cs]
+    cu = _cu([3], gpu)
+    ws = PagedWorkspace(70, 12, 128)
+    assert ws.buf.device == cs[0].k.device
+
+    def step(i, **kw):
+        return (paged_decode_attn(qs[i], *cs[i].args(), 0.1, **cs[i].scales(), **kw),
+                paged_prompt_attn(few[i], *cs[i].args(), cu, 0.1, **cs[i].scales(), **kw))
+
+    want = [step(i) for i in range(2)]
+    graphs, outs = [], []
+    for i in range(2):
+        got = step(i, workspace=ws)
+        assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(i, workspace=ws))
+        graphs.append(g)
+    for i in (0, 1, 1, 0, 0, 1):
+        for o in outs[i]:
+            o.zero_()
+        graphs[i].replay()
+        step(1 - i, workspace=ws)
+        assert all(torch.equal(a, b) for a, b in zip(outs[i], want[i])), i
+    _clean()
+    assert int(torch.count_nonzero(ws.buf[:ws.counters])) == 0
+    E = _lib.WnwError
+    for fn in (lambda: step(1, workspace=PagedWorkspace(70, 11, 128)), lambda: step(1, workspace=PagedWorkspace(5000, 16, 128)),
+               lambda: PagedWorkspace(70, 17, 128), lambda: PagedWorkspace(-1, 1, 128), lambda: PagedWorkspace(4, 4, 128, "cpu")):
+        with pytest.raises(E):
+            fn()
+    _clean()

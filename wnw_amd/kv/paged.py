@@ -44,6 +44,39 @@ _workspaces: dict[tuple[int, int], list] = {}
 _is_capturing = torch.cuda.is_current_stream_capturing
 
 
+class PagedWorkspace:
+    """The workspace of decode attention calls (and of prompt attention calls
+    of up to 16 query rows per segment) that a program keeps itself: room for
+    ``n_seg`` segments of ``rows`` query rows (heads of a group times tokens),
+    cleared once, here, on the current stream.  A captured call that is given one needs no launch to
+    clear its own (about 3 us).  Launches that use one must not overlap: give
+    graphs or streams that run at the same time one each."""
+
+    def __init__(self, n_seg: int, rows: int, head_dim: int, device: torch.device | str | int | None = None):
+        if _is_capturing():
+            raise _lib.WnwError("make the workspace before the capture")
+        dev = torch.device("cuda", device) if isinstance(device, int) else torch.device("cuda" if device is None else device)
+        if dev.type != "cuda":
+            raise _lib.WnwError(f"the workspace must be on a GPU, not {dev}")
+        if dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        need = int(_lib.lib().wnw_paged_decode_workspace_bytes(n_seg, rows, head_dim))
+        if need < 0:
+            raise _lib.WnwError(f"bad workspace sizes: {n_seg} segments, {rows} rows, head_dim {head_dim}")
+        self.counters = int(_lib.lib().wnw_paged_counter_bytes(n_seg))
+        with torch.cuda.device(dev):
+            _lib.ensure_init(dev)
+            self.buf = torch.zeros(need, dtype=torch.uint8, device=dev)
+
+    def get(self, device: torch.device, n_seg: int, need: int) -> Tensor:
+        if self.buf.device != device:
+            raise _lib.WnwError("the workspace is on another device")
+        if self.buf.numel() < need or self.counters != int(_lib.lib().wnw_paged_counter_bytes(n_seg)):
+            raise _lib.WnwError(f"the workspace is too small, or for other segment counts: {self.buf.numel()} bytes, {need} "
+                                "needed")
+        return self.buf
+
+
 def call_workspace(idx: int, stream: int, n_seg: int, need: int) -> Tensor:
     """The workspace of an attention call on ``stream`` of device ``idx`` (the
     current one), its counters zero."""
@@ -61,8 +94,11 @@ def call_workspace(idx: int, stream: int, n_seg: int, need: int) -> Tensor:
     return buf
 
 
-def _workspace(dev: torch.device, n_seg: int, need: int) -> Tensor:
-    return call_workspace(dev.index if dev.index is not None else torch.cuda.current_device(), _lib.raw_stream(dev), n_seg, need)
+def _workspace(dev: torch.device, n_seg: int, need: int, given: PagedWorkspace | None) -> Tensor:
+    if given is not None:
+        return given.get(dev, n_seg, need)
+    idx = dev.index if dev.index is not None else torch.cuda.current_device()
+    return call_workspace(idx, _lib.raw_stream(dev), n_seg, need)
 
 
 def _cache(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seg_len: Tensor, k_scale: Tensor | None,
@@ -240,17 +276,19 @@ def _check_q(q: Tensor, k_pages: Tensor, scale: float) -> None:
 
 
 def paged_decode_attn(q_flat: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seg_len: Tensor, scale: float, *,
-                      k_scale: Tensor | None = None, v_scale: Tensor | None = None, out: Tensor | None = None) -> Tensor:
+                      k_scale: Tensor | None = None, v_scale: Tensor | None = None, out: Tensor | None = None,
+                      workspace: PagedWorkspace | None = None) -> Tensor:
     """Decode attention over the pages: ``decode_attn`` for a paged cache.
 
     ``q_flat`` [N, G, D] in bf16 or f16, G up to 16; returns [N, G, D].  A
     segment without rows gives zeros.  ``out``: a contiguous tensor for the
     result.  The lengths are read on the device; ``page_table.shape[1]`` bounds
-    them and sizes the grid."""
-    done = (_lib._callpath or _lib.callpath()).paged_decode(q_flat, k_pages, v_pages, page_table, seg_len, scale, k_scale,
-                                                            v_scale, out)
-    if done is not None:
-        return done
+    them and sizes the grid.  ``workspace``: the caller's own."""
+    if workspace is None:
+        done = (_lib._callpath or _lib.callpath()).paged_decode(q_flat, k_pages, v_pages, page_table, seg_len, scale, k_scale,
+                                                                v_scale, out)
+        if done is not None:
+            return done
     cache = _cache(k_pages, v_pages, page_table, seg_len, k_scale, v_scale, q_flat, out)
     _check_q(q_flat, k_pages, scale)
     N, D = cache.n_seg, cache.head_dim
@@ -267,7 +305,7 @@ def paged_decode_attn(q_flat: Tensor, k_pages: Tensor, v_pages: Tensor, page_tab
         return o
     with torch.cuda.device(q.device):
         _lib.ensure_init(q.device)
-        ws = _workspace(q.device, N, int(_lib.lib().wnw_paged_decode_workspace_bytes(N, G, D)))
+        ws = _workspace(q.device, N, int(_lib.lib().wnw_paged_decode_workspace_bytes(N, G, D)), workspace)
         _lib.check(_lib.lib().wnw_paged_decode_attn(
             ctypes.byref(cache), _lib.ptr(seg_len), _lib.ptr(q), _lib.ptr(o), G, float(scale), _lib.dtype_code(q.dtype),
             _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(q.device)), "paged_decode_attn")
@@ -276,7 +314,8 @@ def paged_decode_attn(q_flat: Tensor, k_pages: Tensor, v_pages: Tensor, page_tab
 
 def paged_prompt_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seg_len: Tensor, cu_tokens: Tensor,
                       scale: float, *, max_tokens: int | None = None, k_scale: Tensor | None = None,
-                      v_scale: Tensor | None = None, out: Tensor | None = None) -> Tensor:
+                      v_scale: Tensor | None = None, out: Tensor | None = None,
+                      workspace: PagedWorkspace | None = None) -> Tensor:
     """Causal attention of prompts, or of chunks of them, over the pages that
     hold their K and V already (``paged_append`` comes first).
 
@@ -285,11 +324,13 @@ def paged_prompt_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: T
     i of them sees the first seg_len - n + i + 1 (none: zeros).  Returns
     [T, Hq, D].  ``max_tokens``, the most tokens of a sample, sizes the grid
     (default T); a sample with more sets the device error word and its rows of
-    the result are not written."""
-    done = (_lib._callpath or _lib.callpath()).paged_prompt(q, k_pages, v_pages, page_table, seg_len, cu_tokens, scale,
-                                                            max_tokens, k_scale, v_scale, out)
-    if done is not None:
-        return done
+    the result are not written.  ``workspace``: the caller's own, used by calls
+    of up to 16 query rows per segment (max_tokens times heads of a group)."""
+    if workspace is None:
+        done = (_lib._callpath or _lib.callpath()).paged_prompt(q, k_pages, v_pages, page_table, seg_len, cu_tokens, scale,
+                                                                max_tokens, k_scale, v_scale, out)
+        if done is not None:
+            return done
     cache = _cache(k_pages, v_pages, page_table, seg_len, k_scale, v_scale, q, cu_tokens, out)
     _check_q(q, k_pages, scale)
     N, D = cache.n_seg, cache.head_dim
@@ -310,7 +351,7 @@ def paged_prompt_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: T
         _lib.ensure_init(q.device)
         need = int(_lib.lib().wnw_paged_prompt_workspace_bytes(ctypes.byref(cache), G, most))
         if G * most <= 16:
-            ws = _workspace(q.device, N, need)
+            ws = _workspace(q.device, N, need, workspace)
         else:
             ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
         _lib.check(_lib.lib().wnw_paged_prompt_attn(
