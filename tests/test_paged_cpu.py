@@ -12,7 +12,7 @@ PTR = 1 << 20
 
 
 def _cache(**change):
-    f = dict(k_pages=PTR, v_pages=PTR, k_scale=PTR, v_scale=PTR, page_table=PTR, n_seg=8, n_pages=100, max_blocks=10,
+    f = dict(k_pages=PTR, v_pages=PTR * 4, k_scale=PTR, v_scale=PTR * 8, page_table=PTR, n_seg=8, n_pages=100, max_blocks=10,
              page_rows=64, head_dim=128, k_stride=64 * 128, v_stride=64 * 128, table_stride=10, page_dtype=_lib.DT_E4M3)
     f.update(change)
     return _lib.PagedCache(*(f[n] for n, _ in _lib.PagedCache._fields_))
@@ -113,3 +113,9 @@ def test_host_tensors_are_refused():
         paged_decode_attn(x, pages, pages, table, lens, 0.1)
     with pytest.raises(_lib.WnwError):
         paged_prompt_attn(x, pages, pages, table, lens, torch.tensor([0, 1, 2], dtype=torch.int32), 0.1)
+
+
+def test_grids_past_the_launch_limit_are_refused():
+    many = _cache(n_seg=1 << 23, n_pages=1 << 20)
+    assert _append(many, T=1 << 24, B=1 << 20, most=64) == _lib.WNW_EINVAL
+    assert _prompt(many, T=1 << 23, B=1 << 20, most=4096) == _lib.WNW_EINVAL

@@ -495,7 +495,7 @@ extern "C" int wnw_paged_append(const wnw_paged_cache* cache, const int32_t* seg
   const bool q8 = cache->page_dtype == WNW_E4M3;
   const int64_t unit_rows = q8 ? cache->page_rows : std::min(cache->page_rows, 4096 / D);
   const int64_t units = (std::max<int64_t>(most, 1) + unit_rows - 2) / unit_rows + 1;
-  WNW_CHECK_ARG(N * units < (1ll << 31), "too many segments and tokens for one call");
+  WNW_CHECK_ARG(N * units < (1ll << 23), "too many segments and tokens for one call");
   p.t = PagedTokens{cu_tokens, (int32_t)n_tokens, (int32_t)hkv, (int32_t)most};
   p.seg_len = seg_len;
   p.new_len = new_len;

@@ -591,7 +591,7 @@ extern "C" int wnw_paged_prompt_attn(const wnw_paged_cache* cache, const int32_t
     return paged_decode_launch(cache, seg_len, q, out, strides, p.t, group, scale, dtype, workspace, workspace_bytes, stream);
   WNW_CHECK_ARG(most * group < (1ll << 30), "too many query rows");
   const PromptPlan y = prompt_plan(N, group, most, p.c.capacity, D);
-  WNW_CHECK_ARG(N * y.nqb < (1ll << 25), "too many segments and tokens for one call");
+  WNW_CHECK_ARG(N * y.nqb < (1ll << 23), "too many segments and tokens for one call");
   WNW_CHECK_ARG(y.bytes == 0 || (workspace && workspace_bytes >= y.bytes), "workspace too small: %lld bytes, %lld needed",
                 (long long)workspace_bytes, (long long)y.bytes);
   WNW_CHECK_ARG((uintptr_t)workspace % 256 == 0, "the workspace must be 256-byte aligned");

@@ -48,9 +48,10 @@ class PagedWorkspace:
     """The workspace of decode attention calls (and of prompt attention calls
     of up to 16 query rows per segment) that a program keeps itself: room for
     ``n_seg`` segments of ``rows`` query rows (heads of a group times tokens),
-    cleared once, here, on the current stream.  A captured call that is given one needs no launch to
-    clear its own (about 3 us).  Launches that use one must not overlap: give
-    graphs or streams that run at the same time one each."""
+    cleared once, here, on the current stream.  A captured call that is given
+    one needs no launch to clear its own (about 3 us).  Launches that use one
+    must not overlap: give graphs or streams that run at the same time one
+    each."""
 
     def __init__(self, n_seg: int, rows: int, head_dim: int, device: torch.device | str | int | None = None):
         if _is_capturing():
@@ -175,7 +176,8 @@ def paged_append(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_ta
     [cu_tokens[b], cu_tokens[b + 1]) (int32 [B + 1], B = N / Hkv), one each
     without ``cu_tokens``.  ``max_tokens``, the most tokens of a sample, sizes
     the grid (default T); a sample with more sets the device error word and is
-    not appended.
+    not appended.  Rows of the rotated q that belong to no such sample (tokens
+    behind the last) are not written.
 
     ``positions`` (int64 or int32, [T] or [axes, T]) and ``inv_freq`` (float64 or
     float32, [rot / 2], rot a multiple of 16 up to D) rotate q and K: pair j by
