@@ -361,9 +361,9 @@ __global__ __launch_bounds__(NT) void paged_append_kernel(PagedAppendParams p, i
   }
 }
 
-// Workgroups that shares of the q heads are made for: 568 of a 4,564-token prompt
-// take 21.8 us in one or two shares and 28.1 in four (the sines again in each),
-// 256 of ragged chunks 10.8, 9.5 and 9.0.
+// Workgroups that shares of the q heads are made for: 584 of a 4,564-token prompt
+// take 22.0 us in one share, 21.8 in two and 28.1 in four (the sines again in each),
+// 552 of ragged chunks 10.8, 9.5 and 9.0.
 static constexpr int64_t kPaWgs = 1536;
 
 template <typename T, bool Q8>
