@@ -295,3 +295,17 @@ def test_own_workspace(gpu):
         with pytest.raises(E):
             fn()
     _clean()
+
+
+@pytest.mark.parametrize("q8,dtype,D,G", [(True, BF, 128, 4), (False, FP, 64, 8), (True, FP, 256, 2)])
+@pytest.mark.parametrize("new,old", [([300], [0]), ([64, 90], [500, 0]), ([200, 30, 80, 1], [300, 2000, 10, 0]), ([700], [0])],
+                         ids=lambda x: "-".join(map(str, x)))
+def test_prompts_in_a_wide_table(gpu, q8, dtype, D, G, new, old):
+    """A table for far more rows than the segments have: each block of queries is cut by the rows that it sees."""
+    c = Cache(gpu, [o + n for o, n in zip(old, new) for _ in range(2)], 64, D, dtype, q8, seed=30)
+    wide = torch.full((c.table.shape[0], c.table.shape[1] + 500), -1, dtype=torch.int32, device=gpu)
+    wide[:, :c.table.shape[1]] = c.table
+    q = _q(gpu, sum(new), 2 * G, D, dtype)
+    out = paged_prompt_attn(q, c.k, c.v, wide, c.seg_len, _cu(new, gpu), D ** -0.5, max_tokens=max(new), **c.scales())
+    _clean()
+    _prompt_check(c, q, out, new, 2, D ** -0.5)

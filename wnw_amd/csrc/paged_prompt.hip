@@ -85,6 +85,19 @@ __device__ __forceinline__ PromptRows prompt_rows(const PagedPromptParams& p, in
   return r;
 }
 
+// Into how many splits a block's tiles are cut, of the most that the launch has: by
+// the block's own tiles, as the table that the launch was planned for may be far
+// wider than the segments are long (100 tokens in a table of 25,000 rows: 14 us, cut
+// by the table 26; 64 tokens after 500 rows 19 and 26, with pieces of 4 tiles or
+// more 21).
+__device__ __forceinline__ int splits_of(int tiles, int most) { return max(min(tiles / 2, most), 1); }
+// Tiles that a block of query rows walks
+template <int W>
+__device__ __forceinline__ int tiles_of(const PagedPromptParams& p, const PromptRows& r, int qblk) {
+  const int last = r.len - r.count + 1 + min(32 * W * (qblk + 1) - 1, r.rows - 1) / p.G;  // rows that its last one sees
+  return max((last + kPpKeys - 1) / kPpKeys, 0);
+}
+
 // The wave's rows out, 32-element parts dt0 .. dt0 + NT - 1: lane (hi, n) has
 // elements 32 i + 8 j + 4 hi + 0..3 of row n
 template <typename T, int NT>
@@ -134,12 +147,13 @@ __global__ __launch_bounds__((64 * W), (D == 256 && !Q8 ? 1 : 2)) void paged_pro
   const int row = qblk * kPpQ + 32 * w + n;
   const int ri = min(row, r.rows - 1) / p.G, rg = min(row, r.rows - 1) - ri * p.G;
   const int limit = base + ri;
-  // rows that the first and the last query see: of the wave, of the workgroup
+  // rows that the wave's first and last query see
   const int wfirst = base + min(qblk * kPpQ + 32 * w, r.rows - 1) / p.G;
   const int wlast = base + min(qblk * kPpQ + 32 * w + 31, r.rows - 1) / p.G;
-  const int first = base + qblk * kPpQ / p.G, last = base + min(qblk * kPpQ + kPpQ - 1, r.rows - 1) / p.G;
-  const int tiles = max((last + kPpKeys - 1) / kPpKeys, 0);
-  const int t0 = (int)((int64_t)tiles * split / p.splits), t1 = (int)((int64_t)tiles * (split + 1) / p.splits);
+  const int first = base + qblk * kPpQ / p.G;  // and the workgroup's first
+  const int tiles = tiles_of<W>(p, r, qblk), splits = splits_of(tiles, p.splits);
+  if (split >= splits) return;
+  const int t0 = (int)((int64_t)tiles * split / splits), t1 = (int)((int64_t)tiles * (split + 1) / splits);
   const bool busy = qblk * kPpQ + 32 * w < r.rows;  // a wave without rows only moves tiles
   const int mine = busy ? min(t1, (wlast + kPpKeys - 1) / kPpKeys) : t0;  // the wave's tiles end here
   u32x4 qr[KK];
@@ -431,7 +445,7 @@ __global__ __launch_bounds__((64 * W), (D == 256 && !Q8 ? 1 : 2)) void paged_pro
     }
   }
   l = sum_x32(l);
-  if (p.splits == 1) {
+  if (splits == 1) {
     prompt_store<T, DT>(p, r, row, h, hi, 0, o, l, Q8 ? ref : 0.f);
   } else if (busy) {
     float* part = p.part + ((((int64_t)block * N + seg) * p.splits + split) * W + w) * (DT * 16 + 3) * 64;
@@ -459,6 +473,8 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParam
   const int seg = block % N, qblk = p.nqb - 1 - block / N;
   const PromptRows r = prompt_rows(p, seg, false);
   if (qblk * kPpQ + 32 * w >= r.rows) return;
+  const int splits = splits_of(tiles_of<W>(p, r, qblk), p.splits);
+  if (splits == 1) return;
   constexpr int64_t kPart = (DT * 16 + 3) * 64;
   const float* part = p.part + ((int64_t)block * p.splits * W + w) * kPart;
   f32x16 o = f32x16{};
@@ -474,7 +490,7 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParam
     ref = most;
   };
 #pragma unroll 2
-  for (int s = k; s < p.splits; s += 4) {
+  for (int s = k; s < splits; s += 4) {
     const float* at = part + s * W * kPart;
     f32x16 y;
 #pragma unroll
