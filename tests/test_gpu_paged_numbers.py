@@ -1,0 +1,66 @@
+"""The paged cache's attention over numbers that a query must not feel: scales of
+pages that no segment names.  Tolerances as in test_gpu_paged.py, from the same
+bounds."""
+import pytest
+import torch
+
+from tests.paged_ref import Cache
+from tests.test_gpu_paged import BF, FP, _clean, _cu, _decode_check, _q
+from wnw_amd import _lib
+from wnw_amd.kv.paged import paged_decode_attn, paged_prompt_attn
+
+pytestmark = pytest.mark.gpu
+
+
+def _free_page_0(c):
+    """Moves page 0's rows to a page that no segment names, if one does; True where pages are named."""
+    ids = [(s, i) for s, n in enumerate(c.lens) for i in range(-(-n // c.page))]
+    named = torch.zeros(c.P, dtype=torch.bool, device=c.dev)
+    for s, i in ids:
+        named[c.table[s, i].item()] = True
+    spare = int((~named).nonzero()[-1])
+    if bool(named[0]):
+        for t in (c.k, c.v):
+            b = t.view(torch.uint8) if c.q8 else t
+            b[spare] = b[0]
+        for t in (c.k_scale, c.v_scale):
+            if t is not None:
+                t[spare] = t[0]
+        for s, i in ids:
+            if c.table[s, i].item() == 0:
+                c.table[s, i] = spare
+        named[0], named[spare] = False, True
+    return named
+
+
+@pytest.mark.parametrize("dtype,D,G,page", [(BF, 128, 4, 64), (FP, 64, 2, 16), (FP, 256, 16, 32), (BF, 64, 1, 256)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -1.0])
+def test_scales_of_pages_that_nobody_names(gpu, dtype, D, G, page, value):
+    """A pool whose scales nobody has written yet, page 0's among them."""
+    lens = [1, 16, 33, 48, 15, 32, 17, 500, 0, 2000, 9, 9]
+    c = Cache(gpu, lens, page, D, dtype, True, seed=D + page)
+    named = _free_page_0(c)
+    q = _q(gpu, len(lens), G, D, dtype)
+    few = _q(gpu, 6 * 3, 2, D, dtype)  # 3 tokens a sample of 2 heads: the decode kernel's rows
+    long = _q(gpu, 6 * 30, 2 * G, D, dtype)
+    calls = (lambda: paged_decode_attn(q, *c.args(), D ** -0.5, **c.scales()),
+             lambda: paged_prompt_attn(few, *c.args(), _cu([3] * 6, gpu), D ** -0.5, max_tokens=3, **c.scales()),
+             lambda: paged_prompt_attn(long, *c.args(), _cu([30] * 6, gpu), D ** -0.5, max_tokens=30, **c.scales()))
+    c.k_scale[~named] = c.v_scale[~named] = 1.0
+    want = [f() for f in calls]
+    c.k_scale[~named] = c.v_scale[~named] = value
+    got = [f() for f in calls]
+    _clean()
+    _decode_check(c, q, got[0], D ** -0.5)
+    for a, b in zip(got, want):
+        assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
+    # entries that are no page: rows of zeros, whatever page 0's scale is
+    c.table[9, 0], c.table[7, 0] = -1, c.P
+    c.k_scale[~named] = c.v_scale[~named] = 1.0
+    want = [f() for f in calls]
+    c.k_scale[~named] = c.v_scale[~named] = value
+    got = [f() for f in calls]
+    torch.cuda.synchronize()
+    assert _lib.device_error() == _lib.DEVERR_BOUNDS
+    for a, b in zip(got, want):
+        assert bool(torch.isfinite(a).all()) and torch.equal(a, b)

@@ -411,9 +411,10 @@ paged_decode_kernel(PagedDecodeParams p) {
             pid = -1;
           }
         }
-        if (Q8) {
-          ks = p.c.k_scale[max(pid, 0)];
-          vs = p.c.v_scale[max(pid, 0)];
+        if (Q8) {  // a half in no page has weights of 0, or rows of zeros: page 0's scale, whatever it is, is not theirs
+          const float k_of = p.c.k_scale[max(pid, 0)], v_of = p.c.v_scale[max(pid, 0)];
+          ks = pid < 0 ? 1.f : k_of;
+          vs = pid < 0 ? 1.f : v_of;
         }
       };
       u32x4 kr[2][KC], vr[VI];
