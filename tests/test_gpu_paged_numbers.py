@@ -1,11 +1,11 @@
 """The paged cache's attention over numbers that a query must not feel: scales of
-pages that no segment names.  Tolerances as in test_gpu_paged.py, from the same
-bounds."""
+pages that no segment names, infinities in one of a segment's pieces.  Tolerances
+as in test_gpu_paged.py, from the same bounds."""
 import pytest
 import torch
 
-from tests.paged_ref import Cache
-from tests.test_gpu_paged import BF, FP, _clean, _cu, _decode_check, _q
+from tests.paged_ref import HALF, Cache, attend
+from tests.test_gpu_paged import BF, FP, _check, _clean, _cu, _decode_check, _q
 from wnw_amd import _lib
 from wnw_amd.kv.paged import paged_decode_attn, paged_prompt_attn
 
@@ -64,3 +64,30 @@ def test_scales_of_pages_that_nobody_names(gpu, dtype, D, G, page, value):
     assert _lib.device_error() == _lib.DEVERR_BOUNDS
     for a, b in zip(got, want):
         assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("dtype,D,G", [(BF, 128, 4), (FP, 64, 4), (BF, 256, 16), (FP, 128, 4), (BF, 64, 1)])
+@pytest.mark.parametrize("n", [1, 33, 600, 9000])
+def test_decode_infinities_stay_infinities(gpu, q8, dtype, D, G, n):
+    """An infinity of V, with the largest weight and with small ones; 8 bits have NaN in its place."""
+    c = Cache(gpu, [n], 64, D, dtype, q8, seed=n + D)
+    u = torch.randn(D, device=gpu, generator=torch.Generator(device=gpu).manual_seed(5))
+    u = u / u.norm() * D ** 0.5
+    q = (u + 0.2 * _q(gpu, 1, G, D, dtype).float()).to(dtype)
+    for d, (r, size) in enumerate([(n // 2, 3.0), (n - 1, -2.0), (0, 0.0)][:3 if n > 1 else 1]):
+        p, at = c.table[0, r // 64].item(), r % 64
+        if q8:
+            c.k[p, at] = (u * size / c.k_scale[p]).clamp(-448, 448).to(c.k.dtype)
+            c.v.view(torch.uint8)[p, at, 7 * d + 3] = 0xff
+        else:
+            c.k[p, at] = (u * size).to(dtype)
+            c.v[p, at, 7 * d + 3] = float("-inf")
+    out = paged_decode_attn(q, *c.args(), 3.0 / D, **c.scales())
+    _clean()
+    odd = [3, 10, 17][:3 if n > 1 else 1]
+    assert bool((out[..., odd].isnan() if q8 else out[..., odd] == float("-inf")).all())
+    keep = [d for d in range(D) if d not in odd]
+    k, v = c.rows(0)
+    ref, A = attend(q[0].double(), k, v[:, keep], torch.full((G,), n, device=gpu), 3.0 / D)
+    _check(out[0][:, keep], ref, HALF[dtype] * ref.abs() + 2.0 ** -13 * A, n)

@@ -197,7 +197,7 @@ __device__ __forceinline__ void paged_decode_gather(const PagedDecodeParams& p, 
       float pm[8], pl[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int k = min(k0 + i * runs, np - 1);  // past the last: the last again, without weight
+        const int k = min(k0 + i * runs, np - 1);  // past the last: the last again, not added
         const int slot = (2 * (w0 + k) + (k == 0 ? late : 0)) * p.cols;
         po[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(ra, slot * (D * 4) + item * 16, 0, kSc1));
         const auto ml = __builtin_amdgcn_raw_buffer_load_b64(rm, (slot + col) * 8, 0, kSc1);
@@ -213,7 +213,8 @@ __device__ __forceinline__ void paged_decode_gather(const PagedDecodeParams& p, 
       M = now;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float f = k0 + i * runs < np ? __builtin_amdgcn_exp2f(pm[i] - M) : 0.f;
+        if (k0 + i * runs >= np) continue;  // not by a weight of 0: the last one may hold an infinity
+        const float f = __builtin_amdgcn_exp2f(pm[i] - M);
         L += f * pl[i];
         o += f * po[i];
       }
