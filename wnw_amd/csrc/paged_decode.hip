@@ -213,10 +213,11 @@ __device__ __forceinline__ void paged_decode_gather(const PagedDecodeParams& p, 
       M = now;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (k0 + i * runs >= np) continue;  // not by a weight of 0: the last one may hold an infinity
-        const float f = __builtin_amdgcn_exp2f(pm[i] - M);
+        const bool in = k0 + i * runs < np;  // a weight of 0 would not do: the last one may hold an infinity
+        const float f = in ? __builtin_amdgcn_exp2f(pm[i] - M) : 0.f;
         L += f * pl[i];
-        o += f * po[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] += f * (in ? po[i][j] : 0.f);
       }
     }
     if (runs == 1) {
