@@ -1,6 +1,6 @@
 """The paged cache's attention over numbers that a query must not feel: scales of
-pages that no segment names, infinities in one of a segment's pieces.  Tolerances
-as in test_gpu_paged.py, from the same bounds."""
+pages that no segment names, infinities in one of a segment's pieces, rows
+without weight.  Tolerances as in test_gpu_paged.py, from the same bounds."""
 import pytest
 import torch
 
@@ -91,3 +91,20 @@ def test_decode_infinities_stay_infinities(gpu, q8, dtype, D, G, n):
     k, v = c.rows(0)
     ref, A = attend(q[0].double(), k, v[:, keep], torch.full((G,), n, device=gpu), 3.0 / D)
     _check(out[0][:, keep], ref, HALF[dtype] * ref.abs() + 2.0 ** -13 * A, n)
+
+
+@pytest.mark.parametrize("dtype,D,G", [(BF, 128, 4), (BF, 64, 1), (BF, 256, 16), (FP, 128, 4), (FP, 256, 2)])
+@pytest.mark.parametrize("n", [2, 33, 100, 1500, 20000])
+def test_decode_largest_values_without_weight(gpu, dtype, D, G, n):
+    """V at the type's largest number in rows whose weight is 0 in 32 bits: they add nothing."""
+    c = Cache(gpu, [n, 40], 64, D, dtype, False, seed=n + D)
+    u = torch.randn(D, device=gpu, generator=torch.Generator(device=gpu).manual_seed(5))
+    u = u / u.norm() * D ** 0.5
+    q = (u + 0.2 * _q(gpu, 2, G, D, dtype).float()).to(dtype)
+    for r in {0, n // 2, n // 3} if n > 2 else {0}:
+        p, at = c.table[0, r // 64].item(), r % 64
+        c.k[p, at] = (u * -30).to(dtype)
+        c.v[p, at] = torch.finfo(dtype).max
+    out = paged_decode_attn(q, *c.args(), 10.0 / D)
+    _clean()
+    _decode_check(c, q, out, 10.0 / D)

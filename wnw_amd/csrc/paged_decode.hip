@@ -106,18 +106,23 @@ struct PagedDecodeV {
   static constexpr uint32_t read_x(int i) { return (Q8 ? 16 : 32) * i; }
 };
 
-// Two values, positive or zero, as two pairs of 16-bit parts, the lower ones at least `least`
+// Two weights as two pairs of 16-bit parts.  The lower parts of weights that are not 0 are not 0
+// either: an infinity of V times such a part would be NaN.  bf16's are 2^-24 of the upper at least
+// (a weight has 16 bits here), f16's, short of exponents, its least number, 2^-36 of the
+// largest weight; what has no weight adds nothing, however large.
 template <typename T>
-__device__ __forceinline__ void two_parts(float a, float b, float least, uint32_t* hi, uint32_t* lo) {
+__device__ __forceinline__ void two_parts(float a, float b, uint32_t* hi, uint32_t* lo) {
   if constexpr (std::is_same<T, bf16_t>::value) {
     const uint32_t ua = __float_as_uint(a) & 0xffff0000u, ub = __float_as_uint(b) & 0xffff0000u;
     *hi = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
-    const float la = fmaxf(a - __uint_as_float(ua), least), lb = fmaxf(b - __uint_as_float(ub), least);
+    const float ha = __uint_as_float(ua), hb = __uint_as_float(ub);
+    const float la = fmaxf(a - ha, ha * 0x1p-24f), lb = fmaxf(b - hb, hb * 0x1p-24f);
     *lo = __builtin_amdgcn_perm(__float_as_uint(lb), __float_as_uint(la), 0x07060302u);
   } else {
     const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
     *hi = __builtin_bit_cast(uint32_t, h);
-    const float la = fmaxf(a - (float)h[0], least), lb = fmaxf(b - (float)h[1], least);
+    const float ha = (float)h[0], hb = (float)h[1];
+    const float la = fmaxf(a - ha, fminf(ha, 0x1p-24f)), lb = fmaxf(b - hb, fminf(hb, 0x1p-24f));
     *lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(la, lb));
   }
 }
@@ -524,8 +529,6 @@ paged_decode_kernel(PagedDecodeParams p) {
           for (int i = 0; i < DT; ++i) acc[i] *= fall;
           m = mx;
         }
-        // the type's least number, so that an infinity that a column sees stays one; none beside masked rows
-        const float least_part = edge && r.count > 1 ? 0.f : std::is_same<VT, f16_t>::value ? 5.9604645e-8f : 1.17549435e-38f;
         u32x4 hi, lo;
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
@@ -538,7 +541,7 @@ paged_decode_kernel(PagedDecodeParams p) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             uint32_t uh, ul;
-            two_parts<VT>(y[t2][2 * i], y[t2][2 * i + 1], least_part, &uh, &ul);
+            two_parts<VT>(y[t2][2 * i], y[t2][2 * i + 1], &uh, &ul);
             hi[2 * t2 + i] = uh;
             lo[2 * t2 + i] = ul;
           }
