@@ -1,6 +1,12 @@
 """The paged cache's attention over numbers that a query must not feel: scales of
-pages that no segment names, infinities in one of a segment's pieces, rows
-without weight.  Tolerances as in test_gpu_paged.py, from the same bounds."""
+pages that no segment names, V scales of pages that a causal mask hides or that
+have no weight, values of such rows; and infinities that it does see.  Tolerances
+per element, h = half a step of the result's type, A = sum of |weight * value|
+over the rows that the query sees:
+* decode attention: h |ref| + 2^-13 A, as in test_gpu_paged.py;
+* prompt attention: h |ref| + (h + 2^-13) A, and nothing for rows that the query
+  does not see; f16 results below 2^-14 are whole multiples of 2^-24: 2^-25.
+"""
 import pytest
 import torch
 
@@ -108,3 +114,75 @@ def test_decode_largest_values_without_weight(gpu, dtype, D, G, n):
     out = paged_decode_attn(q, *c.args(), 10.0 / D)
     _clean()
     _decode_check(c, q, out, 10.0 / D)
+
+def _rows_check(c, q, out, new, scale, tokens):
+    """The first ``tokens`` tokens of one sample with one KV head, against the rows that each sees alone."""
+    n, G, D = new, q.shape[1], q.shape[2]
+    k, v = c.rows(0)
+    lim = c.lens[0] - n + torch.arange(tokens, device=q.device).repeat_interleave(G) + 1
+    most = int(lim[-1])
+    ref, A = attend(q[:tokens].reshape(-1, D).double(), k[:most], v[:most], lim, scale)
+    h = HALF[q.dtype]
+    bound = h * ref.abs() + (h + 2.0 ** -13) * A + (2.0 ** -25 if q.dtype == FP else 0)
+    _check(out[:tokens].reshape(-1, D), ref, bound, (new, tokens))
+
+
+# new tokens after old rows: one tile, several, splits of a long segment, the few rows of the decode kernel
+SHAPES = [(90, 0), (70, 400), (300, 700), (40, 6000), (3, 110)]
+HIDDEN = [(FP, r) for r in (20, 24, 26, 30, 35, 60)] + [(BF, r) for r in (30, 60, 100, 116)]
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new,old", SHAPES, ids=lambda x: str(x))
+@pytest.mark.parametrize("dtype,ratio", HIDDEN, ids=lambda x: str(x).replace("torch.", ""))
+def test_hidden_pages_have_no_say_in_the_scale(gpu, dtype, ratio, new, old, D):
+    """V pages of later tokens 2^ratio above the others: the tokens before them give what they gave."""
+    page, G = 16, 4
+    c = Cache(gpu, [old + new], page, D, dtype, True, seed=D + new + ratio, room=1)
+    q = _q(gpu, new, G, D, dtype)
+    first = (old + new - 1) // page  # the block of the last rows
+    before = first * page - old      # tokens that do not see it
+    want = paged_prompt_attn(q, *c.args(), _cu([new], gpu), 0.1, **c.scales())
+    c.v_scale[c.table[0, first].item()] *= 2.0 ** ratio
+    got = paged_prompt_attn(q, *c.args(), _cu([new], gpu), 0.1, **c.scales())
+    _clean()
+    assert torch.equal(got[:before], want[:before])
+    _rows_check(c, q, got, new, 0.1, before)
+    if dtype == BF:  # the others see it: its values fit the result's type
+        _rows_check(c, q, got, new, 0.1, new)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new,old", SHAPES, ids=lambda x: str(x))
+@pytest.mark.parametrize("dtype,ratio", HIDDEN, ids=lambda x: str(x).replace("torch.", ""))
+def test_pages_without_weight_have_no_say_in_the_scale(gpu, dtype, ratio, new, old, D):
+    """The first block's V 2^ratio above the others' and its K against every query: seen, and of no weight."""
+    page, G = 16, 4
+    c = Cache(gpu, [old + new + page], page, D, dtype, True, seed=D + new + ratio)
+    u = torch.randn(D, device=gpu, generator=torch.Generator(device=gpu).manual_seed(5))
+    u = u / u.norm() * D ** 0.5
+    q = (u + 0.2 * _q(gpu, new, G, D, dtype).float()).to(dtype)
+    p = c.table[0, 0].item()
+    c.k[p] = (u * -30).clamp(-448, 448).to(c.k.dtype)
+    c.k_scale[p] = 1.0
+    c.v_scale[p] *= 2.0 ** ratio
+    scale = 10.0 / D  # the block's scores: -300 of base e
+    out = paged_prompt_attn(q, *c.args(), _cu([new], gpu), scale, **c.scales())
+    _clean()
+    _rows_check(c, q, out, new, scale, new)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new,old", SHAPES, ids=lambda x: str(x))
+@pytest.mark.parametrize("dtype,low,high", [(FP, -13, 12), (FP, -10, 10), (BF, -70, 10), (BF, -60, 118), (BF, -30, 30)],
+                         ids=lambda x: str(x).replace("torch.", ""))
+def test_prompt_scales_far_apart(gpu, dtype, low, high, new, old, D):
+    """Every third block's V at 2^high and the others' at 2^low, all of them seen: each element to its own sum's bound."""
+    page, G = 16, 4
+    c = Cache(gpu, [old + new], page, D, dtype, True, seed=D + new - low)
+    for i in range(-(-(old + new) // page)):
+        c.v_scale[c.table[0, i].item()] *= 2.0 ** (high if i % 3 == 2 else low)
+    q = _q(gpu, new, G, D, dtype)
+    out = paged_prompt_attn(q, *c.args(), _cu([new], gpu), 0.1, **c.scales())
+    _clean()
+    _rows_check(c, q, out, new, 0.1, new)

@@ -17,8 +17,12 @@
 // elements once for all waves; one barrier per tile, the next tile written among
 // the products of S and the one after it loaded then (head_dim 256: one buffer,
 // two barriers).  K's page scale multiplies the exponent, V's is added to it as
-// its logarithm relative to the largest so far (a part of 2^x either way), so
-// that scales cost a few instructions per 16 keys and any scale fits 16 bits.
+// its logarithm (a part of 2^x either way), so that scales cost a few
+// instructions per 16 keys.  Such weights are held in bf16, whose exponents reach
+// from the append's least scale, 2^-64, to its largest, 2^120: no page but a
+// query's own has a say in how its weights are held.  f16 queries, whose weights
+// have 11 bits over 16-bit pages, have two parts of 8 here (2,048 tokens at
+// head_dim 64 and 128: 46.8 and 71.2 us, bf16 queries 40.7 and 60.2).
 //
 // Few query rows and many keys: the tiles of each block of rows are cut into
 // splits, whose sums a second launch adds up.
@@ -54,7 +58,7 @@ struct PagedPromptParams {
   const void* q;
   void* out;
   int64_t qt, qh, ot, oh;  // strides in elements
-  float* part;             // [blocks, splits, waves]: D / 32 x 16 sums a lane, then max, sum, scale
+  float* part;             // [blocks, splits, waves]: D / 32 x 16 sums a lane, then max, sum
   float scale_log2;
   int32_t G, nqb, splits;
   int32_t* err;
@@ -102,12 +106,12 @@ __device__ __forceinline__ int tiles_of(const PagedPromptParams& p, const Prompt
 // elements 32 i + 8 j + 4 hi + 0..3 of row n
 template <typename T, int NT>
 __device__ __forceinline__ void prompt_store(const PagedPromptParams& p, const PromptRows& r, int row, int h, int hi, int dt0,
-                                             const f32x16* o, float l, float ref) {
+                                             const f32x16* o, float l) {
   if (row >= r.rows) return;
   const int i = row / p.G, g = row - i * p.G;
   T* op = (T*)p.out + (int64_t)(r.first + i) * p.ot + (int64_t)(h * p.G + g) * p.oh;
   const bool none = r.len - r.count + i + 1 <= 0;
-  const float inv = __builtin_amdgcn_exp2f(ref) / l;
+  const float inv = 1.0f / l;
 #pragma unroll
   for (int dt = 0; dt < NT; ++dt)
 #pragma unroll
@@ -119,9 +123,12 @@ __device__ __forceinline__ void prompt_store(const PagedPromptParams& p, const P
     }
 }
 
+// Registers for at most 3 waves per SIMD: made to fit 4, head_dim 64 over 8 bits takes 43.5 us for 40.7 (2,048 tokens).
 template <typename T, int D, bool Q8, int W>
-__global__ __launch_bounds__((64 * W), (D == 256 && !Q8 ? 1 : 2)) void paged_prompt_kernel(PagedPromptParams p) {
-  using Ops = HalfOps<T>;
+__global__ __launch_bounds__((64 * W)) __attribute__((amdgpu_waves_per_eu((D == 256 && !Q8 ? 1 : 2), (D == 256 && !Q8 ? 1 : 3)))) void
+paged_prompt_kernel(PagedPromptParams p) {
+  using VT = typename std::conditional<Q8, bf16_t, T>::type;   // the value product's type
+  using VO = HalfOps<VT>;
   using PE = typename std::conditional<Q8, uint8_t, T>::type;  // the pages' elements
   constexpr int kPpQ = 32 * W;
   constexpr int RB = D * 2, CH = RB / 16, TB = kPpKeys * RB;  // a tile in LDS: 16-bit elements
@@ -130,8 +137,10 @@ __global__ __launch_bounds__((64 * W), (D == 256 && !Q8 ? 1 : 2)) void paged_pro
   constexpr int KK = D / 16, DT = D / 32;
   constexpr int NB = D == 256 ? 1 : 2;  // tiles in LDS
   constexpr bool kAhead = D != 256 || !Q8;  // the next tile's loads are on their way during the products
-  // f16 weights are held times 2^8: normal numbers down to 2^-22 of the largest
-  constexpr float kBias = std::is_same<T, f16_t>::value ? 8.f : 0.f;
+  // f16 weights are held times 2^8: normal numbers down to 2^-22 of the largest;
+  // those with a scale of V times 2^-16: 2^16 times the largest value is a sum yet
+  constexpr float kBias = std::is_same<VT, f16_t>::value ? 8.f : Q8 ? -16.f : 0.f;
+  constexpr bool kTwo = Q8 && std::is_same<T, f16_t>::value;  // weights of two parts
   __shared__ __attribute__((aligned(16))) uint8_t lds[NB * 2 * TB];  // [NB][K, V]
   __shared__ int odd;  // V had infinities or NaN in such a tile
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -267,8 +276,8 @@ __global__ __launch_bounds__((64 * W), (D == 256 && !Q8 ? 1 : 2)) void paged_pro
       if constexpr (Q8) {
         *(u32x4*)(kd + (kput ^ kx)) = e4m3x8<T>(kr[u][0], kr[u][1]);
         *(u32x4*)(kd + (kput ^ kx ^ kHalf)) = e4m3x8<T>(kr[u][2], kr[u][3]);
-        *(u32x4*)(vd + vput) = e4m3x8<T>(vr[u][0], vr[u][1]);
-        *(u32x4*)(vd + (vput ^ kHalf)) = e4m3x8<T>(vr[u][2], vr[u][3]);
+        *(u32x4*)(vd + vput) = e4m3x8<VT>(vr[u][0], vr[u][1]);
+        *(u32x4*)(vd + (vput ^ kHalf)) = e4m3x8<VT>(vr[u][2], vr[u][3]);
       } else {
         *(u32x4*)(kd + (kput ^ kx)) = kr[u];
         *(u32x4*)(vd + vput) = vr[u];
@@ -288,17 +297,12 @@ __global__ __launch_bounds__((64 * W), (D == 256 && !Q8 ? 1 : 2)) void paged_pro
   for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
   float m = kPgLowest, l = 0.f;
   // Q8, per 16 keys of the window that the products are in: what a score is
-  // worth in the exponent, the logarithm of V's scale relative to the largest so
-  // far (ref), and what undoes it
-  float ref = -100.f, wk = 0.f, wl = 0.f, wu = 0.f;
+  // worth in the exponent, the logarithm of V's scale, and what undoes it.  V's
+  // scales below 2^-80 (one of 0 too) count as that.
+  float wk = 0.f, wl = 0.f, wu = 0.f;
   auto enter_scales = [&]() {
     wk = fmaxf(ks, 7.888609e-31f) * p.scale_log2;  // a scale of 0 would make a masked score NaN
-    const float lg = __builtin_amdgcn_logf(vs), most = fmaxf(ref, wave_max(lg));
-    const float f = __builtin_amdgcn_exp2f(ref - most);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
-    ref = most;
-    wl = fmaxf(lg - ref, -100.f);  // less is nothing beside the largest
+    wl = fminf(fmaxf(__builtin_amdgcn_logf(vs), -80.f), 127.f);
     wu = __builtin_amdgcn_exp2f(-wl);
   };
   auto tile = [&](int i, auto masked) {
@@ -353,7 +357,7 @@ __global__ __launch_bounds__((64 * W), (D == 256 && !Q8 ? 1 : 2)) void paged_pro
       for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
       m = mx;
     }
-    u32x4 pb[4];
+    u32x4 pb[4], pc[kTwo ? 4 : 1];
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       const float off = lv[b] - m + kBias;
@@ -363,7 +367,13 @@ __global__ __launch_bounds__((64 * W), (D == 256 && !Q8 ? 1 : 2)) void paged_pro
         const float y0 = __builtin_amdgcn_exp2f(fmaf(s[b >> 1][8 * (b & 1) + 2 * j], ck[b], off));
         const float y1 = __builtin_amdgcn_exp2f(fmaf(s[b >> 1][8 * (b & 1) + 2 * j + 1], ck[b], off));
         sum += y0 + y1;
-        pb[b][j] = Ops::pack2(y0, y1);
+        if constexpr (kTwo) {
+          const uint32_t u0 = __float_as_uint(y0), u1 = __float_as_uint(y1);
+          pb[b][j] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);  // the upper part cut off, what is left rounded
+          pc[b][j] = VO::pack2(y0 - __uint_as_float(u0 & 0xffff0000u), y1 - __uint_as_float(u1 & 0xffff0000u));
+        } else {
+          pb[b][j] = VO::pack2(y0, y1);
+        }
       }
       l = Q8 ? fmaf(sum, un[b], l) : l + sum;
     }
@@ -371,9 +381,11 @@ __global__ __launch_bounds__((64 * W), (D == 256 && !Q8 ? 1 : 2)) void paged_pro
     for (int b = 0; b < 4; ++b)
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const uint64_t v0 = Ops::read_tr(vt + (vget ^ 64 * dt) + 16 * b * RB);
-        const uint64_t v1 = Ops::read_tr(vt + (vget ^ 64 * dt) + (16 * b + 8) * RB);
-        o[dt] = mma32<T>(u32x4{(uint32_t)v0, (uint32_t)(v0 >> 32), (uint32_t)v1, (uint32_t)(v1 >> 32)}, pb[b], o[dt]);
+        const uint64_t v0 = VO::read_tr(vt + (vget ^ 64 * dt) + 16 * b * RB);
+        const uint64_t v1 = VO::read_tr(vt + (vget ^ 64 * dt) + (16 * b + 8) * RB);
+        const u32x4 v{(uint32_t)v0, (uint32_t)(v0 >> 32), (uint32_t)v1, (uint32_t)(v1 >> 32)};
+        o[dt] = mma32<VT>(v, pb[b], o[dt]);
+        if constexpr (kTwo) o[dt] = mma32<VT>(v, pc[b], o[dt]);
       }
   };
   if (t0 < t1) {
@@ -446,9 +458,9 @@ __global__ __launch_bounds__((64 * W), (D == 256 && !Q8 ? 1 : 2)) void paged_pro
   }
   l = sum_x32(l);
   if (splits == 1) {
-    prompt_store<T, DT>(p, r, row, h, hi, 0, o, l, Q8 ? ref : 0.f);
+    prompt_store<T, DT>(p, r, row, h, hi, 0, o, l);
   } else if (busy) {
-    float* part = p.part + ((((int64_t)block * N + seg) * p.splits + split) * W + w) * (DT * 16 + 3) * 64;
+    float* part = p.part + ((((int64_t)block * N + seg) * p.splits + split) * W + w) * (DT * 16 + 2) * 64;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -458,7 +470,6 @@ __global__ __launch_bounds__((64 * W), (D == 256 && !Q8 ? 1 : 2)) void paged_pro
     part += DT * 16 * 64;
     part[lane] = m;
     part[64 + lane] = l;
-    part[128 + lane] = Q8 ? ref : 0.f;
   }
 }
 
@@ -467,7 +478,7 @@ __global__ __launch_bounds__((64 * W), (D == 256 && !Q8 ? 1 : 2)) void paged_pro
 template <typename T, int D, int W>
 __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParams p) {
   constexpr int DT = D / 32, kPpQ = 32 * W;
-  __shared__ float sums[4][19][64];
+  __shared__ float sums[4][18][64];
   const int lane = threadIdx.x & 63, k = threadIdx.x >> 6, hi = lane >> 5, n = lane & 31;
   const int N = p.c.n_seg, block = blockIdx.x / (W * DT), w = blockIdx.x / DT % W, dt = blockIdx.x % DT;
   const int seg = block % N, qblk = p.nqb - 1 - block / N;
@@ -475,19 +486,17 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParam
   if (qblk * kPpQ + 32 * w >= r.rows) return;
   const int splits = splits_of(tiles_of<W>(p, r, qblk), p.splits);
   if (splits == 1) return;
-  constexpr int64_t kPart = (DT * 16 + 3) * 64;
+  constexpr int64_t kPart = (DT * 16 + 2) * 64;
   const float* part = p.part + ((int64_t)block * p.splits * W + w) * kPart;
   f32x16 o = f32x16{};
-  float m = kPgLowest, l = 0.f, ref = -100.f;
-  auto add = [&](float pm, float pl, float pr, const f32x16& y) {
-    const float mx = fmaxf(m, pm), most = fmaxf(ref, pr);
+  float m = kPgLowest, l = 0.f;
+  auto add = [&](float pm, float pl, const f32x16& y) {
+    const float mx = fmaxf(m, pm);
     const float f = __builtin_amdgcn_exp2f(m - mx), g = __builtin_amdgcn_exp2f(pm - mx);
-    const float fo = f * __builtin_amdgcn_exp2f(ref - most), go = g * __builtin_amdgcn_exp2f(pr - most);
     l = l * f + pl * g;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) o[e] = o[e] * fo + y[e] * go;
+    for (int e = 0; e < 16; ++e) o[e] = o[e] * f + y[e] * g;
     m = mx;
-    ref = most;
   };
 #pragma unroll 2
   for (int s = k; s < splits; s += 4) {
@@ -500,13 +509,12 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParam
       for (int e = 0; e < 4; ++e) y[4 * j + e] = z[e];
     }
     at += DT * 16 * 64 + lane;
-    add(gptr<float>(at)[0], gptr<float>(at)[64], gptr<float>(at)[128], y);
+    add(gptr<float>(at)[0], gptr<float>(at)[64], y);
   }
 #pragma unroll
   for (int e = 0; e < 16; ++e) sums[k][e][lane] = o[e];
   sums[k][16][lane] = m;
   sums[k][17][lane] = l;
-  sums[k][18][lane] = ref;
   __syncthreads();
   if (k != 0) return;
 #pragma unroll 1
@@ -514,9 +522,9 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParam
     f32x16 y;
 #pragma unroll
     for (int e = 0; e < 16; ++e) y[e] = sums[i][e][lane];
-    add(sums[i][16][lane], sums[i][17][lane], sums[i][18][lane], y);
+    add(sums[i][16][lane], sums[i][17][lane], y);
   }
-  prompt_store<T, 1>(p, r, qblk * kPpQ + 32 * w + n, seg % p.t.hkv, hi, dt, &o, l, ref);
+  prompt_store<T, 1>(p, r, qblk * kPpQ + 32 * w + n, seg % p.t.hkv, hi, dt, &o, l);
 }
 
 // How a call is cut, from what the host knows of it (us measured on one GPU, bf16
@@ -546,7 +554,7 @@ static PromptPlan prompt_plan(int64_t n_seg, int64_t group, int64_t max_tokens, 
   const int64_t wgs = std::max<int64_t>(n_seg * y.nqb, 1), want = (y.waves == 8 ? 1 : 2) * cus;
   y.splits = std::max<int64_t>(1, std::min({want / wgs, tiles / 4, (int64_t)64}));
   if (tiles - tiles / y.splits < 8) y.splits = 1;
-  y.bytes = y.splits == 1 ? 0 : wgs * y.splits * y.waves * (D / 2 + 3) * 64 * 4;
+  y.bytes = y.splits == 1 ? 0 : wgs * y.splits * y.waves * (D / 2 + 2) * 64 * 4;
   return y;
 }
 
