@@ -1,6 +1,7 @@
 """The paged cache's attention over numbers that a query must not feel: scales of
 pages that no segment names, V scales of pages that a causal mask hides or that
-have no weight, values of such rows; and infinities that it does see.  Tolerances
+have no weight, values of such rows; and of infinities and the type's largest
+values that it does see.  Tolerances
 per element, h = half a step of the result's type, A = sum of |weight * value|
 over the rows that the query sees:
 * decode attention: h |ref| + 2^-13 A, as in test_gpu_paged.py;
@@ -186,3 +187,23 @@ def test_prompt_scales_far_apart(gpu, dtype, low, high, new, old, D):
     out = paged_prompt_attn(q, *c.args(), _cu([new], gpu), 0.1, **c.scales())
     _clean()
     _rows_check(c, q, out, new, 0.1, new)
+
+
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("D,G,new,old", [(128, 4, 1, 3), (128, 4, 1, 9000), (64, 1, 3, 300), (128, 4, 90, 0), (64, 4, 300, 700),
+                                         (256, 4, 60, 100), (128, 4, 40, 6000), (128, 8, 2, 20)])
+def test_sums_of_the_largest_values(gpu, q8, D, G, new, old):
+    """V near bf16's largest number in every row: the mean of such rows is no infinity, though their sum is."""
+    c = Cache(gpu, [old + new], 64, D, BF, q8, seed=D + new + old)
+    sign = torch.where(torch.arange(D, device=gpu) % 3 == 0, -1.0, 1.0)
+    if q8:
+        c.v.copy_((sign * 416).to(c.v.dtype).expand(c.v.shape))
+        c.v_scale.fill_(2.0 ** 119)
+    else:
+        c.v.copy_((sign * 2.75e38).to(BF).expand(c.v.shape))
+    q = _q(gpu, new, G, D, BF)
+    out = paged_prompt_attn(q, *c.args(), _cu([new], gpu), 0.1, **c.scales())
+    _clean()
+    _rows_check(c, q, out, new, 0.1, new)
+    if new == 1:
+        assert torch.equal(paged_decode_attn(q, *c.args(), 0.1, **c.scales()), out)

@@ -263,8 +263,9 @@ paged_decode_kernel(PagedDecodeParams p) {
   using Vl = PagedDecodeV<D, Q8>;
   constexpr int W = Ge::kWaves, NT = 64 * W;
   constexpr int RB = Ge::RB, KC = Ge::KC, VI = Ge::VI, DT = D / 16, KK = D / 32;
-  // weights of f16 are held times 2^12: their lower parts reach 2^-36 of the largest
-  constexpr float kBias = std::is_same<VT, f16_t>::value ? 12.f : 0.f;
+  // weights of f16 are held times 2^12: their lower parts reach 2^-36 of the
+  // largest; of bf16 times 2^-16: 2^16 times the type's largest value is a sum yet
+  constexpr float kBias = std::is_same<VT, f16_t>::value ? 12.f : -16.f;
   __shared__ __attribute__((aligned(16))) uint8_t lds[W * Ge::kPart];
   __shared__ float st[W][16][2];
   __shared__ int32_t sh[2 * W];

@@ -138,8 +138,8 @@ paged_prompt_kernel(PagedPromptParams p) {
   constexpr int NB = D == 256 ? 1 : 2;  // tiles in LDS
   constexpr bool kAhead = D != 256 || !Q8;  // the next tile's loads are on their way during the products
   // f16 weights are held times 2^8: normal numbers down to 2^-22 of the largest;
-  // those with a scale of V times 2^-16: 2^16 times the largest value is a sum yet
-  constexpr float kBias = std::is_same<VT, f16_t>::value ? 8.f : Q8 ? -16.f : 0.f;
+  // bf16 ones times 2^-16: 2^16 times the type's largest value is a sum yet
+  constexpr float kBias = std::is_same<VT, f16_t>::value ? 8.f : -16.f;
   constexpr bool kTwo = Q8 && std::is_same<T, f16_t>::value;  // weights of two parts
   __shared__ __attribute__((aligned(16))) uint8_t lds[NB * 2 * TB];  // [NB][K, V]
   __shared__ int odd;  // V had infinities or NaN in such a tile
