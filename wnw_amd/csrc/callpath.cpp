@@ -318,8 +318,9 @@ PyObject* paged_decode_impl(PyObject* const* a) {
   const bool has_stream = stream_of(dev, &so, &stream);
   Ref stream_ref(so);
   if (!has_stream) return nullptr;
-  Ref ws(PyObject_CallFunction(g_paged_ws, "LOLL", (long long)dev, so, (long long)c.n_seg,
-                               (long long)wnw_paged_decode_workspace_bytes(c.n_seg, g, c.head_dim)));
+  const int64_t need = wnw_paged_decode_workspace_bytes(c.n_seg, g, c.head_dim);
+  if (need < 0) Py_RETURN_NONE;  // the general path says why
+  Ref ws(PyObject_CallFunction(g_paged_ws, "LOLL", (long long)dev, so, (long long)c.n_seg, (long long)need));
   const at::Tensor* buf = buffer(ws);
   if (!buf) return nullptr;
   void *qp = q->data_ptr(), *op = out.data_ptr(), *wp = buf->data_ptr();

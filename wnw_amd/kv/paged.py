@@ -95,7 +95,9 @@ def call_workspace(idx: int, stream: int, n_seg: int, need: int) -> Tensor:
     return buf
 
 
-def _workspace(dev: torch.device, n_seg: int, need: int, given: PagedWorkspace | None) -> Tensor:
+def _workspace(dev: torch.device, n_seg: int, need: int, given: PagedWorkspace | None) -> Tensor | None:
+    if need < 0:  # a cache that the library does not take: the call itself says why
+        return None
     if given is not None:
         return given.get(dev, n_seg, need)
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
