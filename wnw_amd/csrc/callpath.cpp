@@ -14,6 +14,8 @@
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -208,14 +210,19 @@ PyObject* score_impl(PyObject* const* a) {
 }
 
 // The paged cache's operators.  Their tensors may be on another device than
-// the current one, and a call that would need a gradient is left to the general
-// path's refusal.
-bool needs_grad(const at::Tensor* t) { return t && c10::GradMode::is_enabled() && t->requires_grad(); }
+// the current one, and a call that would need a gradient (or has a tangent), or
+// that may be traced, is left to the general path's refusal.
+bool needs_grad(const at::Tensor* t) {
+  return t && ((c10::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined());
+}
+bool watched() {
+  return c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer) || c10::impl::TorchDispatchModeTLS::any_modes_set();
+}
 
 bool paged_cache(PyObject* const* a, PyObject* ks, PyObject* vs, const at::Tensor& q, wnw_paged_cache* c,
                  const int32_t** seg_len) {
   const at::Tensor *k = plain(a[0]), *v = plain(a[1]), *table = plain(a[2]), *len = plain(a[3]);
-  if (!k || !v || !table || !len || k->dim() != 3 || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type())
+  if (watched() || !k || !v || !table || !len || k->dim() != 3 || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type())
     return false;
   const at::ScalarType dt = k->scalar_type();
   const bool q8 = dt == at::kFloat8_e4m3fn;

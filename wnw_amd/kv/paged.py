@@ -20,7 +20,8 @@ are only read may share pages.  Lengths, table entries and token offsets live
 on the device, so launches captured in a HIP graph follow them; bad ones set
 the device error word (``wnw_amd._lib.device_error()``) and nothing outside the
 arrays is touched.  The kernels write behind autograd's back: inputs that
-require a gradient are refused.
+require a gradient or carry a tangent are refused, and so are calls that are
+being traced.
 """
 from __future__ import annotations
 
@@ -29,6 +30,7 @@ from collections.abc import Sequence
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -114,6 +116,12 @@ def _cache(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seg_len: Tensor
         raise _lib.WnwError("all tensors of a call must be on one device")
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise _lib.WnwError("the paged cache's operators have no gradient: call them under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise _lib.WnwError("the paged cache's operators have no forward-mode gradient either")
+    if torch._C._get_tracing_state() is not None \
+            or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise _lib.WnwError("the paged cache's operators cannot be traced: a trace would hold outputs that nothing writes")
     if k_pages.dim() != 3 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype \
             or k_pages.dtype not in _PAGE_DTYPES:
         raise _lib.WnwError(f"k_pages / v_pages must be equal [P, R, D] of bf16, f16 or e4m3: {tuple(k_pages.shape)} "
