@@ -818,6 +818,7 @@ int wnw_paged_append(const wnw_paged_cache* cache, const int32_t* seg_len,
 /*
  * Decode attention over the cache: q, out [n_seg, group, head_dim], group at
  * most 16; 16-bit pages have q's type.  A segment without rows gives zeros.
+ * out may be q itself, but cover no other part of it (prompt attention's too).
  * The first wnw_paged_counter_bytes of the workspace (256-byte aligned, of at
  * least wnw_paged_decode_workspace_bytes(n_seg, group, head_dim)) must be zero
  * before its first use and are left zero by every launch; launches that may

@@ -30,6 +30,7 @@
 // dependent round trips: lengths, table, pages, partial sums, counter (8 segments
 // of at most 813 rows: 11.3 us).
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "paged.h"
@@ -760,6 +761,22 @@ int paged_decode_launch(const wnw_paged_cache* cache, const int32_t* seg_len, co
   return WNW_OK;
 }
 
+// Whether out's rows [tokens, heads, D] overlap q's without being q itself, whose rows other workgroups may yet read.
+bool paged_out_over_q(const void* q, const void* out, const int64_t* strides, int64_t tokens, int64_t heads, int64_t D) {
+  const int64_t qt = tokens > 1 ? strides[0] : 0, qh = heads > 1 ? strides[1] : 0;
+  const int64_t ot = tokens > 1 ? strides[2] : 0, oh = heads > 1 ? strides[3] : 0;
+  const int64_t apart = ((intptr_t)out - (intptr_t)q) / 2;  // elements
+  const bool alike = qt == ot && qh == oh;
+  if (apart >= (tokens - 1) * qt + (heads - 1) * qh + D || -apart >= (tokens - 1) * ot + (heads - 1) * oh + D) return false;
+  if (!alike || apart == 0) return !alike;
+  for (int64_t h = 1 - heads; h < heads; ++h) {  // the nearest rows h heads apart
+    const int64_t x = apart - h * qh, t = qt ? x / qt : 0;
+    for (int64_t i = t - 1; i <= t + 1; ++i)
+      if (i > -tokens && i < tokens && std::abs(x - i * qt) < D) return true;
+  }
+  return false;
+}
+
 // Checks of an attention call that the cache's own do not cover.
 int paged_attn_check(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, const void* out,
                      const int64_t* strides, int64_t group, float scale, int dtype) {
@@ -797,6 +814,7 @@ extern "C" int wnw_paged_decode_attn(const wnw_paged_cache* cache, const int32_t
   const int64_t strides[4] = {group * D, D, group * D, D};
   if (int rc = paged_attn_check(cache, seg_len, q, out, strides, group, scale, dtype)) return rc;
   WNW_CHECK_ARG(group <= 16, "at most 16 query heads per KV head (%lld)", (long long)group);
+  WNW_CHECK_ARG(!paged_out_over_q(q, out, strides, cache->n_seg, group, D), "out covers a part of q");
   // every segment as a sample with one KV head and one token
   const PagedTokens t{nullptr, (int32_t)cache->n_seg, 1, 1};
   return paged_decode_launch(cache, seg_len, q, out, strides, t, group, scale, dtype, workspace, workspace_bytes, stream);

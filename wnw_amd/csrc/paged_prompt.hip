@@ -50,6 +50,7 @@ int paged_decode_launch(const wnw_paged_cache* cache, const int32_t* seg_len, co
                         void* stream);
 int paged_attn_check(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, const void* out,
                      const int64_t* strides, int64_t group, float scale, int dtype);
+bool paged_out_over_q(const void* q, const void* out, const int64_t* strides, int64_t tokens, int64_t heads, int64_t D);
 
 struct PagedPromptParams {
   PagedCache c;
@@ -607,6 +608,7 @@ extern "C" int wnw_paged_prompt_attn(const wnw_paged_cache* cache, const int32_t
     const bool apart = t >= h ? (heads == 1 || h >= D) && (n_tokens == 1 || t >= h * (heads - 1) + D)
                               : (n_tokens == 1 || t >= D) && (heads == 1 || h >= t * (n_tokens - 1) + D);
     WNW_CHECK_ARG(apart, "the rows of out overlap");
+    WNW_CHECK_ARG(!paged_out_over_q(q, out, strides, n_tokens, heads, D), "out covers a part of q");
   }
   const int64_t most = max_tokens;  // as the workspace's size was asked for
   WNW_CHECK_ARG(most > 0, "max_tokens is zero");
