@@ -29,11 +29,13 @@
 //
 // What bounds it: the instructions.  Per tile and wave at head_dim 128 the products
 // take 1,024 cycles of the matrix unit, 32 exponentials 512 and about 230 other
-// vector instructions 920, and on one SIMD these add up: 4,564 tokens take 213 us
-// of kernel, in which matrix instructions run for 37 % and vector ones for 51 % of
-// the cycles.  That is 0.8 PFLOP/s (plain bf16 products of size 8,192: 1.2).
+// vector instructions 920, and on one SIMD these add up: 4,564 tokens take 442,000
+// cycles, for 37 % of which matrix instructions run and for 51 % vector ones.  That
+// is 196 to 211 us a pass (by the card) where passes have pauses between them, 0.8
+// to 0.87 PFLOP/s (plain bf16 products of size 8,192: 1.2), and 233 us in a row of
+// 24, over which the clock falls to 2.1 GHz or less.
 // Without gain: half of the waves a phase behind the others, so that one's
-// products meet the other's exponentials (231 us; 214 without); the next tile's
+// products meet the other's exponentials (8 % slower in one loop); the next tile's
 // scores among the exponentials (2 to 5 % slower); loads two tiles ahead; raised
 // wave priority in the products.
 #include <algorithm>
