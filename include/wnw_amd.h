@@ -758,8 +758,9 @@ int wnw_read_stream(const void* src, int64_t bytes, int64_t n_wg, int form,
  * entries past a segment's rows are not read.
  *
  * page_dtype WNW_BF16 / WNW_F16: the rows themselves.  WNW_E4M3: codes that
- * stand for code * k_scale[page] (v_scale for V); the scales are positive, and
- * prompt attention takes those of V below 2^-80 for 2^-80.
+ * stand for code * k_scale[page] (v_scale for V); the scales are positive, V's
+ * from 2^-80 up (decode attention holds weights by smaller ones with fewer bits,
+ * prompt attention takes them for 2^-80).
  * Bad lengths, table entries and token offsets set the device error word:
  * WNW_DEVERR_BOUNDS (an entry that is no page, a length below zero or past
  * the table, token offsets that decrease or leave the tokens) or

@@ -9,7 +9,8 @@ neighbours, so it grows without being moved:
 * ``k_pages`` / ``v_pages`` [P, R, D]: R = 16, 32, 64, 128 or 256 rows of D =
   64, 128 or 256 elements; bf16 / f16, or e4m3 (``torch.float8_e4m3fn``) codes;
 * ``k_scale`` / ``v_scale`` float32 [P], with e4m3 pages: a code stands for
-  code * scale, one scale for each block of R tokens of one head;
+  code * scale, one positive scale (V's from 2^-80 up) for each block of R
+  tokens of one head;
 * ``page_table`` int32 [N, M]: row i of segment s is row i % R of page
   ``page_table[s, i // R]``; entries past a segment's rows are not read;
 * ``seg_len`` int32 [N]: rows of each segment.
