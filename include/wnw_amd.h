@@ -851,6 +851,37 @@ int wnw_paged_prompt_attn(const wnw_paged_cache* cache, const int32_t* seg_len,
                           float scale, int dtype, void* workspace,
                           int64_t workspace_bytes, void* stream);
 
+/*
+ * Both attentions through a sliding window with first rows that stay visible:
+ * a row at place r of its segment (r = seg_len - n + i for token i of n) sees the
+ * rows j <= r with j < sinks or j > r - window.  Each of window and sinks is a
+ * device array [n_seg] or, where that is NULL, window_all / sinks_all for all
+ * segments (not negative; values past the cache's rows mean all of them).  A row
+ * that sees none gives zeros.  Table entries of blocks that no row of the call
+ * sees are not read: their pages may have been given back.  A negative entry
+ * sets WNW_DEVERR_BOUNDS, and the segment's outputs are zeros.  Workspaces: the
+ * decode attention's as without a window, the prompt attention's by the function
+ * below, with the same window and sinks.
+ */
+int wnw_paged_decode_attn_window(const wnw_paged_cache* cache,
+                                 const int32_t* seg_len, const void* q,
+                                 void* out, int64_t group,
+                                 const int32_t* window, int64_t window_all,
+                                 const int32_t* sinks, int64_t sinks_all,
+                                 float scale, int dtype, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
+int64_t wnw_paged_prompt_window_workspace_bytes(
+    const wnw_paged_cache* cache, int64_t group, int64_t max_tokens,
+    const int32_t* window, int64_t window_all, const int32_t* sinks,
+    int64_t sinks_all);
+int wnw_paged_prompt_attn_window(
+    const wnw_paged_cache* cache, const int32_t* seg_len, const void* q,
+    void* out, const int64_t* strides, int64_t n_tokens, int64_t n_samples,
+    int64_t group, const int32_t* cu_tokens, int64_t max_tokens,
+    const int32_t* window, int64_t window_all, const int32_t* sinks,
+    int64_t sinks_all, float scale, int dtype, void* workspace,
+    int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

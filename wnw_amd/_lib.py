@@ -73,6 +73,10 @@ _SIGNATURES = {
     "wnw_paged_decode_attn": (_i32, [_vp] * 4 + [_i64, _f32, _i32, _vp, _i64, _vp]),
     "wnw_paged_prompt_workspace_bytes": (_i64, [_vp, _i64, _i64]),
     "wnw_paged_prompt_attn": (_i32, [_vp] * 5 + [_i64] * 3 + [_vp, _i64, _f32, _i32, _vp, _i64, _vp]),
+    "wnw_paged_decode_attn_window": (_i32, [_vp] * 4 + [_i64, _vp, _i64, _vp, _i64, _f32, _i32, _vp, _i64, _vp]),
+    "wnw_paged_prompt_window_workspace_bytes": (_i64, [_vp, _i64, _i64, _vp, _i64, _vp, _i64]),
+    "wnw_paged_prompt_attn_window": (_i32, [_vp] * 5 + [_i64] * 3 + [_vp, _i64, _vp, _i64, _vp, _i64, _f32, _i32, _vp, _i64,
+                                                                  _vp]),
     "wnw_read_stream": (_i32, [_vp, _i64, _i64, _i32, _vp, _vp]),
     # host planner (CPU only)
     "wnw_planner_create": (_vp, [_i32, _i32, _i32, _i32]),

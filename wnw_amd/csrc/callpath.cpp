@@ -307,6 +307,30 @@ bool result(PyObject* given, const at::Tensor& q, at::Tensor* out) {
   return true;
 }
 
+// A window and sinks: int32 [n_seg] tensors, or numbers (sinks: None, for none).
+struct View {
+  const int32_t *window = nullptr, *sinks = nullptr;
+  int64_t window_all = 0, sinks_all = 0;
+};
+bool view_of(PyObject* window, PyObject* sinks, const at::Tensor& q, int64_t n_seg, View* y) {
+  PyObject* const o[2] = {window, sinks};
+  const int32_t** p[2] = {&y->window, &y->sinks};
+  int64_t* all[2] = {&y->window_all, &y->sinks_all};
+  for (int i = 0; i < 2; ++i) {
+    if (i == 1 && o[i] == Py_None) continue;
+    if (whole(o[i], all[i])) {
+      if (*all[i] < 0) return false;
+      continue;
+    }
+    const at::Tensor* t = vec(o[i], at::kInt, n_seg);
+    if (!usable(t, q) || t->dim() != 1) return false;
+    *p[i] = t->const_data_ptr<int32_t>();
+  }
+  return true;
+}
+
+// (q, k_pages, v_pages, page_table, seg_len, scale, k_scale, v_scale, out), WIN: and (window, sinks)
+template <bool WIN>
 PyObject* paged_decode_impl(PyObject* const* a) {
   const at::Tensor* q = plain(a[0]);
   wnw_paged_cache c;
@@ -317,6 +341,8 @@ PyObject* paged_decode_impl(PyObject* const* a) {
       !paged_cache(a + 1, a[6], a[7], *q, &c, &len) || q->size(0) != c.n_seg || !heads(*q, c.head_dim) || q->size(1) > 16 ||
       !number(a[5], &scale) || !(scale > 0) || !std::isfinite(scale) || !result(a[8], *q, &out) || !out.is_contiguous())
     Py_RETURN_NONE;
+  View y;
+  if (WIN && !view_of(a[9], a[10], *q, c.n_seg, &y)) Py_RETURN_NONE;
   const int64_t dev = q->device().index(), g = q->size(1);
   const c10::DeviceGuard guard(q->device());
   if (!ready(dev)) Py_RETURN_NONE;
@@ -335,12 +361,16 @@ PyObject* paged_decode_impl(PyObject* const* a) {
   const int dt = dtype_code(q->scalar_type());
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = wnw_paged_decode_attn(&c, len, qp, op, g, (float)scale, dt, wp, bytes, stream);
+  rc = WIN ? wnw_paged_decode_attn_window(&c, len, qp, op, g, y.window, y.window_all, y.sinks, y.sinks_all, (float)scale, dt, wp,
+                                          bytes, stream)
+           : wnw_paged_decode_attn(&c, len, qp, op, g, (float)scale, dt, wp, bytes, stream);
   Py_END_ALLOW_THREADS
   if (rc != WNW_OK) return failed(rc, "paged_decode_attn");
   return a[8] != Py_None ? Py_NewRef(a[8]) : THPVariable_Wrap(std::move(out));
 }
 
+// (q, k_pages, v_pages, page_table, seg_len, cu_tokens, scale, max_tokens, k_scale, v_scale, out), WIN: and (window, sinks)
+template <bool WIN>
 PyObject* paged_prompt_impl(PyObject* const* a) {
   const at::Tensor* q = plain(a[0]);
   wnw_paged_cache c;
@@ -352,6 +382,8 @@ PyObject* paged_prompt_impl(PyObject* const* a) {
       !tokens_of(a[5], a[7], *q, c.n_seg, &cu, &samples, &most) || q->size(1) % (c.n_seg / samples) != 0 ||
       !number(a[6], &scale) || !(scale > 0) || !std::isfinite(scale) || !result(a[10], *q, &out))
     Py_RETURN_NONE;
+  View y;
+  if (WIN && !view_of(a[11], a[12], *q, c.n_seg, &y)) Py_RETURN_NONE;
   const int64_t dev = q->device().index(), g = q->size(1) / (c.n_seg / samples);
   const c10::DeviceGuard guard(q->device());
   if (!ready(dev)) Py_RETURN_NONE;
@@ -360,7 +392,8 @@ PyObject* paged_prompt_impl(PyObject* const* a) {
   const bool has_stream = stream_of(dev, &so, &stream);
   Ref stream_ref(so);
   if (!has_stream) return nullptr;
-  const int64_t need = wnw_paged_prompt_workspace_bytes(&c, g, most);
+  const int64_t need = WIN ? wnw_paged_prompt_window_workspace_bytes(&c, g, most, y.window, y.window_all, y.sinks, y.sinks_all)
+                           : wnw_paged_prompt_workspace_bytes(&c, g, most);
   if (need < 0) Py_RETURN_NONE;  // the general path says why
   at::Tensor own;
   Ref ws(g * most <= 16 ? PyObject_CallFunction(g_paged_ws, "LOLL", (long long)dev, so, (long long)c.n_seg, (long long)need)
@@ -379,7 +412,9 @@ PyObject* paged_prompt_impl(PyObject* const* a) {
   const int dt = dtype_code(q->scalar_type());
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = wnw_paged_prompt_attn(&c, len, qp, op, strides, tokens, samples, g, cu, most, (float)scale, dt, wp, need, stream);
+  rc = WIN ? wnw_paged_prompt_attn_window(&c, len, qp, op, strides, tokens, samples, g, cu, most, y.window, y.window_all, y.sinks,
+                                          y.sinks_all, (float)scale, dt, wp, need, stream)
+           : wnw_paged_prompt_attn(&c, len, qp, op, strides, tokens, samples, g, cu, most, (float)scale, dt, wp, need, stream);
   Py_END_ALLOW_THREADS
   if (rc != WNW_OK) return failed(rc, "paged_prompt_attn");
   return a[10] != Py_None ? Py_NewRef(a[10]) : THPVariable_Wrap(std::move(out));
@@ -504,12 +539,16 @@ PyMethodDef methods[] = {
     {"score", (PyCFunction)(void (*)(void))entry<score_impl, 10>, METH_FASTCALL,
      "score(q, k, starts, ends, audio_starts, audio_ends, acc, offsets, max_audio, scale) -> True, or None: not the "
      "plain form"},
-    {"paged_decode", (PyCFunction)(void (*)(void))entry<paged_decode_impl, 9>, METH_FASTCALL,
+    {"paged_decode", (PyCFunction)(void (*)(void))entry<paged_decode_impl<false>, 9>, METH_FASTCALL,
      "paged_decode(q, k_pages, v_pages, page_table, seg_len, scale, k_scale, v_scale, out) -> out, or None: not the plain "
      "form"},
-    {"paged_prompt", (PyCFunction)(void (*)(void))entry<paged_prompt_impl, 11>, METH_FASTCALL,
+    {"paged_prompt", (PyCFunction)(void (*)(void))entry<paged_prompt_impl<false>, 11>, METH_FASTCALL,
      "paged_prompt(q, k_pages, v_pages, page_table, seg_len, cu_tokens, scale, max_tokens, k_scale, v_scale, out) -> out, or "
      "None: not the plain form"},
+    {"paged_decode_window", (PyCFunction)(void (*)(void))entry<paged_decode_impl<true>, 11>, METH_FASTCALL,
+     "paged_decode_window(..., out, window, sinks): paged_decode through a window"},
+    {"paged_prompt_window", (PyCFunction)(void (*)(void))entry<paged_prompt_impl<true>, 13>, METH_FASTCALL,
+     "paged_prompt_window(..., out, window, sinks): paged_prompt through a window"},
     {"paged_append", (PyCFunction)(void (*)(void))entry<paged_append_impl, 15>, METH_FASTCALL,
      "paged_append(k, v, k_pages, v_pages, page_table, seg_len, q, positions, inv_freq, sections, interleaved, cu_tokens, "
      "max_tokens, k_scale, v_scale) -> (q rotated, new lengths), or None: not the plain form"},

@@ -52,6 +52,21 @@ __device__ __forceinline__ bool paged_tokens_of(const PagedTokens& t, int s, int
   return true;
 }
 
+// What a row sees of its segment: rows r - window + 1 .. r, r itself the last, and
+// the first `sinks` rows up to r.  One pair for all segments, or one for each.
+struct PagedView {
+  const int32_t* window;  // [n_seg], or null: all have window_all
+  const int32_t* sinks;
+  int32_t window_all, sinks_all;
+};
+// Segment s's window and sinks, no larger than its n rows; false where one is negative.
+__device__ __forceinline__ bool paged_view_of(const PagedView& y, int s, int n, int* window, int* sinks) {
+  const int w = y.window ? y.window[s] : y.window_all, z = y.sinks ? y.sinks[s] : y.sinks_all;
+  *window = min(w, n);
+  *sinks = min(z, n);
+  return (w | z) >= 0;
+}
+
 // x, as a value that the compiler does not know: what follows from it is worked
 // out here and not, ahead of the loops around, held in registers all along
 template <typename I>

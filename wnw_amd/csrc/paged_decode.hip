@@ -50,6 +50,7 @@ struct PagedDecodeParams {
   float scale_log2;
   int32_t G, cols;         // cols: query rows of a segment at most
   int32_t* err;
+  PagedView view;          // with a window
 };
 
 static constexpr int kPdStep = 32;  // rows of a step
@@ -144,6 +145,7 @@ __device__ __forceinline__ void load_agent(const float* p, float* a, float* b) {
 // trip), which is why what follows a piece is kept short and rolled.
 struct DecodeRows {
   int first, count, h, n, cols;  // tokens, KV head, rows of the segment, query rows
+  bool blind;                    // WIN: a window of no rows, and no sinks
 };
 __device__ __forceinline__ DecodeRows decode_rows(const PagedDecodeParams& p, int seg, int n) {
   DecodeRows r;
@@ -168,11 +170,12 @@ __device__ __forceinline__ T* out_row(const PagedDecodeParams& p, const DecodeRo
   return (T*)p.out + (int64_t)(r.first + ti) * p.ot + (int64_t)(r.h * p.G + col - ti * p.G) * p.oh;
 }
 // Elements d .. d + 3 of a result, from its sums
-template <typename T>
+template <typename T, bool WIN>
 __device__ __forceinline__ void paged_decode_out(const PagedDecodeParams& p, const DecodeRows& r, int col, int d, const f32x4& o,
                                                  float L) {
   const int ti = token_of(p, r, col);
-  const bool sees = r.n - r.count + ti + 1 > 0;  // else a row without keys
+  bool sees = r.n - r.count + ti + 1 > 0;  // else a row without keys
+  if constexpr (WIN) sees &= !r.blind;
   const float inv = __builtin_amdgcn_rcpf(L);
   float y[4];
 #pragma unroll
@@ -183,7 +186,7 @@ __device__ __forceinline__ void paged_decode_out(const PagedDecodeParams& p, con
 // The partials of workgroups [w0, w1] (the first in slot 2 w0 + late, the
 // others each in its first slot) added up, in as many runs as there are threads
 // for, 8 at a time; the runs by way of lds.
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool WIN>
 __device__ __forceinline__ void paged_decode_gather(const PagedDecodeParams& p, const DecodeRows& r, int tid, int late, int w0,
                                                     int w1, float* lds) {
   constexpr int kSc1 = 16;  // buffer cache policy: coherent over the device
@@ -227,7 +230,7 @@ __device__ __forceinline__ void paged_decode_gather(const PagedDecodeParams& p, 
       }
     }
     if (runs == 1) {
-      paged_decode_out<T>(p, r, col, 4 * (item % (D / 4)), o, L);
+      paged_decode_out<T, WIN>(p, r, col, 4 * (item % (D / 4)), o, L);
     } else {
       float* to = lds + e * 8;
       *(f32x4*)to = o;
@@ -248,11 +251,29 @@ __device__ __forceinline__ void paged_decode_gather(const PagedDecodeParams& p, 
       o = o * f + g * *(const f32x4*)at;
       M = now;
     }
-    paged_decode_out<T>(p, r, tid / (D / 4), 4 * (tid % (D / 4)), o, L);
+    paged_decode_out<T, WIN>(p, r, tid / (D / 4), 4 * (tid % (D / 4)), o, L);
   }
 }
 
-template <typename T, int D, bool Q8>
+// Through a window (WIN), the steps that no row of a segment sees are left out of
+// its steps: those between the sinks' and the first one that the first token's
+// window reaches.  The table's entries there are not read.
+struct DecodeView {
+  int window, sinks;  // no larger than the segment
+  int lo;             // rows from here on are in the first token's window
+  int head, gap;      // the sinks' steps, and how many are left out behind them
+};
+__device__ __forceinline__ DecodeView decode_view(int window, int sinks, int n, int count) {
+  DecodeView y;
+  y.window = window;
+  y.sinks = sinks;
+  y.lo = max(n - count + 1 - window, 0);
+  y.head = (sinks + kPdStep - 1) / kPdStep;
+  y.gap = max(y.lo / kPdStep - y.head, 0);
+  return y;
+}
+
+template <typename T, int D, bool Q8, bool WIN>
 __global__ __launch_bounds__((64 * PagedDecodeGeom<D, Q8>::kWaves),
                              (PagedDecodeGeom<D, Q8>::kWaves * PagedDecodeGeom<D, Q8>::kWgs / 4)) void
 paged_decode_kernel(PagedDecodeParams p) {
@@ -274,6 +295,20 @@ paged_decode_kernel(PagedDecodeParams p) {
   const int N = p.c.n_seg, wg = blockIdx.x;
 
   auto steps_of = [&](int n) { return n >= 0 && n <= p.c.capacity ? (n + kPdStep - 1) / kPdStep : 0; };
+  int lane_w = 0, lane_z = 0;  // WIN: of the lane's segment, as len
+  // segment s's steps, and its window and sinks
+  auto seg_steps = [&](int s, int n, int* w, int* z) {
+    int steps = steps_of(n);
+    if constexpr (WIN) {
+      if (!paged_view_of(p.view, s, n, w, z)) steps = 0;
+      if (steps > 0) {
+        int first, count = 1;
+        if (p.t.cu) paged_tokens_of(p.t, s, &first, &count);
+        steps -= decode_view(*w, *z, n, count).gap;
+      }
+    }
+    return steps;
+  };
   auto scan = [&](int x) {  // inclusive, over the wave
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -290,7 +325,7 @@ paged_decode_kernel(PagedDecodeParams p) {
   const int per = (N + NT - 1) / NT, sa = min(tid * per, N), sb = min(sa + per, N);
   if (N <= 64) {
     len = lane < N ? p.seg_len[lane] : 0;
-    num = steps_of(len);
+    num = seg_steps(min(lane, N - 1), len, &lane_w, &lane_z);
     at = scan(num);
     S = __builtin_amdgcn_readlane(at, 63);
     at -= num;
@@ -298,7 +333,7 @@ paged_decode_kernel(PagedDecodeParams p) {
   } else {
     int most = 0;
     for (int s = sa; s < sb; ++s) {
-      const int n = steps_of(p.seg_len[s]);
+      const int n = seg_steps(s, p.seg_len[s], &lane_w, &lane_z);
       mine += n;
       most = max(most, n);
     }
@@ -342,7 +377,7 @@ paged_decode_kernel(PagedDecodeParams p) {
     } else {
       int e = before + incl - mine;  // steps before the thread's segments
       for (int s = sa; s < sb; ++s) {
-        const int n = steps_of(p.seg_len[s]);
+        const int n = seg_steps(s, p.seg_len[s], &lane_w, &lane_z);
         if (uncut ? s == s0 : e <= x0 && x0 < e + n) {
           sh[0] = s;
           sh[1] = e;
@@ -363,7 +398,7 @@ paged_decode_kernel(PagedDecodeParams p) {
   for (int x = x0; x < x1 && win < N;) {
     if (N > 64) {
       len = win + lane < N ? p.seg_len[win + lane] : 0;
-      num = steps_of(len);
+      num = seg_steps(min(win + lane, N - 1), len, &lane_w, &lane_z);
       at += scan(num) - num;
     }
     // the pieces of this window, and the waves [wf, wt) of each; a piece that
@@ -392,7 +427,13 @@ paged_decode_kernel(PagedDecodeParams p) {
       const int first_step = piece(j, &a, &b);
       a += iw;
       const int mysteps = (b - a + nw - 1) / nw;
-      const DecodeRows r = decode_rows(p, seg, n);
+      DecodeRows r = decode_rows(p, seg, n);
+      DecodeView view = {};
+      if constexpr (WIN) {
+        view = decode_view(__builtin_amdgcn_readlane(lane_w, j), __builtin_amdgcn_readlane(lane_z, j), n, r.count);
+        r.blind = (view.window | view.sinks) == 0;
+      }
+      auto real = [&](int step) { return WIN && step >= view.head ? step + view.gap : step; };
       const int cols = r.cols;
       const int c = min(lc, max(cols - 1, 0)), ti = token_of(p, r, c);
       const int limit = n - r.count + ti + 1;  // rows that the lane's column sees
@@ -411,9 +452,9 @@ paged_decode_kernel(PagedDecodeParams p) {
       float ks = 1.f, vs = 1.f;
       auto window = [&](int k0) {
         const int step = a + nw * (k0 + (lane >> 1));
-        const int row = step * kPdStep + 16 * (lane & 1);
+        const int row = real(step) * kPdStep + 16 * (lane & 1);
         pid = -1;
-        if (step < b && row < n) {
+        if (step < b && row < n && (!WIN || row < view.sinks || row + 16 > view.lo)) {
           pid = p.c.table[seg * p.c.table_stride + (row >> p.c.shift)];
           if (pid < 0 || pid >= p.c.n_pages) {
             raise_device_error(p.err, WNW_DEVERR_BOUNDS);
@@ -431,7 +472,7 @@ paged_decode_kernel(PagedDecodeParams p) {
       int bad = 0;  // halves of the loaded step that no page holds
       auto load = [&](int k) {
         const int from = 2 * (k & 31);
-        const int step = a + nw * k;
+        const int step = real(a + nw * k);
         const int p0 = __builtin_amdgcn_readlane(pid, from), p1 = __builtin_amdgcn_readlane(pid, from + 1);
         bad = (p0 < 0 ? 1 : 0) | (p1 < 0 ? 2 : 0);
         const int in = (step * kPdStep) & ((1 << p.c.shift) - 1);  // first row in its page
@@ -464,8 +505,8 @@ paged_decode_kernel(PagedDecodeParams p) {
 #pragma unroll
       for (int i = 0; i < KK; ++i) qs[64 * i] = qf[i];
       for (int k = 0; k < mysteps; ++k) {
-        const int row0 = (a + nw * k) * kPdStep;
-        const bool edge = row0 + kPdStep > all_see || bad;
+        const int row0 = real(a + nw * k) * kPdStep;
+        const bool edge = row0 + kPdStep > all_see || bad || (WIN && row0 < n - view.window && row0 + kPdStep > view.sinks);
         const int bad_now = bad, from = 2 * (k & 31);
         // the 8 to 16 addresses made of these are worked out where they are used: held, they would cost registers
         asm volatile("" : "+v"(vput), "+v"(vget));
@@ -492,13 +533,16 @@ paged_decode_kernel(PagedDecodeParams p) {
 #pragma unroll
           for (int i = 0; i < VI; ++i) {
             const int rr = (i * 1024 + lane * 16) / RB;
-            if (row0 + rr >= n || (bad_now >> (rr >> 4) & 1)) vr[i] = u32x4{0, 0, 0, 0};
+            if (row0 + rr >= n || (bad_now >> (rr >> 4) & 1) || (WIN && row0 + rr >= view.sinks && row0 + rr < view.lo))
+              vr[i] = u32x4{0, 0, 0, 0};
           }
-          if (row0 + kPdStep > all_see && r.count > 1) {
+          if ((WIN || row0 + kPdStep > all_see) && r.count > 1) {
             bool any = false;
 #pragma unroll
-            for (int i = 0; i < VI; ++i)
-              if (row0 + (i * 1024 + lane * 16) / RB >= all_see) any |= take_odd<PE>(vr[i]);
+            for (int i = 0; i < VI; ++i) {
+              const int row = row0 + (i * 1024 + lane * 16) / RB;
+              if (row >= all_see || (WIN && row >= view.sinks && row < n - view.window)) any |= take_odd<PE>(vr[i]);
+            }
             if (__ballot(any)) odd = 1;
           }
 #pragma unroll
@@ -506,7 +550,8 @@ paged_decode_kernel(PagedDecodeParams p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               if (bad_now >> t2 & 1) y[t2][i] = 0.f;
-              if (row0 + 16 * t2 + 4 * lq + i >= limit) y[t2][i] = -INFINITY;
+              const int row = row0 + 16 * t2 + 4 * lq + i;
+              if (row >= limit || (WIN && row >= view.sinks && row < limit - view.window)) y[t2][i] = -INFINITY;
             }
         }
 #pragma unroll
@@ -570,11 +615,17 @@ paged_decode_kernel(PagedDecodeParams p) {
         __builtin_amdgcn_wave_barrier();
       }
       if (odd) {
+        // rows that some columns see: those that the window leaves between the first token and the last, the last tokens'
+        const int late = max(all_see, 0);
+        int row = late;
+        if constexpr (WIN) row = min(max(view.lo, view.sinks), late);
 #pragma unroll 1
-        for (int row = max(all_see, 0); row < n; ++row) {
-          const int step = row / kPdStep - a;  // nw apart in the wave
-          const uint8_t* from = step >= 0 && step % nw == 0 && row / kPdStep < b ? paged_v_row(p.c, seg, row, RB) : nullptr;
-          if (!from || row >= limit) continue;
+        for (; row < n; ++row) {
+          if (WIN && row < late && row >= n - view.window) row = late;
+          const int of = WIN && row / kPdStep >= view.head + view.gap ? row / kPdStep - view.gap : row / kPdStep;
+          const int step = of - a;  // nw apart in the wave
+          const uint8_t* from = step >= 0 && step % nw == 0 && of < b ? paged_v_row(p.c, seg, row, RB) : nullptr;
+          if (!from || row >= limit || (WIN && row >= view.sinks && row < limit - view.window)) continue;
 #pragma unroll
           for (int i = 0; i < DT; ++i) {
             __builtin_amdgcn_sched_barrier(0);
@@ -595,7 +646,7 @@ paged_decode_kernel(PagedDecodeParams p) {
           }
         } else if (!(cut >> j & 1)) {  // the whole segment
 #pragma unroll
-          for (int i = 0; i < DT; ++i) paged_decode_out<T>(p, r, oc, 16 * i + 4 * oq, acc[i], l);
+          for (int i = 0; i < DT; ++i) paged_decode_out<T, WIN>(p, r, oc, 16 * i + 4 * oq, acc[i], l);
         } else {
           const int64_t slot = (int64_t)(2 * wg + (first_step + a == x0 ? 0 : 1)) * p.cols + oc;
 #pragma unroll
@@ -620,7 +671,8 @@ paged_decode_kernel(PagedDecodeParams p) {
       for (uint64_t todo = several; todo; todo &= todo - 1) {
         const int j = __builtin_ctzll(todo);
         const int f = __builtin_amdgcn_readlane(waves, j) & 255, t = __builtin_amdgcn_readlane(waves, j) >> 8;
-        const DecodeRows r = decode_rows(p, win + j, __builtin_amdgcn_readlane(len, j));
+        DecodeRows r = decode_rows(p, win + j, __builtin_amdgcn_readlane(len, j));
+        if constexpr (WIN) r.blind = (__builtin_amdgcn_readlane(lane_w, j) | __builtin_amdgcn_readlane(lane_z, j)) == 0;
         int a, b;
         const int slot = (2 * wg + (piece(j, &a, &b) + a == x0 ? 0 : 1)) * p.cols;
         for (int e = here(tid); e < r.cols * (D / 4); e += NT) {
@@ -636,7 +688,7 @@ paged_decode_kernel(PagedDecodeParams p) {
             M = now;
           }
           if (!(cut >> j & 1)) {
-            paged_decode_out<T>(p, r, col, d, o, L);
+            paged_decode_out<T, WIN>(p, r, col, d, o, L);
           } else {
             float* to = p.part_acc + (slot + col) * D + d;
             store_agent(to, o[0], o[1]);
@@ -670,7 +722,9 @@ paged_decode_kernel(PagedDecodeParams p) {
       for (int i = 0; i < (j1 != j0 ? 2 : 1); ++i) {
         if (!sh[i]) continue;
         const int j = i ? j1 : j0, b0 = __builtin_amdgcn_readlane(at, j), w0 = owner_of(b0);
-        paged_decode_gather<T, D, NT>(p, decode_rows(p, win + j, __builtin_amdgcn_readlane(len, j)), tid, b0 > start_of(w0), w0,
+        DecodeRows r = decode_rows(p, win + j, __builtin_amdgcn_readlane(len, j));
+        if constexpr (WIN) r.blind = (__builtin_amdgcn_readlane(lane_w, j) | __builtin_amdgcn_readlane(lane_z, j)) == 0;
+        paged_decode_gather<T, D, NT, WIN>(p, r, tid, b0 > start_of(w0), w0,
                                       owner_of(b0 + __builtin_amdgcn_readlane(num, j) - 1), (float*)lds);
       }
     }
@@ -687,7 +741,11 @@ paged_decode_kernel(PagedDecodeParams p) {
       int first, count;
       if (!paged_tokens_of(p.t, s, &first, &count) || n < 0 || n > p.c.capacity) raise_device_error(p.err, WNW_DEVERR_BOUNDS);
     }
-    if (steps_of(n) > 0) continue;
+    int w, z;
+    if constexpr (WIN) {
+      if (!paged_view_of(p.view, s, n, &w, &z) && tid == 0) raise_device_error(p.err, WNW_DEVERR_BOUNDS);
+    }
+    if (seg_steps(s, n, &w, &z) > 0) continue;
     const DecodeRows r = decode_rows(p, s, 0);
     const float zero[4] = {0.f, 0.f, 0.f, 0.f};
     for (int e = here(tid); e < r.cols * (D / 4); e += NT) {
@@ -714,18 +772,22 @@ static PagedDecodeLayout decode_layout(int64_t n_seg, int64_t cols, int64_t D) {
   return y;
 }
 
-template <typename T, int D>
-static void launch_decode(const PagedDecodeParams& p, bool q8, int grid, hipStream_t st) {
+template <typename T, int D, bool WIN>
+static void launch_decode_view(const PagedDecodeParams& p, bool q8, int grid, hipStream_t st) {
   if (q8)
-    hipLaunchKernelGGL((paged_decode_kernel<T, D, true>), dim3(grid), dim3(64 * PagedDecodeGeom<D, true>::kWaves), 0, st, p);
+    hipLaunchKernelGGL((paged_decode_kernel<T, D, true, WIN>), dim3(grid), dim3(64 * PagedDecodeGeom<D, true>::kWaves), 0, st, p);
   else
-    hipLaunchKernelGGL((paged_decode_kernel<T, D, false>), dim3(grid), dim3(64 * PagedDecodeGeom<D, false>::kWaves), 0, st, p);
+    hipLaunchKernelGGL((paged_decode_kernel<T, D, false, WIN>), dim3(grid), dim3(64 * PagedDecodeGeom<D, false>::kWaves), 0, st, p);
+}
+template <typename T, int D>
+static void launch_decode(const PagedDecodeParams& p, bool q8, bool view, int grid, hipStream_t st) {
+  view ? launch_decode_view<T, D, true>(p, q8, grid, st) : launch_decode_view<T, D, false>(p, q8, grid, st);
 }
 
 // Shared with the prompt attention's entry point, which hands it the calls of a few tokens.
 int paged_decode_launch(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, void* out, const int64_t* strides,
-                        const PagedTokens& t, int64_t group, float scale, int dtype, void* workspace, int64_t bytes,
-                        void* stream) {
+                        const PagedTokens& t, const PagedView* view, int64_t group, float scale, int dtype, void* workspace,
+                        int64_t bytes, void* stream) {
   PagedDecodeParams p = {};
   if (int rc = paged_cache_of(cache, &p.c)) return rc;
   const int64_t N = cache->n_seg, D = cache->head_dim, cols = group * t.most;
@@ -733,8 +795,17 @@ int paged_decode_launch(const wnw_paged_cache* cache, const int32_t* seg_len, co
   WNW_CHECK_ARG(workspace && bytes >= y.total, "workspace too small: %lld bytes, %lld needed", (long long)bytes,
                 (long long)y.total);
   WNW_CHECK_ARG((uintptr_t)workspace % 256 == 0, "the workspace must be 256-byte aligned");
-  const int64_t steps = N * ((p.c.capacity + kPdStep - 1) / kPdStep);
+  int64_t steps = N * ((p.c.capacity + kPdStep - 1) / kPdStep);
   WNW_CHECK_ARG(steps < (1ll << 31), "the page table names too many rows for one call");
+  int64_t least = 1;
+  if (view) {
+    p.view = *view;
+    if (!view->window && !view->sinks) {  // steps that a segment has through its window, at most
+      const int64_t rows = (int64_t)view->window_all + view->sinks_all + t.most;
+      steps = std::min(steps, N * (rows / kPdStep + 3));
+      least = std::min<int64_t>(N, decode_grid((int)D, cache->page_dtype == WNW_E4M3));
+    }
+  }
   const bool q8 = cache->page_dtype == WNW_E4M3;
   p.t = t;
   p.seg_len = seg_len;
@@ -748,15 +819,15 @@ int paged_decode_launch(const wnw_paged_cache* cache, const int32_t* seg_len, co
   p.G = (int32_t)group;
   p.cols = (int32_t)cols;
   p.err = device_error_word();
-  const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(decode_grid((int)D, q8), steps / kPdMin + 1));
+  const int grid = (int)std::max<int64_t>(least, std::min<int64_t>(decode_grid((int)D, q8), steps / kPdMin + 1));
   hipStream_t st = (hipStream_t)stream;
   const bool bf = dtype == WNW_BF16;
   if (D == 64)
-    bf ? launch_decode<bf16_t, 64>(p, q8, grid, st) : launch_decode<f16_t, 64>(p, q8, grid, st);
+    bf ? launch_decode<bf16_t, 64>(p, q8, view, grid, st) : launch_decode<f16_t, 64>(p, q8, view, grid, st);
   else if (D == 128)
-    bf ? launch_decode<bf16_t, 128>(p, q8, grid, st) : launch_decode<f16_t, 128>(p, q8, grid, st);
+    bf ? launch_decode<bf16_t, 128>(p, q8, view, grid, st) : launch_decode<f16_t, 128>(p, q8, view, grid, st);
   else
-    bf ? launch_decode<bf16_t, 256>(p, q8, grid, st) : launch_decode<f16_t, 256>(p, q8, grid, st);
+    bf ? launch_decode<bf16_t, 256>(p, q8, view, grid, st) : launch_decode<f16_t, 256>(p, q8, view, grid, st);
   WNW_CHECK_HIP(hipGetLastError(), "paged attention launch");
   return WNW_OK;
 }
@@ -792,6 +863,17 @@ int paged_attn_check(const wnw_paged_cache* cache, const int32_t* seg_len, const
   return WNW_OK;
 }
 
+// A call's window and sinks: `ptr` or the one for all.
+bool paged_view_host(const int32_t* window, int64_t window_all, const int32_t* sinks, int64_t sinks_all, PagedView* out) {
+  if ((!window && window_all < 0) || (!sinks && sinks_all < 0)) {
+    set_error("window and sinks must not be negative (%lld, %lld)", (long long)window_all, (long long)sinks_all);
+    return false;
+  }
+  // a cache has at most 2^30 rows
+  *out = PagedView{window, sinks, (int32_t)std::min<int64_t>(window_all, 1 << 30), (int32_t)std::min<int64_t>(sinks_all, 1 << 30)};
+  return true;
+}
+
 }  // namespace wnw
 
 using namespace wnw;
@@ -805,9 +887,8 @@ extern "C" int64_t wnw_paged_decode_workspace_bytes(int64_t n_seg, int64_t rows,
   return decode_layout(n_seg, rows, head_dim).total;
 }
 
-extern "C" int wnw_paged_decode_attn(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, void* out,
-                                     int64_t group, float scale, int dtype, void* workspace, int64_t workspace_bytes,
-                                     void* stream) {
+static int decode_attn(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, void* out, const PagedView* view,
+                       int64_t group, float scale, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   WNW_CHECK_ARG(cache != nullptr, "the cache description is null");
   if (cache->n_seg == 0) return WNW_OK;
   const int64_t D = cache->head_dim;
@@ -817,5 +898,20 @@ extern "C" int wnw_paged_decode_attn(const wnw_paged_cache* cache, const int32_t
   WNW_CHECK_ARG(!paged_out_over_q(q, out, strides, cache->n_seg, group, D), "out covers a part of q");
   // every segment as a sample with one KV head and one token
   const PagedTokens t{nullptr, (int32_t)cache->n_seg, 1, 1};
-  return paged_decode_launch(cache, seg_len, q, out, strides, t, group, scale, dtype, workspace, workspace_bytes, stream);
+  return paged_decode_launch(cache, seg_len, q, out, strides, t, view, group, scale, dtype, workspace, workspace_bytes, stream);
+}
+
+extern "C" int wnw_paged_decode_attn(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, void* out,
+                                     int64_t group, float scale, int dtype, void* workspace, int64_t workspace_bytes,
+                                     void* stream) {
+  return decode_attn(cache, seg_len, q, out, nullptr, group, scale, dtype, workspace, workspace_bytes, stream);
+}
+
+extern "C" int wnw_paged_decode_attn_window(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, void* out,
+                                            int64_t group, const int32_t* window, int64_t window_all, const int32_t* sinks,
+                                            int64_t sinks_all, float scale, int dtype, void* workspace,
+                                            int64_t workspace_bytes, void* stream) {
+  PagedView view;
+  if (!paged_view_host(window, window_all, sinks, sinks_all, &view)) return WNW_EINVAL;
+  return decode_attn(cache, seg_len, q, out, &view, group, scale, dtype, workspace, workspace_bytes, stream);
 }

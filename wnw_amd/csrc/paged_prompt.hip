@@ -48,8 +48,9 @@ namespace wnw {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 int paged_decode_launch(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, void* out, const int64_t* strides,
-                        const PagedTokens& t, int64_t group, float scale, int dtype, void* workspace, int64_t bytes,
-                        void* stream);
+                        const PagedTokens& t, const PagedView* view, int64_t group, float scale, int dtype, void* workspace,
+                        int64_t bytes, void* stream);
+bool paged_view_host(const int32_t* window, int64_t window_all, const int32_t* sinks, int64_t sinks_all, PagedView* out);
 int paged_attn_check(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, const void* out,
                      const int64_t* strides, int64_t group, float scale, int dtype);
 bool paged_out_over_q(const void* q, const void* out, const int64_t* strides, int64_t tokens, int64_t heads, int64_t D);
@@ -65,6 +66,7 @@ struct PagedPromptParams {
   float scale_log2;
   int32_t G, nqb, splits;
   int32_t* err;
+  PagedView view;          // with a window
 };
 
 static constexpr int kPpKeys = 64;  // keys of a tile
@@ -80,12 +82,19 @@ __device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f3
 // What a workgroup's rows are.
 struct PromptRows {
   int first, count, len, rows;  // the sample's tokens, the segment's rows, query rows
+  int window, sinks;            // WIN: no larger than the segment
+  bool blind;                   // WIN: a window of no rows, and no sinks
 };
+template <bool WIN>
 __device__ __forceinline__ PromptRows prompt_rows(const PagedPromptParams& p, int seg, bool tell) {
   PromptRows r;
   const bool told = paged_tokens_of(p.t, seg, &r.first, &r.count);
   r.len = p.seg_len[seg];
-  const bool good = r.len >= 0 && r.len <= p.c.capacity;
+  bool good = r.len >= 0 && r.len <= p.c.capacity;
+  if constexpr (WIN) {
+    good &= paged_view_of(p.view, seg, r.len, &r.window, &r.sinks);
+    r.blind = (r.window | r.sinks) == 0;
+  }
   if (tell && (!told || !good)) raise_device_error(p.err, WNW_DEVERR_BOUNDS);
   if (!good) r.len = 0;
   r.rows = r.count * p.G;
@@ -98,22 +107,39 @@ __device__ __forceinline__ PromptRows prompt_rows(const PagedPromptParams& p, in
 // by the table 26; 64 tokens after 500 rows 19 and 26, with pieces of 4 tiles or
 // more 21).
 __device__ __forceinline__ int splits_of(int tiles, int most) { return max(min(tiles / 2, most), 1); }
-// Tiles that a block of query rows walks
-template <int W>
-__device__ __forceinline__ int tiles_of(const PagedPromptParams& p, const PromptRows& r, int qblk) {
-  const int last = r.len - r.count + 1 + min(32 * W * (qblk + 1) - 1, r.rows - 1) / p.G;  // rows that its last one sees
-  return max((last + kPpKeys - 1) / kPpKeys, 0);
+// Tiles that a block of query rows walks.  Through a window, those that none of its rows
+// sees are left out: `gap` of them behind the `head` that hold the sinks.  (Places in the
+// walk, not tiles, are what the loops, the splits, the LDS buffers and the pages held in
+// registers count.)
+struct PromptTiles {
+  int n, head, gap;
+  int lo, last_lo;  // rows from here on are in the window of the block's first row, of its last
+};
+template <int W, bool WIN>
+__device__ __forceinline__ PromptTiles tiles_of(const PagedPromptParams& p, const PromptRows& r, int qblk) {
+  const int base = r.len - r.count + 1;
+  const int last = base + min(32 * W * (qblk + 1) - 1, r.rows - 1) / p.G;  // rows that its last one sees
+  PromptTiles y = {max((last + kPpKeys - 1) / kPpKeys, 0), 0, 0, 0, 0};
+  if constexpr (WIN) {
+    y.lo = max(base + 32 * W * qblk / p.G - r.window, 0);
+    y.last_lo = last - r.window;
+    y.head = min((r.sinks + kPpKeys - 1) / kPpKeys, y.n);
+    y.gap = max(min(y.lo / kPpKeys, y.n) - y.head, 0);
+    y.n -= y.gap;
+  }
+  return y;
 }
 
 // The wave's rows out, 32-element parts dt0 .. dt0 + NT - 1: lane (hi, n) has
 // elements 32 i + 8 j + 4 hi + 0..3 of row n
-template <typename T, int NT>
+template <typename T, int NT, bool WIN>
 __device__ __forceinline__ void prompt_store(const PagedPromptParams& p, const PromptRows& r, int row, int h, int hi, int dt0,
                                              const f32x16* o, float l) {
   if (row >= r.rows) return;
   const int i = row / p.G, g = row - i * p.G;
   T* op = (T*)p.out + (int64_t)(r.first + i) * p.ot + (int64_t)(h * p.G + g) * p.oh;
-  const bool none = r.len - r.count + i + 1 <= 0;
+  bool none = r.len - r.count + i + 1 <= 0;
+  if constexpr (WIN) none |= r.blind;
   const float inv = 1.0f / l;
 #pragma unroll
   for (int dt = 0; dt < NT; ++dt)
@@ -127,7 +153,7 @@ __device__ __forceinline__ void prompt_store(const PagedPromptParams& p, const P
 }
 
 // Registers for at most 3 waves per SIMD: made to fit 4, head_dim 64 over 8 bits takes 43.5 us for 40.7 (2,048 tokens).
-template <typename T, int D, bool Q8, int W>
+template <typename T, int D, bool Q8, int W, bool WIN>
 __global__ __launch_bounds__((64 * W)) __attribute__((amdgpu_waves_per_eu((D == 256 && !Q8 ? 1 : 2), (D == 256 && !Q8 ? 1 : 3)))) void
 paged_prompt_kernel(PagedPromptParams p) {
   using VT = typename std::conditional<Q8, bf16_t, T>::type;   // the value product's type
@@ -152,7 +178,7 @@ paged_prompt_kernel(PagedPromptParams p) {
   // the blocks with the most tiles first; workgroups of one segment N apart (8 segments: each in one L2)
   const int seg = blockIdx.x % N, rank = blockIdx.x / N;
   const int block = rank / p.splits, split = rank - block * p.splits, qblk = p.nqb - 1 - block;
-  const PromptRows r = prompt_rows(p, seg, tid == 0 && qblk == 0 && split == 0);
+  const PromptRows r = prompt_rows<WIN>(p, seg, tid == 0 && qblk == 0 && split == 0);
   if (qblk * kPpQ >= r.rows) return;
   const int h = seg % p.t.hkv;
   const int base = r.len - r.count + 1;  // token i sees base + i rows
@@ -163,7 +189,9 @@ paged_prompt_kernel(PagedPromptParams p) {
   const int wfirst = base + min(qblk * kPpQ + 32 * w, r.rows - 1) / p.G;
   const int wlast = base + min(qblk * kPpQ + 32 * w + 31, r.rows - 1) / p.G;
   const int first = base + qblk * kPpQ / p.G;  // and the workgroup's first
-  const int tiles = tiles_of<W>(p, r, qblk), splits = splits_of(tiles, p.splits);
+  const PromptTiles walk = tiles_of<W, WIN>(p, r, qblk);
+  const int tiles = walk.n, splits = splits_of(tiles, p.splits);
+  auto real = [&](int place) { return WIN && place >= walk.head ? place + walk.gap : place; };
   if (split >= splits) return;
   const int t0 = (int)((int64_t)tiles * split / splits), t1 = (int)((int64_t)tiles * (split + 1) / splits);
   const bool busy = qblk * kPpQ + 32 * w < r.rows;  // a wave without rows only moves tiles
@@ -198,9 +226,10 @@ paged_prompt_kernel(PagedPromptParams p) {
   // Rows past the segment's take its last page; an entry that is no page page
   // 0, with its sign bit set.
   auto find = [&](int window) {
-    const int id = table[min((window * 64 + lane) * 16, r.len - 1) >> p.c.shift];
+    const int key = WIN ? real(window * kWin + (lane >> 2)) * kPpKeys + (lane & 3) * 16 : (window * 64 + lane) * 16;
+    const int id = table[min(key, r.len - 1) >> p.c.shift];
     const bool is = (uint32_t)id < (uint32_t)p.c.n_pages;
-    wrong |= !is;
+    wrong |= !is && (!WIN || key < r.sinks || key + 16 > walk.lo);  // others may have been given back
     pid_next = is ? id : (int)0x80000000;
   };
   auto find_scales = [&]() {
@@ -228,8 +257,9 @@ paged_prompt_kernel(PagedPromptParams p) {
     soff = here(soff);
 #pragma unroll
     for (int u = 0; u < NI; ++u) {
-      const int row = tile * kPpKeys + u * RPL + w * (64 / CG);
-      const int id = __builtin_amdgcn_readlane(pid, (row >> 4) & 63);
+      const int in_tile = u * RPL + w * (64 / CG);
+      const int row = real(tile) * kPpKeys + in_tile;
+      const int id = __builtin_amdgcn_readlane(pid, ((tile * kPpKeys + in_tile) >> 4) & 63);
       const int64_t page = id & 0x7fffffff;
       const WNW_GLOBAL uint8_t* kp = gptr<uint8_t>(p.c.k) + (page * p.c.k_stride + (row & in) * GB);
       const WNW_GLOBAL uint8_t* vp = gptr<uint8_t>(p.c.v) + (page * p.c.v_stride + (row & in) * GB);
@@ -246,19 +276,24 @@ paged_prompt_kernel(PagedPromptParams p) {
     }
   };
   auto clear = [&](int tile) {  // rows of kr and vr that are not the segment's
-    int any = (tile + 1) * kPpKeys > r.len;
+    int any = (real(tile) + 1) * kPpKeys > r.len;
 #pragma unroll
     for (int u = 0; u < NI; ++u) any |= gone[u] < 0;
     if (!any) return;
 #pragma unroll
     for (int u = 0; u < NI; ++u) {
       if (gone[u] < 0) kr[u] = u32x4{0, 0, 0, 0};
-      if (gone[u] < 0 || tile * kPpKeys + u * RPL + srow >= r.len) vr[u] = u32x4{0, 0, 0, 0};
+      if (gone[u] < 0 || real(tile) * kPpKeys + u * RPL + srow >= r.len) vr[u] = u32x4{0, 0, 0, 0};
     }
   };
-  // takes infinities and NaN out of the V of a tile that not every row of the workgroup sees whole
+  // whether every row of the workgroup sees the whole of a tile
+  auto whole = [&](int tile) {
+    const int k0 = real(tile) * kPpKeys, k1 = k0 + kPpKeys;
+    return k1 <= first && (!WIN || k0 >= walk.last_lo || k1 <= r.sinks);
+  };
+  // takes infinities and NaN out of the V of one that not every row does
   auto even = [&](int tile) {
-    if ((tile + 1) * kPpKeys <= first) return;
+    if (whole(tile)) return;
     bool any = false;
 #pragma unroll
     for (int u = 0; u < NI; ++u) any |= take_odd<PE>(vr[u]);
@@ -336,13 +371,23 @@ paged_prompt_kernel(PagedPromptParams p) {
       lv[b] = Q8 ? at(wl) : 0.f;
       un[b] = Q8 ? at(wu) : 1.f;
     }
-    if constexpr (decltype(masked)::value) {
-      const int lim = limit - i * kPpKeys - 4 * hi;  // keys 32 mt + 8 j + c (+ 4 hi) below it
+    if (masked) {
+      const int lim = limit - real(i) * kPpKeys - 4 * hi;  // keys 32 mt + 8 j + c (+ 4 hi) below it
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (32 * mt + 8 * (e >> 2) + (e & 3) >= lim) s[mt][e] = -INFINITY;
+      if constexpr (WIN) {  // and those below the window that are no sinks
+        const int lo = lim - r.window, sink = r.sinks - real(i) * kPpKeys - 4 * hi;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int k = 32 * mt + 8 * (e >> 2) + (e & 3);
+            if (k < lo && k >= sink) s[mt][e] = -INFINITY;
+          }
+      }
     }
     float mx = m;
 #pragma unroll
@@ -423,45 +468,67 @@ paged_prompt_kernel(PagedPromptParams p) {
         __syncthreads();
       }
     };
-    // the tiles that every row of the wave sees whole, the others, the turns of the workgroup's later waves
-    int i = t0;
-    for (const int full = min(wfirst / kPpKeys, mine); i < full; ++i) {
-      turn(i);
-      tile(i, std::false_type());
-    }
-    for (; i < mine; ++i) {
-      turn(i);
-      tile(i, std::true_type());
-    }
-    for (; i < t1; ++i) {
-      turn(i);
+    auto pass = [&](int i) {  // a tile that none of the wave's rows sees
       if constexpr (NB == 2) {
         put(i + 1);
         fetch(i + 2);
       }
+    };
+    if constexpr (WIN) {
+      for (int i = t0; i < t1; ++i) {
+        turn(i);
+        const int k0 = real(i) * kPpKeys, k1 = k0 + kPpKeys;
+        if (!busy || k0 >= wlast || (k0 >= r.sinks && k1 <= wfirst - r.window))
+          pass(i);
+        else
+          tile(i, k1 > wfirst || (k0 < wlast - r.window && k1 > r.sinks));
+      }
+    } else {
+      // the tiles that every row of the wave sees whole, the others, the turns of the workgroup's later waves
+      int i = t0;
+      for (const int full = min(wfirst / kPpKeys, mine); i < full; ++i) {
+        turn(i);
+        tile(i, std::false_type());
+      }
+      for (; i < mine; ++i) {
+        turn(i);
+        tile(i, std::true_type());
+      }
+      for (; i < t1; ++i) {
+        turn(i);
+        pass(i);
+      }
     }
     if (wrong) raise_device_error(p.err, WNW_DEVERR_BOUNDS);
     if (odd) {  // what even() took out, to the rows that see it (the wave's tiles are behind a barrier)
-      const int from = max(t0, max(first, 0) / kPpKeys) * kPpKeys, to = min(t1 * kPpKeys, wlast);
+      auto give = [&](int from, int to) {
 #pragma unroll 1
-      for (int key = from; key < to; ++key) {
-        const uint8_t* at = paged_v_row(p.c, seg, key, GB);
-        if (!at || key >= limit) continue;
+        for (int key = from; key < to; ++key) {
+          const uint8_t* at = paged_v_row(p.c, seg, key, GB);
+          if (!at || key >= limit || (WIN && key >= r.sinks && key < limit - r.window)) continue;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+          for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            __builtin_amdgcn_sched_barrier(0);
-            const f32x4 x = odd_quad<PE>(at, 32 * dt + 8 * j + 4 * hi);
+            for (int j = 0; j < 4; ++j) {
+              __builtin_amdgcn_sched_barrier(0);
+              const f32x4 x = odd_quad<PE>(at, 32 * dt + 8 * j + 4 * hi);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[dt][4 * j + e] += x[e];
-          }
+              for (int e = 0; e < 4; ++e) o[dt][4 * j + e] += x[e];
+            }
+        }
+      };
+      if constexpr (WIN) {
+#pragma unroll 1
+        for (int i = t0; i < t1; ++i)
+          if (!whole(i)) give(real(i) * kPpKeys, min((real(i) + 1) * kPpKeys, wlast));
+      } else {
+        give(max(t0, max(first, 0) / kPpKeys) * kPpKeys, min(t1 * kPpKeys, wlast));
       }
     }
   }
   l = sum_x32(l);
   if (splits == 1) {
-    prompt_store<T, DT>(p, r, row, h, hi, 0, o, l);
+    prompt_store<T, DT, WIN>(p, r, row, h, hi, 0, o, l);
   } else if (busy) {
     float* part = p.part + ((((int64_t)block * N + seg) * p.splits + split) * W + w) * (DT * 16 + 2) * 64;
 #pragma unroll
@@ -478,16 +545,16 @@ paged_prompt_kernel(PagedPromptParams p) {
 
 // The splits' sums added up: a workgroup for 32 query rows and 32 elements of
 // them, its four waves a quarter of the splits each, joined through LDS.
-template <typename T, int D, int W>
+template <typename T, int D, int W, bool WIN>
 __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParams p) {
   constexpr int DT = D / 32, kPpQ = 32 * W;
   __shared__ float sums[4][18][64];
   const int lane = threadIdx.x & 63, k = threadIdx.x >> 6, hi = lane >> 5, n = lane & 31;
   const int N = p.c.n_seg, block = blockIdx.x / (W * DT), w = blockIdx.x / DT % W, dt = blockIdx.x % DT;
   const int seg = block % N, qblk = p.nqb - 1 - block / N;
-  const PromptRows r = prompt_rows(p, seg, false);
+  const PromptRows r = prompt_rows<WIN>(p, seg, false);
   if (qblk * kPpQ + 32 * w >= r.rows) return;
-  const int splits = splits_of(tiles_of<W>(p, r, qblk), p.splits);
+  const int splits = splits_of(tiles_of<W, WIN>(p, r, qblk).n, p.splits);
   if (splits == 1) return;
   constexpr int64_t kPart = (DT * 16 + 2) * 64;
   const float* part = p.part + ((int64_t)block * p.splits * W + w) * kPart;
@@ -527,7 +594,7 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParam
     for (int e = 0; e < 16; ++e) y[e] = sums[i][e][lane];
     add(sums[i][16][lane], sums[i][17][lane], y);
   }
-  prompt_store<T, 1>(p, r, qblk * kPpQ + 32 * w + n, seg % p.t.hkv, hi, dt, &o, l);
+  prompt_store<T, 1, WIN>(p, r, qblk * kPpQ + 32 * w + n, seg % p.t.hkv, hi, dt, &o, l);
 }
 
 // How a call is cut, from what the host knows of it (us measured on one GPU, bf16
@@ -548,9 +615,14 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParam
 struct PromptPlan {
   int64_t waves, nqb, splits, bytes;
 };
-static PromptPlan prompt_plan(int64_t n_seg, int64_t group, int64_t max_tokens, int64_t capacity, int64_t D) {
+// view: the windows, null without; then a block's tiles are at most those of its rows' windows.
+static PromptPlan prompt_plan(int64_t n_seg, int64_t group, int64_t max_tokens, int64_t capacity, int64_t D,
+                              const PagedView* view) {
   PromptPlan y;
-  const int64_t rows = max_tokens * group, cus = device_cus(), tiles = (capacity + kPpKeys - 1) / kPpKeys;
+  const int64_t rows = max_tokens * group, cus = device_cus();
+  int64_t tiles = (capacity + kPpKeys - 1) / kPpKeys;
+  if (view && !view->window && !view->sinks)
+    tiles = std::min(tiles, ((int64_t)view->window_all + view->sinks_all + 256 / group) / kPpKeys + 3);
   const bool own = n_seg * ((rows + 255) / 256) <= cus && 2 * max_tokens >= capacity;
   y.waves = D == 128 && !own ? 8 : 4;
   y.nqb = (rows + 32 * y.waves - 1) / (32 * y.waves);
@@ -561,19 +633,24 @@ static PromptPlan prompt_plan(int64_t n_seg, int64_t group, int64_t max_tokens, 
   return y;
 }
 
-template <typename T, int D, bool Q8, int W>
+template <typename T, int D, bool Q8, int W, bool WIN>
 static hipError_t launch_prompt_q(const PagedPromptParams& p, hipStream_t st) {
   const unsigned blocks = (unsigned)(p.c.n_seg * (int64_t)p.nqb);
-  hipLaunchKernelGGL((paged_prompt_kernel<T, D, Q8, W>), dim3(blocks * p.splits), dim3(64 * W), 0, st, p);
-  if (p.splits > 1) hipLaunchKernelGGL((paged_prompt_join_kernel<T, D, W>), dim3(blocks * W * (D / 32)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((paged_prompt_kernel<T, D, Q8, W, WIN>), dim3(blocks * p.splits), dim3(64 * W), 0, st, p);
+  if (p.splits > 1)
+    hipLaunchKernelGGL((paged_prompt_join_kernel<T, D, W, WIN>), dim3(blocks * W * (D / 32)), dim3(256), 0, st, p);
   return hipGetLastError();
 }
+template <typename T, bool WIN>
+static hipError_t launch_prompt_view(const PagedPromptParams& p, int64_t D, bool q8, int64_t waves, hipStream_t st) {
+  if (D == 64) return q8 ? launch_prompt_q<T, 64, true, 4, WIN>(p, st) : launch_prompt_q<T, 64, false, 4, WIN>(p, st);
+  if (D == 256) return q8 ? launch_prompt_q<T, 256, true, 4, WIN>(p, st) : launch_prompt_q<T, 256, false, 4, WIN>(p, st);
+  if (waves == 8) return q8 ? launch_prompt_q<T, 128, true, 8, WIN>(p, st) : launch_prompt_q<T, 128, false, 8, WIN>(p, st);
+  return q8 ? launch_prompt_q<T, 128, true, 4, WIN>(p, st) : launch_prompt_q<T, 128, false, 4, WIN>(p, st);
+}
 template <typename T>
-static hipError_t launch_prompt(const PagedPromptParams& p, int64_t D, bool q8, int64_t waves, hipStream_t st) {
-  if (D == 64) return q8 ? launch_prompt_q<T, 64, true, 4>(p, st) : launch_prompt_q<T, 64, false, 4>(p, st);
-  if (D == 256) return q8 ? launch_prompt_q<T, 256, true, 4>(p, st) : launch_prompt_q<T, 256, false, 4>(p, st);
-  if (waves == 8) return q8 ? launch_prompt_q<T, 128, true, 8>(p, st) : launch_prompt_q<T, 128, false, 8>(p, st);
-  return q8 ? launch_prompt_q<T, 128, true, 4>(p, st) : launch_prompt_q<T, 128, false, 4>(p, st);
+static hipError_t launch_prompt(const PagedPromptParams& p, int64_t D, bool q8, int64_t waves, bool view, hipStream_t st) {
+  return view ? launch_prompt_view<T, true>(p, D, q8, waves, st) : launch_prompt_view<T, false>(p, D, q8, waves, st);
 }
 
 // Query rows of a segment that decode attention takes: four tokens of 8 samples after
@@ -584,19 +661,18 @@ static constexpr int kFewRows = 16;
 
 using namespace wnw;
 
-extern "C" int64_t wnw_paged_prompt_workspace_bytes(const wnw_paged_cache* cache, int64_t group, int64_t max_tokens) {
+static int64_t prompt_workspace(const wnw_paged_cache* cache, int64_t group, int64_t max_tokens, const PagedView* view) {
   PagedCache c;
   if (!cache || group < 1 || group > 1024 || max_tokens < 0 || max_tokens >= (1 << 24)) return -1;
   if (paged_cache_of(cache, &c)) return -1;
   if (max_tokens == 0) return 0;
   if (max_tokens * group <= kFewRows) return wnw_paged_decode_workspace_bytes(cache->n_seg, max_tokens * group, cache->head_dim);
-  return prompt_plan(cache->n_seg, group, max_tokens, c.capacity, cache->head_dim).bytes;
+  return prompt_plan(cache->n_seg, group, max_tokens, c.capacity, cache->head_dim, view).bytes;
 }
 
-extern "C" int wnw_paged_prompt_attn(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, void* out,
-                                     const int64_t* strides, int64_t n_tokens, int64_t n_samples, int64_t group,
-                                     const int32_t* cu_tokens, int64_t max_tokens, float scale, int dtype, void* workspace,
-                                     int64_t workspace_bytes, void* stream) {
+static int prompt_attn(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, void* out, const int64_t* strides,
+                       int64_t n_tokens, int64_t n_samples, int64_t group, const int32_t* cu_tokens, int64_t max_tokens,
+                       const PagedView* view, float scale, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   PagedPromptParams p = {};
   if (int rc = paged_cache_of(cache, &p.c)) return rc;
   const int64_t N = cache->n_seg, D = cache->head_dim;
@@ -616,9 +692,9 @@ extern "C" int wnw_paged_prompt_attn(const wnw_paged_cache* cache, const int32_t
   WNW_CHECK_ARG(most > 0, "max_tokens is zero");
   p.t = PagedTokens{cu_tokens, (int32_t)n_tokens, (int32_t)(N / n_samples), (int32_t)most};
   if (most * group <= kFewRows)
-    return paged_decode_launch(cache, seg_len, q, out, strides, p.t, group, scale, dtype, workspace, workspace_bytes, stream);
+    return paged_decode_launch(cache, seg_len, q, out, strides, p.t, view, group, scale, dtype, workspace, workspace_bytes, stream);
   WNW_CHECK_ARG(most * group < (1ll << 30), "too many query rows");
-  const PromptPlan y = prompt_plan(N, group, most, p.c.capacity, D);
+  const PromptPlan y = prompt_plan(N, group, most, p.c.capacity, D, view);
   WNW_CHECK_ARG(N * y.nqb < (1ll << 23), "too many segments and tokens for one call");
   WNW_CHECK_ARG(y.bytes == 0 || (workspace && workspace_bytes >= y.bytes), "workspace too small: %lld bytes, %lld needed",
                 (long long)workspace_bytes, (long long)y.bytes);
@@ -633,8 +709,41 @@ extern "C" int wnw_paged_prompt_attn(const wnw_paged_cache* cache, const int32_t
   p.nqb = (int32_t)y.nqb;
   p.splits = (int32_t)y.splits;
   p.err = device_error_word();
-  const hipError_t e = dtype == WNW_BF16 ? launch_prompt<bf16_t>(p, D, cache->page_dtype == WNW_E4M3, y.waves, (hipStream_t)stream)
-                                         : launch_prompt<f16_t>(p, D, cache->page_dtype == WNW_E4M3, y.waves, (hipStream_t)stream);
+  if (view) p.view = *view;
+  const bool q8 = cache->page_dtype == WNW_E4M3;
+  const hipError_t e = dtype == WNW_BF16 ? launch_prompt<bf16_t>(p, D, q8, y.waves, view, (hipStream_t)stream)
+                                         : launch_prompt<f16_t>(p, D, q8, y.waves, view, (hipStream_t)stream);
   WNW_CHECK_HIP(e, "paged prompt attention launch");
   return WNW_OK;
+}
+
+extern "C" int64_t wnw_paged_prompt_workspace_bytes(const wnw_paged_cache* cache, int64_t group, int64_t max_tokens) {
+  return prompt_workspace(cache, group, max_tokens, nullptr);
+}
+
+extern "C" int wnw_paged_prompt_attn(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, void* out,
+                                     const int64_t* strides, int64_t n_tokens, int64_t n_samples, int64_t group,
+                                     const int32_t* cu_tokens, int64_t max_tokens, float scale, int dtype, void* workspace,
+                                     int64_t workspace_bytes, void* stream) {
+  return prompt_attn(cache, seg_len, q, out, strides, n_tokens, n_samples, group, cu_tokens, max_tokens, nullptr, scale, dtype,
+                     workspace, workspace_bytes, stream);
+}
+
+extern "C" int64_t wnw_paged_prompt_window_workspace_bytes(const wnw_paged_cache* cache, int64_t group, int64_t max_tokens,
+                                                           const int32_t* window, int64_t window_all, const int32_t* sinks,
+                                                           int64_t sinks_all) {
+  PagedView view;
+  if (!paged_view_host(window, window_all, sinks, sinks_all, &view)) return -1;
+  return prompt_workspace(cache, group, max_tokens, &view);
+}
+
+extern "C" int wnw_paged_prompt_attn_window(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, void* out,
+                                            const int64_t* strides, int64_t n_tokens, int64_t n_samples, int64_t group,
+                                            const int32_t* cu_tokens, int64_t max_tokens, const int32_t* window,
+                                            int64_t window_all, const int32_t* sinks, int64_t sinks_all, float scale, int dtype,
+                                            void* workspace, int64_t workspace_bytes, void* stream) {
+  PagedView view;
+  if (!paged_view_host(window, window_all, sinks, sinks_all, &view)) return WNW_EINVAL;
+  return prompt_attn(cache, seg_len, q, out, strides, n_tokens, n_samples, group, cu_tokens, max_tokens, &view, scale, dtype,
+                     workspace, workspace_bytes, stream);
 }

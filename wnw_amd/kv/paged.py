@@ -288,7 +288,27 @@ def _check_q(q: Tensor, k_pages: Tensor, scale: float) -> None:
         raise _lib.WnwError(f"the scale must be positive, got {scale}")
 
 
+def _tensors(*args) -> list[Tensor]:
+    return [x for x in args if isinstance(x, Tensor)]
+
+
+def _view(window: int | Tensor, sinks: int | Tensor | None, n_seg: int) -> tuple:
+    """The checked window and sinks as the library takes them: (pointer, number) each."""
+    args = []
+    for name, x in (("window", window), ("sinks", 0 if sinks is None else sinks)):
+        if isinstance(x, Tensor):
+            if x.dtype != torch.int32 or x.shape != (n_seg,) or not x.is_contiguous():
+                raise _lib.WnwError(f"{name} must be a contiguous int32 [{n_seg}], or a number")
+            args += [_lib.ptr(x), 0]
+        else:
+            if isinstance(x, bool) or not isinstance(x, int) or x < 0:
+                raise _lib.WnwError(f"{name} must be a whole number, not negative, or int32 [{n_seg}], got {x!r}")
+            args += [None, min(x, 1 << 30)]
+    return tuple(args)
+
+
 def paged_decode_attn(q_flat: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seg_len: Tensor, scale: float, *,
+                      window: int | Tensor | None = None, sinks: int | Tensor | None = None,
                       k_scale: Tensor | None = None, v_scale: Tensor | None = None, out: Tensor | None = None,
                       workspace: PagedWorkspace | None = None) -> Tensor:
     """Decode attention over the pages: ``decode_attn`` for a paged cache.
@@ -296,13 +316,23 @@ def paged_decode_attn(q_flat: Tensor, k_pages: Tensor, v_pages: Tensor, page_tab
     ``q_flat`` [N, G, D] in bf16 or f16, G up to 16; returns [N, G, D].  A
     segment without rows gives zeros.  ``out``: a contiguous tensor for the
     result.  The lengths are read on the device; ``page_table.shape[1]`` bounds
-    them and sizes the grid.  ``workspace``: the caller's own."""
+    them and sizes the grid.  ``workspace``: the caller's own.
+
+    ``window``: each segment's query rows see its last ``window`` rows and its
+    first ``sinks`` (default none) alone; a number for all segments, or int32 [N],
+    one for each (class-A heads a window as long as the cache, class-B heads a
+    short one, in one launch).  0 leaves the sinks; a segment that shows no row
+    gives zeros.  Table entries of blocks that are not seen are not read: their
+    pages may have gone (``wnw_amd.kv.pages``).  Negative entries set the device
+    error word and give zeros."""
     if workspace is None:
-        done = (_lib._callpath or _lib.callpath()).paged_decode(q_flat, k_pages, v_pages, page_table, seg_len, scale, k_scale,
-                                                                v_scale, out)
+        native = _lib._callpath or _lib.callpath()
+        args = (q_flat, k_pages, v_pages, page_table, seg_len, scale, k_scale, v_scale, out)
+        done = native.paged_decode(*args) if window is None and sinks is None else \
+            native.paged_decode_window(*args, window, sinks)
         if done is not None:
             return done
-    cache = _cache(k_pages, v_pages, page_table, seg_len, k_scale, v_scale, q_flat, out)
+    cache = _cache(k_pages, v_pages, page_table, seg_len, k_scale, v_scale, q_flat, out, *_tensors(window, sinks))
     _check_q(q_flat, k_pages, scale)
     N, D = cache.n_seg, cache.head_dim
     if q_flat.dim() != 3 or q_flat.shape[0] != N or q_flat.shape[2] != D or not 1 <= q_flat.shape[1] <= 16:
@@ -312,21 +342,26 @@ def paged_decode_attn(q_flat: Tensor, k_pages: Tensor, v_pages: Tensor, page_tab
         q = q.clone()
     if out is not None and not out.is_contiguous():
         raise _lib.WnwError("out must be contiguous")
+    if window is None and sinks is not None:
+        raise _lib.WnwError("sinks need a window")
+    view = () if window is None else _view(window, sinks, N)
     o = _out(out, q)
     G = q.shape[1]
     if N == 0:
         return o
+    call = _lib.lib().wnw_paged_decode_attn_window if view else _lib.lib().wnw_paged_decode_attn
     with torch.cuda.device(q.device):
         _lib.ensure_init(q.device)
         ws = _workspace(q.device, N, int(_lib.lib().wnw_paged_decode_workspace_bytes(N, G, D)), workspace)
-        _lib.check(_lib.lib().wnw_paged_decode_attn(
-            ctypes.byref(cache), _lib.ptr(seg_len), _lib.ptr(q), _lib.ptr(o), G, float(scale), _lib.dtype_code(q.dtype),
+        _lib.check(call(
+            ctypes.byref(cache), _lib.ptr(seg_len), _lib.ptr(q), _lib.ptr(o), G, *view, float(scale), _lib.dtype_code(q.dtype),
             _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(q.device)), "paged_decode_attn")
     return o
 
 
 def paged_prompt_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seg_len: Tensor, cu_tokens: Tensor,
-                      scale: float, *, max_tokens: int | None = None, k_scale: Tensor | None = None,
+                      scale: float, *, max_tokens: int | None = None, window: int | Tensor | None = None,
+                      sinks: int | Tensor | None = None, k_scale: Tensor | None = None,
                       v_scale: Tensor | None = None, out: Tensor | None = None,
                       workspace: PagedWorkspace | None = None) -> Tensor:
     """Causal attention of prompts, or of chunks of them, over the pages that
@@ -338,13 +373,18 @@ def paged_prompt_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: T
     [T, Hq, D].  ``max_tokens``, the most tokens of a sample, sizes the grid
     (default T); a sample with more sets the device error word and its rows of
     the result are not written.  ``workspace``: the caller's own, used by calls
-    of up to 16 query rows per segment (max_tokens times heads of a group)."""
+    of up to 16 query rows per segment (max_tokens times heads of a group).
+
+    ``window`` and ``sinks`` as for ``paged_decode_attn``: a token at row r sees
+    the rows j <= r with j < sinks or j > r - window."""
     if workspace is None:
-        done = (_lib._callpath or _lib.callpath()).paged_prompt(q, k_pages, v_pages, page_table, seg_len, cu_tokens, scale,
-                                                                max_tokens, k_scale, v_scale, out)
+        native = _lib._callpath or _lib.callpath()
+        args = (q, k_pages, v_pages, page_table, seg_len, cu_tokens, scale, max_tokens, k_scale, v_scale, out)
+        done = native.paged_prompt(*args) if window is None and sinks is None else \
+            native.paged_prompt_window(*args, window, sinks)
         if done is not None:
             return done
-    cache = _cache(k_pages, v_pages, page_table, seg_len, k_scale, v_scale, q, cu_tokens, out)
+    cache = _cache(k_pages, v_pages, page_table, seg_len, k_scale, v_scale, q, cu_tokens, out, *_tensors(window, sinks))
     _check_q(q, k_pages, scale)
     N, D = cache.n_seg, cache.head_dim
     q = _heads("q", q, None, D)
@@ -353,6 +393,9 @@ def paged_prompt_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: T
     H = N // max(B, 1)
     if N and (q.shape[1] < 1 or q.shape[1] % H):
         raise _lib.WnwError(f"{q.shape[1]} query heads are not a multiple of {H} KV heads")
+    if window is None and sinks is not None:
+        raise _lib.WnwError("sinks need a window")
+    view = () if window is None else _view(window, sinks, N)
     o = _out(out, q)
     if N == 0 or T == 0:
         return o
@@ -360,15 +403,18 @@ def paged_prompt_attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: T
         raise _lib.WnwError("max_tokens is zero and there are tokens")
     G = q.shape[1] // H
     strides = (ctypes.c_int64 * 4)(q.stride(0), q.stride(1), o.stride(0), o.stride(1))
+    lib = _lib.lib()
+    call, size = (lib.wnw_paged_prompt_attn_window, lib.wnw_paged_prompt_window_workspace_bytes) if view else \
+        (lib.wnw_paged_prompt_attn, lib.wnw_paged_prompt_workspace_bytes)
     with torch.cuda.device(q.device):
         _lib.ensure_init(q.device)
-        need = int(_lib.lib().wnw_paged_prompt_workspace_bytes(ctypes.byref(cache), G, most))
+        need = int(size(ctypes.byref(cache), G, most, *view))
         if G * most <= 16:
             ws = _workspace(q.device, N, need, workspace)
         else:
             ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-        _lib.check(_lib.lib().wnw_paged_prompt_attn(
+        _lib.check(call(
             ctypes.byref(cache), _lib.ptr(seg_len), _lib.ptr(q), _lib.ptr(o), strides, T, B, G, _lib.ptr(cu_tokens), most,
-            float(scale), _lib.dtype_code(q.dtype), _lib.ptr(ws), max(need, 0), _lib.stream_of(q.device)),
+            *view, float(scale), _lib.dtype_code(q.dtype), _lib.ptr(ws), max(need, 0), _lib.stream_of(q.device)),
             "paged_prompt_attn")
     return o
