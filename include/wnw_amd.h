@@ -46,6 +46,7 @@ extern "C" {
 #define WNW_DEVERR_BOUNDS 1   /* an offset pointed outside the given rows  */
 #define WNW_DEVERR_ORDER 2    /* cu_seqlens decreasing                     */
 #define WNW_DEVERR_CAPACITY 4 /* in-place append beyond segment capacity   */
+#define WNW_DEVERR_VALUES 8   /* NaN or +inf among a beam's logits, or its score */
 
 /* attention kernel selection (wnw_decode_attn_ex) */
 #define WNW_ATTN_AUTO 0 /* fastest kernel that supports the arguments    */
@@ -881,6 +882,119 @@ int wnw_paged_prompt_attn_window(
     const int32_t* window, int64_t window_all, const int32_t* sinks,
     int64_t sinks_all, float scale, int dtype, void* workspace,
     int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Pages of the paged cache                                                  */
+/* ------------------------------------------------------------------------ */
+/*
+ * Which pages of a pool are used: page_refs int32 [n_pages] counts the table
+ * entries that name each (0: free; a caller's own pages, that no table names,
+ * may be counted too).  An entry is a page or -1; others set WNW_DEVERR_BOUNDS
+ * and are taken for -1.  A segment's page that is partly filled is named by no
+ * other entry.  All arrays are device arrays; nothing is waited for.
+ *
+ * Fresh pages are the lowest free ones, handed out in the order of (segment,
+ * block).  Where a call cannot be done, because the free pages do not suffice
+ * (WNW_DEVERR_CAPACITY) or one of its lengths, parents or token counts is bad
+ * (WNW_DEVERR_BOUNDS), nothing is done: see each.
+ *
+ * workspace: wnw_pages_workspace_bytes, 256-byte aligned, in no state that
+ * matters; launches that may overlap must not share one.
+ */
+int64_t wnw_pages_workspace_bytes(int64_t n_seg, int64_t n_samples,
+                                  int64_t n_pages);
+
+/*
+ * Reorders and copies samples: new sample i goes on from sample parents[i]
+ * (int32 [n_new], in [0, n_old), or -1: no rows).  A parent's first child takes
+ * its pages over; others share those that are full and get a fresh one for a
+ * block that is partly filled.  new_table [n_new * kv_heads, max_blocks] (rows
+ * new_stride entries apart), new_len [n_new * kv_heads], new_refs [n_pages], and
+ * copies [n_new * kv_heads, 3]: the page, the fresh page and the rows to copy,
+ * (-1, -1, 0) where there is none; wnw_paged_copy does it, for each layer that
+ * shares the table.  Pages of samples that no one goes on from are given back.
+ * The outputs overlap none of the inputs.  Not done: new_table -1, new_len 0, no
+ * copies, new_refs as page_refs.
+ */
+int wnw_paged_fork(const int32_t* page_table, int64_t table_stride,
+                   const int32_t* seg_len, const int32_t* page_refs,
+                   const int32_t* parents, int64_t n_old, int64_t n_new,
+                   int64_t kv_heads, int64_t max_blocks, int64_t n_pages,
+                   int64_t page_rows, int32_t* new_table, int64_t new_stride,
+                   int32_t* new_len, int32_t* new_refs, int32_t* copies,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Pages for the next rows of each segment: the blocks of rows [seg_len, seg_len
+ * + n) that have none get one, n = cu_tokens[b + 1] - cu_tokens[b] of the
+ * segment's sample b, or `tokens` with cu_tokens NULL.  With a window (window /
+ * window_all >= 0, as wnw_paged_decode_attn_window takes it; window_all < 0 and
+ * window NULL: none) the blocks that neither the row at seg_len nor a later one
+ * sees are given back: those past the sinks that end at or below row seg_len + 1
+ * - window.  They serve later calls, not this one.  new_table and new_refs may
+ * be page_table and page_refs themselves (with the same stride), else overlap
+ * neither.  Not done: both as they were.
+ */
+int wnw_paged_reserve(const int32_t* page_table, int64_t table_stride,
+                      const int32_t* seg_len, const int32_t* page_refs,
+                      int64_t n_seg, int64_t n_samples, int64_t max_blocks,
+                      int64_t n_pages, int64_t page_rows,
+                      const int32_t* cu_tokens, int64_t tokens,
+                      const int32_t* window, int64_t window_all,
+                      const int32_t* sinks, int64_t sinks_all,
+                      int32_t* new_table, int64_t new_stride,
+                      int32_t* new_refs, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/*
+ * The used pages to the front of the pool: with U of them, each one at U or
+ * above moves, in order, to the lowest place below U that is free.  moves
+ * [n_pages / 2, 3]: (page, its new place, page_rows), then (-1, -1, 0); used [1]:
+ * U.  new_table and new_refs as for wnw_paged_reserve.
+ */
+int wnw_paged_compact(const int32_t* page_table, int64_t table_stride,
+                      const int32_t* page_refs, int64_t n_seg,
+                      int64_t max_blocks, int64_t n_pages, int64_t page_rows,
+                      int32_t* new_table, int64_t new_stride,
+                      int32_t* new_refs, int32_t* moves, int32_t* used,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Copies rows [0, n) of page src to page dst for each (src, dst, n) of copies
+ * [n_copies, 3], of K, V and their scales.  Entries with src < 0 are none; one
+ * with a page outside the pool, n outside [0, page_rows] or src == dst sets
+ * WNW_DEVERR_BOUNDS and is left out.  No page is dst twice, or both src and dst.
+ * Of `cache`, n_seg, max_blocks and page_table are not looked at.
+ */
+int wnw_paged_copy(const wnw_paged_cache* cache, const int32_t* copies,
+                   int64_t n_copies, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Beam search                                                               */
+/* ------------------------------------------------------------------------ */
+/*
+ * The k best continuations of each sample: of the candidates (beam w, token v)
+ * with total = scores[b, w] + logits[b, w, v] - log sum_v exp logits[b, w, v],
+ * held in 64 bits, the k largest, equal ones by the lower (w, v).  logits [batch,
+ * beams, vocab] with strides[2] = {sample, beam} in elements, tokens contiguous,
+ * rows at any element; scores [batch, beams]; done [batch, beams] or NULL: a beam
+ * with a non-zero entry has finished and offers (scores[b, w], end) alone, its
+ * logits are not looked at.  Logits of -inf and beams with a score of -inf offer
+ * nothing.  A beam with NaN or +inf among its logits, or as its score, offers
+ * nothing and sets WNW_DEVERR_VALUES.
+ *
+ * out_scores [batch, k] (32 bits), out_parents [batch, k]: b * beams + w, as
+ * wnw_paged_fork takes them, out_tokens [batch, k].  Without a candidate: -inf,
+ * b * beams, end.  At most 64 beams and k 64, vocab below 2^25.
+ */
+int64_t wnw_beam_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab,
+                                 int dtype);
+int wnw_beam_select(const void* logits, const int64_t* strides, int64_t batch,
+                    int64_t beams, int64_t vocab, const float* scores,
+                    const uint8_t* done, int64_t end, int64_t k, int dtype,
+                    float* out_scores, int32_t* out_parents,
+                    int64_t* out_tokens, void* workspace,
+                    int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,275 @@
+"""The pools' operators against tests/pages_ref.py: whole numbers, equal ones."""
+import random
+
+import pytest
+import torch
+
+from tests import pages_ref
+from tests.test_gpu_paged import _clean
+from wnw_amd import _lib
+from wnw_amd.kv.pages import paged_compact, paged_copy, paged_fork, paged_reserve
+
+pytestmark = pytest.mark.gpu
+E4M3 = torch.float8_e4m3fn
+
+
+def _t(x, gpu, shape=None):
+    t = torch.tensor(x, dtype=torch.int32, device=gpu)
+    return t if shape is None else t.reshape(shape)
+
+
+def _wide(table, M, gpu):
+    """A table whose rows lie M + 3 entries apart."""
+    room = torch.full((max(len(table), 1), M + 3), 12345, dtype=torch.int32, device=gpu)
+    view = room[:len(table), :M]
+    if len(table) and M:
+        view.copy_(_t(table, gpu))
+    return view, room
+
+
+def _state(rng, B, H, R, M, P, junk=False, shared=True):
+    """A pool in use: samples of random lengths, some sharing full pages, some entries given back; counts that include pages
+    that no table names."""
+    pages = list(range(P))
+    rng.shuffle(pages)
+    table, lens = [], []
+    for b in range(B):
+        for h in range(H):
+            n = rng.choice([0, 1, R - 1, R, R + 1, rng.randrange(M * R + 1), M * R])
+            n = min(n, M * R)
+            row = []
+            for j in range(M):
+                named = j * R < n or rng.random() < 0.1
+                full = (j + 1) * R <= n
+                if not named or not pages or (full and rng.random() < 0.1):
+                    row.append(-1)
+                elif full and shared and table and rng.random() < 0.3 and any(e >= 0 for e in table[-1]):
+                    k = rng.randrange(M)
+                    e = table[-1][k]
+                    row.append(e if e >= 0 and (k + 1) * R <= lens[-1] else -1)
+                else:
+                    row.append(pages.pop())
+            if junk:
+                row = [rng.choice([P, -2, 0x7fffffff, -2147483648]) if e < 0 and rng.random() < 0.3 else e for e in row]
+            table.append(row)
+            lens.append(n)
+    pinned = [pages.pop() for _ in range(min(3, len(pages)))]
+    return table, lens, pages_ref.counts(table, P, pinned)
+
+
+SIZES = [(1, 1, 16, 1, 3), (1, 1, 64, 4, 10), (3, 2, 16, 9, 70), (8, 4, 32, 20, 700), (5, 8, 128, 300, 20000), (64, 8, 16, 7, 40000),
+         (2, 1, 256, 700, 17001), (300, 1, 16, 3, 2000), (0, 2, 16, 4, 9), (3, 1, 16, 0, 5)]
+
+
+@pytest.mark.parametrize("B,H,R,M,P", SIZES)
+@pytest.mark.parametrize("junk", [False, True])
+def test_fork(gpu, B, H, R, M, P, junk):
+    rng = random.Random(B * 1000 + M)
+    for n_new in (B, 1, 2 * B + 3, 0):
+        table, lens, refs = _state(rng, B, H, R, M, P, junk)
+        parents = [rng.randrange(-1, B) if rng.random() < 0.9 else -1 for _ in range(n_new)]
+        if n_new == 1 and B:
+            parents = [B - 1]
+        want = pages_ref.fork(table, lens, refs, parents, R, H, M)
+        view, room = _wide(table, M, gpu)
+        new, new_len, new_refs, copies = paged_fork(view, _t(lens, gpu), _t(refs, gpu), _t(parents, gpu), R, kv_heads=H)
+        torch.cuda.synchronize()
+        err = _lib.device_error()
+        if want is None:
+            assert err & _lib.DEVERR_CAPACITY
+            assert bool((new == -1).all()) and bool((new_len == 0).all()) and new_refs.tolist() == refs
+            assert copies.tolist() == [[-1, -1, 0]] * (n_new * H)
+        else:
+            assert err in ((0, _lib.DEVERR_BOUNDS) if junk else (0,))
+            assert new.tolist() == want[0] and new_len.tolist() == want[1]
+            assert new_refs.tolist() == want[2] and copies.tolist() == want[3]
+        assert room[:, M:].unique().tolist() in ([12345], []) and view.tolist() == table
+
+
+@pytest.mark.parametrize("B,H,R,M,P", SIZES)
+@pytest.mark.parametrize("junk", [False, True])
+def test_reserve(gpu, B, H, R, M, P, junk):
+    rng = random.Random(B * 999 + M)
+    N = B * H
+    for how in ("one", "none", "chunks", "window", "windows"):
+        table, lens, refs = _state(rng, B, H, R, M, P, junk)
+        cu = view = None
+        tokens = [{"one": 1, "none": 0, "window": min(2, R * M)}.get(how, 0)] * N
+        kw = dict(tokens=tokens[0] if N else 0)
+        if how in ("chunks", "windows"):
+            new = [rng.choice([0, 1, rng.randrange(M * R + 1)]) for _ in range(B)]
+            cu = [sum(new[:b]) for b in range(B + 1)]
+            tokens = [new[s // H] for s in range(N)]
+            lens = [max(0, min(n, M * R - t)) for n, t in zip(lens, tokens)]
+            kw = dict(cu_tokens=_t(cu, gpu))
+        else:
+            lens = [max(0, min(n, M * R - t)) for n, t in zip(lens, tokens)]
+        if how == "window":
+            view = [(R + 3, 5)] * N
+            kw |= dict(window=R + 3, sinks=5)
+        elif how == "windows":
+            view = [(rng.choice([0, 1, R, 3 * R + 1, 0x7fffffff]), rng.choice([0, 1, R, R + 1, 0x7fffffff])) for _ in range(N)]
+            kw |= dict(window=_t([w for w, _ in view], gpu), sinks=_t([z for _, z in view], gpu))
+        want = pages_ref.reserve(table, lens, refs, R, tokens, view)
+        was, room = _wide(table, M, gpu)
+        counts = _t(refs, gpu)
+        new, new_refs = paged_reserve(was, _t(lens, gpu), counts, R, **kw)
+        torch.cuda.synchronize()
+        err = _lib.device_error()
+        if want is None:
+            assert err & _lib.DEVERR_CAPACITY, how
+            want = table, refs
+        else:
+            assert err in ((0, _lib.DEVERR_BOUNDS) if junk else (0,)), how
+        assert new.tolist() == want[0] and new_refs.tolist() == want[1], how
+        assert was.tolist() == table and counts.tolist() == refs
+        paged_reserve(was, _t(lens, gpu), counts, R, out=(was, counts), **kw)  # in place
+        torch.cuda.synchronize()
+        _lib.device_error()
+        assert was.tolist() == want[0] and counts.tolist() == want[1], how
+        assert room[:, M:].unique().tolist() in ([12345], [])
+
+
+@pytest.mark.parametrize("B,H,R,M,P", SIZES + [(20, 4, 16, 40, 50001)])
+@pytest.mark.parametrize("junk", [False, True])
+def test_compact(gpu, B, H, R, M, P, junk):
+    rng = random.Random(B * 77 + M)
+    for _ in range(2):
+        table, lens, refs = _state(rng, B, H, R, M, P, junk)
+        want = pages_ref.compact(table, refs, R)
+        was, room = _wide(table, M, gpu)
+        counts = _t(refs, gpu)
+        new, new_refs, moves, used = paged_compact(was, counts, R)
+        torch.cuda.synchronize()
+        assert _lib.device_error() in ((0, _lib.DEVERR_BOUNDS) if junk else (0,))
+        assert new.tolist() == want[0] and new_refs.tolist() == want[1]
+        assert moves.tolist() == want[2] and used.tolist() == [want[3]]
+        got = paged_compact(was, counts, R, out=(was, counts))
+        torch.cuda.synchronize()
+        _lib.device_error()
+        assert was.tolist() == want[0] and counts.tolist() == want[1] and got[2].tolist() == want[2]
+        again = paged_compact(was, counts, R)  # nothing is left to move
+        assert torch.equal(again[0], was) and torch.equal(again[1], counts) and bool((again[2][:, 0] == -1).all())
+        assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype,D,R", [(E4M3, 128, 64), (E4M3, 64, 16), (torch.bfloat16, 256, 256), (torch.float16, 64, 32),
+                                       (E4M3, 256, 128)])
+def test_copy(gpu, dtype, D, R):
+    rng = random.Random(R)
+    P = 300
+    both = torch.randint(0, 256, (P, 2, R, D * (1 if dtype == E4M3 else 2)), dtype=torch.uint8, device=gpu)
+    both = both if dtype == E4M3 else both
+    k, v = (both[:, i].view(dtype) for i in range(2))  # pages of K and V beside each other
+    scales = [torch.rand(P, device=gpu) for _ in range(2)] if dtype == E4M3 else [None, None]
+    for n in (1, 7, 100, 0):
+        ids = rng.sample(range(P), 2 * n)
+        copies = [[ids[2 * i], ids[2 * i + 1], rng.choice([0, 1, R // 2, R - 1, R])] for i in range(n)]
+        copies += [[-1, -1, 0], [-5, 3, R]]
+        rng.shuffle(copies)
+        want, ws = both.clone(), [None if s is None else s.clone() for s in scales]
+        for a, b, rows in copies:
+            if a >= 0:
+                want[b, :, :rows] = want[a, :, :rows]
+                for s in ws:
+                    if s is not None:
+                        s[b] = s[a]
+        paged_copy(k, v, _t(copies, gpu), k_scale=scales[0], v_scale=scales[1])
+        _clean()
+        assert torch.equal(both, want)
+        assert all(s is None or torch.equal(s, t) for s, t in zip(scales, ws))
+    # entries outside the pool or the page: the error word, and nothing else
+    was = both.clone()
+    for bad in ([P, 0, R], [0, P, R], [0, -1, R], [4, 4, R], [0, 1, R + 1], [0, 1, -1], [0x7fffffff, 1, 1]):
+        paged_copy(k, v, _t([bad], gpu), k_scale=scales[0], v_scale=scales[1])
+        torch.cuda.synchronize()
+        assert _lib.device_error() == _lib.DEVERR_BOUNDS, bad
+    assert torch.equal(both, was)
+
+
+def test_bad_numbers_change_nothing(gpu):
+    """Lengths, parents, token counts and windows that cannot be: the error word, outputs as documented."""
+    table, refs, R = [[0, 1, -1, -1], [2, -1, -1, -1]], [1, 1, 1, 0, 0, 0], 16
+    bounds, room = _lib.DEVERR_BOUNDS, _lib.DEVERR_CAPACITY
+
+    def fork(lens=(20, 5), parents=(1, 0)):
+        return paged_fork(_t(table, gpu), _t(lens, gpu), _t(refs, gpu), _t(parents, gpu), R, kv_heads=1)
+
+    for kw in (dict(lens=(-1, 5)), dict(lens=(20, 65)), dict(parents=(2, 0)), dict(parents=(-2,)), dict(parents=(0, 0x7fffffff))):
+        new, new_len, new_refs, copies = fork(**kw)
+        torch.cuda.synchronize()
+        assert _lib.device_error() == bounds, kw
+        assert bool((new == -1).all()) and bool((new_len == 0).all()) and new_refs.tolist() == refs and bool((copies[:, 0] == -1).all())
+
+    def reserve(lens=(20, 5), **kw):
+        return paged_reserve(_t(table, gpu), _t(lens, gpu), _t(refs, gpu), R, **kw)
+
+    for want, kw in ((bounds, dict(lens=(-1, 5))), (bounds, dict(lens=(20, 65), tokens=0)), (room, dict(tokens=60)),
+                     (room, dict(tokens=44)), (bounds, dict(cu_tokens=_t([0, 5, 3], gpu))), (bounds, dict(cu_tokens=_t([-1, 5, 9], gpu))),
+                     (bounds, dict(window=_t([5, -1], gpu))), (bounds, dict(window=5, sinks=_t([-3, 0], gpu))),
+                     (room, dict(tokens=1 << 30)), (room, dict(cu_tokens=_t([0, 5, 0x7fffffff], gpu)))):
+        new, new_refs = reserve(**kw)
+        torch.cuda.synchronize()
+        assert _lib.device_error() == want, kw
+        assert new.tolist() == table and new_refs.tolist() == refs
+
+
+def test_captured_in_place(gpu):
+    """A captured reserve that keeps its table and counts in place, replayed as segments grow, beside eager calls."""
+    rng = random.Random(5)
+    B, H, R, M, P = 3, 2, 16, 30, 400
+    table, refs = [[-1] * M for _ in range(B * H)], [0] * P
+    lens = [0] * (B * H)
+    view = [(40, 5)] * (B * H)
+    dt, dl, dr = _t(table, gpu), _t(lens, gpu), _t(refs, gpu)
+    keep = dt.clone(), dr.clone()
+    paged_reserve(dt, dl, dr, R, tokens=7, window=40, sinks=5)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged_reserve(dt, dl, dr, R, tokens=7, window=40, sinks=5, out=(dt, dr))
+    assert torch.equal(dt, keep[0]) and torch.equal(dr, keep[1])  # captured, not run
+    for step in range(40):
+        graph.replay()
+        table, refs = pages_ref.reserve(table, lens, refs, R, [7] * (B * H), view)
+        if step % 7 == 3:
+            paged_reserve(dt.clone(), dl, dr.clone(), R, tokens=16)
+        torch.cuda.synchronize()
+        assert dt.tolist() == table and dr.tolist() == refs and refs == pages_ref.counts(table, P)
+        lens = [n + rng.choice([7, 3]) for n in lens]
+        dl.copy_(_t(lens, gpu))
+    _clean()
+
+
+def test_refusals(gpu):
+    table, lens, refs = _t([[0, 1], [2, -1]], gpu), _t([20, 5], gpu), _t([1, 1, 1, 0], gpu)
+    parents = _t([0, 1], gpu)
+    E = _lib.WnwError
+    for bad in (dict(t=table.long()), dict(t=table[0]), dict(t=table.t()), dict(l=lens.long()), dict(l=lens[:1]), dict(r=refs.float()),
+                dict(r=refs.view(2, 2)), dict(p=parents.long()), dict(p=parents.view(1, 2)), dict(R=24), dict(R=512), dict(h=0), dict(h=3),
+                dict(t=table.cpu()), dict(p=parents.cpu())):
+        c = dict(t=table, l=lens, r=refs, p=parents, R=16, h=1)
+        c.update(bad)
+        with pytest.raises(E):
+            paged_fork(c["t"], c["l"], c["r"], c["p"], c["R"], kv_heads=c["h"])
+    for kw in (dict(tokens=-1), dict(sinks=3), dict(window=-1), dict(window=3, sinks=-1), dict(cu_tokens=_t([0, 1, 2, 3], gpu)),
+               dict(cu_tokens=lens.long()), dict(out=(table[:1], refs)), dict(out=(table, refs[:2])), dict(out=(table.long(), refs)),
+               dict(out=(table, refs.clone()[:3])), dict(window=lens.cpu())):
+        with pytest.raises(E):
+            paged_reserve(table, lens, refs, 16, **kw)
+    room = torch.zeros(40, dtype=torch.int32, device=gpu)
+    with pytest.raises(E, match="overlaps"):  # one row further on in the same memory
+        paged_reserve(room[:20].view(5, 4), torch.zeros(5, dtype=torch.int32, device=gpu), refs, 16,
+                      out=(room[4:24].view(5, 4), refs.clone()))
+    with pytest.raises(E, match="overlaps"):
+        paged_compact(room[:20].view(5, 4), room[20:30], 16, out=(room[:20].view(5, 4), room[21:31]))
+    with pytest.raises(E, match="overlaps"):
+        paged_reserve(room[:20].view(5, 4), torch.zeros(5, dtype=torch.int32, device=gpu), room[20:30], 16,
+                      out=(room[20:40].view(5, 4), refs.new_zeros(10)))
+    k = torch.zeros(4, 16, 64, dtype=torch.bfloat16, device=gpu)
+    for bad in (dict(c=_t([[0, 1]], gpu)), dict(c=_t([[0, 1, 2]], gpu).long()), dict(v=k[:2]), dict(v=k.half()), dict(s=torch.ones(4, device=gpu)),
+                dict(k=k.float(), v=k.float()), dict(k=k.transpose(1, 2), v=k.transpose(1, 2)), dict(c=torch.zeros(1, 3, dtype=torch.int32))):
+        c = dict(k=k, v=k.clone(), c=_t([[0, 1, 2]], gpu), s=None)
+        c.update(bad)
+        with pytest.raises(E):
+            paged_copy(c["k"], c["v"], c["c"], k_scale=c["s"])
+    _clean()

@@ -17,7 +17,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libwnw_amd.
 WNW_OK, WNW_EINVAL, WNW_EHIP, WNW_ENOTSUP = 0, 1, 2, 3
 DT_F32, DT_F16, DT_BF16, DT_E4M3 = 0, 1, 2, 3
 ATTN_AUTO, ATTN_MFMA, ATTN_VALU, ATTN_STREAM = 0, 1, 2, 3
-DEVERR_BOUNDS, DEVERR_ORDER, DEVERR_CAPACITY = 1, 2, 4
+DEVERR_BOUNDS, DEVERR_ORDER, DEVERR_CAPACITY, DEVERR_VALUES = 1, 2, 4, 8
 NOALLOC_SCRATCH_BYTES, NOALLOC_MAX_SEG = 16 << 20, 4096
 TOPK_MAX_CHUNKS, TOPK_MAX_K = 8192, 64  # wnw_chunk_topk: chunks of one sample, k
 
@@ -77,6 +77,14 @@ _SIGNATURES = {
     "wnw_paged_prompt_window_workspace_bytes": (_i64, [_vp, _i64, _i64, _vp, _i64, _vp, _i64]),
     "wnw_paged_prompt_attn_window": (_i32, [_vp] * 5 + [_i64] * 3 + [_vp, _i64, _vp, _i64, _vp, _i64, _f32, _i32, _vp, _i64,
                                                                   _vp]),
+    "wnw_pages_workspace_bytes": (_i64, [_i64] * 3),
+    "wnw_paged_fork": (_i32, [_vp, _i64, _vp, _vp, _vp] + [_i64] * 6 + [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "wnw_paged_reserve": (_i32, [_vp, _i64, _vp, _vp] + [_i64] * 5 + [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp,
+                                                                    _i64, _vp]),
+    "wnw_paged_compact": (_i32, [_vp, _i64, _vp] + [_i64] * 4 + [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "wnw_paged_copy": (_i32, [_vp, _vp, _i64, _vp]),
+    "wnw_beam_workspace_bytes": (_i64, [_i64] * 3 + [_i32]),
+    "wnw_beam_select": (_i32, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
     "wnw_read_stream": (_i32, [_vp, _i64, _i64, _i32, _vp, _vp]),
     # host planner (CPU only)
     "wnw_planner_create": (_vp, [_i32, _i32, _i32, _i32]),

@@ -1,0 +1,440 @@
+// Selection of a beam search's next beams (gfx950): the k best continuations of
+// each sample, over all of its beams and the vocabulary.
+//
+// Mathematics: candidate (w, v) has total(w, v) = score_w + (x_wv - lse_w), lse_w =
+// log sum_v exp x_wv, in 64 bits; the k largest totals, equal ones by the lower
+// (w, v).  Within a beam totals go with the logits, so a beam need not be sorted.
+//
+// Two launches.  The first reads the logits once: a wave takes 2,048 of a row and
+// leaves their maximum, sum exp(x - max) and the maximum of each group of 256
+// bytes.  In the second, a workgroup a sample puts the sums together, finds the
+// k best groups by their maxima (the k best elements lie in those: each other
+// group is behind k maxima), reads these alone again, and ranks what is not
+// below the k-th group's maximum.
+#include "wnw_common.h"
+
+namespace wnw {
+
+static constexpr int kBeamTask = 2048;    // logits of a wave
+static constexpr int kBeamThreads = 1024; // of a sample's workgroup
+static constexpr int kBeamMax = 64;       // beams, and candidates to select
+static constexpr int kBeamList = 512;     // candidates that are ranked against each other
+static constexpr float kBeamLog2e = 1.4426950408889634f;
+static constexpr float kBeamLowest = -3.402823466e38f;  // running maxima start here
+
+struct BeamParams {
+  const void* logits;
+  const float* scores;  // [B, W]
+  const uint8_t* done;  // [B, W] or null
+  double* part_sum;     // [rows, tasks]
+  float* part_max;      // [rows, tasks]
+  float* group_max;     // [rows, tasks, groups of a task]
+  float* out_scores;    // [B, k]
+  int32_t* out_parents;
+  int64_t* out_tokens;
+  int32_t* err;
+  int64_t stride_b, stride_w;  // in elements
+  int32_t B, W, V, k, tasks, end;
+};
+
+template <typename T>
+struct BeamGeom {
+  static constexpr int kVec = 16 / Elem<T>::kBytes;  // elements of a load
+  static constexpr int kGroup = 16 * kVec;           // of a group: 16 lanes' loads
+  static constexpr int kLoads = kBeamTask / (64 * kVec);
+  static constexpr int kGroups = kBeamTask / kGroup;  // of a task
+};
+
+// Elements e .. e + kVec - 1 of a row of V, those past its end -inf.  Rows may
+// start at any element: a load near the end is taken from the row's last kVec.
+template <typename T>
+__device__ __forceinline__ void beam_load(const T* row, int e, int V, u32x4* raw, int* from) {
+  constexpr int N = BeamGeom<T>::kVec;
+  struct __attribute__((packed, aligned(Elem<T>::kBytes))) Any {
+    u32x4 x;
+  };
+  *from = max(min(e, V - N), 0);
+  if (V >= N) {
+    *raw = ((const WNW_GLOBAL Any*)(uintptr_t)(row + *from))->x;
+  } else {
+    uint32_t w[4] = {0, 0, 0, 0};
+    for (int i = 0; i < V; ++i) {
+      if constexpr (Elem<T>::kBytes == 4)
+        w[i] = ((const uint32_t*)row)[i];
+      else
+        w[i >> 1] |= (uint32_t)((const uint16_t*)row)[i] << (16 * (i & 1));
+    }
+    *raw = u32x4{w[0], w[1], w[2], w[3]};
+  }
+}
+template <typename T>
+__device__ __forceinline__ void beam_values(const u32x4& raw, int e, int from, int V, float* x) {
+  constexpr int N = BeamGeom<T>::kVec;
+  if constexpr (Elem<T>::kBytes == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = __uint_as_float(raw[i]);
+  } else {
+    unpack8(raw, x, (T*)nullptr);
+  }
+  if (from != e || e + N > V) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (from + i < e || from + i >= V) x[i] = -INFINITY;
+  }
+}
+
+template <int kCtrl>
+__device__ __forceinline__ float dpp_max(float x) {
+  return fmaxf(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), kCtrl, 0xf, 0xf, false)));
+}
+// Maximum over the 16 lanes of a row
+__device__ __forceinline__ float max_row16(float x) {
+  x = dpp_max<0xB1>(x);   // quad_perm [1, 0, 3, 2]
+  x = dpp_max<0x4E>(x);   // quad_perm [2, 3, 0, 1]
+  x = dpp_max<0x141>(x);  // row_half_mirror
+  return dpp_max<0x140>(x);
+}
+__device__ __forceinline__ double wave_sum64(double x) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void beam_rows_kernel(BeamParams p) {
+  using Ge = BeamGeom<T>;
+  constexpr int N = Ge::kVec, U = Ge::kLoads;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t at = (int64_t)blockIdx.x * 4 + w;  // the task
+  if (at >= (int64_t)p.B * p.W * p.tasks) return;
+  const int row = (int)(at / p.tasks), task = (int)(at - (int64_t)row * p.tasks);
+  if (p.done && p.done[row]) return;  // its logits are not looked at
+  const T* x0 = (const T*)p.logits + (int64_t)(row / p.W) * p.stride_b + (int64_t)(row % p.W) * p.stride_w;
+  const int first = task * kBeamTask + lane * N;
+  u32x4 raw[U];
+  int from[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) beam_load<T>(x0, first + u * 64 * N, p.V, &raw[u], &from[u]);
+  float x[U][N], most[U];
+  float m = kBeamLowest;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    beam_values<T>(raw[u], first + u * 64 * N, from[u], p.V, x[u]);
+    float y = x[u][0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) y = fmaxf(y, x[u][i]);
+    most[u] = max_row16(y);
+    m = fmaxf(m, most[u]);
+  }
+  m = max_x32(max_x16(m));
+  // (a logit of NaN or +inf leaves NaN in the sum: the pick refuses the beam)
+  double sum = 0.0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s += __builtin_amdgcn_exp2f((x[u][i] - m) * kBeamLog2e);
+    sum += (double)s;
+  }
+  sum = wave_sum64(sum);
+  if (lane == 0) {
+    p.part_max[at] = m;
+    p.part_sum[at] = sum;
+  }
+  float mine = most[0];
+#pragma unroll
+  for (int u = 1; u < U; ++u) mine = (lane & 15) == u ? most[u] : mine;
+  if ((lane & 15) < U) p.group_max[at * Ge::kGroups + (lane & 15) * 4 + (lane >> 4)] = mine;
+}
+
+// A candidate's place in the order: its total as an ordered integer, and (w, v).
+struct BeamKey {
+  uint64_t total;
+  uint32_t id;
+};
+__device__ __forceinline__ uint64_t ordered(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);  // -0 is 0
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double unordered(uint64_t u) {
+  return __builtin_bit_cast(double, u >> 63 ? u & ~(1ull << 63) : ~u);
+}
+static constexpr BeamKey kBeamNone = {0, 0xffffffffu};  // behind every candidate
+__device__ __forceinline__ bool ahead(const BeamKey& a, const BeamKey& b) {
+  return a.total > b.total || (a.total == b.total && a.id < b.id);
+}
+__device__ __forceinline__ BeamKey ahead_of(const BeamKey& a, const BeamKey& b) { return ahead(a, b) ? a : b; }
+__device__ __forceinline__ BeamKey wave_first(BeamKey x) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const BeamKey y = {(uint64_t)__shfl_xor((unsigned long long)x.total, o), (uint32_t)__shfl_xor((int)x.id, o)};
+    x = ahead_of(x, y);
+  }
+  return x;
+}
+
+struct BeamShared {
+  double lse[kBeamMax];
+  float score[kBeamMax];
+  int state[kBeamMax];  // 1: continues, 2: finished, 0: neither
+  BeamKey list[kBeamList];
+  BeamKey best[kBeamMax];
+  BeamKey wave[kBeamThreads / 64];
+  int count, found;
+};
+
+// The k first candidates, one after the other: next(last) gives a thread's first one behind `last`.
+template <typename F>
+__device__ __forceinline__ void beam_rounds(BeamShared& sh, int k, F next) {
+  BeamKey last = {~0ull, 0};
+  int r = 0;
+  for (; r < k; ++r) {
+    const BeamKey mine = wave_first(next(last));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = mine;
+    __syncthreads();
+    BeamKey x = sh.wave[0];
+    for (int i = 1; i < kBeamThreads / 64; ++i) x = ahead_of(x, sh.wave[i]);
+    if (x.id == kBeamNone.id) break;
+    if (threadIdx.x == 0) sh.best[r] = x;
+    last = x;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) sh.found = r;
+  __syncthreads();
+}
+// The k first of the list's n, by their ranks.
+__device__ __forceinline__ void beam_ranks(BeamShared& sh, int k, int n) {
+  for (int i = threadIdx.x; i < n; i += kBeamThreads) {
+    const BeamKey x = sh.list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += ahead(sh.list[j], x);
+    if (rank < k) sh.best[rank] = x;
+  }
+  if (threadIdx.x == 0) sh.found = min(n, k);
+  __syncthreads();
+}
+
+template <typename T>
+__global__ __launch_bounds__(kBeamThreads) void beam_pick_kernel(BeamParams p) {
+  using Ge = BeamGeom<T>;
+  constexpr int N = Ge::kVec;
+  __shared__ BeamShared sh;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int W = p.W, k = p.k, groups = p.tasks * Ge::kGroups;
+  // the rows' sums
+  for (int w = wave; w < W; w += kBeamThreads / 64) {
+    const int row = b * W + w;
+    const float score = p.scores[row];
+    int state = p.done && p.done[row] ? 2 : 1;
+    double lse = 0.0;
+    bool bad = !(score < INFINITY);
+    if (state == 1) {
+      const float* pm = p.part_max + (int64_t)row * p.tasks;
+      const double* ps = p.part_sum + (int64_t)row * p.tasks;
+      float m = kBeamLowest;
+      for (int i = lane; i < p.tasks; i += 64) m = fmaxf(m, pm[i]);
+      m = wave_max(m);
+      double s = 0.0;
+      for (int i = lane; i < p.tasks; i += 64) s += ps[i] * exp((double)pm[i] - (double)m);
+      s = wave_sum64(s);
+      lse = (double)m + log(s);
+      bad |= !(s < (double)INFINITY);
+      if (s == 0.0) state = 0;
+    }
+    if (bad || score == -INFINITY) state = 0;
+    if (lane == 0) {
+      sh.lse[w] = lse;
+      sh.score[w] = score;
+      sh.state[w] = state;
+      if (bad) raise_device_error(p.err, WNW_DEVERR_VALUES);
+    }
+  }
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  auto total_of = [&](int w, float x) { return (double)sh.score[w] + ((double)x - sh.lse[w]); };
+
+  // the k best groups
+  const int n = W * groups;
+  auto group_key = [&](int g) {
+    const int w = g / groups;
+    if (sh.state[w] != 1) return kBeamNone;
+    const float x = p.group_max[(int64_t)b * n + g];
+    return x == -INFINITY ? kBeamNone : BeamKey{ordered(total_of(w, x)), (uint32_t)g};
+  };
+  {
+    BeamKey mine = kBeamNone;
+    for (int g = tid; g < n; g += kBeamThreads) mine = ahead_of(group_key(g), mine);
+    // rows of 16 lanes: k of their 64 maxima are no further back than the k-th of them
+    BeamKey x = mine;
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) {
+      const BeamKey y = {(uint64_t)__shfl_xor((unsigned long long)x.total, o), (uint32_t)__shfl_xor((int)x.id, o)};
+      x = ahead_of(x, y);
+    }
+    if ((lane & 15) == 0) sh.best[tid >> 4] = x;
+    __syncthreads();
+    const BeamKey y = sh.best[lane];
+    int rank = 0;
+    for (int j = 0; j < 64; ++j) rank += ahead(sh.best[j], y) || (j < lane && sh.best[j].id == y.id && sh.best[j].total == y.total);
+    const int at = __builtin_ctzll(__ballot(rank == k - 1));
+    const BeamKey least = sh.best[at];
+    __syncthreads();
+    for (int g = tid; g < n; g += kBeamThreads) {
+      const BeamKey key = group_key(g);
+      if (key.id != kBeamNone.id && !ahead(least, key)) {
+        const int slot = atomicAdd(&sh.count, 1);
+        if (slot < kBeamList) sh.list[slot] = key;
+      }
+    }
+    __syncthreads();
+    const int c = sh.count;
+    if (c <= kBeamList)
+      beam_ranks(sh, k, c);
+    else
+      beam_rounds(sh, k, [&](const BeamKey& last) {
+        BeamKey first = kBeamNone;
+        for (int g = tid; g < n; g += kBeamThreads) {
+          const BeamKey key = group_key(g);
+          if (ahead(last, key)) first = ahead_of(key, first);
+        }
+        return first;
+      });
+  }
+  // their elements, and the finished beams
+  const int found = sh.found;
+  const uint64_t floor_total = found == k ? sh.best[k - 1].total : 0;
+  const int mine = tid >> 4;  // the thread's group, 16 threads each
+  BeamKey keys[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) keys[i] = kBeamNone;
+  if (mine < found) {
+    const int g = (int)sh.best[mine].id, w = g / groups, e = (g - w * groups) * Ge::kGroup + (tid & 15) * N;
+    const T* row = (const T*)p.logits + (int64_t)b * p.stride_b + (int64_t)w * p.stride_w;
+    u32x4 raw;
+    int from;
+    float x[N];
+    beam_load<T>(row, e, p.V, &raw, &from);
+    beam_values<T>(raw, e, from, p.V, x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint64_t t = ordered(total_of(w, x[i]));
+      if (x[i] > -INFINITY && t >= floor_total) keys[i] = BeamKey{t, (uint32_t)w * (uint32_t)p.V + (uint32_t)(from + i)};
+    }
+  }
+  BeamKey lone = kBeamNone;
+  if (tid < W && sh.state[tid] == 2)
+    lone = BeamKey{ordered((double)sh.score[tid]), (uint32_t)tid * (uint32_t)p.V + (uint32_t)p.end};
+  __syncthreads();
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  auto put = [&](const BeamKey& x) {
+    if (x.id == kBeamNone.id) return;
+    const int slot = atomicAdd(&sh.count, 1);
+    if (slot < kBeamList) sh.list[slot] = x;
+  };
+#pragma unroll
+  for (int i = 0; i < N; ++i) put(keys[i]);
+  put(lone);
+  __syncthreads();
+  const int c = sh.count;
+  if (c <= kBeamList)
+    beam_ranks(sh, k, c);
+  else
+    beam_rounds(sh, k, [&](const BeamKey& last) {
+      BeamKey first = ahead(last, lone) ? lone : kBeamNone;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (ahead(last, keys[i])) first = ahead_of(keys[i], first);
+      return first;
+    });
+  if (tid < k) {
+    const bool is = tid < sh.found;
+    const BeamKey x = is ? sh.best[tid] : kBeamNone;
+    const int w = is ? (int)(x.id / (uint32_t)p.V) : 0;
+    const int64_t at = (int64_t)b * k + tid;
+    p.out_scores[at] = is ? (float)unordered(x.total) : -INFINITY;
+    p.out_parents[at] = b * W + w;
+    p.out_tokens[at] = is ? (int64_t)(x.id - (uint32_t)w * (uint32_t)p.V) : (int64_t)p.end;
+  }
+}
+
+struct BeamLayout {
+  int64_t tasks, max, groups, total;  // bytes, the sums first
+};
+static BeamLayout beam_layout(int64_t rows, int64_t vocab, int dtype) {
+  BeamLayout y;
+  y.tasks = (vocab + kBeamTask - 1) / kBeamTask;
+  const int64_t per = dtype == WNW_F32 ? BeamGeom<float>::kGroups : BeamGeom<bf16_t>::kGroups;
+  y.max = (rows * y.tasks * 8 + 255) / 256 * 256;
+  y.groups = y.max + (rows * y.tasks * 4 + 255) / 256 * 256;
+  y.total = y.groups + rows * y.tasks * per * 4;
+  return y;
+}
+static bool beam_sizes(int64_t batch, int64_t beams, int64_t vocab, int dtype) {
+  return batch >= 0 && batch < (1 << 20) && beams >= 1 && beams <= kBeamMax && vocab >= 1 && vocab < (1 << 25) &&
+         (dtype == WNW_F32 || dtype == WNW_F16 || dtype == WNW_BF16);
+}
+
+template <typename T>
+static void launch_beam(const BeamParams& p, hipStream_t st) {
+  const int64_t tasks = (int64_t)p.B * p.W * p.tasks;
+  hipLaunchKernelGGL((beam_rows_kernel<T>), dim3((unsigned)((tasks + 3) / 4)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((beam_pick_kernel<T>), dim3((unsigned)p.B), dim3(kBeamThreads), 0, st, p);
+}
+
+}  // namespace wnw
+
+using namespace wnw;
+
+extern "C" int64_t wnw_beam_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int dtype) {
+  return beam_sizes(batch, beams, vocab, dtype) ? beam_layout(batch * beams, vocab, dtype).total : -1;
+}
+
+extern "C" int wnw_beam_select(const void* logits, const int64_t* strides, int64_t batch, int64_t beams, int64_t vocab,
+                               const float* scores, const uint8_t* done, int64_t end, int64_t k, int dtype, float* out_scores,
+                               int32_t* out_parents, int64_t* out_tokens, void* workspace, int64_t workspace_bytes, void* stream) {
+  WNW_CHECK_ARG(dtype == WNW_F32 || dtype == WNW_F16 || dtype == WNW_BF16, "logits must be f32, f16 or bf16");
+  WNW_CHECK_ARG(beam_sizes(batch, beams, vocab, dtype), "bad sizes: %lld samples of %lld beams (at most %d), vocabulary %lld",
+                (long long)batch, (long long)beams, kBeamMax, (long long)vocab);
+  WNW_CHECK_ARG(k >= 1 && k <= kBeamMax, "k must be 1 to %d", kBeamMax);
+  WNW_CHECK_ARG(end >= 0 && end < vocab, "end must be a token of the vocabulary");
+  if (batch == 0) return WNW_OK;
+  WNW_CHECK_ARG(logits && strides && scores && out_scores && out_parents && out_tokens, "null pointer argument");
+  const int64_t elem = elem_bytes(dtype);
+  WNW_CHECK_ARG(strides[0] >= 0 && strides[1] >= 0 && strides[0] < (1ll << 40) && strides[1] < (1ll << 40), "bad strides");
+  WNW_CHECK_ARG((uintptr_t)logits % elem == 0, "the logits are not aligned to their type");
+  const BeamLayout y = beam_layout(batch * beams, vocab, dtype);
+  WNW_CHECK_ARG((batch * beams * y.tasks + 3) / 4 < (1ll << 24), "too many logits for one call");
+  WNW_CHECK_ARG(workspace && workspace_bytes >= y.total, "workspace too small: %lld bytes, %lld needed",
+                (long long)workspace_bytes, (long long)y.total);
+  WNW_CHECK_ARG((uintptr_t)workspace % 256 == 0, "the workspace must be 256-byte aligned");
+  BeamParams p;
+  p.logits = logits;
+  p.scores = scores;
+  p.done = done;
+  p.part_sum = (double*)workspace;
+  p.part_max = (float*)((uint8_t*)workspace + y.max);
+  p.group_max = (float*)((uint8_t*)workspace + y.groups);
+  p.out_scores = out_scores;
+  p.out_parents = out_parents;
+  p.out_tokens = out_tokens;
+  p.err = device_error_word();
+  p.stride_b = strides[0];
+  p.stride_w = strides[1];
+  p.B = (int32_t)batch;
+  p.W = (int32_t)beams;
+  p.V = (int32_t)vocab;
+  p.k = (int32_t)k;
+  p.tasks = (int32_t)y.tasks;
+  p.end = (int32_t)end;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == WNW_F32)
+    launch_beam<float>(p, st);
+  else if (dtype == WNW_F16)
+    launch_beam<f16_t>(p, st);
+  else
+    launch_beam<bf16_t>(p, st);
+  WNW_CHECK_HIP(hipGetLastError(), "beam selection launch");
+  return WNW_OK;
+}

@@ -107,13 +107,10 @@ def _workspace(dev: torch.device, n_seg: int, need: int, given: PagedWorkspace |
     return call_workspace(idx, _lib.raw_stream(dev), n_seg, need)
 
 
-def _cache(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seg_len: Tensor, k_scale: Tensor | None,
-           v_scale: Tensor | None, *others: Tensor | None) -> _lib.PagedCache:
-    """The checked cache as the library takes it; ``others``: tensors of the call that share its device."""
-    tensors = [t for t in (k_pages, v_pages, page_table, seg_len, k_scale, v_scale, *others) if t is not None]
+def _refuse_watched(tensors: list[Tensor]) -> None:
+    """Refuses tensors on the host or on several devices, and calls that autograd or a trace would have to follow."""
     _lib.require_gpu(*tensors)
-    dev = k_pages.device
-    if any(t.device != dev for t in tensors):
+    if any(t.device != tensors[0].device for t in tensors):
         raise _lib.WnwError("all tensors of a call must be on one device")
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise _lib.WnwError("the paged cache's operators have no gradient: call them under torch.no_grad()")
@@ -123,6 +120,13 @@ def _cache(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seg_len: Tensor
     if torch._C._get_tracing_state() is not None \
             or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
         raise _lib.WnwError("the paged cache's operators cannot be traced: a trace would hold outputs that nothing writes")
+
+
+def _cache(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seg_len: Tensor, k_scale: Tensor | None,
+           v_scale: Tensor | None, *others: Tensor | None) -> _lib.PagedCache:
+    """The checked cache as the library takes it; ``others``: tensors of the call that share its device."""
+    tensors = [t for t in (k_pages, v_pages, page_table, seg_len, k_scale, v_scale, *others) if t is not None]
+    _refuse_watched(tensors)
     if k_pages.dim() != 3 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype \
             or k_pages.dtype not in _PAGE_DTYPES:
         raise _lib.WnwError(f"k_pages / v_pages must be equal [P, R, D] of bf16, f16 or e4m3: {tuple(k_pages.shape)} "
