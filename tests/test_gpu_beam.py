@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from tests.test_gpu_paged import _clean
+from tests.test_gpu_paged_edges import _General
 from wnw_amd import _lib
 from wnw_amd.kv.beam import beam_select
 
@@ -229,3 +230,14 @@ def test_refusals(gpu):
             beam_select(c["x"], c["s"], c["k"], done=c["done"], end=c["end"])
     assert beam_select(x[:0], s[:0], 3)[0].shape == (0, 3)
     _clean()
+
+
+def test_both_ways_into_a_call(gpu, monkeypatch):
+    """The native way of the plain calls and the general way give the same bits."""
+    x, s = _logits(gpu, 3, 4, 5001, FP, 11, 3)
+    done = torch.rand(3, 4, device=gpu) < 0.3
+    native = [beam_select(x, s), beam_select(x, s, 9, done=done, end=7), beam_select(x.float(), s, 1)]
+    monkeypatch.setattr(_lib, "_callpath", _General())
+    general = [beam_select(x, s), beam_select(x, s, 9, done=done, end=7), beam_select(x.float(), s, 1)]
+    _clean()
+    assert all(torch.equal(a, b) for n, g in zip(native, general) for a, b in zip(n, g))

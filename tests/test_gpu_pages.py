@@ -3,9 +3,11 @@ import random
 
 import pytest
 import torch
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from tests import pages_ref
 from tests.test_gpu_paged import _clean
+from tests.test_gpu_paged_edges import _General
 from wnw_amd import _lib
 from wnw_amd.kv.pages import paged_compact, paged_copy, paged_fork, paged_reserve
 
@@ -272,4 +274,44 @@ def test_refusals(gpu):
         c.update(bad)
         with pytest.raises(E):
             paged_copy(c["k"], c["v"], c["c"], k_scale=c["s"])
+    _clean()
+
+
+def test_both_ways_into_a_call(gpu, monkeypatch):
+    """The native way of the plain calls and the general way give the same results."""
+    rng = random.Random(3)
+    B, H, R, M, P = 4, 2, 32, 11, 300
+    table, lens, refs = _state(rng, B, H, R, M, P)
+    lens = [min(n, M * R - 40) for n in lens]
+    k = torch.randn(P, R, 64, device=gpu).to(torch.bfloat16)
+    results = []
+    for general in (False, True):
+        if general:
+            monkeypatch.setattr(_lib, "_callpath", _General())
+        t, n, r = _t(table, gpu), _t(lens, gpu), _t(refs, gpu)
+        kk, vv = k.clone(), -k
+        forked = paged_fork(t, n, r, _t([1, 1, 0, -1, 3], gpu), R, kv_heads=H)
+        paged_copy(kk, vv, forked[3])
+        room = torch.full((B * H, M + 5), 9, dtype=torch.int32, device=gpu)[:, :M], torch.empty_like(r)
+        got = [*forked, kk, vv, *paged_reserve(t, n, r, R), *paged_reserve(t, n, r, R, cu_tokens=_t([0, 5, 40, 40, 41], gpu), out=room),
+               *paged_reserve(t, n, r, R, tokens=0, window=n + 3, sinks=4), *paged_compact(t, r, R), *paged_compact(t, r, R, out=(t, r))]
+        torch.cuda.synchronize()
+        results.append((_lib.device_error(), [x.clone() for x in got]))
+    assert results[0][0] == results[1][0] == 0
+    assert all(torch.equal(a, b) for a, b in zip(results[0][1], results[1][1]))
+    want = pages_ref.fork(table, lens, refs, [1, 1, 0, -1, 3], R, H, M)
+    assert results[0][1][0].tolist() == want[0]
+
+
+def test_watched_calls_are_refused(gpu):
+    """Pages that require a gradient, and traces."""
+    k = torch.zeros(4, 16, 64, device=gpu, dtype=torch.bfloat16, requires_grad=True)
+    copies = _t([[0, 1, 2]], gpu)
+    with pytest.raises(_lib.WnwError, match="gradient"):
+        paged_copy(k, k.detach().clone(), copies)
+    with torch.no_grad():
+        paged_copy(k, k.detach().clone(), copies)
+    table, refs = _t([[0]], gpu), _t([1], gpu)
+    with pytest.raises(_lib.WnwError, match="trace"):
+        make_fx(lambda r: paged_compact(table, r, 16)[0])(refs)
     _clean()

@@ -6,8 +6,7 @@
 // (w, v).  Within a beam totals go with the logits, so a beam need not be sorted.
 //
 // Two launches.  The first reads the logits once: a wave takes 2,048 of a row and
-// leaves their maximum, sum exp(x - max) and the maximum of each group of 256
-// bytes.  In the second, a workgroup a sample puts the sums together, finds the
+// leaves their maximum, sum exp(x - max) and the maximum of each group of 128.  In the second, a workgroup a sample puts the sums together, finds the
 // k best groups by their maxima (the k best elements lie in those: each other
 // group is behind k maxima), reads these alone again, and ranks what is not
 // below the k-th group's maximum.
@@ -28,7 +27,7 @@ struct BeamParams {
   const uint8_t* done;  // [B, W] or null
   double* part_sum;     // [rows, tasks]
   float* part_max;      // [rows, tasks]
-  float* group_max;     // [rows, tasks, groups of a task]
+  float* group_max;     // [rows, tasks, kBeamGroups]
   float* out_scores;    // [B, k]
   int32_t* out_parents;
   int64_t* out_tokens;
@@ -37,12 +36,16 @@ struct BeamParams {
   int32_t B, W, V, k, tasks, end;
 };
 
+static constexpr int kBeamGroup = 128;                     // logits of a group
+static constexpr int kBeamGroups = kBeamTask / kBeamGroup;  // of a task
+static constexpr int kBeamWaves = kBeamThreads / 64;
+static constexpr int kBeamHeld = 8;  // chunks of 64 groups whose maxima a wave of the pick holds
+
 template <typename T>
 struct BeamGeom {
-  static constexpr int kVec = 16 / Elem<T>::kBytes;  // elements of a load
-  static constexpr int kGroup = 16 * kVec;           // of a group: 16 lanes' loads
-  static constexpr int kLoads = kBeamTask / (64 * kVec);
-  static constexpr int kGroups = kBeamTask / kGroup;  // of a task
+  static constexpr int kVec = 16 / Elem<T>::kBytes;        // elements of a load
+  static constexpr int kLoads = kBeamTask / (64 * kVec);   // of a lane in a task
+  static constexpr int kEach = kBeamGroup / 16;            // elements of a thread of the 16 that read a group again
 };
 
 // Elements e .. e + kVec - 1 of a row of V, those past its end -inf.  Rows may
@@ -104,6 +107,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void beam_rows_kernel(BeamParams p) {
   using Ge = BeamGeom<T>;
   constexpr int N = Ge::kVec, U = Ge::kLoads;
+  static_assert(U <= 16, "a lane of 16 for each load's maximum");
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t at = (int64_t)blockIdx.x * 4 + w;  // the task
   if (at >= (int64_t)p.B * p.W * p.tasks) return;
@@ -141,10 +145,17 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(BeamParams p) {
     p.part_max[at] = m;
     p.part_sum[at] = sum;
   }
+  // a group is a row of 16 lanes' load, or two rows' with 4 elements a load
+  if constexpr (N == 4) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) most[u] = max_x16(most[u]);
+  }
+  constexpr int R = N == 8 ? 4 : 2;  // groups of a load
   float mine = most[0];
 #pragma unroll
   for (int u = 1; u < U; ++u) mine = (lane & 15) == u ? most[u] : mine;
-  if ((lane & 15) < U) p.group_max[at * Ge::kGroups + (lane & 15) * 4 + (lane >> 4)] = mine;
+  if ((lane & 15) < U && (N == 8 || !(lane & 16)))
+    p.group_max[at * kBeamGroups + (lane & 15) * R + (lane >> (N == 8 ? 4 : 5))] = mine;
 }
 
 // A candidate's place in the order: its total as an ordered integer, and (w, v).
@@ -179,7 +190,8 @@ struct BeamShared {
   int state[kBeamMax];  // 1: continues, 2: finished, 0: neither
   BeamKey list[kBeamList];
   BeamKey best[kBeamMax];
-  BeamKey wave[kBeamThreads / 64];
+  BeamKey wave[kBeamWaves];
+  uint32_t high[64];
   int count, found;
 };
 
@@ -194,7 +206,7 @@ __device__ __forceinline__ void beam_rounds(BeamShared& sh, int k, F next) {
     if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = mine;
     __syncthreads();
     BeamKey x = sh.wave[0];
-    for (int i = 1; i < kBeamThreads / 64; ++i) x = ahead_of(x, sh.wave[i]);
+    for (int i = 1; i < kBeamWaves; ++i) x = ahead_of(x, sh.wave[i]);
     if (x.id == kBeamNone.id) break;
     if (threadIdx.x == 0) sh.best[r] = x;
     last = x;
@@ -203,42 +215,76 @@ __device__ __forceinline__ void beam_rounds(BeamShared& sh, int k, F next) {
   if (threadIdx.x == 0) sh.found = r;
   __syncthreads();
 }
-// The k first of the list's n, by their ranks.
+template <int kCtrl>
+__device__ __forceinline__ int dpp_add(int x) {
+  return x + __builtin_amdgcn_mov_dpp(x, kCtrl, 0xf, 0xf, false);
+}
+// The k first of the list's n, by their ranks: 16 threads count those ahead of one.
 __device__ __forceinline__ void beam_ranks(BeamShared& sh, int k, int n) {
-  for (int i = threadIdx.x; i < n; i += kBeamThreads) {
-    const BeamKey x = sh.list[i];
+  for (int base = 0; base < n; base += kBeamThreads / 16) {
+    const int i = base + (int)(threadIdx.x >> 4);
+    const BeamKey x = sh.list[min(i, n - 1)];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += ahead(sh.list[j], x);
-    if (rank < k) sh.best[rank] = x;
+    for (int j = threadIdx.x & 15; j < n; j += 16) rank += ahead(sh.list[j], x);
+    rank = dpp_add<0xB1>(rank);
+    rank = dpp_add<0x4E>(rank);
+    rank = dpp_add<0x141>(rank);
+    rank = dpp_add<0x140>(rank);
+    if (i < n && rank < k && (threadIdx.x & 15) == 0) sh.best[rank] = x;
   }
   if (threadIdx.x == 0) sh.found = min(n, k);
   __syncthreads();
 }
 
+// A group of a sample: its beam, and its place among the beam's.
+struct BeamPlace {
+  int w, group;
+};
+
 template <typename T>
 __global__ __launch_bounds__(kBeamThreads) void beam_pick_kernel(BeamParams p) {
   using Ge = BeamGeom<T>;
-  constexpr int N = Ge::kVec;
+  constexpr int N = Ge::kVec, E = Ge::kEach;
   __shared__ BeamShared sh;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int W = p.W, k = p.k, groups = p.tasks * Ge::kGroups;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int W = p.W, k = p.k, groups = p.tasks * kBeamGroups, chunks = (groups + 63) / 64, n = W * chunks;
+  // Chunk c of the sample's: 64 groups of beam c / chunks.  A wave takes every 16th, and
+  // has the first of them on their way before anything else.
+  auto place_of = [&](int c) {
+    const int w = c / chunks;
+    return BeamPlace{w, (c - w * chunks) * 64 + lane};
+  };
+  auto max_of = [&](const BeamPlace& x) {
+    return x.group < groups ? p.group_max[((int64_t)b * W + x.w) * groups + x.group] : -INFINITY;
+  };
+  float held[kBeamHeld];
+#pragma unroll
+  for (int i = 0; i < kBeamHeld; ++i) {
+    const int c = wave + i * kBeamWaves;
+    held[i] = c < n ? max_of(place_of(c)) : -INFINITY;
+  }
   // the rows' sums
-  for (int w = wave; w < W; w += kBeamThreads / 64) {
+  for (int w = wave; w < W; w += kBeamWaves) {
     const int row = b * W + w;
+    const float* pm = p.part_max + (int64_t)row * p.tasks;
+    const double* ps = p.part_sum + (int64_t)row * p.tasks;
+    const bool in = lane < p.tasks;
+    float m = in ? pm[lane] : kBeamLowest;
+    double s = in ? ps[lane] : 0.0;
     const float score = p.scores[row];
     int state = p.done && p.done[row] ? 2 : 1;
-    double lse = 0.0;
     bool bad = !(score < INFINITY);
+    double lse = 0.0;
     if (state == 1) {
-      const float* pm = p.part_max + (int64_t)row * p.tasks;
-      const double* ps = p.part_sum + (int64_t)row * p.tasks;
-      float m = kBeamLowest;
-      for (int i = lane; i < p.tasks; i += 64) m = fmaxf(m, pm[i]);
-      m = wave_max(m);
-      double s = 0.0;
-      for (int i = lane; i < p.tasks; i += 64) s += ps[i] * exp((double)pm[i] - (double)m);
-      s = wave_sum64(s);
-      lse = (double)m + log(s);
+      for (int i = lane + 64; i < p.tasks; i += 64) {  // (a vocabulary past 131,072)
+        const float y = pm[i], now = fmaxf(m, y);
+        s = s * (double)__builtin_amdgcn_exp2f((m - now) * kBeamLog2e) +
+            ps[i] * (double)__builtin_amdgcn_exp2f((y - now) * kBeamLog2e);
+        m = now;
+      }
+      const float most = wave_max(m);
+      s = wave_sum64(s * (double)__builtin_amdgcn_exp2f((m - most) * kBeamLog2e));
+      lse = (double)most + log(s);
       bad |= !(s < (double)INFINITY);
       if (s == 0.0) state = 0;
     }
@@ -253,99 +299,118 @@ __global__ __launch_bounds__(kBeamThreads) void beam_pick_kernel(BeamParams p) {
   if (tid == 0) sh.count = 0;
   __syncthreads();
   auto total_of = [&](int w, float x) { return (double)sh.score[w] + ((double)x - sh.lse[w]); };
-
-  // the k best groups
-  const int n = W * groups;
-  auto group_key = [&](int g) {
-    const int w = g / groups;
-    if (sh.state[w] != 1) return kBeamNone;
-    const float x = p.group_max[(int64_t)b * n + g];
-    return x == -INFINITY ? kBeamNone : BeamKey{ordered(total_of(w, x)), (uint32_t)g};
+  auto key_of = [&](const BeamPlace& at, float x) {
+    return sh.state[at.w] == 1 && x > -INFINITY
+               ? BeamKey{ordered(total_of(at.w, x)), (uint32_t)(at.w * groups + at.group)}
+               : kBeamNone;
   };
+
+  // The k best groups.  First what they are not behind: the k-th largest of 16 waves'
+  // maxima, or of 64 rows' of 16 lanes, by the totals' upper words, of which 20 bits are enough.
+  BeamKey keys[kBeamHeld];
+  uint32_t high = 0;
+#pragma unroll
+  for (int i = 0; i < kBeamHeld; ++i) {
+    const int c = wave + i * kBeamWaves;
+    keys[i] = kBeamNone;
+    if (c < n) keys[i] = key_of(place_of(c), held[i]);
+    high = max(high, (uint32_t)(keys[i].total >> 32));
+  }
+  for (int c = wave + kBeamHeld * kBeamWaves; c < n; c += kBeamWaves) {
+    const BeamPlace at = place_of(c);
+    high = max(high, (uint32_t)(key_of(at, max_of(at)).total >> 32));
+  }
+  high = max(high, (uint32_t)__builtin_amdgcn_mov_dpp((int)high, 0xB1, 0xf, 0xf, false));
+  high = max(high, (uint32_t)__builtin_amdgcn_mov_dpp((int)high, 0x4E, 0xf, 0xf, false));
+  high = max(high, (uint32_t)__builtin_amdgcn_mov_dpp((int)high, 0x141, 0xf, 0xf, false));
+  high = max(high, (uint32_t)__builtin_amdgcn_mov_dpp((int)high, 0x140, 0xf, 0xf, false));
+  if ((lane & 15) == 0) sh.high[tid >> 4] = high;
+  __syncthreads();
+  uint32_t least = 0;
   {
-    BeamKey mine = kBeamNone;
-    for (int g = tid; g < n; g += kBeamThreads) mine = ahead_of(group_key(g), mine);
-    // rows of 16 lanes: k of their 64 maxima are no further back than the k-th of them
-    BeamKey x = mine;
-#pragma unroll
-    for (int o = 8; o >= 1; o >>= 1) {
-      const BeamKey y = {(uint64_t)__shfl_xor((unsigned long long)x.total, o), (uint32_t)__shfl_xor((int)x.id, o)};
-      x = ahead_of(x, y);
+    uint32_t y = sh.high[lane];
+    if (k <= kBeamWaves) {  // one a wave: the other rows' lanes count nothing
+      y = max(y, (uint32_t)__builtin_amdgcn_mov_dpp((int)y, 0xB1, 0xf, 0xf, false));
+      y = max(y, (uint32_t)__builtin_amdgcn_mov_dpp((int)y, 0x4E, 0xf, 0xf, false));
+      if (lane & 3) y = 0;
     }
-    if ((lane & 15) == 0) sh.best[tid >> 4] = x;
-    __syncthreads();
-    const BeamKey y = sh.best[lane];
-    int rank = 0;
-    for (int j = 0; j < 64; ++j) rank += ahead(sh.best[j], y) || (j < lane && sh.best[j].id == y.id && sh.best[j].total == y.total);
-    const int at = __builtin_ctzll(__ballot(rank == k - 1));
-    const BeamKey least = sh.best[at];
-    __syncthreads();
-    for (int g = tid; g < n; g += kBeamThreads) {
-      const BeamKey key = group_key(g);
-      if (key.id != kBeamNone.id && !ahead(least, key)) {
-        const int slot = atomicAdd(&sh.count, 1);
-        if (slot < kBeamList) sh.list[slot] = key;
-      }
-    }
-    __syncthreads();
-    const int c = sh.count;
-    if (c <= kBeamList)
-      beam_ranks(sh, k, c);
-    else
-      beam_rounds(sh, k, [&](const BeamKey& last) {
-        BeamKey first = kBeamNone;
-        for (int g = tid; g < n; g += kBeamThreads) {
-          const BeamKey key = group_key(g);
-          if (ahead(last, key)) first = ahead_of(key, first);
-        }
-        return first;
-      });
-  }
-  // their elements, and the finished beams
-  const int found = sh.found;
-  const uint64_t floor_total = found == k ? sh.best[k - 1].total : 0;
-  const int mine = tid >> 4;  // the thread's group, 16 threads each
-  BeamKey keys[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) keys[i] = kBeamNone;
-  if (mine < found) {
-    const int g = (int)sh.best[mine].id, w = g / groups, e = (g - w * groups) * Ge::kGroup + (tid & 15) * N;
-    const T* row = (const T*)p.logits + (int64_t)b * p.stride_b + (int64_t)w * p.stride_w;
-    u32x4 raw;
-    int from;
-    float x[N];
-    beam_load<T>(row, e, p.V, &raw, &from);
-    beam_values<T>(raw, e, from, p.V, x);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const uint64_t t = ordered(total_of(w, x[i]));
-      if (x[i] > -INFINITY && t >= floor_total) keys[i] = BeamKey{t, (uint32_t)w * (uint32_t)p.V + (uint32_t)(from + i)};
+    for (int bit = 31; bit >= 12; --bit) {
+      const uint32_t up = least | 1u << bit;
+      if (__popcll(__ballot(y >= up)) >= k) least = up;
     }
   }
-  BeamKey lone = kBeamNone;
-  if (tid < W && sh.state[tid] == 2)
-    lone = BeamKey{ordered((double)sh.score[tid]), (uint32_t)tid * (uint32_t)p.V + (uint32_t)p.end};
-  __syncthreads();
-  if (tid == 0) sh.count = 0;
-  __syncthreads();
   auto put = [&](const BeamKey& x) {
-    if (x.id == kBeamNone.id) return;
     const int slot = atomicAdd(&sh.count, 1);
     if (slot < kBeamList) sh.list[slot] = x;
   };
+  auto offer = [&](const BeamKey& x) {
+    if (x.id != kBeamNone.id && (uint32_t)(x.total >> 32) >= least) put(x);
+  };
 #pragma unroll
-  for (int i = 0; i < N; ++i) put(keys[i]);
-  put(lone);
+  for (int i = 0; i < kBeamHeld; ++i) offer(keys[i]);
+  for (int c = wave + kBeamHeld * kBeamWaves; c < n; c += kBeamWaves) {
+    const BeamPlace at = place_of(c);
+    offer(key_of(at, max_of(at)));
+  }
   __syncthreads();
-  const int c = sh.count;
-  if (c <= kBeamList)
-    beam_ranks(sh, k, c);
+  const int near = sh.count;
+  if (near <= kBeamList)
+    beam_ranks(sh, k, near);
+  else
+    beam_rounds(sh, k, [&](const BeamKey& last) {
+      BeamKey first = kBeamNone;
+      for (int c = wave; c < n; c += kBeamWaves) {
+        const BeamPlace at = place_of(c);
+        const BeamKey key = key_of(at, max_of(at));
+        if (ahead(last, key)) first = ahead_of(key, first);
+      }
+      return first;
+    });
+
+  // their elements, 16 threads a group, and the finished beams
+  const int found = sh.found, mine = tid >> 4;
+  const uint64_t floor_total = found == k ? sh.best[k - 1].total : 0;
+  if (tid == 0) sh.count = 0;  // (behind the barrier that ended the ranks)
+  BeamKey each[E], lone = kBeamNone;
+#pragma unroll
+  for (int i = 0; i < E; ++i) each[i] = kBeamNone;
+  if (mine < found) {
+    const int g = (int)sh.best[mine].id, w = g / groups, e = (g - w * groups) * kBeamGroup + (tid & 15) * N;
+    const T* row = (const T*)p.logits + (int64_t)b * p.stride_b + (int64_t)w * p.stride_w;
+    u32x4 raw[E / N];
+    int from[E / N];
+    float x[E];
+#pragma unroll
+    for (int u = 0; u < E / N; ++u) beam_load<T>(row, e + 16 * N * u, p.V, &raw[u], &from[u]);
+#pragma unroll
+    for (int u = 0; u < E / N; ++u) {
+      beam_values<T>(raw[u], e + 16 * N * u, from[u], p.V, x + N * u);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint64_t t = ordered(total_of(w, x[N * u + i]));
+        if (x[N * u + i] > -INFINITY && t >= floor_total)
+          each[N * u + i] = BeamKey{t, (uint32_t)w * (uint32_t)p.V + (uint32_t)(from[u] + i)};
+      }
+    }
+  }
+  if (tid < W && sh.state[tid] == 2)
+    lone = BeamKey{ordered((double)sh.score[tid]), (uint32_t)tid * (uint32_t)p.V + (uint32_t)p.end};
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    if (each[i].id != kBeamNone.id) put(each[i]);
+  if (lone.id != kBeamNone.id && lone.total >= floor_total) put(lone);
+  __syncthreads();
+  const int last_few = sh.count;
+  if (last_few <= kBeamList)
+    beam_ranks(sh, k, last_few);
   else
     beam_rounds(sh, k, [&](const BeamKey& last) {
       BeamKey first = ahead(last, lone) ? lone : kBeamNone;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (ahead(last, keys[i])) first = ahead_of(keys[i], first);
+      for (int i = 0; i < E; ++i)
+        if (ahead(last, each[i])) first = ahead_of(each[i], first);
       return first;
     });
   if (tid < k) {
@@ -362,13 +427,12 @@ __global__ __launch_bounds__(kBeamThreads) void beam_pick_kernel(BeamParams p) {
 struct BeamLayout {
   int64_t tasks, max, groups, total;  // bytes, the sums first
 };
-static BeamLayout beam_layout(int64_t rows, int64_t vocab, int dtype) {
+static BeamLayout beam_layout(int64_t rows, int64_t vocab) {
   BeamLayout y;
   y.tasks = (vocab + kBeamTask - 1) / kBeamTask;
-  const int64_t per = dtype == WNW_F32 ? BeamGeom<float>::kGroups : BeamGeom<bf16_t>::kGroups;
   y.max = (rows * y.tasks * 8 + 255) / 256 * 256;
   y.groups = y.max + (rows * y.tasks * 4 + 255) / 256 * 256;
-  y.total = y.groups + rows * y.tasks * per * 4;
+  y.total = y.groups + rows * y.tasks * kBeamGroups * 4;
   return y;
 }
 static bool beam_sizes(int64_t batch, int64_t beams, int64_t vocab, int dtype) {
@@ -388,7 +452,7 @@ static void launch_beam(const BeamParams& p, hipStream_t st) {
 using namespace wnw;
 
 extern "C" int64_t wnw_beam_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int dtype) {
-  return beam_sizes(batch, beams, vocab, dtype) ? beam_layout(batch * beams, vocab, dtype).total : -1;
+  return beam_sizes(batch, beams, vocab, dtype) ? beam_layout(batch * beams, vocab).total : -1;
 }
 
 extern "C" int wnw_beam_select(const void* logits, const int64_t* strides, int64_t batch, int64_t beams, int64_t vocab,
@@ -404,7 +468,7 @@ extern "C" int wnw_beam_select(const void* logits, const int64_t* strides, int64
   const int64_t elem = elem_bytes(dtype);
   WNW_CHECK_ARG(strides[0] >= 0 && strides[1] >= 0 && strides[0] < (1ll << 40) && strides[1] < (1ll << 40), "bad strides");
   WNW_CHECK_ARG((uintptr_t)logits % elem == 0, "the logits are not aligned to their type");
-  const BeamLayout y = beam_layout(batch * beams, vocab, dtype);
+  const BeamLayout y = beam_layout(batch * beams, vocab);
   WNW_CHECK_ARG((batch * beams * y.tasks + 3) / 4 < (1ll << 24), "too many logits for one call");
   WNW_CHECK_ARG(workspace && workspace_bytes >= y.total, "workspace too small: %lld bytes, %lld needed",
                 (long long)workspace_bytes, (long long)y.total);

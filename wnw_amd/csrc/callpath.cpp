@@ -500,6 +500,241 @@ PyObject* paged_append_impl(PyObject* const* a) {
   return first.o && second.o ? PyTuple_Pack(2, first.o, second.o) : nullptr;
 }
 
+// The current stream and device of a call on t's device; false: leave it to the general path, or (stream) an exception.
+struct Call {
+  const c10::DeviceGuard guard;
+  PyObject* so = nullptr;
+  void* stream = nullptr;
+  bool ok = false, has_stream = false;
+  explicit Call(const at::Tensor& t) : guard(t.device()) {
+    ok = ready(t.device().index());
+    if (ok) has_stream = stream_of(t.device().index(), &so, &stream);
+  }
+  ~Call() { Py_XDECREF(so); }
+};
+at::Tensor like(const at::Tensor& t, at::IntArrayRef shape, at::ScalarType type) {
+  return at::empty(shape, t.options().dtype(type).requires_grad(false));
+}
+
+// A pool's table and counts, and (len) its segments' lengths
+struct Pool {
+  const at::Tensor *table, *refs, *len = nullptr;
+  int64_t N, M, P, stride;
+};
+bool pool_of(PyObject* table, PyObject* refs, PyObject* len, Pool* p) {
+  p->table = plain(table);
+  p->refs = plain(refs);
+  if (watched() || !p->table || !usable(p->refs, *p->table) || p->table->dim() != 2 || p->table->scalar_type() != at::kInt ||
+      p->refs->scalar_type() != at::kInt || p->refs->dim() != 1 || !p->refs->is_contiguous())
+    return false;
+  p->N = p->table->size(0);
+  p->M = p->table->size(1);
+  p->P = p->refs->size(0);
+  if (p->N < 1 || p->M < 1 || p->P < 1 || p->table->stride(1) != 1) return false;
+  p->stride = p->N > 1 ? p->table->stride(0) : p->M;
+  if (!len) return true;
+  p->len = vec(len, at::kInt, p->N);
+  return usable(p->len, *p->table) && p->len->dim() == 1;
+}
+// Where a pool's new state goes: the two tensors given, or new ones
+bool pool_out(PyObject* out, const Pool& p, at::Tensor* table, at::Tensor* refs) {
+  if (out == Py_None) {
+    *table = like(*p.table, {p.N, p.M}, at::kInt);
+    *refs = like(*p.table, {p.P}, at::kInt);
+    return true;
+  }
+  if (!PyTuple_CheckExact(out) || PyTuple_GET_SIZE(out) != 2) return false;
+  Pool o;
+  if (!pool_of(PyTuple_GET_ITEM(out, 0), PyTuple_GET_ITEM(out, 1), nullptr, &o) || o.table->device() != p.table->device() ||
+      o.N != p.N || o.M != p.M || o.P != p.P || o.stride < o.M)
+    return false;
+  *table = *o.table;
+  *refs = *o.refs;
+  return true;
+}
+PyObject* wrapped(PyObject* given, at::Tensor&& t) { return given ? Py_NewRef(given) : THPVariable_Wrap(std::move(t)); }
+
+// (page_table, seg_len, page_refs, parents, page_rows, kv_heads)
+PyObject* paged_fork_impl(PyObject* const* a) {
+  Pool p;
+  int64_t rows, heads;
+  const at::Tensor* parents = plain(a[3]);
+  if (!pool_of(a[0], a[2], a[1], &p) || !usable(parents, *p.table) || parents->scalar_type() != at::kInt || parents->dim() != 1 ||
+      !parents->is_contiguous() || !whole(a[4], &rows) || !whole(a[5], &heads) || heads < 1 || p.N % heads != 0 ||
+      parents->size(0) < 1)
+    Py_RETURN_NONE;
+  const int64_t n_new = parents->size(0), S = n_new * heads;
+  const int64_t need = wnw_pages_workspace_bytes(std::max(p.N, S), p.N / heads, p.P);
+  if (need < 0) Py_RETURN_NONE;
+  Call call(*p.table);
+  if (!call.ok) Py_RETURN_NONE;
+  if (!call.has_stream) return nullptr;
+  at::Tensor table = like(*p.table, {S, p.M}, at::kInt), len = like(*p.table, {S}, at::kInt), refs = like(*p.table, {p.P}, at::kInt);
+  at::Tensor copies = like(*p.table, {S, 3}, at::kInt), ws = like(*p.table, {need}, at::kByte);
+  const int32_t *t = p.table->const_data_ptr<int32_t>(), *l = p.len->const_data_ptr<int32_t>(), *r = p.refs->const_data_ptr<int32_t>();
+  const int32_t* pa = parents->const_data_ptr<int32_t>();
+  int32_t *nt = table.data_ptr<int32_t>(), *nl = len.data_ptr<int32_t>(), *nr = refs.data_ptr<int32_t>(), *cp = copies.data_ptr<int32_t>();
+  void* w = ws.data_ptr();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = wnw_paged_fork(t, p.stride, l, r, pa, p.N / heads, n_new, heads, p.M, p.P, rows, nt, p.M, nl, nr, cp, w, need, call.stream);
+  Py_END_ALLOW_THREADS
+  if (rc != WNW_OK) return failed(rc, "paged_fork");
+  Ref o0(THPVariable_Wrap(std::move(table))), o1(THPVariable_Wrap(std::move(len))), o2(THPVariable_Wrap(std::move(refs))),
+      o3(THPVariable_Wrap(std::move(copies)));
+  return o0.o && o1.o && o2.o && o3.o ? PyTuple_Pack(4, o0.o, o1.o, o2.o, o3.o) : nullptr;
+}
+
+// (page_table, seg_len, page_refs, page_rows, tokens, cu_tokens, window, sinks, out)
+PyObject* paged_reserve_impl(PyObject* const* a) {
+  Pool p;
+  int64_t rows, tokens;
+  if (!pool_of(a[0], a[2], a[1], &p) || !whole(a[3], &rows) || !whole(a[4], &tokens) || tokens < 0) Py_RETURN_NONE;
+  const int32_t* cu = nullptr;
+  int64_t samples = p.N;
+  if (a[5] != Py_None) {
+    const at::Tensor* t = plain(a[5]);
+    if (!usable(t, *p.table) || t->scalar_type() != at::kInt || t->dim() != 1 || t->size(0) < 2 || !t->is_contiguous()) Py_RETURN_NONE;
+    samples = t->size(0) - 1;
+    if (p.N % samples != 0) Py_RETURN_NONE;
+    cu = t->const_data_ptr<int32_t>();
+  }
+  View y;
+  y.window_all = -1;
+  if (a[6] == Py_None ? a[7] != Py_None : !view_of(a[6], a[7], *p.table, p.N, &y)) Py_RETURN_NONE;
+  const int64_t need = wnw_pages_workspace_bytes(p.N, samples, p.P);
+  if (need < 0) Py_RETURN_NONE;
+  Call call(*p.table);
+  if (!call.ok) Py_RETURN_NONE;
+  if (!call.has_stream) return nullptr;
+  at::Tensor table, refs;
+  if (!pool_out(a[8], p, &table, &refs)) Py_RETURN_NONE;
+  at::Tensor ws = like(*p.table, {need}, at::kByte);
+  const int32_t *t = p.table->const_data_ptr<int32_t>(), *l = p.len->const_data_ptr<int32_t>(), *r = p.refs->const_data_ptr<int32_t>();
+  int32_t *nt = table.data_ptr<int32_t>(), *nr = refs.data_ptr<int32_t>();
+  const int64_t ns = p.N > 1 ? table.stride(0) : p.M;
+  void* w = ws.data_ptr();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = wnw_paged_reserve(t, p.stride, l, r, p.N, samples, p.M, p.P, rows, cu, tokens, y.window, y.window_all, y.sinks, y.sinks_all, nt,
+                         ns, nr, w, need, call.stream);
+  Py_END_ALLOW_THREADS
+  if (rc != WNW_OK) return failed(rc, "paged_reserve");
+  const bool given = a[8] != Py_None;
+  Ref o0(wrapped(given ? PyTuple_GET_ITEM(a[8], 0) : nullptr, std::move(table))),
+      o1(wrapped(given ? PyTuple_GET_ITEM(a[8], 1) : nullptr, std::move(refs)));
+  return o0.o && o1.o ? PyTuple_Pack(2, o0.o, o1.o) : nullptr;
+}
+
+// (page_table, page_refs, page_rows, out)
+PyObject* paged_compact_impl(PyObject* const* a) {
+  Pool p;
+  int64_t rows;
+  if (!pool_of(a[0], a[1], nullptr, &p) || !whole(a[2], &rows)) Py_RETURN_NONE;
+  const int64_t need = wnw_pages_workspace_bytes(p.N, 0, p.P);
+  if (need < 0) Py_RETURN_NONE;
+  Call call(*p.table);
+  if (!call.ok) Py_RETURN_NONE;
+  if (!call.has_stream) return nullptr;
+  at::Tensor table, refs;
+  if (!pool_out(a[3], p, &table, &refs)) Py_RETURN_NONE;
+  at::Tensor moves = like(*p.table, {p.P / 2, 3}, at::kInt), used = like(*p.table, {1}, at::kInt), ws = like(*p.table, {need}, at::kByte);
+  const int32_t *t = p.table->const_data_ptr<int32_t>(), *r = p.refs->const_data_ptr<int32_t>();
+  int32_t *nt = table.data_ptr<int32_t>(), *nr = refs.data_ptr<int32_t>(), *mv = moves.data_ptr<int32_t>(), *us = used.data_ptr<int32_t>();
+  const int64_t ns = p.N > 1 ? table.stride(0) : p.M;
+  void* w = ws.data_ptr();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = wnw_paged_compact(t, p.stride, r, p.N, p.M, p.P, rows, nt, ns, nr, mv, us, w, need, call.stream);
+  Py_END_ALLOW_THREADS
+  if (rc != WNW_OK) return failed(rc, "paged_compact");
+  const bool given = a[3] != Py_None;
+  Ref o0(wrapped(given ? PyTuple_GET_ITEM(a[3], 0) : nullptr, std::move(table))),
+      o1(wrapped(given ? PyTuple_GET_ITEM(a[3], 1) : nullptr, std::move(refs))), o2(THPVariable_Wrap(std::move(moves))),
+      o3(THPVariable_Wrap(std::move(used)));
+  return o0.o && o1.o && o2.o && o3.o ? PyTuple_Pack(4, o0.o, o1.o, o2.o, o3.o) : nullptr;
+}
+
+// (k_pages, v_pages, copies, k_scale, v_scale)
+PyObject* paged_copy_impl(PyObject* const* a) {
+  const at::Tensor *k = plain(a[0]), *v = plain(a[1]), *copies = plain(a[2]);
+  if (watched() || !k || needs_grad(k) || !usable(v, *k) || !usable(copies, *k) || k->dim() != 3 || k->sizes() != v->sizes() ||
+      k->scalar_type() != v->scalar_type())
+    Py_RETURN_NONE;
+  const at::ScalarType dt = k->scalar_type();
+  const bool q8 = dt == at::kFloat8_e4m3fn;
+  const int64_t P = k->size(0), R = k->size(1), D = k->size(2);
+  if ((!q8 && !half_type(*k)) || P < 1 || k->stride(2) != 1 || v->stride(2) != 1 || k->stride(1) != D || v->stride(1) != D ||
+      copies->scalar_type() != at::kInt || copies->dim() != 2 || copies->size(1) != 3 || !copies->is_contiguous())
+    Py_RETURN_NONE;
+  const at::Tensor* sc[2] = {nullptr, nullptr};
+  for (int i = 0; i < 2; ++i) {
+    if (q8 ? !usable(sc[i] = vec(a[3 + i], at::kFloat, P), *k) || sc[i]->dim() != 1 : a[3 + i] != Py_None) Py_RETURN_NONE;
+  }
+  wnw_paged_cache c = {};
+  c.k_pages = k->data_ptr();
+  c.v_pages = v->data_ptr();
+  c.k_scale = q8 ? sc[0]->data_ptr<float>() : nullptr;
+  c.v_scale = q8 ? sc[1]->data_ptr<float>() : nullptr;
+  c.n_pages = P;
+  c.page_rows = R;
+  c.head_dim = D;
+  c.k_stride = P > 1 ? k->stride(0) : R * D;
+  c.v_stride = P > 1 ? v->stride(0) : R * D;
+  c.page_dtype = q8 ? WNW_E4M3 : dtype_code(dt);
+  Call call(*k);
+  if (!call.ok) Py_RETURN_NONE;
+  if (!call.has_stream) return nullptr;
+  const int32_t* cp = copies->const_data_ptr<int32_t>();
+  const int64_t n = copies->size(0);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = wnw_paged_copy(&c, cp, n, call.stream);
+  Py_END_ALLOW_THREADS
+  if (rc != WNW_OK) return failed(rc, "paged_copy");
+  Py_RETURN_TRUE;
+}
+
+// (logits, scores, k, done, end)
+PyObject* beam_select_impl(PyObject* const* a) {
+  const at::Tensor *x = plain(a[0]), *s = plain(a[1]), *done = nullptr;
+  if (watched() || !x || needs_grad(x) || !usable(s, *x) || x->dim() != 3 || x->stride(2) != 1) Py_RETURN_NONE;
+  const int64_t B = x->size(0), W = x->size(1), V = x->size(2);
+  const int dt = dtype_code(x->scalar_type());
+  int64_t k = W, end = 0;
+  if (dt < 0 || B < 1 || s->scalar_type() != at::kFloat || s->dim() != 2 || s->size(0) != B || s->size(1) != W || !s->is_contiguous() ||
+      (a[2] != Py_None && !whole(a[2], &k)) || k < 1 || k > 64 || !whole(a[4], &end))
+    Py_RETURN_NONE;
+  if (a[3] != Py_None) {
+    done = plain(a[3]);
+    if (!usable(done, *x) || done->scalar_type() != at::kBool || done->dim() != 2 || done->size(0) != B || done->size(1) != W ||
+        !done->is_contiguous())
+      Py_RETURN_NONE;
+  }
+  const int64_t need = wnw_beam_workspace_bytes(B, W, V, dt);
+  if (need < 0) Py_RETURN_NONE;
+  Call call(*x);
+  if (!call.ok) Py_RETURN_NONE;
+  if (!call.has_stream) return nullptr;
+  at::Tensor out = like(*x, {B, k}, at::kFloat), parents = like(*x, {B, k}, at::kInt), tokens = like(*x, {B, k}, at::kLong);
+  at::Tensor ws = like(*x, {need}, at::kByte);
+  const int64_t strides[2] = {x->stride(0), x->stride(1)};
+  const void* xp = x->const_data_ptr();
+  const float* sp = s->const_data_ptr<float>();
+  const uint8_t* dp = done ? (const uint8_t*)done->const_data_ptr() : nullptr;
+  float* op = out.data_ptr<float>();
+  int32_t* pp = parents.data_ptr<int32_t>();
+  int64_t* tp = tokens.data_ptr<int64_t>();
+  void* w = ws.data_ptr();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = wnw_beam_select(xp, strides, B, W, V, sp, dp, end, k, dt, op, pp, tp, w, need, call.stream);
+  Py_END_ALLOW_THREADS
+  if (rc != WNW_OK) return failed(rc, "beam_select");
+  Ref o0(THPVariable_Wrap(std::move(out))), o1(THPVariable_Wrap(std::move(parents))), o2(THPVariable_Wrap(std::move(tokens)));
+  return o0.o && o1.o && o2.o ? PyTuple_Pack(3, o0.o, o1.o, o2.o) : nullptr;
+}
+
 // No C++ exception leaves an entry: such a call takes the general path.
 template <PyObject* (*f)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -552,6 +787,18 @@ PyMethodDef methods[] = {
     {"paged_append", (PyCFunction)(void (*)(void))entry<paged_append_impl, 15>, METH_FASTCALL,
      "paged_append(k, v, k_pages, v_pages, page_table, seg_len, q, positions, inv_freq, sections, interleaved, cu_tokens, "
      "max_tokens, k_scale, v_scale) -> (q rotated, new lengths), or None: not the plain form"},
+    {"paged_fork", (PyCFunction)(void (*)(void))entry<paged_fork_impl, 6>, METH_FASTCALL,
+     "paged_fork(page_table, seg_len, page_refs, parents, page_rows, kv_heads) -> (table, lengths, counts, copies), or None: not "
+     "the plain form"},
+    {"paged_reserve", (PyCFunction)(void (*)(void))entry<paged_reserve_impl, 9>, METH_FASTCALL,
+     "paged_reserve(page_table, seg_len, page_refs, page_rows, tokens, cu_tokens, window, sinks, out) -> (table, counts), or None: "
+     "not the plain form"},
+    {"paged_compact", (PyCFunction)(void (*)(void))entry<paged_compact_impl, 4>, METH_FASTCALL,
+     "paged_compact(page_table, page_refs, page_rows, out) -> (table, counts, moves, used), or None: not the plain form"},
+    {"paged_copy", (PyCFunction)(void (*)(void))entry<paged_copy_impl, 5>, METH_FASTCALL,
+     "paged_copy(k_pages, v_pages, copies, k_scale, v_scale) -> True, or None: not the plain form"},
+    {"beam_select", (PyCFunction)(void (*)(void))entry<beam_select_impl, 5>, METH_FASTCALL,
+     "beam_select(logits, scores, k, done, end) -> (scores, parents, tokens), or None: not the plain form"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_callpath", "Plain calls of the per-layer operators.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

@@ -32,6 +32,9 @@ def beam_select(logits: Tensor, scores: Tensor, k: int | None = None, *, done: T
     ``parents`` are rows of a [B * W] batch, b * W + w, as ``paged_fork`` takes
     them.  Where a sample has fewer than k candidates the rest have the score
     -inf, the sample's first beam and the token ``end``."""
+    native = (_lib._callpath or _lib.callpath()).beam_select(logits, scores, k, done, end)
+    if native is not None:  # the plain form: checked and launched natively
+        return native
     tensors = [t for t in (logits, scores, done) if t is not None]
     _refuse_watched(tensors)
     if logits.dim() != 3 or logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):

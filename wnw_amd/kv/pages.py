@@ -82,6 +82,9 @@ def paged_fork(page_table: Tensor, seg_len: Tensor, page_refs: Tensor, parents: 
     fresh page, rows) or (-1, -1, 0): ``paged_copy`` does it, once for each layer
     that shares the table.  Where the call cannot be done the new table has no
     pages and the new lengths are 0; the old ones hold.  At most 8,192 samples."""
+    done = (_lib._callpath or _lib.callpath()).paged_fork(page_table, seg_len, page_refs, parents, page_rows, kv_heads)
+    if done is not None:  # the plain form: checked and launched natively
+        return done
     N, M, P, stride = _table(page_table, page_refs, seg_len, parents)
     if parents.dtype != torch.int32 or parents.dim() != 1 or not parents.is_contiguous():
         raise _lib.WnwError("parents must be a contiguous int32 [B']")
@@ -117,6 +120,10 @@ def paged_reserve(page_table: Tensor, seg_len: Tensor, page_refs: Tensor, page_r
 
     ``out``: (table, counts) to write to, which may be the given ones themselves,
     for programs and captured graphs that keep them in one place."""
+    done = (_lib._callpath or _lib.callpath()).paged_reserve(page_table, seg_len, page_refs, page_rows, tokens, cu_tokens, window,
+                                                             sinks, out)
+    if done is not None:
+        return done
     N, M, P, stride = _table(page_table, page_refs, seg_len, cu_tokens, *(out or ()), *_tensors(window, sinks))
     if cu_tokens is not None:
         if cu_tokens.dtype != torch.int32 or cu_tokens.dim() != 1 or cu_tokens.numel() < 1 or not cu_tokens.is_contiguous():
@@ -151,6 +158,9 @@ def paged_compact(page_table: Tensor, page_refs: Tensor, page_rows: int, *,
     order, to the lowest place below U that is free: ``moves`` int32 [P // 2, 3],
     (page, its new place, page_rows), then (-1, -1, 0), for ``paged_copy``.
     ``out`` as for ``paged_reserve``."""
+    done = (_lib._callpath or _lib.callpath()).paged_compact(page_table, page_refs, page_rows, out)
+    if done is not None:
+        return done
     N, M, P, stride = _table(page_table, page_refs, None, *(out or ()))
     new_table, new_refs, new_stride = _out(out, page_table, page_refs)
     moves, used = page_refs.new_empty((P // 2, 3)), page_refs.new_empty(1)
@@ -172,6 +182,8 @@ def paged_copy(k_pages: Tensor, v_pages: Tensor, copies: Tensor, *, k_scale: Ten
     or the page sets the device error word and is left out.  No page may be dst
     twice, or both src and dst (``paged_fork``'s and ``paged_compact``'s are
     not)."""
+    if (_lib._callpath or _lib.callpath()).paged_copy(k_pages, v_pages, copies, k_scale, v_scale) is not None:
+        return
     tensors = [t for t in (k_pages, v_pages, copies, k_scale, v_scale) if t is not None]
     _refuse_watched(tensors)
     if k_pages.dim() != 3 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype \
