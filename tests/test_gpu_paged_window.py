@@ -359,3 +359,37 @@ def test_refusals(gpu):
             with pytest.raises(_lib.WnwError):
                 call()
     _clean()
+
+
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("dtype,D,G,new,old", [(BF, 128, 4, [300], [9000]), (FP, 64, 1, [70, 200, 0], [6000, 300, 12000]),
+                                               (BF, 256, 2, [90, 33], [5000, 7000]), (FP, 128, 16, [64], [8000])])
+def test_prompt_blocks_of_different_lengths(gpu, q8, dtype, D, G, new, old):
+    """Few blocks, cut into shares by their own tiles: heads that see everything beside heads with short windows."""
+    H = 4
+    lens = [o + n for o, n in zip(old, new) for _ in range(H)]
+    c = Cache(gpu, lens, 64, D, dtype, q8, seed=D + G)
+    N = len(lens)
+    window = torch.tensor([(ALL, 500, 64, 0)[s % 4] for s in range(N)], dtype=torch.int32, device=gpu)
+    sinks = torch.tensor([(0, 4, 130, 0)[s % 4] for s in range(N)], dtype=torch.int32, device=gpu)
+    _hide(c, new, window, sinks)
+    q = _q(gpu, sum(new), H * G, D, dtype)
+    out = paged_prompt_attn(q, *c.args(), _cu(new, gpu), D ** -0.5, max_tokens=max(new), window=window, sinks=sinks, **c.scales())
+    _clean()
+    _prompt_check(c, q, out, new, window, sinks, D ** -0.5)
+    assert torch.equal(out, paged_prompt_attn(q, *c.args(), _cu(new, gpu), D ** -0.5, max_tokens=max(new), window=window,
+                                              sinks=sinks, **c.scales()))
+    # a sample with more tokens than the call says: the error word, its rows not written, the others' right
+    if len(new) > 1:
+        most = sorted(new)[-2]
+        room = torch.full_like(q, 7.0)
+        paged_prompt_attn(q, *c.args(), _cu(new, gpu), D ** -0.5, max_tokens=most, window=window, sinks=sinks, out=room, **c.scales())
+        torch.cuda.synchronize()
+        assert _lib.device_error() == _lib.DEVERR_BOUNDS
+        at = 0
+        for b, n in enumerate(new):
+            if n > most:
+                assert bool((room[at:at + n] == 7).all())
+                room[at:at + n] = out[at:at + n]
+            at += n
+        _prompt_check(c, q, room, new, window, sinks, D ** -0.5)

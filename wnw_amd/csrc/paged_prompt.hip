@@ -62,14 +62,17 @@ struct PagedPromptParams {
   const void* q;
   void* out;
   int64_t qt, qh, ot, oh;  // strides in elements
-  float* part;             // [blocks, splits, waves]: D / 32 x 16 sums a lane, then max, sum
+  float* part;             // [blocks, splits, waves] (WIN: [shares, waves]): D / 32 x 16 sums a lane, then max, sum
   float scale_log2;
   int32_t G, nqb, splits;
   int32_t* err;
-  PagedView view;          // with a window
+  PagedView view;          // WIN: the windows, the workgroups of the launch if blocks are shared out
+  int32_t wgs;             // (else 0), and each block's first share and shares
+  int32_t* shares;
 };
 
 static constexpr int kPpKeys = 64;  // keys of a tile
+static constexpr int kPpLeast = 4;  // tiles of a share at least
 
 template <typename T>
 __device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f32x16& c) {
@@ -130,6 +133,90 @@ __device__ __forceinline__ PromptTiles tiles_of(const PagedPromptParams& p, cons
   return y;
 }
 
+// Through windows of different lengths the blocks' tiles differ (512 tokens after
+// 22,116 rows: 354 where a head sees everything, 36 through 2,048), so where there are few
+// blocks each is cut by its own: all of them into shares of at most `most` tiles, the
+// least number with which the launch's workgroups have a share each.  Every workgroup
+// finds that out for itself, a wave over at most 512 blocks, from numbers that
+// are on the device.
+static constexpr int kPpShared = 512;  // blocks at most
+struct PromptShare {
+  int block, split, splits;  // block -1: none
+};
+__device__ __forceinline__ int div_up(int x, int y, float inv) {  // inv = 1 / y, y >= 4
+  x += y - 1;
+  int q = (int)((float)x * inv);
+  const int rest = x - q * y;
+  q += rest >= y ? 1 : 0;
+  return q - (rest < 0 ? 1 : 0);
+}
+template <int W>
+__device__ __forceinline__ PromptShare prompt_share(const PagedPromptParams& p, int id, int lane, bool tell) {
+  constexpr int L = kPpShared / 64;
+  const int blocks = p.c.n_seg * p.nqb;
+  int tiles[L], longest = 0;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < L; ++i) {
+    const int b = i * 64 + lane;
+    tiles[i] = 0;
+    if (i * 64 < blocks && b < blocks) {
+      const int qblk = p.nqb - 1 - b / p.c.n_seg;
+      const PromptRows r = prompt_rows<true>(p, b % p.c.n_seg, tell && qblk == 0);
+      if (qblk * 32 * W < r.rows) tiles[i] = max(tiles_of<W, true>(p, r, qblk).n, 1);  // (rows that see none are written too)
+    }
+    sum += (float)tiles[i];
+    longest = max(longest, tiles[i]);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) longest = max(longest, __shfl_xor(longest, o));
+  sum = wave_sum(sum);
+  auto shares_of = [&](int most, int* mine) {
+    const float inv = 1.0f / (float)most;
+    int all = 0;
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      if (i * 64 < blocks) {
+        mine[i] = min(div_up(tiles[i], most, inv), p.wgs + 1);
+        all += mine[i];
+      } else {
+        mine[i] = 0;
+      }
+    return all;
+  };
+  int mine[L];
+  int lo = max((int)(0.999f * sum / (float)p.wgs), kPpLeast), hi = max(longest, lo);
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    int all = shares_of(mid, mine);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) all += __shfl_xor(all, o);
+    if (all <= p.wgs)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  const int own = shares_of(lo, mine);
+  int incl = own;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(incl, o);
+    if (lane >= o) incl += y;
+  }
+  PromptShare y = {-1, 0, 1};
+  int at = incl - own;
+#pragma unroll
+  for (int i = 0; i < L; ++i) {
+    if (id >= at && id < at + mine[i]) y = PromptShare{i * 64 + lane, id - at, mine[i]};
+    at += mine[i];
+  }
+  const uint64_t who = __ballot(y.block >= 0);
+  if (!who) return PromptShare{-1, 0, 1};
+  const int from = __builtin_ctzll(who);
+  return PromptShare{__builtin_amdgcn_readlane(y.block, from), __builtin_amdgcn_readlane(y.split, from),
+                     __builtin_amdgcn_readlane(y.splits, from)};
+}
+
 // The wave's rows out, 32-element parts dt0 .. dt0 + NT - 1: lane (hi, n) has
 // elements 32 i + 8 j + 4 hi + 0..3 of row n
 template <typename T, int NT, bool WIN>
@@ -176,8 +263,25 @@ paged_prompt_kernel(PagedPromptParams p) {
   const int hi = lane >> 5, n = lane & 31;
   const int N = p.c.n_seg;
   // the blocks with the most tiles first; workgroups of one segment N apart (8 segments: each in one L2)
-  const int seg = blockIdx.x % N, rank = blockIdx.x / N;
-  const int block = rank / p.splits, split = rank - block * p.splits, qblk = p.nqb - 1 - block;
+  int seg, block, split, shared = 1;
+  if (WIN && p.wgs > 0) {
+    const PromptShare mine = prompt_share<W>(p, blockIdx.x, lane, blockIdx.x == 0 && w == 0);
+    if (mine.block < 0) return;
+    seg = mine.block % N;
+    block = mine.block / N;
+    split = mine.split;
+    shared = mine.splits;
+    if (split == 0 && tid == 0) {
+      p.shares[2 * mine.block] = blockIdx.x;
+      p.shares[2 * mine.block + 1] = shared;
+    }
+  } else {
+    const int rank = blockIdx.x / N;
+    seg = blockIdx.x % N;
+    block = rank / p.splits;
+    split = rank - block * p.splits;
+  }
+  const int qblk = p.nqb - 1 - block;
   const PromptRows r = prompt_rows<WIN>(p, seg, tid == 0 && qblk == 0 && split == 0);
   if (qblk * kPpQ >= r.rows) return;
   const int h = seg % p.t.hkv;
@@ -190,7 +294,7 @@ paged_prompt_kernel(PagedPromptParams p) {
   const int wlast = base + min(qblk * kPpQ + 32 * w + 31, r.rows - 1) / p.G;
   const int first = base + qblk * kPpQ / p.G;  // and the workgroup's first
   const PromptTiles walk = tiles_of<W, WIN>(p, r, qblk);
-  const int tiles = walk.n, splits = splits_of(tiles, p.splits);
+  const int tiles = walk.n, splits = WIN ? shared : splits_of(tiles, p.splits);
   auto real = [&](int place) { return WIN && place >= walk.head ? place + walk.gap : place; };
   if (split >= splits) return;
   const int t0 = (int)((int64_t)tiles * split / splits), t1 = (int)((int64_t)tiles * (split + 1) / splits);
@@ -530,7 +634,8 @@ paged_prompt_kernel(PagedPromptParams p) {
   if (splits == 1) {
     prompt_store<T, DT, WIN>(p, r, row, h, hi, 0, o, l);
   } else if (busy) {
-    float* part = p.part + ((((int64_t)block * N + seg) * p.splits + split) * W + w) * (DT * 16 + 2) * 64;
+    const int64_t place = WIN ? blockIdx.x : ((int64_t)block * N + seg) * p.splits + split;
+    float* part = p.part + (place * W + w) * (DT * 16 + 2) * 64;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -554,10 +659,11 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParam
   const int seg = block % N, qblk = p.nqb - 1 - block / N;
   const PromptRows r = prompt_rows<WIN>(p, seg, false);
   if (qblk * kPpQ + 32 * w >= r.rows) return;
-  const int splits = splits_of(tiles_of<W, WIN>(p, r, qblk).n, p.splits);
+  const int splits = WIN ? p.shares[2 * block + 1] : splits_of(tiles_of<W, WIN>(p, r, qblk).n, p.splits);
   if (splits == 1) return;
   constexpr int64_t kPart = (DT * 16 + 2) * 64;
-  const float* part = p.part + ((int64_t)block * p.splits * W + w) * kPart;
+  const int64_t place = WIN ? p.shares[2 * block] : (int64_t)block * p.splits;
+  const float* part = p.part + (place * W + w) * kPart;
   f32x16 o = f32x16{};
   float m = kPgLowest, l = 0.f;
   auto add = [&](float pm, float pl, const f32x16& y) {
@@ -614,6 +720,7 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedPromptParam
 // tokens, 11 tiles: 25 us, cut in two 31).
 struct PromptPlan {
   int64_t waves, nqb, splits, bytes;
+  int64_t wgs = 0, part = 0;  // through windows: the workgroups that blocks are shared out to, bytes ahead of the partial sums
 };
 // view: the windows, null without; then a block's tiles are at most those of its rows' windows.
 static PromptPlan prompt_plan(int64_t n_seg, int64_t group, int64_t max_tokens, int64_t capacity, int64_t D,
@@ -629,6 +736,19 @@ static PromptPlan prompt_plan(int64_t n_seg, int64_t group, int64_t max_tokens, 
   const int64_t wgs = std::max<int64_t>(n_seg * y.nqb, 1), want = (y.waves == 8 ? 1 : 2) * cus;
   y.splits = std::max<int64_t>(1, std::min({want / wgs, tiles / 4, (int64_t)64}));
   if (tiles - tiles / y.splits < 8) y.splits = 1;
+  if (view) {
+    // (of windows on the device nothing is known: they may differ)
+    const bool alike = !view->window && !view->sinks;
+    if (alike ? y.splits > 1 : wgs <= std::min<int64_t>(want, kPpShared) && tiles - tiles / 4 >= 8) {
+      y.wgs = want;
+      y.part = (wgs * 8 + 255) / 256 * 256;
+      y.bytes = y.part + want * y.waves * (D / 2 + 2) * 64 * 4;
+    } else {
+      y.bytes = 0;
+    }
+    y.splits = 1;
+    return y;
+  }
   y.bytes = y.splits == 1 ? 0 : wgs * y.splits * y.waves * (D / 2 + 2) * 64 * 4;
   return y;
 }
@@ -636,8 +756,8 @@ static PromptPlan prompt_plan(int64_t n_seg, int64_t group, int64_t max_tokens, 
 template <typename T, int D, bool Q8, int W, bool WIN>
 static hipError_t launch_prompt_q(const PagedPromptParams& p, hipStream_t st) {
   const unsigned blocks = (unsigned)(p.c.n_seg * (int64_t)p.nqb);
-  hipLaunchKernelGGL((paged_prompt_kernel<T, D, Q8, W, WIN>), dim3(blocks * p.splits), dim3(64 * W), 0, st, p);
-  if (p.splits > 1)
+  hipLaunchKernelGGL((paged_prompt_kernel<T, D, Q8, W, WIN>), dim3(WIN && p.wgs ? p.wgs : blocks * p.splits), dim3(64 * W), 0, st, p);
+  if (p.splits > 1 || (WIN && p.wgs > 0))
     hipLaunchKernelGGL((paged_prompt_join_kernel<T, D, W, WIN>), dim3(blocks * W * (D / 32)), dim3(256), 0, st, p);
   return hipGetLastError();
 }
@@ -703,7 +823,9 @@ static int prompt_attn(const wnw_paged_cache* cache, const int32_t* seg_len, con
   p.q = q;
   p.out = out;
   p.qt = strides[0], p.qh = strides[1], p.ot = strides[2], p.oh = strides[3];
-  p.part = (float*)workspace;
+  p.part = (float*)((uint8_t*)workspace + y.part);
+  p.shares = (int32_t*)workspace;
+  p.wgs = (int32_t)y.wgs;
   p.scale_log2 = scale * kPgLog2e;
   p.G = (int32_t)group;
   p.nqb = (int32_t)y.nqb;
