@@ -256,20 +256,19 @@ __device__ __forceinline__ void paged_decode_gather(const PagedDecodeParams& p, 
 }
 
 // Through a window (WIN), the steps that no row of a segment sees are left out of
-// its steps: those between the sinks' and the first one that the first token's
-// window reaches.  The table's entries there are not read.
+// its steps: those between the sinks' and the first one that the window of the
+// first of the most tokens reaches.  (A sample with fewer may have a step that
+// none of them sees: the table's entries there are not read either.)
 struct DecodeView {
   int window, sinks;  // no larger than the segment
-  int lo;             // rows from here on are in the first token's window
   int head, gap;      // the sinks' steps, and how many are left out behind them
 };
-__device__ __forceinline__ DecodeView decode_view(int window, int sinks, int n, int count) {
+__device__ __forceinline__ DecodeView decode_view(int window, int sinks, int n, int most) {
   DecodeView y;
   y.window = window;
   y.sinks = sinks;
-  y.lo = max(n - count + 1 - window, 0);
   y.head = (sinks + kPdStep - 1) / kPdStep;
-  y.gap = max(y.lo / kPdStep - y.head, 0);
+  y.gap = max(max(n - most + 1 - window, 0) / kPdStep - y.head, 0);
   return y;
 }
 
@@ -295,17 +294,23 @@ paged_decode_kernel(PagedDecodeParams p) {
   const int N = p.c.n_seg, wg = blockIdx.x;
 
   auto steps_of = [&](int n) { return n >= 0 && n <= p.c.capacity ? (n + kPdStep - 1) / kPdStep : 0; };
-  int lane_w = 0, lane_z = 0;  // WIN: of the lane's segment, as len
+  // WIN: the windows and sinks of the segments that the lanes have, as len (in LDS: registers are short)
+  __shared__ int32_t views[WIN ? W : 1][2][64];
+  auto keep = [&](int window, int sinks) {
+    if constexpr (WIN) {
+      views[w][0][lane] = window;
+      views[w][1][lane] = sinks;
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+  int unused[2];
+  auto kept = [&](int i, int j) { return __builtin_amdgcn_readfirstlane(views[w][i][j]); };
   // segment s's steps, and its window and sinks
   auto seg_steps = [&](int s, int n, int* w, int* z) {
     int steps = steps_of(n);
     if constexpr (WIN) {
       if (!paged_view_of(p.view, s, n, w, z)) steps = 0;
-      if (steps > 0) {
-        int first, count = 1;
-        if (p.t.cu) paged_tokens_of(p.t, s, &first, &count);
-        steps -= decode_view(*w, *z, n, count).gap;
-      }
+      steps = steps > 0 ? steps - decode_view(*w, *z, n, p.t.most).gap : 0;
     }
     return steps;
   };
@@ -325,7 +330,9 @@ paged_decode_kernel(PagedDecodeParams p) {
   const int per = (N + NT - 1) / NT, sa = min(tid * per, N), sb = min(sa + per, N);
   if (N <= 64) {
     len = lane < N ? p.seg_len[lane] : 0;
-    num = seg_steps(min(lane, N - 1), len, &lane_w, &lane_z);
+    int win_of, sinks_of;
+    num = seg_steps(min(lane, N - 1), len, &win_of, &sinks_of);
+    keep(win_of, sinks_of);
     at = scan(num);
     S = __builtin_amdgcn_readlane(at, 63);
     at -= num;
@@ -333,7 +340,7 @@ paged_decode_kernel(PagedDecodeParams p) {
   } else {
     int most = 0;
     for (int s = sa; s < sb; ++s) {
-      const int n = seg_steps(s, p.seg_len[s], &lane_w, &lane_z);
+      const int n = seg_steps(s, p.seg_len[s], &unused[0], &unused[1]);
       mine += n;
       most = max(most, n);
     }
@@ -377,7 +384,7 @@ paged_decode_kernel(PagedDecodeParams p) {
     } else {
       int e = before + incl - mine;  // steps before the thread's segments
       for (int s = sa; s < sb; ++s) {
-        const int n = seg_steps(s, p.seg_len[s], &lane_w, &lane_z);
+        const int n = seg_steps(s, p.seg_len[s], &unused[0], &unused[1]);
         if (uncut ? s == s0 : e <= x0 && x0 < e + n) {
           sh[0] = s;
           sh[1] = e;
@@ -398,7 +405,9 @@ paged_decode_kernel(PagedDecodeParams p) {
   for (int x = x0; x < x1 && win < N;) {
     if (N > 64) {
       len = win + lane < N ? p.seg_len[win + lane] : 0;
-      num = seg_steps(min(win + lane, N - 1), len, &lane_w, &lane_z);
+      int win_of, sinks_of;
+      num = seg_steps(min(win + lane, N - 1), len, &win_of, &sinks_of);
+      keep(win_of, sinks_of);
       at += scan(num) - num;
     }
     // the pieces of this window, and the waves [wf, wt) of each; a piece that
@@ -429,8 +438,10 @@ paged_decode_kernel(PagedDecodeParams p) {
       const int mysteps = (b - a + nw - 1) / nw;
       DecodeRows r = decode_rows(p, seg, n);
       DecodeView view = {};
+      int lo = 0;  // rows from here on are in the first token's window
       if constexpr (WIN) {
-        view = decode_view(__builtin_amdgcn_readlane(lane_w, j), __builtin_amdgcn_readlane(lane_z, j), n, r.count);
+        view = decode_view(kept(0, j), kept(1, j), n, p.t.most);
+        lo = max(n - r.count + 1 - view.window, 0);
         r.blind = (view.window | view.sinks) == 0;
       }
       auto real = [&](int step) { return WIN && step >= view.head ? step + view.gap : step; };
@@ -454,7 +465,7 @@ paged_decode_kernel(PagedDecodeParams p) {
         const int step = a + nw * (k0 + (lane >> 1));
         const int row = real(step) * kPdStep + 16 * (lane & 1);
         pid = -1;
-        if (step < b && row < n && (!WIN || row < view.sinks || row + 16 > view.lo)) {
+        if (step < b && row < n && (!WIN || row < view.sinks || row + 16 > lo)) {
           pid = p.c.table[seg * p.c.table_stride + (row >> p.c.shift)];
           if (pid < 0 || pid >= p.c.n_pages) {
             raise_device_error(p.err, WNW_DEVERR_BOUNDS);
@@ -533,7 +544,7 @@ paged_decode_kernel(PagedDecodeParams p) {
 #pragma unroll
           for (int i = 0; i < VI; ++i) {
             const int rr = (i * 1024 + lane * 16) / RB;
-            if (row0 + rr >= n || (bad_now >> (rr >> 4) & 1) || (WIN && row0 + rr >= view.sinks && row0 + rr < view.lo))
+            if (row0 + rr >= n || (bad_now >> (rr >> 4) & 1) || (WIN && row0 + rr >= view.sinks && row0 + rr < lo))
               vr[i] = u32x4{0, 0, 0, 0};
           }
           if ((WIN || row0 + kPdStep > all_see) && r.count > 1) {
@@ -618,7 +629,7 @@ paged_decode_kernel(PagedDecodeParams p) {
         // rows that some columns see: those that the window leaves between the first token and the last, the last tokens'
         const int late = max(all_see, 0);
         int row = late;
-        if constexpr (WIN) row = min(max(view.lo, view.sinks), late);
+        if constexpr (WIN) row = min(max(lo, view.sinks), late);
 #pragma unroll 1
         for (; row < n; ++row) {
           if (WIN && row < late && row >= n - view.window) row = late;
@@ -672,7 +683,7 @@ paged_decode_kernel(PagedDecodeParams p) {
         const int j = __builtin_ctzll(todo);
         const int f = __builtin_amdgcn_readlane(waves, j) & 255, t = __builtin_amdgcn_readlane(waves, j) >> 8;
         DecodeRows r = decode_rows(p, win + j, __builtin_amdgcn_readlane(len, j));
-        if constexpr (WIN) r.blind = (__builtin_amdgcn_readlane(lane_w, j) | __builtin_amdgcn_readlane(lane_z, j)) == 0;
+        if constexpr (WIN) r.blind = (kept(0, j) | kept(1, j)) == 0;
         int a, b;
         const int slot = (2 * wg + (piece(j, &a, &b) + a == x0 ? 0 : 1)) * p.cols;
         for (int e = here(tid); e < r.cols * (D / 4); e += NT) {
@@ -723,7 +734,7 @@ paged_decode_kernel(PagedDecodeParams p) {
         if (!sh[i]) continue;
         const int j = i ? j1 : j0, b0 = __builtin_amdgcn_readlane(at, j), w0 = owner_of(b0);
         DecodeRows r = decode_rows(p, win + j, __builtin_amdgcn_readlane(len, j));
-        if constexpr (WIN) r.blind = (__builtin_amdgcn_readlane(lane_w, j) | __builtin_amdgcn_readlane(lane_z, j)) == 0;
+        if constexpr (WIN) r.blind = (kept(0, j) | kept(1, j)) == 0;
         paged_decode_gather<T, D, NT, WIN>(p, r, tid, b0 > start_of(w0), w0,
                                       owner_of(b0 + __builtin_amdgcn_readlane(num, j) - 1), (float*)lds);
       }
