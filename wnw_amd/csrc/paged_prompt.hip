@@ -110,13 +110,20 @@ __device__ __forceinline__ PromptRows prompt_rows(const PagedPromptParams& p, in
 // by the table 26; 64 tokens after 500 rows 19 and 26, with pieces of 4 tiles or
 // more 21).
 __device__ __forceinline__ int splits_of(int tiles, int most) { return max(min(tiles / 2, most), 1); }
-// Tiles that a block of query rows walks.  Through a window, those that none of its rows
-// sees are left out: `gap` of them behind the `head` that hold the sinks.  (Places in the
-// walk, not tiles, are what the loops, the splits, the LDS buffers and the pages held in
-// registers count.)
+// Tiles that a block of query rows walks.  Through a window, the groups of 16 keys that
+// none of its rows sees are left out: `gap` of them behind the `head` that hold the
+// sinks, and what is left is put together, four groups a tile (a page has whole
+// groups).  Places in that walk, not keys, are what the loops, the splits, the LDS
+// buffers and the pages held in registers count.
 struct PromptTiles {
   int n, head, gap;
   int lo, last_lo;  // rows from here on are in the window of the block's first row, of its last
+  __device__ __forceinline__ int group(int place) const { return place < head ? place : place + gap; }
+  // the place of the first group at or past row x
+  __device__ __forceinline__ int place_of(int x) const {
+    const int g = (max(x, 0) + 15) >> 4;
+    return g < head ? g : max(g - gap, head);
+  }
 };
 template <int W, bool WIN>
 __device__ __forceinline__ PromptTiles tiles_of(const PagedPromptParams& p, const PromptRows& r, int qblk) {
@@ -124,11 +131,12 @@ __device__ __forceinline__ PromptTiles tiles_of(const PagedPromptParams& p, cons
   const int last = base + min(32 * W * (qblk + 1) - 1, r.rows - 1) / p.G;  // rows that its last one sees
   PromptTiles y = {max((last + kPpKeys - 1) / kPpKeys, 0), 0, 0, 0, 0};
   if constexpr (WIN) {
+    const int groups = max((last + 15) >> 4, 0);
     y.lo = max(base + 32 * W * qblk / p.G - r.window, 0);
     y.last_lo = last - r.window;
-    y.head = min((r.sinks + kPpKeys - 1) / kPpKeys, y.n);
-    y.gap = max(min(y.lo / kPpKeys, y.n) - y.head, 0);
-    y.n -= y.gap;
+    y.head = min((r.sinks + 15) >> 4, groups);
+    y.gap = max(min(y.lo >> 4, groups) - y.head, 0);
+    y.n = (groups - y.gap + 3) >> 2;
   }
   return y;
 }
@@ -295,7 +303,8 @@ paged_prompt_kernel(PagedPromptParams p) {
   const int first = base + qblk * kPpQ / p.G;  // and the workgroup's first
   const PromptTiles walk = tiles_of<W, WIN>(p, r, qblk);
   const int tiles = walk.n, splits = WIN ? shared : splits_of(tiles, p.splits);
-  auto real = [&](int place) { return WIN && place >= walk.head ? place + walk.gap : place; };
+  // the first key of group b of a tile
+  auto key_of = [&](int tile, int b) { return WIN ? walk.group(4 * tile + b) * 16 : tile * kPpKeys + 16 * b; };
   if (split >= splits) return;
   const int t0 = (int)((int64_t)tiles * split / splits), t1 = (int)((int64_t)tiles * (split + 1) / splits);
   const bool busy = qblk * kPpQ + 32 * w < r.rows;  // a wave without rows only moves tiles
@@ -330,7 +339,7 @@ paged_prompt_kernel(PagedPromptParams p) {
   // Rows past the segment's take its last page; an entry that is no page page
   // 0, with its sign bit set.
   auto find = [&](int window) {
-    const int key = WIN ? real(window * kWin + (lane >> 2)) * kPpKeys + (lane & 3) * 16 : (window * 64 + lane) * 16;
+    const int key = (WIN ? walk.group(window * 64 + lane) : window * 64 + lane) * 16;
     const int id = table[min(key, r.len - 1) >> p.c.shift];
     const bool is = (uint32_t)id < (uint32_t)p.c.n_pages;
     wrong |= !is && (!WIN || key < r.sinks || key + 16 > walk.lo);  // others may have been given back
@@ -362,7 +371,7 @@ paged_prompt_kernel(PagedPromptParams p) {
 #pragma unroll
     for (int u = 0; u < NI; ++u) {
       const int in_tile = u * RPL + w * (64 / CG);
-      const int row = real(tile) * kPpKeys + in_tile;
+      const int row = WIN ? key_of(tile, in_tile >> 4) + (in_tile & 15) : tile * kPpKeys + in_tile;
       const int id = __builtin_amdgcn_readlane(pid, ((tile * kPpKeys + in_tile) >> 4) & 63);
       const int64_t page = id & 0x7fffffff;
       const WNW_GLOBAL uint8_t* kp = gptr<uint8_t>(p.c.k) + (page * p.c.k_stride + (row & in) * GB);
@@ -380,21 +389,27 @@ paged_prompt_kernel(PagedPromptParams p) {
     }
   };
   auto clear = [&](int tile) {  // rows of kr and vr that are not the segment's
-    int any = (real(tile) + 1) * kPpKeys > r.len;
+    int any = WIN ? key_of(tile, 3) + 16 > r.len : (tile + 1) * kPpKeys > r.len;
 #pragma unroll
     for (int u = 0; u < NI; ++u) any |= gone[u] < 0;
     if (!any) return;
 #pragma unroll
     for (int u = 0; u < NI; ++u) {
       if (gone[u] < 0) kr[u] = u32x4{0, 0, 0, 0};
-      if (gone[u] < 0 || real(tile) * kPpKeys + u * RPL + srow >= r.len) vr[u] = u32x4{0, 0, 0, 0};
+      const int at = u * RPL + srow;
+      const int row = WIN ? key_of(tile, (u * RPL + w * (64 / CG)) >> 4) + (at & 15) : tile * kPpKeys + at;
+      if (gone[u] < 0 || row >= r.len) vr[u] = u32x4{0, 0, 0, 0};
     }
   };
-  // whether every row of the workgroup sees the whole of a tile
-  auto whole = [&](int tile) {
-    const int k0 = real(tile) * kPpKeys, k1 = k0 + kPpKeys;
-    return k1 <= first && (!WIN || k0 >= walk.last_lo || k1 <= r.sinks);
+  // Whether rows see the whole of a tile, the first of them `seen` rows and the last from the group at place `late` on:
+  // every group before it is of sinks alone.
+  auto all_see = [&](int tile, int seen, int late) {
+    if constexpr (!WIN) return (tile + 1) * kPpKeys <= seen;
+    const int early = r.sinks >> 4;
+    return key_of(tile, 3) + 16 <= seen && (4 * tile >= late || 4 * tile + 4 <= early || early >= late);
   };
+  const int late = WIN ? walk.place_of(walk.last_lo) : 0;
+  auto whole = [&](int tile) { return all_see(tile, first, late); };  // every row of the workgroup
   // takes infinities and NaN out of the V of one that not every row does
   auto even = [&](int tile) {
     if (whole(tile)) return;
@@ -476,21 +491,23 @@ paged_prompt_kernel(PagedPromptParams p) {
       un[b] = Q8 ? at(wu) : 1.f;
     }
     if (masked) {
-      const int lim = limit - real(i) * kPpKeys - 4 * hi;  // keys 32 mt + 8 j + c (+ 4 hi) below it
+      if constexpr (WIN) {
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+        for (int b = 0; b < 4; ++b) {
+          const int key = key_of(i, b) + 4 * hi, lim = limit - key, lo = lim - r.window, sink = r.sinks - key;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (32 * mt + 8 * (e >> 2) + (e & 3) >= lim) s[mt][e] = -INFINITY;
-      if constexpr (WIN) {  // and those below the window that are no sinks
-        const int lo = lim - r.window, sink = r.sinks - real(i) * kPpKeys - 4 * hi;
+          for (int e = 0; e < 8; ++e) {
+            const int k = 8 * (e >> 2) + (e & 3);  // of the group's keys
+            if (k >= lim || (k < lo && k >= sink)) s[b >> 1][8 * (b & 1) + e] = -INFINITY;
+          }
+        }
+      } else {
+        const int lim = limit - i * kPpKeys - 4 * hi;  // keys 32 mt + 8 j + c (+ 4 hi) below it
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int k = 32 * mt + 8 * (e >> 2) + (e & 3);
-            if (k < lo && k >= sink) s[mt][e] = -INFINITY;
-          }
+          for (int e = 0; e < 16; ++e)
+            if (32 * mt + 8 * (e >> 2) + (e & 3) >= lim) s[mt][e] = -INFINITY;
       }
     }
     float mx = m;
@@ -579,13 +596,14 @@ paged_prompt_kernel(PagedPromptParams p) {
       }
     };
     if constexpr (WIN) {
+      // places of the first group that the wave's first row sees past the sinks, and of the first that its last row sees whole
+      const int from = walk.place_of(wfirst - r.window - 15), wlate = walk.place_of(wlast - r.window);
       for (int i = t0; i < t1; ++i) {
         turn(i);
-        const int k0 = real(i) * kPpKeys, k1 = k0 + kPpKeys;
-        if (!busy || k0 >= wlast || (k0 >= r.sinks && k1 <= wfirst - r.window))
+        if (!busy || key_of(i, 0) >= wlast || (4 * i >= walk.head && 4 * i + 4 <= from))
           pass(i);
         else
-          tile(i, k1 > wfirst || (k0 < wlast - r.window && k1 > r.sinks));
+          tile(i, !all_see(i, wfirst, wlate));
       }
     } else {
       // the tiles that every row of the wave sees whole, the others, the turns of the workgroup's later waves
@@ -624,7 +642,7 @@ paged_prompt_kernel(PagedPromptParams p) {
       if constexpr (WIN) {
 #pragma unroll 1
         for (int i = t0; i < t1; ++i)
-          if (!whole(i)) give(real(i) * kPpKeys, min((real(i) + 1) * kPpKeys, wlast));
+          for (int b = 0; b < 4 && !whole(i); ++b) give(key_of(i, b), min(key_of(i, b) + 16, wlast));
       } else {
         give(max(t0, max(first, 0) / kPpKeys) * kPpKeys, min(t1 * kPpKeys, wlast));
       }
@@ -729,7 +747,7 @@ static PromptPlan prompt_plan(int64_t n_seg, int64_t group, int64_t max_tokens, 
   const int64_t rows = max_tokens * group, cus = device_cus();
   int64_t tiles = (capacity + kPpKeys - 1) / kPpKeys;
   if (view && !view->window && !view->sinks)
-    tiles = std::min(tiles, ((int64_t)view->window_all + view->sinks_all + 256 / group) / kPpKeys + 3);
+    tiles = std::min(tiles, ((int64_t)view->window_all + view->sinks_all + 256 / group) / kPpKeys + 2);
   const bool own = n_seg * ((rows + 255) / 256) <= cus && 2 * max_tokens >= capacity;
   y.waves = D == 128 && !own ? 8 : 4;
   y.nqb = (rows + 32 * y.waves - 1) / (32 * y.waves);
