@@ -50,8 +50,7 @@ def test_workspace_sizes():
 
     assert size(c, 4, 2) == lib.wnw_paged_decode_workspace_bytes(8, 8, 128)
     assert size(c, 4, 100) == 0  # a short walk is not cut
-    assert size(c, 4, 100, window_all=1 << 40) == size(c, 4, 100, window=PTR) == \
-        lib.wnw_paged_prompt_workspace_bytes(ctypes.byref(c), 4, 100) > 0
+    assert size(c, 4, 100, window_all=1 << 40) == size(c, 4, 100, window=PTR) > 0  # shared out
     assert size(c, 4, 100, window_all=-1) == size(c, 0, 100) == size(_cache(head_dim=96), 4, 100) == -1
 
 

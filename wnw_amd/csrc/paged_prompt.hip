@@ -264,6 +264,11 @@ paged_prompt_kernel(PagedPromptParams p) {
   // f16 weights are held times 2^8: normal numbers down to 2^-22 of the largest;
   // bf16 ones times 2^-16: 2^16 times the type's largest value is a sum yet
   constexpr float kBias = std::is_same<VT, f16_t>::value ? 8.f : -16.f;
+  // How a window's tiles run over 8-bit pages at head_dim 128: 4,564 tokens, window 1,024,
+  // 105 us for 114 one after the other (in a row of such calls, the clock falling, 109 for
+  // 111).  16-bit pages, which have no codes to convert, lose by it (a ragged batch 69 for
+  // 66), and so does head_dim 64, whose products are short (window 500: 53 for 48).
+  constexpr bool kSideBySide = WIN && Q8 && D == 128;
   constexpr bool kTwo = Q8 && std::is_same<T, f16_t>::value;  // weights of two parts
   __shared__ __attribute__((aligned(16))) uint8_t lds[NB * 2 * TB];  // [NB][K, V]
   __shared__ int odd;  // V had infinities or NaN in such a tile
@@ -462,6 +467,23 @@ paged_prompt_kernel(PagedPromptParams p) {
     wl = fminf(fmaxf(__builtin_amdgcn_logf(vs), -80.f), 127.f);
     wu = __builtin_amdgcn_exp2f(-wl);
   };
+  // Scores of keys that a row does not see, in the tile's groups that not all of the wave's rows see whole (as all_see)
+  auto hide = [&](int i, int wlate, f32x16* s) {
+    const int early = r.sinks >> 4;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int place = 4 * i + b, key = walk.group(place) * 16;
+      if (key + 16 <= wfirst && (place >= wlate || place < early)) continue;
+      const int lo = limit - r.window - key - 4 * hi, sink = min(r.sinks, limit) - key - 4 * hi;
+      const bool sinks = place < walk.head;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int k = 8 * (e >> 2) + (e & 3);  // of the group's keys (+ 4 hi)
+        const bool sees = (uint32_t)(k - lo) < (uint32_t)r.window || (sinks && k < sink);
+        s[b >> 1][8 * (b & 1) + e] = sees ? s[b >> 1][8 * (b & 1) + e] : -INFINITY;
+      }
+    }
+  };
   auto tile = [&](int i, auto masked) {
     const uint8_t* kt = lds + (NB == 2 ? (i & 1) * 2 * TB : 0);
     const uint8_t* vt = kt + TB;
@@ -492,15 +514,7 @@ paged_prompt_kernel(PagedPromptParams p) {
     }
     if (masked) {
       if constexpr (WIN) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const int key = key_of(i, b) + 4 * hi, lim = limit - key, lo = lim - r.window, sink = r.sinks - key;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int k = 8 * (e >> 2) + (e & 3);  // of the group's keys
-            if (k >= lim || (k < lo && k >= sink)) s[b >> 1][8 * (b & 1) + e] = -INFINITY;
-          }
-        }
+        hide(i, walk.place_of(wlast - r.window), s);
       } else {
         const int lim = limit - i * kPpKeys - 4 * hi;  // keys 32 mt + 8 j + c (+ 4 hi) below it
 #pragma unroll
@@ -557,7 +571,355 @@ paged_prompt_kernel(PagedPromptParams p) {
         if constexpr (kTwo) o[dt] = mma32<VT>(v, pc[b], o[dt]);
       }
   };
-  if (t0 < t1) {
+  auto finish = [&]() {  // (the wave's tiles are behind a barrier)
+    if (wrong) raise_device_error(p.err, WNW_DEVERR_BOUNDS);
+    if (odd) {  // what even() took out, to the rows that see it
+      auto give = [&](int from, int to) {
+#pragma unroll 1
+        for (int key = from; key < to; ++key) {
+          const uint8_t* at = paged_v_row(p.c, seg, key, GB);
+          if (!at || key >= limit || (WIN && key >= r.sinks && key < limit - r.window)) continue;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              __builtin_amdgcn_sched_barrier(0);
+              const f32x4 x = odd_quad<PE>(at, 32 * dt + 8 * j + 4 * hi);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[dt][4 * j + e] += x[e];
+            }
+        }
+      };
+      if constexpr (WIN) {
+#pragma unroll 1
+        for (int i = t0; i < t1; ++i)
+          for (int b = 0; b < 4 && !whole(i); ++b) give(key_of(i, b), min(key_of(i, b) + 16, wlast));
+      } else {
+        give(max(t0, max(first, 0) / kPpKeys) * kPpKeys, min(t1 * kPpKeys, wlast));
+      }
+    }
+  };
+  if constexpr (kSideBySide) {
+    // A tile's products and vector instructions run side by side where they are of
+    // different tiles: the next tile's scores among this one's exponentials, this one's
+    // values among the next one's maximum and the staging.  So K is staged a tile ahead of
+    // V: when tile i is used, K of i + 1 and V of i are in LDS, K of i + 2 and V of i + 1 in
+    // registers on their way there, K of i + 3 and V of i + 2 on their way from memory.
+    // What a group's page and scales are lies in LDS, kRef tiles from tile ref0 on.
+    if (t0 < t1) {
+      if (tid == 0) odd = 0;
+      constexpr int kRef = 64;
+      struct Refs {
+        int32_t id[4 * kRef];
+        float k[Q8 ? 4 * kRef : 4], l[Q8 ? 4 * kRef : 4], u[Q8 ? 4 * kRef : 4];
+      };
+      __shared__ __attribute__((aligned(16))) Refs refs;
+      int ref0 = t0;
+      auto refer_pages = [&](int tile) {  // the thread's group's page, or -1
+        ref0 = tile;
+        int id = -1;
+        if (tid < 4 * kRef) {
+          const int key = walk.group(4 * tile + tid) * 16;
+          id = table[min(key, r.len - 1) >> p.c.shift];
+          const bool is = (uint32_t)id < (uint32_t)p.c.n_pages;
+          wrong |= !is && (key < r.sinks || key + 16 > walk.lo);  // others may have been given back
+          id = is ? id : -1;
+          refs.id[tid] = is ? id : (int)0x80000000;
+        }
+        return id;
+      };
+      auto refer_scales = [&](int id) {
+        if (Q8 && tid < 4 * kRef) {
+          const float k_of = p.c.k_scale[max(id, 0)], v_of = p.c.v_scale[max(id, 0)];
+          refs.k[tid] = fmaxf(id >= 0 ? k_of : 1.f, 7.888609e-31f) * p.scale_log2;  // a scale of 0 would make a masked score NaN
+          const float log_v = fminf(fmaxf(__builtin_amdgcn_logf(id >= 0 ? v_of : 1.f), -80.f), 127.f);
+          refs.l[tid] = log_v;
+          refs.u[tid] = __builtin_amdgcn_exp2f(-log_v);
+        }
+      };
+      auto load = [&](int tile, const uint8_t* pages, int64_t stride, u32x4* to, int* none) {
+        const int in = (1 << p.c.shift) - 1;
+        typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+        soff = here(soff);
+#pragma unroll
+        for (int u = 0; u < NI; ++u) {
+          const int in_tile = u * RPL + w * (64 / CG);
+          const int row = key_of(tile, in_tile >> 4) + (in_tile & 15);
+          const int id = __builtin_amdgcn_readfirstlane(refs.id[4 * (tile - ref0) + (in_tile >> 4)]);
+          const WNW_GLOBAL uint8_t* at = gptr<uint8_t>(pages) + ((int64_t)(id & 0x7fffffff) * stride + (row & in) * GB);
+          if constexpr (Q8) {
+            const u32x2_t x0 = *(const WNW_GLOBAL u32x2_t*)(at + soff), x1 = *(const WNW_GLOBAL u32x2_t*)(at + (soff + GB / 2));
+            to[u] = u32x4{x0[0], x0[1], x1[0], x1[1]};
+          } else {
+            to[u] = *(const WNW_GLOBAL u32x4*)(at + soff);
+          }
+          none[u] = id;
+        }
+      };
+      int vgone[NI];
+      auto load_k = [&](int tile) { load(tile, p.c.k, p.c.k_stride, kr, gone); };
+      auto load_v = [&](int tile) { load(tile, p.c.v, p.c.v_stride, vr, vgone); };
+      auto clear_k = [&]() {
+#pragma unroll
+        for (int u = 0; u < NI; ++u)
+          if (gone[u] < 0) kr[u] = u32x4{0, 0, 0, 0};
+      };
+      auto clear_v = [&](int tile) {
+        int any = key_of(tile, 3) + 16 > r.len;
+#pragma unroll
+        for (int u = 0; u < NI; ++u) any |= vgone[u] < 0;
+        if (any) {
+#pragma unroll
+          for (int u = 0; u < NI; ++u) {
+            const int row = key_of(tile, (u * RPL + w * (64 / CG)) >> 4) + ((u * RPL + srow) & 15);
+            if (vgone[u] < 0 || row >= r.len) vr[u] = u32x4{0, 0, 0, 0};
+          }
+        }
+        even(tile);
+      };
+      constexpr int kAheadK = 2, kAheadV = 3;  // steps that K's and V's operands are read ahead of their products
+      // what the staging of K's tile and of V's writes to LDS, in kPut pieces each
+      constexpr int kPut = NI * (Q8 ? 2 : 1);
+      auto put_k = [&](int tile, int piece) {
+        const int u = Q8 ? piece / 2 : piece;
+        constexpr int kRot = RPL % CH;
+        const uint32_t kx = kRot ? ((u * kRot) % CH) * 16 : 0;
+        uint8_t* kd = lds + (tile & 1) * 2 * TB + u * RPL * RB;
+        if constexpr (Q8) {
+          if (piece % 2 == 0)
+            *(u32x4*)(kd + (kput ^ kx)) = e4m3x8<T>(kr[u][0], kr[u][1]);
+          else
+            *(u32x4*)(kd + (kput ^ kx ^ kHalf)) = e4m3x8<T>(kr[u][2], kr[u][3]);
+        } else {
+          *(u32x4*)(kd + (kput ^ kx)) = kr[u];
+        }
+      };
+      auto put_v = [&](int tile, int piece) {
+        const int u = Q8 ? piece / 2 : piece;
+        uint8_t* vd = lds + (tile & 1) * 2 * TB + TB + u * RPL * RB;
+        if constexpr (Q8) {
+          if (piece % 2 == 0)
+            *(u32x4*)(vd + vput) = e4m3x8<VT>(vr[u][0], vr[u][1]);
+          else
+            *(u32x4*)(vd + (vput ^ kHalf)) = e4m3x8<VT>(vr[u][2], vr[u][3]);
+        } else {
+          *(u32x4*)(vd + vput) = vr[u];
+        }
+      };
+      auto put_all = [&](auto put, int tile) {
+#pragma unroll
+        for (int piece = 0; piece < kPut; ++piece) put(tile, piece);
+      };
+      {
+        const int id = refer_pages(t0);
+        __syncthreads();
+        u32x4 first_k[NI];
+        int first_gone[NI];
+        load(t0, p.c.k, p.c.k_stride, first_k, first_gone);
+        load_v(t0);
+        load_k(t0 + 1);
+        refer_scales(id);
+#pragma unroll
+        for (int u = 0; u < NI; ++u) {  // K of t0 by way of kr
+          const u32x4 x = kr[u];
+          const int none = gone[u];
+          kr[u] = first_k[u];
+          gone[u] = first_gone[u];
+          first_k[u] = x;
+          first_gone[u] = none;
+        }
+        clear_k();
+        put_all(put_k, t0);
+        clear_v(t0);
+        put_all(put_v, t0);
+        load_v(t0 + 1);
+#pragma unroll
+        for (int u = 0; u < NI; ++u) {
+          kr[u] = first_k[u];
+          gone[u] = first_gone[u];
+        }
+        clear_k();
+        put_all(put_k, t0 + 1);
+        load_k(t0 + 2);
+      }
+      __syncthreads();
+      // the score's worth in the exponent, V's scale and what undoes it, of a tile's groups
+      f32x4 ck, lv, un;
+      auto numbers = [&](int i) {
+        const int at = 4 * (i - ref0);
+        ck = Q8 ? *(const f32x4*)(refs.k + at) : f32x4{p.scale_log2, p.scale_log2, p.scale_log2, p.scale_log2};
+        lv = Q8 ? *(const f32x4*)(refs.l + at) : f32x4{0.f, 0.f, 0.f, 0.f};
+        un = Q8 ? *(const f32x4*)(refs.u + at) : f32x4{1.f, 1.f, 1.f, 1.f};
+      };
+      auto scores = [&](int i, f32x16* s) {
+        const uint8_t* kt = lds + (i & 1) * 2 * TB;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) s[mt] = f32x16{};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) s[mt] = mma32<T>(*(const u32x4*)(kt + (kget ^ 32 * kk) + mt * 32 * RB), qr[kk], s[mt]);
+      };
+      auto most = [&](const f32x16* s) {
+        float mx = m;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          float y = s[b >> 1][8 * (b & 1)];
+#pragma unroll
+          for (int e = 1; e < 8; ++e) y = fmaxf(y, s[b >> 1][8 * (b & 1) + e]);
+          mx = fmaxf(mx, y * ck[b]);
+        }
+        return mx;
+      };
+      const int wlate = walk.place_of(wlast - r.window);
+      float mx = m;
+      // tile i, whose scores s are there; next: the next one's
+      auto turn = [&](int i) {
+        __syncthreads();
+        if (i + 3 >= ref0 + kRef) {
+          refer_scales(refer_pages(i));
+          __syncthreads();
+        }
+      };
+      auto use = [&](int i, f32x16* s, f32x16* next) {
+          turn(i);
+          const float f = __builtin_amdgcn_exp2f(m - mx);
+          const bool grown = __ballot(mx > m) != 0;
+          m = mx;
+          l *= f;
+          // Each step below is a product or two and the vector instructions that run in their
+          // shadow; operands from LDS are read a step ahead.
+          __builtin_amdgcn_sched_barrier(0);
+          u32x4 pb[4], pc[kTwo ? 4 : 1];
+          const uint8_t* vt = lds + (i & 1) * 2 * TB + TB;
+          constexpr int kSteps = 4 * DT, kHalfway = kSteps / 2;
+          u32x4 va[kAheadV + 1];
+          auto read_v = [&](int t) {
+            const int b = t / DT, dt = t % DT;
+            const uint64_t v0 = VO::read_tr(vt + (vget ^ 64 * dt) + 16 * b * RB);
+            const uint64_t v1 = VO::read_tr(vt + (vget ^ 64 * dt) + (16 * b + 8) * RB);
+            va[t % (kAheadV + 1)] = u32x4{(uint32_t)v0, (uint32_t)(v0 >> 32), (uint32_t)v1, (uint32_t)(v1 >> 32)};
+          };
+          {
+            const uint8_t* kt = lds + ((i + 1) & 1) * 2 * TB;
+            u32x4 ka[kAheadK + 1][2];
+            auto read = [&](int kk) {
+#pragma unroll
+              for (int mt = 0; mt < 2; ++mt) ka[kk % (kAheadK + 1)][mt] = *(const u32x4*)(kt + (kget ^ 32 * kk) + mt * 32 * RB);
+            };
+#pragma unroll
+            for (int kk = 0; kk < kAheadK; ++kk) read(kk);
+            constexpr int kEach = 32 / KK;  // of the lane's weights to a step
+            float sum = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+              if (kk + kAheadK < KK) read(kk + kAheadK);
+              if (kk == KK - 1) {
+#pragma unroll
+                for (int t = 0; t < kAheadV; ++t) read_v(t);
+              }
+#pragma unroll
+              for (int mt = 0; mt < 2; ++mt) next[mt] = mma32<T>(ka[kk % (kAheadK + 1)][mt], qr[kk], kk == 0 ? f32x16{} : next[mt]);
+              const int b = kk * kEach / 8;
+              const float off = lv[b] - m + kBias;
+#pragma unroll
+              for (int j = kk * kEach % 8 / 2; j < (kk * kEach % 8 + kEach) / 2; ++j) {
+                const float y0 = __builtin_amdgcn_exp2f(fmaf(s[b >> 1][8 * (b & 1) + 2 * j], ck[b], off));
+                const float y1 = __builtin_amdgcn_exp2f(fmaf(s[b >> 1][8 * (b & 1) + 2 * j + 1], ck[b], off));
+                sum += y0 + y1;
+                if constexpr (kTwo) {
+                  const uint32_t u0 = __float_as_uint(y0), u1 = __float_as_uint(y1);
+                  pb[b][j] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);  // the upper part cut off, what is left rounded
+                  pc[b][j] = VO::pack2(y0 - __uint_as_float(u0 & 0xffff0000u), y1 - __uint_as_float(u1 & 0xffff0000u));
+                } else {
+                  pb[b][j] = VO::pack2(y0, y1);
+                }
+              }
+              if ((kk + 1) * kEach % 8 == 0) {
+                l = Q8 ? fmaf(sum, un[b], l) : l + sum;
+                sum = 0.f;
+                asm volatile("" : "+v"(pb[b]), "+v"(l));  // here, not where they are used
+                if constexpr (kTwo) asm volatile("" : "+v"(pc[b]));
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+          if (grown) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
+          }
+          numbers(i + 1);
+          if (!all_see(i + 1, wfirst, wlate)) hide(i + 1, wlate, next);
+          kput = here(kput);
+          vput = here(vput);
+          float y = 0.f;
+          mx = m;
+          auto value = [&](int t) {
+            const int b = t / DT, dt = t % DT;
+            if (t + kAheadV < kSteps) read_v(t + kAheadV);
+            o[dt] = mma32<VT>(va[t % (kAheadV + 1)], pb[b], o[dt]);
+            if constexpr (kTwo) o[dt] = mma32<VT>(va[t % (kAheadV + 1)], pc[b], o[dt]);
+          };
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int t = 0; t < kHalfway; ++t) {
+            value(t);
+            constexpr int kEach = 32 / kHalfway;
+#pragma unroll
+            for (int e = t * kEach; e < (t + 1) * kEach; ++e) {
+              const float x = next[e >> 4][e & 15];
+              y = e % 8 == 0 ? x : fmaxf(y, x);
+              if (e % 8 == 7) mx = fmaxf(mx, y * ck[e / 8]);
+            }
+            asm volatile("" : "+v"(y), "+v"(mx));
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          clear_k();
+          clear_v(i + 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int t = kHalfway; t < kSteps; ++t) {
+            value(t);
+#pragma unroll
+            for (int piece = 0; piece < 2 * kPut; ++piece)
+              if (piece * kHalfway / (2 * kPut) == t - kHalfway) {
+                if (piece < kPut)
+                  put_v(i + 1, piece);
+                else
+                  put_k(i + 2, piece - kPut);
+              }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          mx = i + 1 < t1 ? max_x32(mx) : m;
+          load_v(i + 2);
+          load_k(i + 3);
+      };
+      if (busy) {
+        f32x16 s[2], next[2];
+        numbers(t0);
+        scores(t0, s);
+        if (!all_see(t0, wfirst, wlate)) hide(t0, wlate, s);
+        mx = max_x32(most(s));
+        int i = t0;
+        for (; i + 1 < t1; i += 2) {
+          use(i, s, next);
+          use(i + 1, next, s);
+        }
+        if (i < t1) use(i, s, next);
+      } else {
+        for (int i = t0; i < t1; ++i) {
+          turn(i);
+          clear_k();
+          clear_v(i + 1);
+          put_all(put_k, i + 2);
+          put_all(put_v, i + 1);
+          load_v(i + 2);
+          load_k(i + 3);
+        }
+      }
+      finish();
+    }
+  } else if (t0 < t1) {
     if (tid == 0) odd = 0;
     __syncthreads();
     find(t0 / kWin);
@@ -621,32 +983,7 @@ paged_prompt_kernel(PagedPromptParams p) {
         pass(i);
       }
     }
-    if (wrong) raise_device_error(p.err, WNW_DEVERR_BOUNDS);
-    if (odd) {  // what even() took out, to the rows that see it (the wave's tiles are behind a barrier)
-      auto give = [&](int from, int to) {
-#pragma unroll 1
-        for (int key = from; key < to; ++key) {
-          const uint8_t* at = paged_v_row(p.c, seg, key, GB);
-          if (!at || key >= limit || (WIN && key >= r.sinks && key < limit - r.window)) continue;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              __builtin_amdgcn_sched_barrier(0);
-              const f32x4 x = odd_quad<PE>(at, 32 * dt + 8 * j + 4 * hi);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[dt][4 * j + e] += x[e];
-            }
-        }
-      };
-      if constexpr (WIN) {
-#pragma unroll 1
-        for (int i = t0; i < t1; ++i)
-          for (int b = 0; b < 4 && !whole(i); ++b) give(key_of(i, b), min(key_of(i, b) + 16, wlast));
-      } else {
-        give(max(t0, max(first, 0) / kPpKeys) * kPpKeys, min(t1 * kPpKeys, wlast));
-      }
-    }
+    finish();
   }
   l = sum_x32(l);
   if (splits == 1) {
@@ -740,34 +1077,50 @@ struct PromptPlan {
   int64_t waves, nqb, splits, bytes;
   int64_t wgs = 0, part = 0;  // through windows: the workgroups that blocks are shared out to, bytes ahead of the partial sums
 };
-// view: the windows, null without; then a block's tiles are at most those of its rows' windows.
-static PromptPlan prompt_plan(int64_t n_seg, int64_t group, int64_t max_tokens, int64_t capacity, int64_t D,
-                              const PagedView* view) {
+static PromptPlan prompt_plan(int64_t n_seg, int64_t group, int64_t max_tokens, int64_t capacity, int64_t D) {
   PromptPlan y;
-  const int64_t rows = max_tokens * group, cus = device_cus();
-  int64_t tiles = (capacity + kPpKeys - 1) / kPpKeys;
-  if (view && !view->window && !view->sinks)
-    tiles = std::min(tiles, ((int64_t)view->window_all + view->sinks_all + 256 / group) / kPpKeys + 2);
+  const int64_t rows = max_tokens * group, cus = device_cus(), tiles = (capacity + kPpKeys - 1) / kPpKeys;
   const bool own = n_seg * ((rows + 255) / 256) <= cus && 2 * max_tokens >= capacity;
   y.waves = D == 128 && !own ? 8 : 4;
   y.nqb = (rows + 32 * y.waves - 1) / (32 * y.waves);
   const int64_t wgs = std::max<int64_t>(n_seg * y.nqb, 1), want = (y.waves == 8 ? 1 : 2) * cus;
   y.splits = std::max<int64_t>(1, std::min({want / wgs, tiles / 4, (int64_t)64}));
   if (tiles - tiles / y.splits < 8) y.splits = 1;
-  if (view) {
-    // (of windows on the device nothing is known: they may differ)
-    const bool alike = !view->window && !view->sinks;
-    if (alike ? y.splits > 1 : wgs <= std::min<int64_t>(want, kPpShared) && tiles - tiles / 4 >= 8) {
-      y.wgs = want;
-      y.part = (wgs * 8 + 255) / 256 * 256;
-      y.bytes = y.part + want * y.waves * (D / 2 + 2) * 64 * 4;
-    } else {
-      y.bytes = 0;
-    }
-    y.splits = 1;
-    return y;
-  }
   y.bytes = y.splits == 1 ? 0 : wgs * y.splits * y.waves * (D / 2 + 2) * 64 * 4;
+  return y;
+}
+
+// Through windows: a block's tiles are at most those of its rows' windows, where these are
+// known (on the device they may be anything, and differ).
+//
+// Few blocks, of tiles that may differ or be cut with a gain as above, are shared out to
+// as many workgroups as the CUs hold, of 8 waves at head_dim 128 (512 tokens after
+// 22,116 rows, two of eight heads unwindowed: 93 us, with 4 waves 97).  Others have about
+// the same walk each, and smaller workgroups walk less beyond their own rows, two at a
+// time on a CU: 4,564 tokens, head_dim 128, window 100 54 us (8 waves: 60), 500 81 (91),
+// 1,024 105 (107), but 2,000 165 (161): 8 from 25 tiles on.
+static PromptPlan window_plan(int64_t n_seg, int64_t group, int64_t max_tokens, int64_t capacity, int64_t D, const PagedView& view) {
+  const bool alike = !view.window && !view.sinks;
+  const int64_t rows = max_tokens * group, cus = device_cus();
+  int64_t tiles = (capacity + kPpKeys - 1) / kPpKeys;
+  if (alike) tiles = std::min(tiles, ((int64_t)view.window_all + view.sinks_all + 256 / group) / kPpKeys + 2);
+  PromptPlan y;
+  auto blocks = [&](int64_t waves) {
+    y.waves = waves;
+    y.nqb = (rows + 32 * waves - 1) / (32 * waves);
+    return std::max<int64_t>(n_seg * y.nqb, 1);
+  };
+  y.splits = 1;
+  y.bytes = 0;
+  const int64_t wgs = blocks(D == 128 ? 8 : 4), want = (y.waves == 8 ? 1 : 2) * cus;
+  const int64_t most = alike ? std::min(want / wgs, tiles / 4) : wgs <= std::min<int64_t>(want, kPpShared) ? 4 : 1;
+  if (most > 1 && tiles - tiles / most >= 8) {
+    y.wgs = want;
+    y.part = (wgs * 8 + 255) / 256 * 256;
+    y.bytes = y.part + want * y.waves * (D / 2 + 2) * 64 * 4;
+  } else {
+    blocks(D == 128 && tiles > 24 ? 8 : 4);
+  }
   return y;
 }
 
@@ -805,7 +1158,8 @@ static int64_t prompt_workspace(const wnw_paged_cache* cache, int64_t group, int
   if (paged_cache_of(cache, &c)) return -1;
   if (max_tokens == 0) return 0;
   if (max_tokens * group <= kFewRows) return wnw_paged_decode_workspace_bytes(cache->n_seg, max_tokens * group, cache->head_dim);
-  return prompt_plan(cache->n_seg, group, max_tokens, c.capacity, cache->head_dim, view).bytes;
+  const int64_t N = cache->n_seg, D = cache->head_dim;
+  return (view ? window_plan(N, group, max_tokens, c.capacity, D, *view) : prompt_plan(N, group, max_tokens, c.capacity, D)).bytes;
 }
 
 static int prompt_attn(const wnw_paged_cache* cache, const int32_t* seg_len, const void* q, void* out, const int64_t* strides,
@@ -832,7 +1186,7 @@ static int prompt_attn(const wnw_paged_cache* cache, const int32_t* seg_len, con
   if (most * group <= kFewRows)
     return paged_decode_launch(cache, seg_len, q, out, strides, p.t, view, group, scale, dtype, workspace, workspace_bytes, stream);
   WNW_CHECK_ARG(most * group < (1ll << 30), "too many query rows");
-  const PromptPlan y = prompt_plan(N, group, most, p.c.capacity, D, view);
+  const PromptPlan y = view ? window_plan(N, group, most, p.c.capacity, D, *view) : prompt_plan(N, group, most, p.c.capacity, D);
   WNW_CHECK_ARG(N * y.nqb < (1ll << 23), "too many segments and tokens for one call");
   WNW_CHECK_ARG(y.bytes == 0 || (workspace && workspace_bytes >= y.bytes), "workspace too small: %lld bytes, %lld needed",
                 (long long)workspace_bytes, (long long)y.bytes);
