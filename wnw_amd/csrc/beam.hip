@@ -97,10 +97,32 @@ __device__ __forceinline__ float max_row16(float x) {
   x = dpp_max<0x141>(x);  // row_half_mirror
   return dpp_max<0x140>(x);
 }
-__device__ __forceinline__ double wave_sum64(double x) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
-  return x;
+// Maximum and sum over the wave, without LDS
+__device__ __forceinline__ float beam_max(float x) { return max_x32(max_x16(max_row16(x))); }
+__device__ __forceinline__ double f64_of(uint32_t lo, uint32_t hi) {
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int kCtrl>
+__device__ __forceinline__ double dpp_sum64(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  return x + f64_of(__builtin_amdgcn_mov_dpp((int)(uint32_t)u, kCtrl, 0xf, 0xf, false),
+                    __builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), kCtrl, 0xf, 0xf, false));
+}
+__device__ __forceinline__ double beam_sum64(double x) {
+  x = dpp_sum64<0xB1>(x);
+  x = dpp_sum64<0x4E>(x);
+  x = dpp_sum64<0x141>(x);
+  x = dpp_sum64<0x140>(x);
+  {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)u, (uint32_t)u, false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+    x = f64_of(lo[0], hi[0]) + f64_of(lo[1], hi[1]);
+  }
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const auto lo = __builtin_amdgcn_permlane32_swap((uint32_t)u, (uint32_t)u, false, false);
+  const auto hi = __builtin_amdgcn_permlane32_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+  return f64_of(lo[0], hi[0]) + f64_of(lo[1], hi[1]);
 }
 
 template <typename T>
@@ -140,7 +162,7 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(BeamParams p) {
     for (int i = 0; i < N; ++i) s += __builtin_amdgcn_exp2f((x[u][i] - m) * kBeamLog2e);
     sum += (double)s;
   }
-  sum = wave_sum64(sum);
+  sum = beam_sum64(sum);
   if (lane == 0) {
     p.part_max[at] = m;
     p.part_sum[at] = sum;
@@ -247,21 +269,33 @@ __global__ __launch_bounds__(kBeamThreads) void beam_pick_kernel(BeamParams p) {
   constexpr int N = Ge::kVec, E = Ge::kEach;
   __shared__ BeamShared sh;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int W = p.W, k = p.k, groups = p.tasks * kBeamGroups, chunks = (groups + 63) / 64, n = W * chunks;
+  const int W = p.W, k = p.k, groups = p.tasks * kBeamGroups, chunks = (groups + 63) / 64;
   // Chunk c of the sample's: 64 groups of beam c / chunks.  A wave takes every 16th, and
   // has the first of them on their way before anything else.
-  auto place_of = [&](int c) {
-    const int w = c / chunks;
-    return BeamPlace{w, (c - w * chunks) * 64 + lane};
+  struct Chunk {
+    int w, c;  // the beam, and the chunk of its own
   };
+  const int more_w = kBeamWaves / chunks, more_c = kBeamWaves % chunks;
+  const Chunk chunk0 = {wave / chunks, wave % chunks};
+  auto next_of = [&](Chunk x) {
+    x.w += more_w;
+    x.c += more_c;
+    if (x.c >= chunks) {
+      x.c -= chunks;
+      ++x.w;
+    }
+    return x;
+  };
+  auto place_of = [&](const Chunk& x) { return BeamPlace{x.w, x.c * 64 + lane}; };
   auto max_of = [&](const BeamPlace& x) {
     return x.group < groups ? p.group_max[((int64_t)b * W + x.w) * groups + x.group] : -INFINITY;
   };
   float held[kBeamHeld];
+  Chunk rest = chunk0;  // the first that is not held
 #pragma unroll
   for (int i = 0; i < kBeamHeld; ++i) {
-    const int c = wave + i * kBeamWaves;
-    held[i] = c < n ? max_of(place_of(c)) : -INFINITY;
+    held[i] = rest.w < W ? max_of(place_of(rest)) : -INFINITY;
+    rest = next_of(rest);
   }
   // the rows' sums
   for (int w = wave; w < W; w += kBeamWaves) {
@@ -282,8 +316,8 @@ __global__ __launch_bounds__(kBeamThreads) void beam_pick_kernel(BeamParams p) {
             ps[i] * (double)__builtin_amdgcn_exp2f((y - now) * kBeamLog2e);
         m = now;
       }
-      const float most = wave_max(m);
-      s = wave_sum64(s * (double)__builtin_amdgcn_exp2f((m - most) * kBeamLog2e));
+      const float most = beam_max(m);
+      s = beam_sum64(s * (double)__builtin_amdgcn_exp2f((m - most) * kBeamLog2e));
       lse = (double)most + log(s);
       bad |= !(s < (double)INFINITY);
       if (s == 0.0) state = 0;
@@ -309,15 +343,16 @@ __global__ __launch_bounds__(kBeamThreads) void beam_pick_kernel(BeamParams p) {
   // maxima, or of 64 rows' of 16 lanes, by the totals' upper words, of which 20 bits are enough.
   BeamKey keys[kBeamHeld];
   uint32_t high = 0;
+  Chunk x = chunk0;
 #pragma unroll
   for (int i = 0; i < kBeamHeld; ++i) {
-    const int c = wave + i * kBeamWaves;
     keys[i] = kBeamNone;
-    if (c < n) keys[i] = key_of(place_of(c), held[i]);
+    if (x.w < W) keys[i] = key_of(place_of(x), held[i]);
     high = max(high, (uint32_t)(keys[i].total >> 32));
+    x = next_of(x);
   }
-  for (int c = wave + kBeamHeld * kBeamWaves; c < n; c += kBeamWaves) {
-    const BeamPlace at = place_of(c);
+  for (x = rest; x.w < W; x = next_of(x)) {
+    const BeamPlace at = place_of(x);
     high = max(high, (uint32_t)(key_of(at, max_of(at)).total >> 32));
   }
   high = max(high, (uint32_t)__builtin_amdgcn_mov_dpp((int)high, 0xB1, 0xf, 0xf, false));
@@ -349,8 +384,8 @@ __global__ __launch_bounds__(kBeamThreads) void beam_pick_kernel(BeamParams p) {
   };
 #pragma unroll
   for (int i = 0; i < kBeamHeld; ++i) offer(keys[i]);
-  for (int c = wave + kBeamHeld * kBeamWaves; c < n; c += kBeamWaves) {
-    const BeamPlace at = place_of(c);
+  for (x = rest; x.w < W; x = next_of(x)) {
+    const BeamPlace at = place_of(x);
     offer(key_of(at, max_of(at)));
   }
   __syncthreads();
@@ -360,8 +395,8 @@ __global__ __launch_bounds__(kBeamThreads) void beam_pick_kernel(BeamParams p) {
   else
     beam_rounds(sh, k, [&](const BeamKey& last) {
       BeamKey first = kBeamNone;
-      for (int c = wave; c < n; c += kBeamWaves) {
-        const BeamPlace at = place_of(c);
+      for (Chunk x = chunk0; x.w < W; x = next_of(x)) {
+        const BeamPlace at = place_of(x);
         const BeamKey key = key_of(at, max_of(at));
         if (ahead(last, key)) first = ahead_of(key, first);
       }

@@ -20,7 +20,7 @@ namespace wnw {
 static constexpr int kPlanThreads = 1024;
 static constexpr int kPlanWaves = kPlanThreads / 64;
 static constexpr int kPlanPer = 16;          // pages of a thread at a time
-static constexpr int kPlanCopy = 8192;       // counts that another workgroup of the plan copies
+static constexpr int kPlanCopy = 4096;       // counts that another workgroup of the plan copies
 static constexpr int kMaxSamples = 8192;     // of a fork
 
 // A workspace, in 32-bit words: the head, then lists.
@@ -54,6 +54,7 @@ struct CompactParams {
   PagesParams g;
   int32_t* moves;
   int32_t* used;
+  int32_t range;
 };
 
 // Where the lists of a workspace begin
@@ -61,7 +62,7 @@ __device__ __forceinline__ int32_t* ws_fresh(const PagesParams& g) { return g.ws
 __device__ __forceinline__ int32_t* ws_place(const PagesParams& g) { return ws_fresh(g) + g.n_pages; }  // [segments] or [n_pages]
 
 struct PlanShared {
-  int wave[kPlanWaves];
+  int wave[kPlanWaves], second[kPlanWaves];
 };
 // x summed over the threads before, *all over all of them
 __device__ __forceinline__ int plan_scan(PlanShared& sh, int x, int* all) {
@@ -84,6 +85,28 @@ __device__ __forceinline__ int plan_scan(PlanShared& sh, int x, int* all) {
   }
   *all = sum;
   return before + incl - x;
+}
+
+// Sums of two numbers over all threads
+__device__ __forceinline__ void plan_sums(PlanShared& sh, int* a, int* b) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    *a += __shfl_xor(*a, o);
+    *b += __shfl_xor(*b, o);
+  }
+  __syncthreads();
+  if (lane == 0) {
+    sh.wave[w] = *a;
+    sh.second[w] = *b;
+  }
+  __syncthreads();
+  *a = *b = 0;
+#pragma unroll
+  for (int i = 0; i < kPlanWaves; ++i) {
+    *a += sh.wave[i];
+    *b += sh.second[i];
+  }
 }
 
 // The counts of 16 pages from `at` on; -1 past the pool
@@ -109,15 +132,15 @@ __device__ __forceinline__ Counts plan_counts(const PagesParams& g, int at) {
   return c;
 }
 
-// The first `need` free pages into the fresh list; whether there are as many.
-__device__ __forceinline__ bool plan_fresh(const PagesParams& g, PlanShared& sh, int need) {
+// The first `need` free pages into the fresh list; whether there are as many.  c: the
+// thread's counts of the pool's first pages, on their way since before the need was known.
+__device__ __forceinline__ bool plan_fresh(const PagesParams& g, PlanShared& sh, int need, Counts c) {
   int have = 0;
   for (int base = 0; base < g.n_pages && have < need; base += kPlanThreads * kPlanPer) {
     const int at = base + (int)threadIdx.x * kPlanPer;
-    Counts c;
     int mine = 0;
     if (at < g.n_pages) {
-      c = plan_counts(g, at);
+      if (base > 0) c = plan_counts(g, at);
 #pragma unroll
       for (int i = 0; i < kPlanPer; ++i) mine += c.n[i] == 0;
     }
@@ -138,8 +161,14 @@ __device__ __forceinline__ bool plan_fresh(const PagesParams& g, PlanShared& sh,
 
 // The plan's other workgroups copy the counts
 __device__ __forceinline__ void plan_copy(const PagesParams& g) {
-  const int from = ((int)blockIdx.x - 1) * kPlanCopy, to = min(from + kPlanCopy, g.n_pages);
-  for (int i = from + (int)threadIdx.x; i < to; i += kPlanThreads) g.new_refs[i] = g.refs[i];
+  constexpr int N = kPlanCopy / kPlanThreads;
+  const int from = ((int)blockIdx.x - 1) * kPlanCopy + (int)threadIdx.x;
+  int32_t x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = g.refs[min(from + i * kPlanThreads, g.n_pages - 1)];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (from + i * kPlanThreads < g.n_pages) g.new_refs[from + i * kPlanThreads] = x[i];
 }
 // A table entry: the page, or -1
 __device__ __forceinline__ int entry_of(const PagesParams& g, int e, bool tell) {
@@ -170,6 +199,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(ForkParams p) {
     return;
   }
   const int tid = threadIdx.x, rows = g.max_blocks << g.shift;
+  const Counts counts = plan_counts(g, tid * kPlanPer);
   bool good = true;
   for (int i = tid; i < p.n_old; i += kPlanThreads) {
     first[i] = 0x7fffffff;
@@ -209,7 +239,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(ForkParams p) {
       if (s < segs) ws_place(g)[s] = mine ? at : -1;
       need += all;
     }
-    room = plan_fresh(g, sh, need);
+    room = plan_fresh(g, sh, need, counts);
     for (int i = tid; i < p.n_old; i += kPlanThreads) {
       fork_first(p)[i] = first[i];
       fork_first(p)[p.n_old + i] = count[i];
@@ -301,10 +331,37 @@ __global__ __launch_bounds__(kPlanThreads) void reserve_plan_kernel(ReserveParam
     return;
   }
   const int tid = threadIdx.x, rows = g.max_blocks << g.shift;
+  const Counts counts = plan_counts(g, tid * kPlanPer);
   bool good = true, room = true;
   if (tid == 0) total = 0;
   __syncthreads();
   // a segment's needs: of one thread where they are a block or two, of a wave otherwise
+  if (!p.wide && g.n_seg <= kPlanThreads) {  // (a decode step's call: nothing goes through memory)
+    __shared__ int bad;
+    if (tid == 0) bad = 0;
+    __syncthreads();
+    int mine = 0;
+    if (tid < g.n_seg) {
+      const ReserveSeg r = reserve_seg(p, tid);
+      const int b0 = r.n >> g.shift;
+      if (!r.good || r.end > rows) {
+        atomicOr(&bad, r.good ? 2 : 1);
+      } else if (r.end > r.n) {
+        const int e0 = g.table[tid * g.stride + b0], e1 = g.table[tid * g.stride + min(b0 + 1, g.max_blocks - 1)];
+        mine = (entry_of(g, e0, false) < 0) + ((b0 + 1) << g.shift < r.end && entry_of(g, e1, false) < 0);
+      }
+    }
+    int need;
+    const int before = plan_scan(sh, mine, &need);
+    good = !(bad & 1);
+    room = !(bad & 2) && need <= g.n_pages;
+    if (good && room) {
+      if (tid < g.n_seg) ws_place(g)[tid] = before;
+      room = plan_fresh(g, sh, need, counts);
+    }
+    plan_end(g, good, room);
+    return;
+  }
   if (p.wide) {
     const int lane = tid & 63;
     for (int s = tid >> 6; s < g.n_seg; s += kPlanWaves) {
@@ -346,7 +403,7 @@ __global__ __launch_bounds__(kPlanThreads) void reserve_plan_kernel(ReserveParam
       if (s < g.n_seg) ws_place(g)[s] = need + before;
       need += all;
     }
-    room = plan_fresh(g, sh, need);
+    room = plan_fresh(g, sh, need, counts);
   }
   plan_end(g, good, room);
 }
@@ -401,64 +458,70 @@ __global__ __launch_bounds__(256) void reserve_kernel(ReserveParams p) {
 __device__ __forceinline__ int32_t* compact_page(const PagesParams& g) { return ws_place(g) + g.n_pages; }
 __device__ __forceinline__ int32_t* compact_refs(const PagesParams& g) { return compact_page(g) + g.n_pages / 2 + 1; }
 
+// A workgroup for `range` pages, which counts the used ones of the whole pool for itself:
+// how many there are, U, how many below its pages, and (where these lie past U) below U.
 __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactParams p) {
   __shared__ PlanShared sh;
   const PagesParams& g = p.g;
-  const int tid = threadIdx.x;
-  int used = 0;
-  for (int base = 0; base < g.n_pages; base += kPlanThreads * kPlanPer) {
-    const int at = base + tid * kPlanPer;
-    int mine = 0, all;
-    if (at < g.n_pages) {
-      const Counts c = plan_counts(g, at);
-#pragma unroll
-      for (int i = 0; i < kPlanPer; ++i) mine += c.n[i] > 0;
-    }
-    plan_scan(sh, mine, &all);
-    used += all;
-  }
-  int holes = 0, movers = 0;
-  for (int base = 0; base < g.n_pages; base += kPlanThreads * kPlanPer) {
-    const int at = base + tid * kPlanPer;
-    Counts c;
-    int h = 0, m = 0, all;
-    if (at < g.n_pages) {
-      c = plan_counts(g, at);
+  const int tid = threadIdx.x, from = (int)blockIdx.x * p.range, to = min(from + p.range, g.n_pages);
+  const Counts head = plan_counts(g, tid * kPlanPer);
+  auto count = [&](int x, int* below) {  // used pages, and those below page x
+    int all = 0, low = 0;
+    for (int at = tid * kPlanPer; at < g.n_pages; at += kPlanThreads * kPlanPer) {
+      const Counts c = at < kPlanThreads * kPlanPer ? head : plan_counts(g, at);
 #pragma unroll
       for (int i = 0; i < kPlanPer; ++i) {
-        h += at + i < used && c.n[i] <= 0;
-        m += at + i >= used && c.n[i] > 0;
+        all += c.n[i] > 0;
+        low += c.n[i] > 0 && at + i < x;
       }
     }
-    int hr = holes + plan_scan(sh, h, &all);
-    holes += all;
-    int mr = movers + plan_scan(sh, m, &all);
-    movers += all;
-    if (at < g.n_pages) {
-#pragma unroll
-      for (int i = 0; i < kPlanPer; ++i) {
-        if (at + i < used && c.n[i] <= 0) {
-          ws_fresh(g)[hr] = at + i;
-          ws_place(g)[at + i] = hr++;
+    plan_sums(sh, &all, &low);
+    *below = low;
+    return all;
+  };
+  int before, under;
+  const int used = count(from, &before);
+  if (from > used)
+    count(used, &under);
+  else
+    under = -1;  // found on the way
+  int at_u = under;
+  // its pages, 1,024 at a time
+  int seen = before;  // used ones below the thread's
+  for (int base = from; base < to; base += kPlanThreads) {
+    const int i = base + tid, c = i < to ? g.refs[i] : 0;
+    int all;
+    const int mine = seen + plan_scan(sh, c > 0, &all);
+    if (at_u < 0 && base <= used && used < base + kPlanThreads) {  // uniform
+      __shared__ int found;
+      if (i == used) found = mine;
+      __syncthreads();
+      at_u = found;
+    }
+    if (i < to) {
+      if (i < used) {
+        if (c <= 0) {
+          ws_fresh(g)[i - mine] = i;
+          ws_place(g)[i] = i - mine;
         }
-        if (at + i >= used && at + i < g.n_pages) {
-          const bool moves = c.n[i] > 0;
-          if (moves) {
-            compact_page(g)[mr] = at + i;
-            compact_refs(g)[mr] = c.n[i];
-          }
-          ws_place(g)[at + i] = moves ? mr++ : -1;
+      } else {
+        const int rank = mine - at_u;
+        if (c > 0) {
+          compact_page(g)[rank] = i;
+          compact_refs(g)[rank] = c;
         }
+        ws_place(g)[i] = c > 0 ? rank : -1;
       }
     }
+    seen += all;
   }
-  if (tid == 0) {
+  if (blockIdx.x == gridDim.x - 1 && tid == 0) {
     g.ws[kUsed] = used;
-    g.ws[kMoves] = movers;
+    g.ws[kMoves] = at_u < 0 ? 0 : used - at_u;
   }
 }
 
-// Workgroups of the segments, then of 1,024 pages each
+// Workgroups of the segments, then of 256 pages each
 __global__ __launch_bounds__(256) void compact_kernel(CompactParams p) {
   const PagesParams& g = p.g;
   const int tid = threadIdx.x, used = g.ws[kUsed], movers = g.ws[kMoves];
@@ -474,9 +537,9 @@ __global__ __launch_bounds__(256) void compact_kernel(CompactParams p) {
     }
     return;
   }
-  const int from = ((int)blockIdx.x - g.n_seg) * 1024;
-  if (from == 0 && tid == 0) *p.used = used;
-  for (int i = from + tid; i < min(from + 1024, g.n_pages); i += 256) {
+  const int i = ((int)blockIdx.x - g.n_seg) * 256 + tid;
+  if (i == 0) *p.used = used;
+  if (i < g.n_pages) {
     if (i < g.n_pages / 2) {
       const bool is = i < movers;
       p.moves[3 * i] = is ? compact_page(g)[i] : -1;
@@ -643,8 +706,11 @@ extern "C" int wnw_paged_compact(const int32_t* page_table, int64_t table_stride
   WNW_CHECK_ARG(used && (n_pages < 2 || moves), "null pointer argument");
   p.moves = moves;
   p.used = used;
-  hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, p);
-  const unsigned blocks = (unsigned)(n_seg + std::max<int64_t>((n_pages + 1023) / 1024, 1));
+  // each of at most 64 workgroups reads all counts: from its L2
+  p.range = (int32_t)(((n_pages + 63) / 64 + kPlanThreads - 1) / kPlanThreads * kPlanThreads);
+  const unsigned plan = n_pages ? (unsigned)((n_pages + p.range - 1) / p.range) : 1;
+  hipLaunchKernelGGL(compact_plan_kernel, dim3(plan), dim3(kPlanThreads), 0, (hipStream_t)stream, p);
+  const unsigned blocks = (unsigned)(n_seg + std::max<int64_t>((n_pages + 255) / 256, 1));
   hipLaunchKernelGGL(compact_kernel, dim3(blocks), dim3(256), 0, (hipStream_t)stream, p);
   WNW_CHECK_HIP(hipGetLastError(), "compact launch");
   return WNW_OK;
