@@ -361,7 +361,7 @@ paged_prompt_kernel(PagedPromptParams p) {
     pid = pid_next;
     ks = ks_next;
     vs = vs_next;
-    find(window + 1);
+    if (!WIN || (window + 1) * kWin <= t1 + 1) find(window + 1);  // (short walks end before: no round trip for nothing)
   };
   u32x4 kr[NI], vr[NI];
   int gone[NI];  // rows of kr and vr in no page: negative
