@@ -241,3 +241,43 @@ def test_both_ways_into_a_call(gpu, monkeypatch):
     general = [beam_select(x, s), beam_select(x, s, 9, done=done, end=7), beam_select(x.float(), s, 1)]
     _clean()
     assert all(torch.equal(a, b) for n, g in zip(native, general) for a, b in zip(n, g))
+
+
+def test_on_another_stream(gpu):
+    """A selection on a stream of the caller's, behind work there that writes its logits."""
+    x, s = _logits(gpu, 3, 5, 12001, BF, 12)
+    want = beam_select(x, s, 7)
+    stream = torch.cuda.Stream()
+    for _ in range(3):
+        late = torch.zeros_like(x)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(2_000_000)
+            late.copy_(x)
+            got = beam_select(late, s, 7)
+        stream.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    _clean()
+
+
+def test_rows_far_apart(gpu):
+    """Samples and beams whose elements lie past 32 bits of offset."""
+    room = torch.empty(2 ** 32 + 2 ** 21, dtype=FP, device=gpu)
+    for strides in ((2 ** 32, 5001), (5001, 2 ** 32)):
+        x = room.as_strided((2, 2, 5000), (*strides, 1))
+        y, s = _logits(gpu, 2, 2, 5000, FP, 13)
+        x.copy_(y)
+        got = beam_select(x, s, 6)
+        _clean()
+        _check(y, s, 6, got)
+
+
+def test_numbers_that_are_none(gpu):
+    """k and end that are not whole numbers are refused; numpy's are taken."""
+    import numpy as np
+    x, s = _logits(gpu, 2, 3, 50, BF, 1)
+    for kw in (dict(k=3.0), dict(k="3"), dict(end=1.5), dict(end=None)):
+        with pytest.raises((_lib.WnwError, TypeError)):
+            beam_select(x, s, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(beam_select(x, s, np.int64(3)), beam_select(x, s, 3)))
+    _clean()

@@ -393,3 +393,20 @@ def test_prompt_blocks_of_different_lengths(gpu, q8, dtype, D, G, new, old):
                 room[at:at + n] = out[at:at + n]
             at += n
         _prompt_check(c, q, room, new, window, sinks, D ** -0.5)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (FP, 128), (BF, 64)])
+def test_prompt_long_walks(gpu, dtype, D):
+    """Blocks that walk more tiles than a workgroup keeps the pages of, in a call that is not cut."""
+    new, old, H, G = [2100], [6000], 8, 8
+    c = Cache(gpu, [8100] * H, 64, D, dtype, True, seed=D)
+    window, sinks = 5003, 37
+    _hide(c, new, window, sinks)
+    q = _q(gpu, 2100, H * G, D, dtype)
+    out = paged_prompt_attn(q, *c.args(), _cu(new, gpu), D ** -0.5, window=window, sinks=sinks, **c.scales())
+    _clean()
+    for s in (0, 7):
+        keep = torch.tensor([0, 1, 63, 64, 65, 1000, 1001, 2036, 2098, 2099], device=gpu)
+        pos = (6000 + keep).repeat_interleave(G)
+        place = (keep, slice(s * G, (s + 1) * G))
+        _check_rows(c, s, q[place].reshape(-1, D), out[place].reshape(-1, D), pos, window, sinks, D ** -0.5, 1)

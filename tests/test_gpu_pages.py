@@ -315,3 +315,128 @@ def test_watched_calls_are_refused(gpu):
     with pytest.raises(_lib.WnwError, match="trace"):
         make_fx(lambda r: paged_compact(table, r, 16)[0])(refs)
     _clean()
+
+
+def test_in_place_of_one_output(gpu):
+    """The table written where it is and the counts elsewhere, and the other way round."""
+    rng = random.Random(21)
+    B, H, R, M, P = 6, 2, 16, 12, 5000
+    table, lens, refs = _state(rng, B, H, R, M, P)
+    lens = [min(n, M * R - 20) for n in lens]
+    reserved, compacted = pages_ref.reserve(table, lens, refs, R, [20] * (B * H)), pages_ref.compact(table, refs, R)
+    for mine in (0, 1):
+        for call, want in ((lambda t, r, out: paged_reserve(t, _t(lens, gpu), r, R, tokens=20, out=out), reserved),
+                           (lambda t, r, out: paged_compact(t, r, R, out=out), compacted)):
+            given = _t(table, gpu), _t(refs, gpu)
+            out = tuple(x if i == mine else torch.full_like(x, 77) for i, x in enumerate(given))
+            got = call(*given, out)
+            _clean()
+            assert got[0] is out[0] and got[1] is out[1]
+            assert out[0].tolist() == want[0] and out[1].tolist() == want[1]
+            kept = given[1 - mine].tolist()  # the input that is not written
+            assert kept == (refs if mine == 0 else table)
+
+
+def test_on_another_stream(gpu):
+    """Calls on a stream of the caller's, behind work of its own that writes their inputs."""
+    rng = random.Random(22)
+    B, H, R, M, P = 5, 2, 32, 40, 3000
+    table, lens, refs = _state(rng, B, H, R, M, P)
+    parents = [4, 4, 0, 1, 1, -1, 2]
+    want = pages_ref.fork(table, lens, refs, parents, R, H, M)
+    after = pages_ref.compact(want[0], want[2], R)
+    ready = [_t(x, gpu) for x in (table, lens, refs, parents)]
+    stream = torch.cuda.Stream()
+    for _ in range(3):
+        late = [torch.zeros_like(x) for x in ready]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(2_000_000)
+            for x, y in zip(late, ready):
+                x.copy_(y)
+            new, new_len, new_refs, copies = paged_fork(*late, R, kv_heads=H)
+            packed = paged_compact(new, new_refs, R)
+        stream.synchronize()
+        assert new.tolist() == want[0] and new_len.tolist() == want[1] and new_refs.tolist() == want[2] and copies.tolist() == want[3]
+        assert packed[0].tolist() == after[0] and packed[2].tolist() == after[2]
+    _clean()
+
+
+def test_captured_fork_and_compact(gpu):
+    """A captured step that forks, copies and compacts, replayed with other parents; eager calls in between."""
+    rng = random.Random(23)
+    B, H, R, M, P = 4, 2, 16, 9, 400
+    table, lens, refs = _state(rng, B, H, R, M, P)
+    dt, dl, dr = _t(table, gpu), _t(lens, gpu), _t(refs, gpu)
+    parents = _t([0] * B, gpu)
+    k = torch.randn(P, R, 64, device=gpu).to(torch.bfloat16)
+    v = k.clone()
+
+    def step():
+        forked = paged_fork(dt, dl, dr, parents, R, kv_heads=H)
+        return (*forked, *paged_compact(forked[0], forked[2], R))
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+        paged_copy(k, v, got[3])
+    for _ in range(6):
+        now = [rng.randrange(-1, B) for _ in range(B)]
+        parents.copy_(_t(now, gpu))
+        before = k.clone()
+        graph.replay()
+        eager = step()
+        want = pages_ref.fork(table, lens, refs, now, R, H, M)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, eager))
+        assert got[0].tolist() == want[0] and got[2].tolist() == want[2] and got[3].tolist() == want[3]
+        for a, b, n in want[3]:
+            if a >= 0:
+                before[b, :n] = before[a, :n]
+        assert torch.equal(k, before) and torch.equal(v, before)
+    _clean()
+
+
+def test_most_samples(gpu):
+    """8,192 samples before and after, all going on from few parents or each from its own; 8,193 are refused."""
+    R, M, P = 16, 2, 30000
+    rng = random.Random(24)
+    table, lens, refs = _state(rng, 8192, 1, R, M, P, shared=False)
+    for parents in ([rng.randrange(8192) for _ in range(8192)], [8191] * 8192, list(range(8191, -1, -1))):
+        want = pages_ref.fork(table, lens, refs, parents, R, 1, M)
+        new, new_len, new_refs, copies = paged_fork(_t(table, gpu), _t(lens, gpu), _t(refs, gpu), _t(parents, gpu), R, kv_heads=1)
+        _clean()
+        assert new.tolist() == want[0] and new_len.tolist() == want[1] and new_refs.tolist() == want[2] and copies.tolist() == want[3]
+    with pytest.raises(_lib.WnwError, match="8192 samples"):
+        paged_fork(_t(table, gpu), _t(lens, gpu), _t(refs, gpu), _t([0] * 8193, gpu), R, kv_heads=1)
+    _clean()
+
+
+def test_copy_far_apart(gpu):
+    """Pages whose bytes lie past 32 bits of offset."""
+    P, R, D = 70001, 256, 128
+    k = torch.empty(P, R, D, dtype=torch.bfloat16, device=gpu)
+    v = torch.empty(P, R, D, dtype=torch.bfloat16, device=gpu)
+    assert k.numel() * 2 > 2 ** 32
+    g = torch.Generator(device=gpu).manual_seed(1)
+    for at in (0, 3, 69999, 70000):
+        k[at] = torch.randn(R, D, device=gpu, generator=g).to(k.dtype)
+        v[at] = torch.randn(R, D, device=gpu, generator=g).to(k.dtype)
+    far, near = (k[70000].clone(), v[70000].clone()), (k[0].clone(), v[0].clone())
+    paged_copy(k, v, _t([[70000, 3, R], [0, 69999, R]], gpu))
+    _clean()
+    assert torch.equal(k[3], far[0]) and torch.equal(v[3], far[1]) and torch.equal(k[69999], near[0]) and torch.equal(v[69999], near[1])
+
+
+def test_numbers_that_are_none(gpu):
+    """Sizes that are not whole numbers are refused; numpy's are taken."""
+    import numpy as np
+    table, lens, refs, parents = _t([[0, 1], [2, -1]], gpu), _t([20, 5], gpu), _t([1, 1, 1, 0], gpu), _t([0, 1], gpu)
+    for call in (lambda: paged_fork(table, lens, refs, parents, 16, kv_heads=1.0), lambda: paged_fork(table, lens, refs, parents, 16.0, kv_heads=1),
+                 lambda: paged_reserve(table, lens, refs, 16, tokens=1.0), lambda: paged_reserve(table, lens, refs, "16"),
+                 lambda: paged_compact(table, refs, None)):
+        with pytest.raises((_lib.WnwError, TypeError)):
+            call()
+    a, b = paged_fork(table, lens, refs, parents, np.int64(16), kv_heads=np.int32(1)), paged_fork(table, lens, refs, parents, 16, kv_heads=1)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    _clean()

@@ -5,6 +5,7 @@ forked by the parents found here (``wnw_amd.kv.pages.paged_fork``)."""
 from __future__ import annotations
 
 import ctypes
+from operator import index
 
 import torch
 from torch import Tensor
@@ -44,14 +45,14 @@ def beam_select(logits: Tensor, scores: Tensor, k: int | None = None, *, done: T
         raise _lib.WnwError(f"scores must be float32 [{B}, {W}], got {scores.dtype} {tuple(scores.shape)}")
     if done is not None and (done.dtype != torch.bool or done.shape != (B, W)):
         raise _lib.WnwError(f"done must be bool [{B}, {W}], got {done.dtype} {tuple(done.shape)}")
-    k = W if k is None else k
+    k, end = W if k is None else index(k), index(end)
     if logits.numel() and logits.stride(2) != 1 or any(logits.stride(i) < 0 for i in range(2)):
         logits = logits.clone(memory_format=torch.contiguous_format)
     scores = scores.contiguous()
     done = None if done is None else done.contiguous()
     need = int(_lib.lib().wnw_beam_workspace_bytes(B, W, V, _lib.dtype_code(logits.dtype)))
     if need < 0:
-        raise _lib.WnwError(f"{B} samples of {W} beams over {V} tokens: 1 to 64 beams, 1 to 2^25 - 1 tokens")
+        raise _lib.WnwError(f"{B} samples of {W} beams over {V} tokens: below 2^20 samples, 1 to 64 beams, 1 to 2^25 - 1 tokens")
     if not 1 <= k <= 64:
         raise _lib.WnwError(f"k must be 1 to 64, got {k}")
     dev = logits.device
