@@ -410,3 +410,84 @@ def test_prompt_long_walks(gpu, dtype, D):
         pos = (6000 + keep).repeat_interleave(G)
         place = (keep, slice(s * G, (s + 1) * G))
         _check_rows(c, s, q[place].reshape(-1, D), out[place].reshape(-1, D), pos, window, sinks, D ** -0.5, 1)
+
+
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("D", [64, 128])
+def test_offsets_past_32_bits(gpu, q8, D):
+    """Pages 3 GiB apart, tokens 2 GiB apart, through a window; calls of few rows, of many, and cut into shares."""
+    G, R, pages = 4, 256, 5
+    small = Cache(gpu, [R * (pages - 1) + 20], R, D, BF, q8, seed=21, spare=0, room=1)
+    assert small.P == pages
+    room = torch.empty(pages * (3 << 30) + (1 << 20), dtype=torch.uint8, device=gpu).view(small.k.dtype)
+    far = (3 << 30) // (1 if q8 else 2)
+    k, v = (room.as_strided((pages, R, D), (far, D, 1), i * R * D) for i in range(2))
+    for to, of in ((k, small.k), (v, small.v)):
+        (to.view(torch.uint8) if q8 else to).copy_(of.view(torch.uint8) if q8 else of)
+    q = _q(gpu, 1, G, D, BF)
+    view = dict(window=700, sinks=5)
+    args, scales = (k, v, small.table, small.seg_len), small.scales()
+    assert torch.equal(paged_decode_attn(q, *small.args(), 0.1, **view, **scales), paged_decode_attn(q, *args, 0.1, **view, **scales))
+    for new in (3, 40, 600):
+        rows = _q(gpu, new, G, D, BF)
+        want = paged_prompt_attn(rows, *small.args(), _cu([new], gpu), 0.1, **view, **scales)
+        assert torch.equal(want, paged_prompt_attn(rows, *args, _cu([new], gpu), 0.1, **view, **scales))
+        _prompt_check(small, rows, want, [new], 700, 5, 0.1)
+    for new in (3, 6):
+        wide = torch.empty((new - 1) * (1 << 30) + G * D, dtype=BF, device=gpu).as_strided((new, G, D), (1 << 30, D, 1))
+        rows = _q(gpu, new, G, D, BF)
+        wide.copy_(rows)
+        want = paged_prompt_attn(rows, *small.args(), _cu([new], gpu), 0.1, **view, **scales)
+        assert torch.equal(want, paged_prompt_attn(wide, *args, _cu([new], gpu), 0.1, **view, **scales))
+        assert torch.equal(want, paged_prompt_attn(wide, *args, _cu([new], gpu), 0.1, out=wide, **view, **scales))
+    _clean()
+
+
+@pytest.mark.parametrize("dtype,D,q8", [(BF, 128, True), (FP, 128, False), (BF, 256, False), (FP, 64, True)])
+def test_out_is_q(gpu, dtype, D, q8):
+    """The result in q's own memory: few rows, many, cut into shares and not."""
+    window = torch.tensor([ALL, 40, 333, 0], dtype=torch.int32, device=gpu)
+    for new, old in ([1, 1], [900, 5]), ([2, 3], [900, 5]), ([70, 33], [3000, 900]), ([600, 1], [0, 10]):
+        c = Cache(gpu, [n + o for n, o in zip(new, old) for _ in range(2)], 32, D, dtype, q8, seed=sum(new))
+        q = _q(gpu, sum(new), 16, D, dtype)
+        for w, z in ((64, 3), (window, 2)):
+            want = paged_prompt_attn(q, *c.args(), _cu(new, gpu), 0.1, max_tokens=max(new), window=w, sinks=z, **c.scales())
+            room = q.clone()
+            got = paged_prompt_attn(room, *c.args(), _cu(new, gpu), 0.1, max_tokens=max(new), window=w, sinks=z, out=room, **c.scales())
+            assert got is room and torch.equal(got, want)
+            _prompt_check(c, q, want, new, w, z, 0.1)
+        qd = _q(gpu, 4, 16, D, dtype)
+        want = paged_decode_attn(qd, *c.args(), 0.1, window=window, sinks=2, **c.scales())
+        room = qd.clone()
+        assert torch.equal(paged_decode_attn(room, *c.args(), 0.1, window=window, sinks=2, out=room, **c.scales()), want)
+    _clean()
+
+
+def test_captured_shares(gpu):
+    """Captured calls that are cut into shares, two graphs and eager ones in turn, as lengths and windows change."""
+    lens = [4000] * 8
+    c = Cache(gpu, lens, 64, 128, BF, True, seed=31)
+    q, cu = _q(gpu, 100, 32, 128, BF), _cu([100], gpu)
+    window = torch.tensor([ALL, 500] * 4, dtype=torch.int32, device=gpu)
+    calls = [lambda: paged_prompt_attn(q, *c.args(), cu, 0.1, window=window, sinks=4, **c.scales()),
+             lambda: paged_prompt_attn(q, *c.args(), cu, 0.1, window=3000, sinks=4, **c.scales())]
+    graphs = []
+    for call in calls:
+        call()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        graphs.append((g, out))
+    for step in range(5):
+        c.lens = [4000 - 700 * step] * 8
+        c.seg_len.copy_(torch.tensor(c.lens, dtype=torch.int32))
+        window[step] = 900 * step
+        for g, _ in graphs:
+            g.replay()
+        want = [call() for call in calls]
+        for g, _ in graphs[::-1]:
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, x) for (_, out), x in zip(graphs, want))
+        _prompt_check(c, q, want[0], [100], window, 4, 0.1)
+    _clean()
