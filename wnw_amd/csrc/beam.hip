@@ -12,20 +12,20 @@
 // maxima), reads these alone again, and ranks what is not below the k-th group's
 // maximum.
 //
-// What bounds it: memory for many rows (512 of 51,865 f16 logits, 53 MB: 13.3 us for
-// the first launch, 4.0 TB/s; 8.2 for the second), else the launches and a chain of
-// dependent loads (5 rows of 32,000: 3.8 and 6.4; 32 of 131,072 f32: 6.8 and 8.2).
-// One launch, whose last workgroup of a sample to arrive does the second's work: 10.5,
-// 14.5 and 35.0 us in all, for 10.8, 13.8 and 19.2: what is left for another
-// workgroup has to pass by the caches.
+// What bounds it: memory for many rows (512 of 51,865 f16 logits, a fifth of the beams
+// finished, 43 MB: 12.9 us for the first launch, 3.3 TB/s; 7.7 for the second), else the
+// launches and a chain of dependent loads (5 rows of 32,000: 3.5 and 6.7; 32 of
+// 131,072 f32: 6.6 and 8.0).  One launch, whose last workgroup of a sample to arrive does
+// the second's work: 10.5, 14.5 and 35.0 us in all, for 10.6, 13.8 and 19.2: what is left
+// for another workgroup has to pass by the caches.
 #include "wnw_common.h"
 
 namespace wnw {
 
-static constexpr int kBeamTask = 2048;    // logits of a wave
+static constexpr int kBeamTask = 2048;    // logits of a wave: four to eight loads in flight
 static constexpr int kBeamThreads = 1024; // of a sample's workgroup
 static constexpr int kBeamMax = 64;       // beams, and candidates to select
-static constexpr int kBeamList = 512;     // candidates that are ranked against each other
+static constexpr int kBeamList = 512;     // candidates that are ranked against each other; more go in k rounds of a maximum
 static constexpr float kBeamLog2e = 1.4426950408889634f;
 static constexpr float kBeamLowest = -3.402823466e38f;  // running maxima start here
 

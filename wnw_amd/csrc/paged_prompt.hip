@@ -38,6 +38,18 @@
 // products meet the other's exponentials (8 % slower in one loop); the next tile's
 // scores among the exponentials (2 to 5 % slower); loads two tiles ahead; raised
 // wave priority in the products.
+//
+// Through a window (WIN): what none of a block's rows sees is left out, in groups of 16
+// keys, and the rest put together to tiles (PromptTiles): tiles of 64 keys in their own
+// places walked a tile more at each border (ragged f16 prompts through 301 rows 72 us,
+// in groups 66).  Masks at both ends of the window only; tiles between take none.
+// Few blocks are cut into shares by the tiles that each has (prompt_share).  8-bit
+// pages at head_dim 128 have the products of one tile beside the vector work of the
+// next (kSideBySide).  Bound as above: 4,564 tokens through 1,024 rows 103 us (0.66
+// PFLOP/s; 117 in a row of 24), 512 tokens after 22,116 rows, 2 of 8 heads unwindowed, 93
+// (8.9 of them the join); there blocks are short, and of the 25 us of a workgroup of
+// the ragged prompts (63 us, 3.2 rounds of two a CU) its tiles take 17, the lengths, pages and
+// q 2.2, the first tiles' round trips 3.3 and the rows out 2.6.
 #include <algorithm>
 #include <type_traits>
 
@@ -72,7 +84,7 @@ struct PagedPromptParams {
 };
 
 static constexpr int kPpKeys = 64;  // keys of a tile
-static constexpr int kPpLeast = 4;  // tiles of a share at least
+static constexpr int kPpLeast = 4;  // tiles of a share at least (as pieces without a window, below)
 
 template <typename T>
 __device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f32x16& c) {
@@ -147,7 +159,7 @@ __device__ __forceinline__ PromptTiles tiles_of(const PagedPromptParams& p, cons
 // least number with which the launch's workgroups have a share each.  Every workgroup
 // finds that out for itself, a wave over at most 512 blocks, from numbers that
 // are on the device.
-static constexpr int kPpShared = 512;  // blocks at most
+static constexpr int kPpShared = 512;  // blocks at most: 8 a lane, as many as workgroups of 4 waves at a time
 struct PromptShare {
   int block, split, splits;  // block -1: none
 };
