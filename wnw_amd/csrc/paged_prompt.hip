@@ -45,11 +45,11 @@
 // in groups 66).  Masks at both ends of the window only; tiles between take none.
 // Few blocks are cut into shares by the tiles that each has (prompt_share).  8-bit
 // pages at head_dim 128 have the products of one tile beside the vector work of the
-// next (kSideBySide).  Bound as above: 4,564 tokens through 1,024 rows 103 us (0.66
-// PFLOP/s; 117 in a row of 24), 512 tokens after 22,116 rows, 2 of 8 heads unwindowed, 93
-// (8.9 of them the join); there blocks are short, and of the 25 us of a workgroup of
-// the ragged prompts (63 us, 3.2 rounds of two a CU) its tiles take 17, the lengths, pages and
-// q 2.2, the first tiles' round trips 3.3 and the rows out 2.6.
+// next (kSideBySide); 16-bit pages go straight into LDS (kDirect).  Bound as above: 4,564
+// tokens through 1,024 rows 103 us (0.66 PFLOP/s; 117 in a row of 24), 512 tokens after
+// 22,116 rows, 2 of 8 heads unwindowed, 92 (8.9 of them the join).  The ragged prompts, 57
+// us, have short blocks: a workgroup's lengths, pages and q, its first tiles' round trips
+// and its rows out are a third of its time, and two are on a CU.
 #include <algorithm>
 #include <type_traits>
 
@@ -259,9 +259,15 @@ __device__ __forceinline__ void prompt_store(const PagedPromptParams& p, const P
     }
 }
 
-// Registers for at most 3 waves per SIMD: made to fit 4, head_dim 64 over 8 bits takes 43.5 us for 40.7 (2,048 tokens).
+// Waves per SIMD that the registers are for, at least and at most: 3 at most, as made to
+// fit 4, head_dim 64 over 8 bits takes 43.5 us for 40.7 (2,048 tokens).  Windows over 16-bit
+// pages, whose tiles do not go through registers, take 4 at head_dim 64 and 2 at 256.
+constexpr int prompt_waves(int d, bool q8, bool win, bool most) {
+  if (win && !q8 && d != 128) return d == 64 ? 4 : 2;
+  return d == 256 && !q8 ? 1 : most ? 3 : 2;
+}
 template <typename T, int D, bool Q8, int W, bool WIN>
-__global__ __launch_bounds__((64 * W)) __attribute__((amdgpu_waves_per_eu((D == 256 && !Q8 ? 1 : 2), (D == 256 && !Q8 ? 1 : 3)))) void
+__global__ __launch_bounds__((64 * W)) __attribute__((amdgpu_waves_per_eu(prompt_waves(D, Q8, WIN, false), prompt_waves(D, Q8, WIN, true)))) void
 paged_prompt_kernel(PagedPromptParams p) {
   using VT = typename std::conditional<Q8, bf16_t, T>::type;   // the value product's type
   using VO = HalfOps<VT>;
@@ -272,6 +278,12 @@ paged_prompt_kernel(PagedPromptParams p) {
   constexpr int NI = kPpKeys * GB / (1024 * W);                     // 16-byte loads per thread and tensor
   constexpr int KK = D / 16, DT = D / 32;
   constexpr int NB = D == 256 ? 1 : 2;  // tiles in LDS
+  // Windows over 16-bit pages: the tiles go straight into LDS, by loads that need no
+  // registers (through 301 rows, ragged f16 prompts at head_dim 128 67 us for 72, 4,564
+  // tokens through 1,024 rows 113 for 119, at head_dim 64 61 for 67, at 256, whose
+  // registers then are enough for a second workgroup on a CU, 206 for 296; but 23 -> 25 for
+  // 300 tokens, where each has a CU of its own).
+  constexpr bool kDirect = WIN && !Q8;
   constexpr bool kAhead = D != 256 || !Q8;  // the next tile's loads are on their way during the products
   // f16 weights are held times 2^8: normal numbers down to 2^-22 of the largest;
   // bf16 ones times 2^-16: 2^16 times the type's largest value is a sum yet
@@ -282,7 +294,7 @@ paged_prompt_kernel(PagedPromptParams p) {
   // 66), and so does head_dim 64, whose products are short (window 500: 53 for 48).
   constexpr bool kSideBySide = WIN && Q8 && D == 128;
   constexpr bool kTwo = Q8 && std::is_same<T, f16_t>::value;  // weights of two parts
-  __shared__ __attribute__((aligned(16))) uint8_t lds[NB * 2 * TB];  // [NB][K, V]
+  __shared__ __attribute__((aligned(16))) uint8_t lds[NB * 2 * TB];  // [NB][K, V]; kDirect: [NB] K, [NB] V
   __shared__ int odd;  // V had infinities or NaN in such a tile
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hi = lane >> 5, n = lane & 31;
@@ -375,6 +387,32 @@ paged_prompt_kernel(PagedPromptParams p) {
     vs = vs_next;
     if (!WIN || (window + 1) * kWin <= t1 + 1) find(window + 1);  // (short walks end before: no round trip for nothing)
   };
+  // kDirect: a lane's 16 bytes of a load go to its place in the load's rows, so it fetches the
+  // chunk that the swizzle puts there.  What is in no page, or not seen by all, is taken out in LDS.
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds);
+  const uint32_t ksrc = (lane / CG) * GB + (((lane % CG) ^ (srow % CH)) * 16);
+  const uint32_t vsrc = (lane / CG) * GB + (((lane % CG) ^ (2 * (srow & 3))) * 16);
+  uint32_t knone = 0, vnone = 0;  // loads of the tile's K, of its V, whose rows are in no page: a bit each
+  auto issue = [&](int tile, bool v, uint32_t to) __attribute__((always_inline)) {
+    const int in = (1 << p.c.shift) - 1;
+    uint32_t none = 0;
+#pragma unroll
+    for (int u = 0; u < NI; ++u) {
+      const int in_tile = u * RPL + w * (64 / CG);
+      const int row = key_of(tile, in_tile >> 4) + (in_tile & 15);
+      const int id = __builtin_amdgcn_readlane(pid, ((tile * kPpKeys + in_tile) >> 4) & 63);
+      const uint8_t* from = (v ? p.c.v : p.c.k) + ((int64_t)(id & 0x7fffffff) * (v ? p.c.v_stride : p.c.k_stride) + (row & in) * GB);
+      constexpr uint32_t kRot = RPL % CH;  // load u's rows lie u * RPL further: as in put()
+      lds_copy16(uniform_ptr(from), v ? vsrc : ksrc ^ (u * kRot % CH * 16), to + in_tile * RB);
+      none |= id < 0 ? 1u << u : 0;
+    }
+    return none;
+  };
+  auto issue_k = [&](int tile) __attribute__((always_inline)) {
+    if (tile % kWin == 0) enter(tile / kWin);
+    knone = issue(tile, false, lds0 + (tile & (NB - 1)) * TB);
+  };
+  auto issue_v = [&](int tile) __attribute__((always_inline)) { vnone = issue(tile, true, lds0 + (NB + (tile & (NB - 1))) * TB); };
   u32x4 kr[NI], vr[NI];
   int gone[NI];  // rows of kr and vr in no page: negative
   auto fetch = [&](int tile) {
@@ -496,9 +534,35 @@ paged_prompt_kernel(PagedPromptParams p) {
       }
     }
   };
-  auto tile = [&](int i, auto masked) {
-    const uint8_t* kt = lds + (NB == 2 ? (i & 1) * 2 * TB : 0);
-    const uint8_t* vt = kt + TB;
+  // kDirect: takes out of a tile's V, which has landed, what some of the rows do not see
+  auto only_seen = [&](int i) __attribute__((always_inline)) {
+    const bool all = whole(i);
+    if (all && !vnone) return;
+    bool any = false;
+#pragma unroll
+    for (int u = 0; u < NI; ++u) {
+      const int in_tile = u * RPL + w * (64 / CG);
+      const int row = key_of(i, in_tile >> 4) + ((in_tile + lane / CG) & 15);
+      u32x4* at = (u32x4*)(lds + (NB + (i & (NB - 1))) * TB + in_tile * RB + lane * 16);
+      u32x4 x = *at;
+      if ((vnone >> u & 1) || row >= r.len) x = u32x4{0, 0, 0, 0};
+      if (!all) any |= take_odd<PE>(x);
+      *at = x;
+    }
+    if (any) odd = 1;
+  };
+  // kDirect, one buffer: V is loaded during the scores, the next K during V's products
+  auto landed = [&](int i) __attribute__((always_inline)) {
+    if constexpr (NB == 1) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      only_seen(i);
+      __syncthreads();
+      if (i + 1 < t1) issue_k(i + 1);
+    }
+  };
+  auto tile = [&](int i, auto masked) __attribute__((always_inline)) {
+    const uint8_t* kt = lds + (kDirect ? (i & (NB - 1)) * TB : NB == 2 ? (i & 1) * 2 * TB : 0);
+    const uint8_t* vt = kDirect ? lds + (NB + (i & (NB - 1))) * TB : kt + TB;
     if (D == 256) {
       kget = here(kget);
       vget = here(vget);
@@ -510,7 +574,7 @@ paged_prompt_kernel(PagedPromptParams p) {
     for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) s[mt] = mma32<T>(*(const u32x4*)(kt + (kget ^ 32 * kk) + mt * 32 * RB), qr[kk], s[mt]);
-    if constexpr (NB == 2) {  // among the products: the next tile into the other buffer, the one after it on its way
+    if constexpr (NB == 2 && !kDirect) {  // among the products: the next tile into the other buffer, the one after it on its way
       put(i + 1);
       fetch(i + 2);
     }
@@ -572,6 +636,7 @@ paged_prompt_kernel(PagedPromptParams p) {
       }
       l = Q8 ? fmaf(sum, un[b], l) : l + sum;
     }
+    if constexpr (kDirect) landed(i);
 #pragma unroll
     for (int b = 0; b < 4; ++b)
 #pragma unroll
@@ -937,18 +1002,43 @@ paged_prompt_kernel(PagedPromptParams p) {
     find(t0 / kWin);
     find_scales();
     if (t0 % kWin != 0) enter(t0 / kWin);
-    if (kAhead) fetch(t0);
+    if (kDirect) {
+      issue_k(t0);
+      issue_v(t0);
+    } else if (kAhead) {
+      fetch(t0);
+    }
     if (t0 % kWin >= kWin / 2) find_scales();
-    if constexpr (NB == 2) {
+    if constexpr (NB == 2 && !kDirect) {
       clear(t0);
       even(t0);
       put(t0);
     }
     if (Q8 && kAhead) enter_scales();
-    if constexpr (NB == 2) fetch(t0 + 1);
+    if constexpr (NB == 2 && !kDirect) fetch(t0 + 1);
     // (the tile after next is fetched while a tile is used, or the next one with
     // one buffer: the window of the products follows that of fetch() by as much)
     auto turn = [&](int i) {
+      if constexpr (kDirect) {  // the loads of a tile are on their way while the one before it is used
+        if (NB == 1 && i == t0)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI) : "memory");  // V behind K
+        else
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (knone) {
+#pragma unroll
+          for (int u = 0; u < NI; ++u)
+            if (knone >> u & 1)
+              *(u32x4*)(lds + (i & (NB - 1)) * TB + (u * RPL + w * (64 / CG)) * RB + lane * 16) = u32x4{0, 0, 0, 0};
+        }
+        if constexpr (NB == 2) only_seen(i);
+        __syncthreads();  // tile i, K of it at least, is in LDS; everyone is done with tile i - 1
+        if (NB == 1 && i > t0) issue_v(i);
+        if (NB == 2 && i + 1 < t1) {
+          issue_k(i + 1);
+          issue_v(i + 1);
+        }
+        return;
+      }
       if (!kAhead) fetch(i);
       if (Q8 && (kAhead ? i % kWin == 0 && i > t0 : i % kWin == 0 || i == t0)) enter_scales();
       __syncthreads();  // everyone is done with tile i - 1; with two buffers tile i is in LDS
@@ -964,7 +1054,9 @@ paged_prompt_kernel(PagedPromptParams p) {
       }
     };
     auto pass = [&](int i) {  // a tile that none of the wave's rows sees
-      if constexpr (NB == 2) {
+      if constexpr (kDirect) {
+        landed(i);
+      } else if constexpr (NB == 2) {
         put(i + 1);
         fetch(i + 2);
       }
@@ -999,7 +1091,34 @@ paged_prompt_kernel(PagedPromptParams p) {
   }
   l = sum_x32(l);
   if (splits == 1) {
-    prompt_store<T, DT, WIN>(p, r, row, h, hi, 0, o, l);
+    if constexpr (WIN) {  // whole rows, by way of LDS: a window of 300 rows 64.4 us for 68.5 (4,564 tokens, 8-bit pages)
+      static_assert(W * 32 * RB <= (int)sizeof(lds), "the waves' rows");
+      __syncthreads();  // everyone is done with the tiles
+      uint8_t* const rows = lds + w * 32 * RB;
+      const bool none = limit <= 0 || r.blind;
+      const float inv = 1.0f / l;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = none ? 0.f : o[dt][4 * j + e] * inv;
+          *(uint64_t*)(rows + n * RB + (((4 * dt + j) ^ (n % CH)) * 16) + hi * 8) =
+              (uint64_t)HalfOps<T>::pack2(y[2], y[3]) << 32 | HalfOps<T>::pack2(y[0], y[1]);
+        }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+      for (int at = lane / CH; at < 32; at += 64 / CH) {
+        const int to = qblk * kPpQ + 32 * w + at;
+        if (to >= r.rows) break;
+        const int i = to / p.G;
+        T* const op = (T*)p.out + (int64_t)(r.first + i) * p.ot + (int64_t)(h * p.G + to - i * p.G) * p.oh;
+        *gptr_w<u32x4>(op + 8 * ((lane % CH) ^ (at % CH))) = *(const u32x4*)(rows + at * RB + (lane % CH) * 16);
+      }
+    } else {
+      prompt_store<T, DT, WIN>(p, r, row, h, hi, 0, o, l);
+    }
   } else if (busy) {
     const int64_t place = WIN ? blockIdx.x : ((int64_t)block * N + seg) * p.splits + split;
     float* part = p.part + (place * W + w) * (DT * 16 + 2) * 64;

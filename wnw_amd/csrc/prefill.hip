@@ -91,28 +91,6 @@ struct PromptAttnParams {
 static constexpr int kPaQ = 128;   // queries per workgroup
 static constexpr int kPaKeys = 64;  // keys per tile
 
-// 16 bytes per lane from gbase + voff into LDS at lds_addr + 16 * lane (M0
-// carries the LDS address and is restored).  One wait state between M0's write
-// and the load, five between a vector instruction's write of the base and the
-// load, the two moves among them.
-__device__ __forceinline__ void prompt_copy16(const void* gbase, uint32_t voff, uint32_t lds_addr) {
-  uint32_t save;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %3\n\t"
-      "s_nop 2\n\t"
-      "global_load_lds_dwordx4 %1, %2\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(save)
-      : "v"(voff), "s"(gbase), "s"(lds_addr)
-      : "memory");
-}
-__device__ __forceinline__ const void* uniform_ptr(const void* p) {
-  const uint64_t x = (uint64_t)(uintptr_t)p;
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
-  return (const void*)(uintptr_t)(((uint64_t)hi << 32) | lo);
-}
-
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(PromptAttnParams p) {
   using Ops = PromptOps<T>;
@@ -160,8 +138,8 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(PromptAttnParams p
     if (key0 + kPaKeys > S) copy_offsets(S - 1 - key0);
 #pragma unroll
     for (int u = 0; u < NI; ++u) {
-      prompt_copy16(kt, kdma[u], dst + (w * NI + u) * 1024);
-      prompt_copy16(vt, vdma[u], dst + TB + (w * NI + u) * 1024);
+      lds_copy16(kt, kdma[u], dst + (w * NI + u) * 1024);
+      lds_copy16(vt, vdma[u], dst + TB + (w * NI + u) * 1024);
     }
   };
   // lane offsets of the operands inside a tile
