@@ -395,11 +395,12 @@ def test_prompt_blocks_of_different_lengths(gpu, q8, dtype, D, G, new, old):
         _prompt_check(c, q, room, new, window, sinks, D ** -0.5)
 
 
-@pytest.mark.parametrize("dtype,D", [(BF, 128), (FP, 128), (BF, 64)])
-def test_prompt_long_walks(gpu, dtype, D):
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (FP, 128), (BF, 64), (BF, 256)])
+def test_prompt_long_walks(gpu, q8, dtype, D):
     """Blocks that walk more tiles than a workgroup keeps the pages of, in a call that is not cut."""
     new, old, H, G = [2100], [6000], 8, 8
-    c = Cache(gpu, [8100] * H, 64, D, dtype, True, seed=D)
+    c = Cache(gpu, [8100] * H, 64, D, dtype, q8, seed=D)
     window, sinks = 5003, 37
     _hide(c, new, window, sinks)
     q = _q(gpu, 2100, H * G, D, dtype)
@@ -491,3 +492,35 @@ def test_captured_shares(gpu):
         assert all(torch.equal(out, x) for (_, out), x in zip(graphs, want))
         _prompt_check(c, q, want[0], [100], window, 4, 0.1)
     _clean()
+
+
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("dtype,D,G", [(BF, 128, 4), (FP, 64, 2), (BF, 256, 4), (FP, 128, 8)])
+@pytest.mark.parametrize("new,old", [(1, 900), (2, 900), (60, 900), (700, 300), (40, 9000)])
+def test_rows_without_a_page_read_as_zeros(gpu, q8, dtype, D, G, new, old):
+    """Blocks that are seen and have no page: the error word, and rows of zeros, beside NaN in page 0 and the last."""
+    n, R, window, sinks = new + old, 32, 200 + new, 70
+    c = Cache(gpu, [n], R, D, dtype, q8, seed=new + D)
+    first = max(old + 1 - window, 0)
+    gone = sorted({1, first // R + 1, first // R + 2, n // R - 1})
+    used = {int(c.table[0, j]) for j in range(-(-n // R)) if j not in gone}
+    k, v = c.rows(0)
+    for j in gone:
+        k[j * R:(j + 1) * R] = 0
+        v[j * R:(j + 1) * R] = 0
+        c.table[0, j] = (-1, 0x7fffffff, c.P, -5)[j % 4]
+    for page in {0, c.P - 1} - used:
+        for pages in (c.k, c.v):
+            (pages.view(torch.uint8) if q8 else pages)[page] = 0x7f if q8 else float("nan")
+    q = _q(gpu, new, G, D, dtype)
+    out = paged_prompt_attn(q, *c.args(), _cu([new], gpu), D ** -0.5, window=window, sinks=sinks, **c.scales())
+    torch.cuda.synchronize()
+    assert _lib.device_error() == _lib.DEVERR_BOUNDS
+    pos = (old + torch.arange(new, device=gpu)).repeat_interleave(G)
+    seen = _seen(n, pos, window, sinks)
+    p = torch.softmax((q.reshape(-1, D).double() @ k.t().contiguous() * D ** -0.5).masked_fill(~seen, -torch.inf), dim=1)
+    ref, A, h = p @ v, p @ v.abs(), HALF[dtype]
+    bound = h * ref.abs() + (h + 2.0 ** -13) * A
+    if dtype == FP:
+        bound = bound + seen.sum(1, keepdim=True) * 2.0 ** -25 * v.abs().max()
+    _check(out.reshape(-1, D), ref, bound, (new, old))
