@@ -14,12 +14,12 @@
 // show.  The plan says whether the call can be done; the second launch leaves
 // everything as it was where it cannot.  A compaction needs the whole pool's counts:
 // up to 64 workgroups each sum all of them, from their L2, and rank their own pages
-// (13,653 pages and their copies: 31 us a pass, planned by one workgroup 41).
+// (13,653 pages and their copies: 30 us a pass, planned by one workgroup 41).
 //
 // What bounds it: the launches and the plan's chain of loads; the bytes are few.
 // Forking 256 segments (6,060 pages) 5.7 us for the plan, 3.7 for the rest, and 3.2 for the
 // copies; reserving for 256 segments of up to 313 blocks (30,677 pages) 5.0 and 3.6;
-// compacting 13,653 pages 6.7 and 4.0.  The page copy is bound by memory: up to 4,096
+// compacting 13,653 pages 5.5 and 3.4.  The page copy is bound by memory: up to 4,096
 // workgroups for K and for V, a page at a time by 256 threads with four 16-byte loads in
 // flight (3,277 pages of 8 KB, 107 MB read and written with K and V: 21.4 us, 5.0 TB/s).
 #include <algorithm>
@@ -98,14 +98,26 @@ __device__ __forceinline__ int plan_scan(PlanShared& sh, int x, int* all) {
   return before + incl - x;
 }
 
+// Sum over the wave's lanes
+template <int kCtrl>
+__device__ __forceinline__ int lane_add(int x) {
+  return x + __builtin_amdgcn_mov_dpp(x, kCtrl, 0xf, 0xf, false);
+}
+__device__ __forceinline__ int lane_sum(int x) {
+  x = lane_add<0xB1>(x);   // quad_perm [1, 0, 3, 2]
+  x = lane_add<0x4E>(x);   // quad_perm [2, 3, 0, 1]
+  x = lane_add<0x141>(x);  // row_half_mirror
+  x = lane_add<0x140>(x);  // row_mirror
+  const auto y = __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false);
+  x = (int)(y[0] + y[1]);
+  const auto z = __builtin_amdgcn_permlane32_swap((uint32_t)x, (uint32_t)x, false, false);
+  return (int)(z[0] + z[1]);
+}
 // Sums of two numbers over all threads
 __device__ __forceinline__ void plan_sums(PlanShared& sh, int* a, int* b) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    *a += __shfl_xor(*a, o);
-    *b += __shfl_xor(*b, o);
-  }
+  *a = lane_sum(*a);
+  *b = lane_sum(*b);
   __syncthreads();
   if (lane == 0) {
     sh.wave[w] = *a;
@@ -476,6 +488,7 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactParam
   const PagesParams& g = p.g;
   const int tid = threadIdx.x, from = (int)blockIdx.x * p.range, to = min(from + p.range, g.n_pages);
   const Counts head = plan_counts(g, tid * kPlanPer);
+  const int own0 = from + tid < to ? g.refs[from + tid] : 0;
   auto count = [&](int x, int* below) {  // used pages, and those below page x
     int all = 0, low = 0;
     for (int at = tid * kPlanPer; at < g.n_pages; at += kPlanThreads * kPlanPer) {
@@ -500,7 +513,7 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactParam
   // its pages, 1,024 at a time
   int seen = before;  // used ones below the thread's
   for (int base = from; base < to; base += kPlanThreads) {
-    const int i = base + tid, c = i < to ? g.refs[i] : 0;
+    const int i = base + tid, c = base == from ? own0 : i < to ? g.refs[i] : 0;
     int all;
     const int mine = seen + plan_scan(sh, c > 0, &all);
     if (at_u < 0 && base <= used && used < base + kPlanThreads) {  // uniform
