@@ -447,10 +447,10 @@ paged_decode_kernel(PagedDecodeParams p) {
       const int mysteps = (b - a + nw - 1) / nw;
       DecodeRows r = decode_rows(p, seg, n);
       DecodeView view = {};
-      int lo = 0;  // rows from here on are in the first token's window
+      int lo = 0;  // rows from here on are in the first token's window; none with a window of 0
       if constexpr (WIN) {
         view = decode_view(kept(0, j), kept(1, j), n, p.t.most);
-        lo = max(n - r.count + 1 - view.window, 0);
+        lo = view.window > 0 ? max(n - r.count + 1 - view.window, 0) : 0x7fffffff;
         r.blind = (view.window | view.sinks) == 0;
       }
       auto real = [&](int step) { return WIN && step >= view.head ? step + view.gap : step; };

@@ -129,7 +129,7 @@ __device__ __forceinline__ int splits_of(int tiles, int most) { return max(min(t
 // buffers and the pages held in registers count.
 struct PromptTiles {
   int n, head, gap;
-  int lo, last_lo;  // rows from here on are in the window of the block's first row, of its last
+  int lo, last_lo;  // rows from here on are in the window of the block's first row (none with a window of 0), of its last
   __device__ __forceinline__ int group(int place) const { return place < head ? place : place + gap; }
   // the place of the first group at or past row x
   __device__ __forceinline__ int place_of(int x) const {
@@ -144,7 +144,7 @@ __device__ __forceinline__ PromptTiles tiles_of(const PagedPromptParams& p, cons
   PromptTiles y = {max((last + kPpKeys - 1) / kPpKeys, 0), 0, 0, 0, 0};
   if constexpr (WIN) {
     const int groups = max((last + 15) >> 4, 0);
-    y.lo = max(base + 32 * W * qblk / p.G - r.window, 0);
+    y.lo = r.window > 0 ? max(base + 32 * W * qblk / p.G - r.window, 0) : 0x7fffffff;
     y.last_lo = last - r.window;
     y.head = min((r.sinks + 15) >> 4, groups);
     y.gap = max(min(y.lo >> 4, groups) - y.head, 0);
