@@ -85,3 +85,20 @@ def test_prompt_of_sinks_alone(gpu, q8, dtype, D, G, page, new, old):
                                 **c.scales())
         _clean()
         _prompt_check(c, q, out, new, window, sinks, D ** -0.5)
+
+
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("new", [[2, 0, 1, 0], [60, 0, 7, 0]], ids=["few", "long"])
+@pytest.mark.parametrize("window,sinks", [(40, 4), (0, 20), (1 << 30, 0)])
+def test_samples_without_tokens(gpu, q8, new, window, sinks):
+    """No row of a sample without tokens is seen: none of its blocks is looked up, whatever its length."""
+    H, G, D = 2, 4, 64
+    lens = [n for n in (90, 500, 33, 16) for _ in range(H)]
+    c = Cache(gpu, lens, 16, D, BF, q8, seed=5)
+    _hide_unseen(c, new, window, sinks)
+    for b, n in enumerate(new):
+        assert n or int(c.table[b * H:(b + 1) * H, 0].max()) == -1
+    q = _q(gpu, sum(new), H * G, D, BF)
+    out = paged_prompt_attn(q, *c.args(), _cu(new, gpu), 0.2, max_tokens=max(new), window=window, sinks=sinks, **c.scales())
+    _clean()
+    _prompt_check(c, q, out, new, window, sinks, 0.2)

@@ -450,6 +450,7 @@ paged_decode_kernel(PagedDecodeParams p) {
       int lo = 0;  // rows from here on are in the first token's window; none with a window of 0
       if constexpr (WIN) {
         view = decode_view(kept(0, j), kept(1, j), n, p.t.most);
+        if (r.count == 0) view.window = view.sinks = 0;  // a sample without tokens: no row is seen
         lo = view.window > 0 ? max(n - r.count + 1 - view.window, 0) : 0x7fffffff;
         r.blind = (view.window | view.sinks) == 0;
       }
