@@ -888,10 +888,13 @@ int wnw_paged_prompt_attn_window(
 /* ------------------------------------------------------------------------ */
 /*
  * Which pages of a pool are used: page_refs int32 [n_pages] counts the table
- * entries that name each (0: free; a caller's own pages, that no table names,
- * may be counted too).  An entry is a page or -1; others set WNW_DEVERR_BOUNDS
- * and are taken for -1.  A segment's page that is partly filled is named by no
- * other entry.  All arrays are device arrays; nothing is waited for.
+ * entries that name each (0: free, any other number: used; a caller's own pages,
+ * that no table names, may be counted too).  An entry is a page or -1; others set
+ * WNW_DEVERR_BOUNDS and are taken for -1.  An entry's page is not free: a
+ * compaction takes one that is in the same way, a fork and a reservation go by
+ * the counts alone and may hand it out again.  A segment's page that is partly
+ * filled is named by no other entry.  All arrays are device arrays; nothing is
+ * waited for.
  *
  * Fresh pages are the lowest free ones, handed out in the order of (segment,
  * block).  Where a call cannot be done, because the free pages do not suffice

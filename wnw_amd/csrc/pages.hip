@@ -2,8 +2,8 @@
 // for the next rows and given back behind a window, a pool's used pages moved to
 // its front, rows copied from page to page.
 //
-// Which pages are used is counted: refs[p] table entries name page p.  With U used
-// pages, need_s fresh pages of segment s and the free pages f_0 < f_1 < ..., segment s
+// Which pages are used is counted: refs[p] table entries name page p, 0: it is free.  With
+// U used pages, need_s fresh pages of segment s and the free pages f_0 < f_1 < ..., segment s
 // gets f_i, i from sum_{s' < s} need_s' on; a compaction moves the i-th used page
 // at or above U to the i-th free one below.  All of it is prefix sums.
 //
@@ -477,7 +477,8 @@ __global__ __launch_bounds__(256) void reserve_kernel(ReserveParams p) {
 // compact
 // ---------------------------------------------------------------------------
 // The lists: of a used page at U or above, or a free one below, its rank among such
-// (place); by rank, the free ones (fresh), and the others and their counts.
+// (place; -1 of the others); by rank, the free ones (fresh), and the used ones above and
+// their counts.
 __device__ __forceinline__ int32_t* compact_page(const PagesParams& g) { return ws_place(g) + g.n_pages; }
 __device__ __forceinline__ int32_t* compact_refs(const PagesParams& g) { return compact_page(g) + g.n_pages / 2 + 1; }
 
@@ -495,9 +496,10 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactParam
       const Counts c = at < kPlanThreads * kPlanPer ? head : plan_counts(g, at);
 #pragma unroll
       for (int i = 0; i < kPlanPer; ++i) {
-        all += c.n[i] > 0;
-        low += c.n[i] > 0 && at + i < x;
+        all += c.n[i] != 0;
+        low += c.n[i] != 0 && at + i < x;
       }
+      all -= max(at + kPlanPer - g.n_pages, 0);  // those past the pool
     }
     plan_sums(sh, &all, &low);
     *below = low;
@@ -515,7 +517,7 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactParam
   for (int base = from; base < to; base += kPlanThreads) {
     const int i = base + tid, c = base == from ? own0 : i < to ? g.refs[i] : 0;
     int all;
-    const int mine = seen + plan_scan(sh, c > 0, &all);
+    const int mine = seen + plan_scan(sh, c != 0, &all);
     if (at_u < 0 && base <= used && used < base + kPlanThreads) {  // uniform
       __shared__ int found;
       if (i == used) found = mine;
@@ -524,17 +526,15 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactParam
     }
     if (i < to) {
       if (i < used) {
-        if (c <= 0) {
-          ws_fresh(g)[i - mine] = i;
-          ws_place(g)[i] = i - mine;
-        }
+        if (c == 0) ws_fresh(g)[i - mine] = i;
+        ws_place(g)[i] = c == 0 ? i - mine : -1;
       } else {
         const int rank = mine - at_u;
-        if (c > 0) {
+        if (c != 0) {
           compact_page(g)[rank] = i;
           compact_refs(g)[rank] = c;
         }
-        ws_place(g)[i] = c > 0 ? rank : -1;
+        ws_place(g)[i] = c != 0 ? rank : -1;
       }
     }
     seen += all;
@@ -553,9 +553,14 @@ __global__ __launch_bounds__(256) void compact_kernel(CompactParams p) {
     const int s = blockIdx.x;
     for (int j = tid; j < g.max_blocks; j += 256) {
       int e = entry_of(g, g.table[s * g.stride + j], true);
-      if (e >= used) {  // (one that the counts call free has no place to go to)
+      if (e >= 0) {
         const int rank = ws_place(g)[e];
-        e = rank >= 0 ? ws_fresh(g)[rank] : -1;
+        if (e < used ? rank >= 0 : rank < 0) {  // the counts call it free: another page may land in it
+          raise_device_error(g.err, WNW_DEVERR_BOUNDS);
+          e = -1;
+        } else if (e >= used) {
+          e = ws_fresh(g)[rank];
+        }
       }
       g.new_table[s * g.new_stride + j] = e;
     }
@@ -571,7 +576,7 @@ __global__ __launch_bounds__(256) void compact_kernel(CompactParams p) {
       p.moves[3 * i + 2] = is ? 1 << g.shift : 0;
     }
     const int c = g.refs[i];
-    g.new_refs[i] = i >= used ? 0 : c > 0 ? c : compact_refs(g)[ws_place(g)[i]];
+    g.new_refs[i] = i >= used ? 0 : c != 0 ? c : compact_refs(g)[ws_place(g)[i]];
   }
 }
 

@@ -7,8 +7,8 @@ A pool's state, beside the pages of each layer that shares it
 * ``page_table`` int32 [N, M]: the page of each block of each segment, -1 where
   there is none;
 * ``seg_len`` int32 [N];
-* ``page_refs`` int32 [P]: how many entries name each page (0: free).  A program
-  may count pages of its own too, that no entry names.
+* ``page_refs`` int32 [P]: how many entries name each page (0: free, any other
+  number: used).  A program may count pages of its own too, that no entry names.
 
 Every call gives the new table and the new counts, which agree again:
 ``page_refs`` + the new table's entries - the old one's.  Fresh pages are the
@@ -20,6 +20,8 @@ call that cannot be done, because the free pages do not suffice or because one
 of its lengths, parents or token counts is bad, sets the device error word
 (``wnw_amd._lib.device_error()``: DEVERR_CAPACITY, DEVERR_BOUNDS) and changes
 nothing.  Entries that are neither a page nor -1 set it too, and are taken for -1.
+So does, for ``paged_compact``, an entry whose page the counts call free; the
+other calls go by the counts alone, and may hand such a page out again.
 """
 from __future__ import annotations
 
