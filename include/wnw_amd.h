@@ -978,7 +978,9 @@ int wnw_paged_copy(const wnw_paged_cache* cache, const int32_t* copies,
 /*
  * The k best continuations of each sample: of the candidates (beam w, token v)
  * with total = scores[b, w] + logits[b, w, v] - log sum_v exp logits[b, w, v],
- * held in 64 bits, the k largest, equal ones by the lower (w, v).  logits [batch,
+ * the k largest, equal ones by the lower (w, v).  Totals are formed and compared in
+ * 64 bits, from a log-sum that is off by less than 2^-18 (up to 2^20 tokens): the
+ * order within a beam is exact, between beams up to that.  logits [batch,
  * beams, vocab] with strides[2] = {sample, beam} in elements, tokens contiguous,
  * rows at any element; scores [batch, beams]; done [batch, beams] or NULL: a beam
  * with a non-zero entry has finished and offers (scores[b, w], end) alone, its
