@@ -934,7 +934,7 @@ int wnw_paged_fork(const int32_t* page_table, int64_t table_stride,
  * window_all >= 0, as wnw_paged_decode_attn_window takes it; window_all < 0 and
  * window NULL: none) the blocks that neither the row at seg_len nor a later one
  * sees are given back: those past the sinks that end at or below row seg_len + 1
- * - window.  They serve later calls, not this one.  new_table and new_refs may
+ * - max(window, 1) (the row at seg_len is written, whether seen or not).  They serve later calls, not this one.  new_table and new_refs may
  * be page_table and page_refs themselves (with the same stride), else overlap
  * neither.  Not done: both as they were.
  */

@@ -9,7 +9,8 @@ import torch
 from tests.paged_ref import Cache
 from tests.test_gpu_paged import BF, FP, _clean, _cu, _q
 from tests.test_gpu_paged_window import _decode_check, _each, _prompt_check, _seen
-from wnw_amd.kv.paged import paged_decode_attn, paged_prompt_attn
+from wnw_amd.kv.paged import paged_append, paged_decode_attn, paged_prompt_attn
+from wnw_amd.kv.pages import paged_reserve
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +103,28 @@ def test_samples_without_tokens(gpu, q8, new, window, sinks):
     out = paged_prompt_attn(q, *c.args(), _cu(new, gpu), 0.2, max_tokens=max(new), window=window, sinks=sinks, **c.scales())
     _clean()
     _prompt_check(c, q, out, new, window, sinks, 0.2)
+
+
+@pytest.mark.parametrize("sinks", [0, 4, 16])
+def test_a_loop_of_sinks_alone(gpu, sinks):
+    """Pages reserved, a row appended, attention through a window of 0: a segment keeps its sinks' block and the one of the row
+    that is written, the last of a block too (row + 1 a multiple of the page's rows)."""
+    N, G, D, R = 2, 4, 64, 16
+    g = torch.Generator(device=gpu).manual_seed(7)
+    table = torch.full((N, 6), -1, dtype=torch.int32, device=gpu)
+    refs, lens = torch.zeros(5, dtype=torch.int32, device=gpu), torch.zeros(N, dtype=torch.int32, device=gpu)
+    k_pages, v_pages = (torch.zeros(5, R, D, device=gpu, dtype=BF) for _ in range(2))
+    rows = torch.randn(2, 90, N, D, device=gpu, generator=g).to(BF)
+    for i in range(90):
+        paged_reserve(table, lens, refs, R, window=0, sinks=sinks, out=(table, refs))
+        assert int(table[0, i // R]) >= 0 and int((table[0] >= 0).sum()) == (2 if sinks and i >= R else 1)
+        _, lens = paged_append(rows[0, i].unsqueeze(0), rows[1, i].unsqueeze(0), k_pages, v_pages, table, lens)
+        q = torch.randn(N, G, D, device=gpu, generator=g).to(BF)
+        out = paged_decode_attn(q, k_pages, v_pages, table, lens, 0.2, window=0, sinks=sinks)
+        _clean()
+        n = min(i + 1, sinks)
+        for s in range(N):
+            k, v = rows[0, :n, s].double(), rows[1, :n, s].double()
+            w = torch.softmax(q[s].double() @ k.t().contiguous() * 0.2, dim=1)
+            ref, A = w @ v, w @ v.abs()
+            assert bool(((out[s].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -13 * A).all()), (i, s)

@@ -120,7 +120,8 @@ def paged_reserve(page_table: Tensor, seg_len: Tensor, page_refs: Tensor, page_r
     With ``window`` (and ``sinks``; as ``paged_decode_attn`` takes them) the blocks
     that neither the next row nor a later one sees are given back, for later
     calls to hand out: those behind the sinks that end at or below row seg_len + 1
-    - window.  ``tokens`` may be 0.
+    - max(window, 1) (the row at seg_len is written, whether it is seen or not).
+    ``tokens`` may be 0.
 
     ``out``: (table, counts) to write to, which may be the given ones themselves,
     for programs and captured graphs that keep them in one place."""
