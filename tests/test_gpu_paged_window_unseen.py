@@ -110,10 +110,11 @@ def test_a_loop_of_sinks_alone(gpu, sinks):
     """Pages reserved, a row appended, attention through a window of 0: a segment keeps its sinks' block and the one of the row
     that is written, the last of a block too (row + 1 a multiple of the page's rows)."""
     N, G, D, R = 2, 4, 64, 16
+    P = 3 * N  # pages that a call gives back serve the next one
     g = torch.Generator(device=gpu).manual_seed(7)
     table = torch.full((N, 6), -1, dtype=torch.int32, device=gpu)
-    refs, lens = torch.zeros(5, dtype=torch.int32, device=gpu), torch.zeros(N, dtype=torch.int32, device=gpu)
-    k_pages, v_pages = (torch.zeros(5, R, D, device=gpu, dtype=BF) for _ in range(2))
+    refs, lens = torch.zeros(P, dtype=torch.int32, device=gpu), torch.zeros(N, dtype=torch.int32, device=gpu)
+    k_pages, v_pages = (torch.zeros(P, R, D, device=gpu, dtype=BF) for _ in range(2))
     rows = torch.randn(2, 90, N, D, device=gpu, generator=g).to(BF)
     for i in range(90):
         paged_reserve(table, lens, refs, R, window=0, sinks=sinks, out=(table, refs))
