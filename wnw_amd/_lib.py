@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from operator import index
 
 import torch  # loads torch's HIP runtime first; the library binds to it
 
@@ -184,6 +185,14 @@ def dtype_code(dt: torch.dtype) -> int:
         return _TORCH_DTYPES[dt]
     except KeyError:
         raise WnwError(f"unsupported dtype {dt}") from None
+
+
+def whole(name: str, x) -> int:
+    """A whole number as the library's 64 bits hold it (ctypes would take it modulo 2^64)."""
+    x = index(x)
+    if not -1 << 63 <= x < 1 << 63:
+        raise WnwError(f"{name} is out of range: {x}")
+    return x
 
 
 def ptr(t: torch.Tensor | None):

@@ -5,7 +5,6 @@ forked by the parents found here (``wnw_amd.kv.pages.paged_fork``)."""
 from __future__ import annotations
 
 import ctypes
-from operator import index
 
 import torch
 from torch import Tensor
@@ -47,7 +46,7 @@ def beam_select(logits: Tensor, scores: Tensor, k: int | None = None, *, done: T
         raise _lib.WnwError(f"scores must be float32 [{B}, {W}], got {scores.dtype} {tuple(scores.shape)}")
     if done is not None and (done.dtype != torch.bool or done.shape != (B, W)):
         raise _lib.WnwError(f"done must be bool [{B}, {W}], got {done.dtype} {tuple(done.shape)}")
-    k, end = W if k is None else index(k), index(end)
+    k, end = W if k is None else _lib.whole("k", k), _lib.whole("end", end)
     if logits.numel() and logits.stride(2) != 1 or any(logits.stride(i) < 0 for i in range(2)):
         logits = logits.clone(memory_format=torch.contiguous_format)
     scores = scores.contiguous()

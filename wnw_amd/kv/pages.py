@@ -26,7 +26,6 @@ other calls go by the counts alone, and may hand such a page out again.
 from __future__ import annotations
 
 import ctypes
-from operator import index
 
 import torch
 from torch import Tensor
@@ -91,7 +90,7 @@ def paged_fork(page_table: Tensor, seg_len: Tensor, page_refs: Tensor, parents: 
     N, M, P, stride = _table(page_table, page_refs, seg_len, parents)
     if parents.dtype != torch.int32 or parents.dim() != 1 or not parents.is_contiguous():
         raise _lib.WnwError("parents must be a contiguous int32 [B']")
-    kv_heads, page_rows = index(kv_heads), index(page_rows)
+    kv_heads, page_rows = _lib.whole("kv_heads", kv_heads), _lib.whole("page_rows", page_rows)
     if kv_heads < 1 or N % kv_heads:
         raise _lib.WnwError(f"{N} segments are not samples x {kv_heads} KV heads")
     n_new = parents.numel()
@@ -138,7 +137,7 @@ def paged_reserve(page_table: Tensor, seg_len: Tensor, page_refs: Tensor, page_r
             raise _lib.WnwError(f"{N} segments are not {B} samples x KV heads")
     else:
         B = N
-    tokens, page_rows = index(tokens), index(page_rows)
+    tokens, page_rows = _lib.whole("tokens", tokens), _lib.whole("page_rows", page_rows)
     if tokens < 0:
         raise _lib.WnwError("tokens must not be negative")
     if window is None and sinks is not None:
@@ -168,7 +167,7 @@ def paged_compact(page_table: Tensor, page_refs: Tensor, page_rows: int, *,
     if done is not None:
         return done
     N, M, P, stride = _table(page_table, page_refs, None, *(out or ()))
-    page_rows = index(page_rows)
+    page_rows = _lib.whole("page_rows", page_rows)
     new_table, new_refs, new_stride = _out(out, page_table, page_refs)
     moves, used = page_refs.new_empty((P // 2, 3)), page_refs.new_empty(1)
     with torch.cuda.device(page_table.device):
