@@ -683,12 +683,13 @@ paged_prompt_kernel(PagedPromptParams p) {
     // V: when tile i is used, K of i + 1 and V of i are in LDS, K of i + 2 and V of i + 1 in
     // registers on their way there, K of i + 3 and V of i + 2 on their way from memory.
     // What a group's page and scales are lies in LDS, kRef tiles from tile ref0 on.
+    static_assert(Q8, "16-bit pages go straight into LDS");
     if (t0 < t1) {
       if (tid == 0) odd = 0;
       constexpr int kRef = 64;
       struct Refs {
         int32_t id[4 * kRef];
-        float k[Q8 ? 4 * kRef : 4], l[Q8 ? 4 * kRef : 4], u[Q8 ? 4 * kRef : 4];
+        float k[4 * kRef], l[4 * kRef], u[4 * kRef];
       };
       __shared__ __attribute__((aligned(16))) Refs refs;
       int ref0 = t0;
@@ -706,7 +707,7 @@ paged_prompt_kernel(PagedPromptParams p) {
         return id;
       };
       auto refer_scales = [&](int id) {
-        if (Q8 && tid < 4 * kRef) {
+        if (tid < 4 * kRef) {
           const float k_of = p.c.k_scale[max(id, 0)], v_of = p.c.v_scale[max(id, 0)];
           refs.k[tid] = fmaxf(id >= 0 ? k_of : 1.f, 7.888609e-31f) * p.scale_log2;  // a scale of 0 would make a masked score NaN
           const float log_v = fminf(fmaxf(__builtin_amdgcn_logf(id >= 0 ? v_of : 1.f), -80.f), 127.f);
@@ -724,12 +725,8 @@ paged_prompt_kernel(PagedPromptParams p) {
           const int row = key_of(tile, in_tile >> 4) + (in_tile & 15);
           const int id = __builtin_amdgcn_readfirstlane(refs.id[4 * (tile - ref0) + (in_tile >> 4)]);
           const WNW_GLOBAL uint8_t* at = gptr<uint8_t>(pages) + ((int64_t)(id & 0x7fffffff) * stride + (row & in) * GB);
-          if constexpr (Q8) {
-            const u32x2_t x0 = *(const WNW_GLOBAL u32x2_t*)(at + soff), x1 = *(const WNW_GLOBAL u32x2_t*)(at + (soff + GB / 2));
-            to[u] = u32x4{x0[0], x0[1], x1[0], x1[1]};
-          } else {
-            to[u] = *(const WNW_GLOBAL u32x4*)(at + soff);
-          }
+          const u32x2_t x0 = *(const WNW_GLOBAL u32x2_t*)(at + soff), x1 = *(const WNW_GLOBAL u32x2_t*)(at + (soff + GB / 2));
+          to[u] = u32x4{x0[0], x0[1], x1[0], x1[1]};
           none[u] = id;
         }
       };
@@ -756,32 +753,24 @@ paged_prompt_kernel(PagedPromptParams p) {
       };
       constexpr int kAheadK = 2, kAheadV = 3;  // steps that K's and V's operands are read ahead of their products
       // what the staging of K's tile and of V's writes to LDS, in kPut pieces each
-      constexpr int kPut = NI * (Q8 ? 2 : 1);
+      constexpr int kPut = NI * 2;
       auto put_k = [&](int tile, int piece) {
-        const int u = Q8 ? piece / 2 : piece;
+        const int u = piece / 2;
         constexpr int kRot = RPL % CH;
         const uint32_t kx = kRot ? ((u * kRot) % CH) * 16 : 0;
         uint8_t* kd = lds + (tile & 1) * 2 * TB + u * RPL * RB;
-        if constexpr (Q8) {
-          if (piece % 2 == 0)
-            *(u32x4*)(kd + (kput ^ kx)) = e4m3x8<T>(kr[u][0], kr[u][1]);
-          else
-            *(u32x4*)(kd + (kput ^ kx ^ kHalf)) = e4m3x8<T>(kr[u][2], kr[u][3]);
-        } else {
-          *(u32x4*)(kd + (kput ^ kx)) = kr[u];
-        }
+        if (piece % 2 == 0)
+          *(u32x4*)(kd + (kput ^ kx)) = e4m3x8<T>(kr[u][0], kr[u][1]);
+        else
+          *(u32x4*)(kd + (kput ^ kx ^ kHalf)) = e4m3x8<T>(kr[u][2], kr[u][3]);
       };
       auto put_v = [&](int tile, int piece) {
-        const int u = Q8 ? piece / 2 : piece;
+        const int u = piece / 2;
         uint8_t* vd = lds + (tile & 1) * 2 * TB + TB + u * RPL * RB;
-        if constexpr (Q8) {
-          if (piece % 2 == 0)
-            *(u32x4*)(vd + vput) = e4m3x8<VT>(vr[u][0], vr[u][1]);
-          else
-            *(u32x4*)(vd + (vput ^ kHalf)) = e4m3x8<VT>(vr[u][2], vr[u][3]);
-        } else {
-          *(u32x4*)(vd + vput) = vr[u];
-        }
+        if (piece % 2 == 0)
+          *(u32x4*)(vd + vput) = e4m3x8<VT>(vr[u][0], vr[u][1]);
+        else
+          *(u32x4*)(vd + (vput ^ kHalf)) = e4m3x8<VT>(vr[u][2], vr[u][3]);
       };
       auto put_all = [&](auto put, int tile) {
 #pragma unroll
@@ -824,9 +813,9 @@ paged_prompt_kernel(PagedPromptParams p) {
       f32x4 ck, lv, un;
       auto numbers = [&](int i) {
         const int at = 4 * (i - ref0);
-        ck = Q8 ? *(const f32x4*)(refs.k + at) : f32x4{p.scale_log2, p.scale_log2, p.scale_log2, p.scale_log2};
-        lv = Q8 ? *(const f32x4*)(refs.l + at) : f32x4{0.f, 0.f, 0.f, 0.f};
-        un = Q8 ? *(const f32x4*)(refs.u + at) : f32x4{1.f, 1.f, 1.f, 1.f};
+        ck = *(const f32x4*)(refs.k + at);
+        lv = *(const f32x4*)(refs.l + at);
+        un = *(const f32x4*)(refs.u + at);
       };
       auto scores = [&](int i, f32x16* s) {
         const uint8_t* kt = lds + (i & 1) * 2 * TB;
@@ -913,7 +902,7 @@ paged_prompt_kernel(PagedPromptParams p) {
                 }
               }
               if ((kk + 1) * kEach % 8 == 0) {
-                l = Q8 ? fmaf(sum, un[b], l) : l + sum;
+                l = fmaf(sum, un[b], l);
                 sum = 0.f;
                 asm volatile("" : "+v"(pb[b]), "+v"(l));  // here, not where they are used
                 if constexpr (kTwo) asm volatile("" : "+v"(pc[b]));
