@@ -1217,8 +1217,9 @@ static PromptPlan prompt_plan(int64_t n_seg, int64_t group, int64_t max_tokens, 
 // as many workgroups as the CUs hold, of 8 waves at head_dim 128 (512 tokens after
 // 22,116 rows, two of eight heads unwindowed: 93 us, with 4 waves 97).  Others have about
 // the same walk each, and smaller workgroups walk less beyond their own rows, two at a
-// time on a CU: 4,564 tokens, head_dim 128, window 100 54 us (8 waves: 60), 500 81 (91),
-// 1,024 105 (107), but 2,000 165 (161): 8 from 25 tiles on.
+// time on a CU (8-bit pages, 4,564 tokens, window 300: 61 us, with 8 waves 71; 500 73 and
+// 88; 1,024 105 and 107; 1,400 129 and 125; 2,000 153 and 158; the whole prompt 211 and
+// 208; 9,000 tokens, window 1,024 206 and 224, the whole prompt 722 and 703).
 static PromptPlan window_plan(int64_t n_seg, int64_t group, int64_t max_tokens, int64_t capacity, int64_t D, const PagedView& view) {
   const bool alike = !view.window && !view.sinks;
   const int64_t rows = max_tokens * group, cus = device_cus();
@@ -1239,7 +1240,7 @@ static PromptPlan window_plan(int64_t n_seg, int64_t group, int64_t max_tokens, 
     y.part = (wgs * 8 + 255) / 256 * 256;
     y.bytes = y.part + want * y.waves * (D / 2 + 2) * 64 * 4;
   } else {
-    blocks(D == 128 && tiles > 24 ? 8 : 4);
+    blocks(4);
   }
   return y;
 }
@@ -1307,7 +1308,7 @@ static int prompt_attn(const wnw_paged_cache* cache, const int32_t* seg_len, con
     return paged_decode_launch(cache, seg_len, q, out, strides, p.t, view, group, scale, dtype, workspace, workspace_bytes, stream);
   WNW_CHECK_ARG(most * group < (1ll << 30), "too many query rows");
   const PromptPlan y = view ? window_plan(N, group, most, p.c.capacity, D, *view) : prompt_plan(N, group, most, p.c.capacity, D);
-  WNW_CHECK_ARG(N * y.nqb < (1ll << 23), "too many segments and tokens for one call");
+  WNW_CHECK_ARG(N * y.nqb * y.waves < (1ll << 26), "too many segments and tokens for one call");  // 2^32 threads
   WNW_CHECK_ARG(y.bytes == 0 || (workspace && workspace_bytes >= y.bytes), "workspace too small: %lld bytes, %lld needed",
                 (long long)workspace_bytes, (long long)y.bytes);
   WNW_CHECK_ARG((uintptr_t)workspace % 256 == 0, "the workspace must be 256-byte aligned");
