@@ -67,7 +67,7 @@ def test_decode_of_some_windows_zero(gpu, q8, lens):
     _decode_check(c, q, out, window, sinks, 0.2)
 
 
-# few: the decode kernel's; two head counts so that both workgroup sizes at head_dim 128 run; long: shares of a block
+# few: the decode kernel's; the others the prompt kernel's, blocks shared out where windows are on the device
 PROMPTS = [([1, 2, 3], [0, 70, 1]), ([33, 5, 64, 7], [0, 9, 100, 1000]), ([129, 200], [0, 333]), ([300], [9000])]
 
 

@@ -33,11 +33,15 @@
 // Through a window (WIN): the same sums over rows below `sinks` and the last `window`.
 // The steps between, which no row of a call sees, are taken out of a segment's steps
 // before these are cut, so that the split stays even and their table entries are not
-// read; what is left of a step is masked.  A kernel of its own: the windows, the
-// steps' places and the masks cost 1.7 us a launch.  One launch for heads that see
-// everything and heads that do not (64 segments, 16 of 7,564 rows and 48 of 512, 37 MB):
-// 23.3 us, the chain of round trips above; 8 segments of 128 rows: 9.6; 256 segments of
-// up to 2,057 16-bit rows, 224 MB: 48.4, 4.6 TB/s.
+// read; what is left of a step is masked.  A window of 0, and a sample without tokens,
+// see no row past the sinks, or none.  A kernel of its own: 16 segments of 7,564 rows and
+// 48 of 512 (8-bit pages, 37 MB) take 18.4 us without windows and 21.3 through windows
+// that show everything: the windows' loads, the steps' places, the masks and the
+// registers that these need (14 spilled for 3).  The same rows as windows of 64 segments of
+// 7,564: 22.2, the short ones having a step or two more; the chain of round trips above
+// bounds it.  8 segments of 128 rows: 9.6; 256 segments of up to 2,057 16-bit rows, 224 MB:
+// 48.4, 4.6 TB/s.  Prompt calls of four tokens (16 query rows of 64 segments, 1,024 of
+// 7,564 8-bit rows each, 17 MB): 17.1 to 18.1, of 8 segments 15.6.
 #include <algorithm>
 #include <cstdlib>
 #include <type_traits>

@@ -32,7 +32,7 @@
 // vector instructions 920, and on one SIMD these add up: 4,564 tokens take 442,000
 // cycles, for 37 % of which matrix instructions run and for 51 % vector ones.  That
 // is 196 to 211 us a pass (by the card) where passes have pauses between them, 0.8
-// to 0.87 PFLOP/s (plain bf16 products of size 8,192: 1.2), and 233 us in a row of
+// to 0.87 PFLOP/s (plain bf16 products of size 8,192: 1.2 to 1.4), and 233 us in a row of
 // 24, over which the clock falls to 2.1 GHz or less.
 // Without gain: half of the waves a phase behind the others, so that one's
 // products meet the other's exponentials (8 % slower in one loop); the next tile's
@@ -45,11 +45,19 @@
 // in groups 66).  Masks at both ends of the window only; tiles between take none.
 // Few blocks are cut into shares by the tiles that each has (prompt_share).  8-bit
 // pages at head_dim 128 have the products of one tile beside the vector work of the
-// next (kSideBySide); 16-bit pages go straight into LDS (kDirect).  Bound as above: 4,564
-// tokens through 1,024 rows 103 us (0.66 PFLOP/s; 117 in a row of 24), 512 tokens after
-// 22,116 rows, 2 of 8 heads unwindowed, 92 (8.9 of them the join).  The ragged prompts, 57
-// us, have short blocks: a workgroup's lengths, pages and q, its first tiles' round trips
-// and its rows out are a third of its time, and two are on a CU.
+// next (kSideBySide); 16-bit pages go straight into LDS (kDirect).
+//
+// What bounds it: 4,564 tokens through 1,024 rows take 101 to 107 us (0.66 PFLOP/s; up to
+// 117 in a row of 24, by the card), 512 tokens after 22,116 rows, 2 of 8 heads unwindowed,
+// 92 (8.9 of them the join).  Over 2,048 to 6,144 tokens the time is a line, 16.5 us and
+// 5.1 ns a tile of 128 rows, within 3 us wherever the workgroups fill the CUs a whole
+// number of times or not.  The 16.5 are the launch, the first tiles' round trips, the rows out and the
+// last workgroups; the 5.1, 1.3 us of a CU, are 2,700 to 3,150 cycles (2.06 to 2.4 GHz) of
+// its SIMDs for a wave's tile, whose matrix and vector instructions one after the other
+// are 2,450: beside the instructions, which overlap in part, it is the barrier of each tile
+// and its waits for LDS, not measured one by one.  The ragged prompts, 57 us, have short
+// blocks: a workgroup's lengths, pages and q, its first tiles' round trips and its rows
+// out are a third of its time, and two are on a CU.
 #include <algorithm>
 #include <type_traits>
 

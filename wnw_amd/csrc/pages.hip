@@ -18,10 +18,13 @@
 //
 // What bounds it: the launches and the plan's chain of loads; the bytes are few.
 // Forking 256 segments (6,060 pages) 5.7 us for the plan, 3.7 for the rest, and 3.2 for the
-// copies; reserving for 256 segments of up to 313 blocks (30,677 pages) 5.0 and 3.6;
+// copies; reserving a row for 256 segments of up to 313 blocks (30,677 pages) 5.0 and 3.6;
 // compacting 13,653 pages 5.5 and 3.4.  The page copy is bound by memory: up to 4,096
 // workgroups for K and for V, a page at a time by 256 threads with four 16-byte loads in
 // flight (3,277 pages of 8 KB, 107 MB read and written with K and V: 21.4 us, 5.0 TB/s).
+// Reserving for prompts the plan is bound by its waves, each of which looks 16 segments'
+// blocks over one after the other: 256 segments of 500 to 2,000 new rows 24 us a pass with
+// pages of 64 (5,132 of them), 34 with pages of 16 (21,920); a row each 9.4.
 #include <algorithm>
 
 #include "paged.h"
